@@ -29,6 +29,9 @@ SOURCES = {
     "capi.hip": [],
     "bin.hip": ["-ffp-contract=off"],
     "render.hip": [],
+    "norm.hip": [],
+    "linear.hip": [],
+    "attend.hip": [],
 }
 
 

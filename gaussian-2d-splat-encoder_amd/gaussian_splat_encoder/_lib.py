@@ -29,7 +29,16 @@ class SplatLevels(ctypes.Structure):
                 ("coarse_H", _I), ("coarse_W", _I)]
 
 
+class SplatAttention(ctypes.Structure):
+    """struct splat_attention: the shapes, strides and masks of a cross attention."""
+    _fields_ = [("dtype", _I), ("B", _I), ("H", _I), ("Hk", _I), ("D", _I), ("scale", _F), ("Lq", _LL), ("Lk", _LL),
+                ("qb", _LL), ("ql", _LL), ("qh", _LL), ("kb", _LL), ("kl", _LL), ("kh", _LL),
+                ("vb", _LL), ("vl", _LL), ("vh", _LL), ("gb", _LL), ("gl", _LL), ("gh", _LL),
+                ("mb", _LL), ("ml", _LL), ("kv_lengths", _VP), ("key_mask", _VP)]
+
+
 _LV = ctypes.POINTER(SplatLevels)
+_AT = ctypes.POINTER(SplatAttention)
 _U = ctypes.c_uint
 
 # name -> (restype, argtypes)
@@ -81,6 +90,18 @@ _SIGS = {
     "splat_exact_render_bwd_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "splat_exact_render_bwd": (_I, [_VP, _VP, _I, _I, _VP, _VP, _I, _I, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
                                     _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "splat_group_norm_workspace_bytes": (_SZ, [_I, _I, _LL, _I, _I]),
+    "splat_group_norm_fwd": (_I, [_VP, _LL, _LL, _VP, _VP, _I, _I, _LL, _I, _I, _F, _I, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "splat_group_norm_bwd_workspace_bytes": (_SZ, [_I, _I, _LL, _I, _I]),
+    "splat_group_norm_bwd": (_I, [_VP, _LL, _LL, _VP, _LL, _LL, _VP, _VP, _VP, _VP, _I, _I, _LL, _I, _I, _I, _I, _VP, _VP,
+                                  _VP, _VP, _SZ, _VP]),
+    "splat_linear_fwd": (_I, [_VP, _LL, _VP, _VP, _VP, _LL, _I, _LL, _I, _I, _I, _VP, _VP, _VP]),
+    "splat_linear_bwd_workspace_bytes": (_SZ, [_I, _LL, _I, _I, _I]),
+    "splat_linear_bwd": (_I, [_VP, _LL, _VP, _VP, _VP, _I, _LL, _I, _I, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "splat_attention_workspace_bytes": (_SZ, [_AT]),
+    "splat_attention_fwd": (_I, [_AT, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "splat_attention_bwd_workspace_bytes": (_SZ, [_AT]),
+    "splat_attention_bwd": (_I, [_AT, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
 }
 
 EXPORTED = tuple(_SIGS)

@@ -1,0 +1,338 @@
+"""Operators of channels-last feature maps and of models that read them, on hand-written HIP kernels (gfx950), forward and
+backward: group norm with an activation, products with an epilogue, cross attention.
+
+Tensors are float32 or bfloat16 on a HIP device, the last dimension dense (anything else is copied first); sums, softmax
+statistics and norms are float32 whatever the type. Results are deterministic: no atomics, fixed orders of summation.
+Everything runs on the current stream and returns without waiting. Device work goes through libsplat_hip.so
+(include/splat_render.h). The reference has no counterpart: its network runs on stock torch operations.
+
+Activations: "none", "gelu" (x Phi(x)), "silu", "relu", "tanh", "sigmoid".
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._lib import SplatAttention, check
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_ACTS = {"none": 0, "gelu": 1, "silu": 2, "relu": 3, "tanh": 4, "sigmoid": 5}
+MAX_HEAD = 128   # values of a head at most
+
+
+def _args(act, x, *others):
+    """Type and activation codes of a call; x's type is every other tensor's too."""
+    for t in (x, *others):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("the HIP feature operators need device tensors (got a CPU tensor)")
+        if t.dtype is not x.dtype:
+            raise ValueError(f"tensors of one type are needed, got {x.dtype} and {t.dtype}")
+        if t.device != x.device:
+            raise ValueError(f"tensors of one device are needed, got {x.device} and {t.device}")
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"float32 or bfloat16 is needed, got {x.dtype}")
+    code = _ACTS.get(act)
+    if code is None:
+        raise ValueError(f"unknown activation {act!r}: one of {sorted(_ACTS)}")
+    return dt, code
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _scratch(nbytes, x):
+    """(tensor that keeps the workspace, its pointer); the caller's stream owns it like any torch tensor."""
+    if not nbytes:
+        return None, None
+    t = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    return t, t.data_ptr()
+
+
+class _On:
+    """Makes x's device current for a call where it is not (the library launches on the current device)."""
+
+    def __init__(self, x):
+        i = x.device.index
+        self.guard = None if i == torch.cuda.current_device() else torch.cuda.device(i)
+        self.index = i
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return _lib.stream_ptr(self.index)
+
+    def __exit__(self, *e):
+        if self.guard is not None:
+            self.guard.__exit__(*e)
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+# ------------------------------------------------------------------------------------------------ group norm
+def _positions(x):
+    """x [B, ..., C] as [B, L, C] with dense channels (a view where the strides allow it)."""
+    B, C = x.shape[0], x.shape[-1]
+    x = x.reshape(B, math.prod(x.shape[1:-1]), C)
+    return x if C == 1 or x.stride(2) == 1 else x.contiguous()
+
+
+def _norm_fwd(x3, weight, bias, G, eps, dt, act, first, save):
+    B, L, C = x3.shape
+    lib = _lib.load()
+    y = torch.empty((B, L, C), dtype=x3.dtype, device=x3.device)
+    stat = torch.empty((2, B, G), dtype=torch.float32, device=x3.device) if save else None
+    if y.numel():
+        with _On(x3) as stream:
+            n = lib.splat_group_norm_workspace_bytes(dt, B, L, C, G)
+            keep, ws = _scratch(n, x3)
+            sp = _ptr(stat)
+            check(lib.splat_group_norm_fwd(x3.data_ptr(), x3.stride(0), x3.stride(1), _ptr(weight), _ptr(bias), dt, B, L, C, G,
+                                           eps, act, first, y.data_ptr(), sp, sp + 4 * B * G if save else None, ws, n,
+                                           stream), "splat_group_norm_fwd")
+    return y, stat
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, G, eps, dt, act, first):
+        x3 = _positions(x)
+        y, stat = _norm_fwd(x3, weight, bias, G, eps, dt, act, first, True)
+        ctx.save_for_backward(x3, weight, bias, stat)
+        ctx.args = (x.shape, G, dt, act, first)
+        return y.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x3, weight, bias, stat = ctx.saved_tensors
+        shape, G, dt, act, first = ctx.args
+        B, L, C = x3.shape
+        lib = _lib.load()
+        new = torch.empty if x3.numel() else torch.zeros
+        dx = torch.empty((B, L, C), dtype=x3.dtype, device=x3.device)
+        dw = new(C, dtype=torch.float32, device=x3.device) if ctx.needs_input_grad[1] else None
+        db = new(C, dtype=torch.float32, device=x3.device) if ctx.needs_input_grad[2] else None
+        if x3.numel():
+            g3 = _positions(dy)
+            with _On(x3) as stream:
+                n = lib.splat_group_norm_bwd_workspace_bytes(dt, B, L, C, G)
+                keep, ws = _scratch(n, x3)
+                sp = stat.data_ptr()
+                check(lib.splat_group_norm_bwd(x3.data_ptr(), x3.stride(0), x3.stride(1), g3.data_ptr(), g3.stride(0),
+                                               g3.stride(1), _ptr(weight), _ptr(bias), sp, sp + 4 * B * G, dt, B, L, C, G,
+                                               act, first, dx.data_ptr(), _ptr(dw), _ptr(db), ws, n, stream),
+                      "splat_group_norm_bwd")
+        return dx.view(shape) if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None, None
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="gelu", act_first=False):
+    """Group norm and an activation on a channels-last map: x [B, ..., C] -> the same shape and type.
+
+    act_first=False: act(weight * norm(x) + bias). act_first=True: weight * norm(act(x)) + bias, the order of the encoder's
+    stages (conv -> GELU -> norm). The mean and the biased variance run over the C / num_groups channels of a group and all
+    positions of an image. weight and bias [C] may be None; they are used, and their gradients returned, in float32."""
+    dt, code = _args(act, x)
+    if x.dim() < 2:
+        raise ValueError(f"x must be [B, ..., C], got {list(x.shape)}")
+    C, G = x.shape[-1], int(num_groups)
+    if G < 1 or C < 1 or C % G:
+        raise ValueError(f"{C} channels do not divide into {num_groups} groups")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            if t.shape != (C,):
+                raise ValueError(f"{name} must be [{C}], got {list(t.shape)}")
+            if t.device != x.device:
+                raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    weight = None if weight is None else weight.float().contiguous()
+    bias = None if bias is None else bias.float().contiguous()
+    first = 1 if act_first else 0
+    if _wants_grad(x, weight, bias):
+        return _GroupNormAct.apply(x, weight, bias, G, float(eps), dt, code, first)
+    return _norm_fwd(_positions(x), weight, bias, G, float(eps), dt, code, first, False)[0].view(x.shape)
+
+
+# ------------------------------------------------------------------------------------------------ products
+def _rows(x):
+    """x [..., K] as [M, K] with dense rows (a view where the strides allow it)."""
+    if x.dim() != 2:
+        x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
+
+
+def _linear_fwd(x2, weight, bias, r2, dt, act, save):
+    M, K = x2.shape
+    N = weight.shape[0]
+    y = torch.empty((M, N), dtype=x2.dtype, device=x2.device)
+    z = torch.empty_like(y) if save and act else None
+    if M:
+        with _On(x2) as stream:
+            check(_lib.load().splat_linear_fwd(x2.data_ptr(), x2.stride(0), weight.data_ptr(), _ptr(bias), _ptr(r2),
+                                               0 if r2 is None else r2.stride(0), dt, M, N, K, act, y.data_ptr(), _ptr(z),
+                                               stream), "splat_linear_fwd")
+    return y, z
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, dt, act):
+        x2 = _rows(x)
+        y, z = _linear_fwd(x2, weight, bias, None if residual is None else _rows(residual), dt, act, True)
+        ctx.save_for_backward(x2, weight, z)
+        ctx.args = (x.shape, dt, act, bias is not None)
+        return y.view(x.shape[:-1] + (weight.shape[0],))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x2, weight, z = ctx.saved_tensors
+        shape, dt, act, has_bias = ctx.args
+        need = ctx.needs_input_grad
+        M, K = x2.shape
+        N = weight.shape[0]
+        new = torch.empty if M else torch.zeros
+        dx = torch.empty((M, K), dtype=x2.dtype, device=x2.device) if need[0] else None
+        dw = new((N, K), dtype=x2.dtype, device=x2.device) if need[1] else None
+        db = new(N, dtype=x2.dtype, device=x2.device) if need[2] and has_bias else None
+        if M and (need[0] or need[1] or db is not None):
+            g = dy.contiguous()
+            lib = _lib.load()
+            with _On(x2) as stream:
+                n = lib.splat_linear_bwd_workspace_bytes(dt, M, N, K, act)
+                keep, ws = _scratch(n, x2)
+                check(lib.splat_linear_bwd(x2.data_ptr(), x2.stride(0), weight.data_ptr(), g.data_ptr(), _ptr(z), dt, M, N, K,
+                                           act, _ptr(dx), _ptr(dw), _ptr(db), ws, n, stream), "splat_linear_bwd")
+        return None if dx is None else dx.view(shape), dw, db, dy if need[3] else None, None, None
+
+
+def linear_act(x, weight, bias=None, act="none", residual=None):
+    """act(x weight^T + bias) + residual in one kernel: x [..., K], weight [N, K] (nn.Linear's, or a 1x1 convolution's
+    flattened), bias [N] or None, residual [..., N] or None -> [..., N]. All of one type; the product, the bias, the
+    activation and the residual are added in float32 and rounded once."""
+    dt, code = _args(act, x, weight, bias, residual)
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x [..., K] and weight [N, K] are needed, got {list(x.shape)} and {list(weight.shape)}")
+    N, K = weight.shape
+    if N < 1 or K < 1:
+        raise ValueError(f"weight must not be empty, got {list(weight.shape)}")
+    if bias is not None and bias.shape != (N,):
+        raise ValueError(f"bias must be [{N}], got {list(bias.shape)}")
+    out = x.shape[:-1] + (N,)
+    if residual is not None and residual.shape != out:
+        raise ValueError(f"residual must be {list(out)}, got {list(residual.shape)}")
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if _wants_grad(x, weight, bias, residual):
+        return _LinearAct.apply(x, weight, bias, residual, dt, code)
+    return _linear_fwd(_rows(x), weight, bias, None if residual is None else _rows(residual), dt, code, False)[0].view(out)
+
+
+# ------------------------------------------------------------------------------------------------ cross attention
+def _dense(t):
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _describe(q, k, v, lengths, mask, scale, dt):
+    B, Lq, H, D = q.shape
+    a = SplatAttention(dt, B, H, k.shape[2], D, scale, Lq, k.shape[1], *q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    if lengths is not None:
+        a.kv_lengths = lengths.data_ptr()
+    if mask is not None:
+        a.key_mask = mask.data_ptr()
+        a.mb, a.ml = mask.stride()
+    return a
+
+
+def _attention_fwd(q, k, v, lengths, mask, scale, dt, save):
+    B, Lq, H, D = q.shape
+    lib = _lib.load()
+    o = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty(B * Lq * H, dtype=torch.float32, device=q.device) if save else None
+    if o.numel():
+        a = _describe(q, k, v, lengths, mask, scale, dt)
+        ref = ctypes.byref(a)
+        with _On(q) as stream:
+            n = lib.splat_attention_workspace_bytes(ref)
+            keep, ws = _scratch(n, q)
+            check(lib.splat_attention_fwd(ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), ws, n,
+                                          stream), "splat_attention_fwd")
+    return o, lse
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, mask, scale, dt):
+        q, k, v = _dense(q), _dense(k), _dense(v)
+        o, lse = _attention_fwd(q, k, v, lengths, mask, scale, dt, True)
+        ctx.save_for_backward(q, k, v, o, lse, lengths, mask)
+        ctx.args = (scale, dt)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, o, lse, lengths, mask = ctx.saved_tensors
+        scale, dt = ctx.args
+        lib = _lib.load()
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if dq.numel() or dk.numel():
+            g = _dense(g)
+            a = _describe(q, k, v, lengths, mask, scale, dt)
+            a.gb, a.gl, a.gh = g.stride()[:3]
+            ref = ctypes.byref(a)
+            with _On(q) as stream:
+                n = lib.splat_attention_bwd_workspace_bytes(ref)
+                keep, ws = _scratch(n, q)
+                check(lib.splat_attention_bwd(ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                                              g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws, n, stream),
+                      "splat_attention_bwd")
+        need = ctx.needs_input_grad
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
+
+
+def cross_attention(q, k, v, kv_lengths=None, key_mask=None, scale=None):
+    """Attention of one sequence's queries over another's keys and values: q [B, Lq, H, D], k and v [B, Lk, Hk, D] ->
+    [B, Lq, H, D]. H is a multiple of Hk (each key head serves H / Hk neighbouring query heads), D at most 128; the three
+    may be views (halves of one projection, transposed heads) as long as the head vectors are dense.
+
+    kv_lengths [B] (integers, on the device): an image's keys past its length do not count. key_mask [B, Lk] (bool): keys
+    that are False do not count. What such keys hold has no effect, and their gradients are zero; a query without any key
+    gives zeros. scale defaults to D ** -0.5."""
+    dt, _ = _args("none", q, k, v)
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q [B, Lq, H, D] and k, v [B, Lk, Hk, D] are needed, got {list(q.shape)}, {list(k.shape)} and "
+                         f"{list(v.shape)}")
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    if H < 1 or Hk < 1 or H % Hk:
+        raise ValueError(f"{H} query heads do not divide over {Hk} key heads")
+    if not 1 <= D <= MAX_HEAD:
+        raise ValueError(f"heads of 1 to {MAX_HEAD} values are needed, got {D}")
+    if kv_lengths is not None:
+        if kv_lengths.shape != (B,) or kv_lengths.dtype not in (torch.int32, torch.int64) or kv_lengths.device != q.device:
+            raise ValueError(f"kv_lengths must be [{B}] int32 or int64 on {q.device}, got {list(kv_lengths.shape)} "
+                             f"{kv_lengths.dtype} on {kv_lengths.device}")
+        if kv_lengths.dtype is torch.int64:
+            kv_lengths = kv_lengths.clamp(0, Lk).to(torch.int32)
+        kv_lengths = kv_lengths.contiguous()
+    if key_mask is not None and (key_mask.shape != (B, Lk) or key_mask.dtype is not torch.bool
+                                 or key_mask.device != q.device):
+        raise ValueError(f"key_mask must be [{B}, {Lk}] bool on {q.device}, got {list(key_mask.shape)} {key_mask.dtype} on "
+                         f"{key_mask.device}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if _wants_grad(q, k, v):
+        return _CrossAttention.apply(q, k, v, kv_lengths, key_mask, scale, dt)
+    return _attention_fwd(_dense(q), _dense(k), _dense(v), kv_lengths, key_mask, scale, dt, False)[0]

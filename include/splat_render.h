@@ -302,6 +302,58 @@ int splat_exact_render_bwd(const float *rec, const float *reach, int N, int C, c
                            float *g_theta, float *g_op, float *g_color, float *g_bg, void *ws, size_t ws_bytes,
                            void *stream);
 
+/* ------------------------------------------------------------------------------------------- feature operators
+ * Operators of the encoder's feature maps and of models that read them (no counterpart in the reference, whose network
+ * runs on stock torch operations): channels-last group norm with an activation, products with an epilogue, and cross
+ * attention. dtype: 0 float32, 1 bfloat16 (features, product weights and biases; statistics and sums are 32-bit floats).
+ * act: 0 none, 1 gelu (x Phi(x)), 2 silu, 3 relu, 4 tanh, 5 sigmoid. Rows may start at any element. A zero size is no
+ * error: nothing is launched, and nothing written where a gradient has no term (the caller clears it). */
+
+/* y[B, L, C] = group norm over G groups of C / G channels and all L positions of an image, then act (act_first = 0), or
+ * of act(x) (act_first = 1). x has strides xsb (images) and xsl (positions), dense channels; y is contiguous; weight[C] and
+ * bias[C] may be NULL. mean[B, G] and rstd[B, G] (both or neither) are what the backward takes.
+ * Backward: dx contiguous, dweight[C], dbias[C] (NULL skips), dy with strides gsb, gsl. */
+size_t splat_group_norm_workspace_bytes(int dtype, int B, long long L, int C, int G);
+int splat_group_norm_fwd(const void *x, long long xsb, long long xsl, const float *weight, const float *bias, int dtype,
+                         int B, long long L, int C, int G, float eps, int act, int act_first, void *y, float *mean,
+                         float *rstd, void *ws, size_t ws_bytes, void *stream);
+size_t splat_group_norm_bwd_workspace_bytes(int dtype, int B, long long L, int C, int G);
+int splat_group_norm_bwd(const void *x, long long xsb, long long xsl, const void *dy, long long gsb, long long gsl,
+                         const float *weight, const float *bias, const float *mean, const float *rstd, int dtype, int B,
+                         long long L, int C, int G, int act, int act_first, void *dx, float *dweight, float *dbias,
+                         void *ws, size_t ws_bytes, void *stream);
+
+/* y[M, N] = act(x[M, K] weight[N, K]^T + bias[N]) + residual[M, N]; bias and residual may be NULL; ldx, ldr: elements from
+ * row to row. z[M, N] (or NULL) receives the activation's input, which the backward of act != 0 takes.
+ * Backward from dy[M, N]: dx[M, K], dweight[N, K], dbias[N] (NULL skips). */
+int splat_linear_fwd(const void *x, long long ldx, const void *weight, const void *bias, const void *residual,
+                     long long ldr, int dtype, long long M, int N, int K, int act, void *y, void *z, void *stream);
+size_t splat_linear_bwd_workspace_bytes(int dtype, long long M, int N, int K, int act);
+int splat_linear_bwd(const void *x, long long ldx, const void *weight, const void *dy, const void *z, int dtype,
+                     long long M, int N, int K, int act, void *dx, void *dweight, void *dbias, void *ws, size_t ws_bytes,
+                     void *stream);
+
+/* o[B, Lq, H, D] = softmax(scale q k^T) v over the keys that count, q[B, Lq, H, D], k and v[B, Lk, Hk, D]; H is a multiple
+ * of Hk (query heads j H / Hk .. share key head j), D at most 128, head vectors dense. Rows without keys give zeros. lse
+ * [B, Hk, Lq H / Hk] (or NULL) is what the backward takes; dq, dk and dv are contiguous. */
+typedef struct splat_attention {
+  int dtype, B, H, Hk, D;                          /* element type; images; query heads; key heads; values per head */
+  float scale;                                     /* of the scores */
+  long long Lq, Lk;                                /* queries and keys of an image */
+  long long qb, ql, qh, kb, kl, kh, vb, vl, vh;    /* elements from image to image, token to token, head to head */
+  long long gb, gl, gh;                            /* the same of the output's gradient (backward) */
+  long long mb, ml;                                /* key_mask: bytes from image to image and from key to key */
+  const int *kv_lengths;                           /* [B] keys of each image that count, the first ones; or NULL */
+  const unsigned char *key_mask;                   /* [B, Lk], 0: the key is left out; or NULL */
+} splat_attention;
+size_t splat_attention_workspace_bytes(const splat_attention *a);
+int splat_attention_fwd(const splat_attention *a, const void *q, const void *k, const void *v, void *o, float *lse,
+                        void *ws, size_t ws_bytes, void *stream);
+size_t splat_attention_bwd_workspace_bytes(const splat_attention *a);
+int splat_attention_bwd(const splat_attention *a, const void *q, const void *k, const void *v, const void *o,
+                        const float *lse, const void *g, void *dq, void *dk, void *dv, void *ws, size_t ws_bytes,
+                        void *stream);
+
 #ifdef __cplusplus
 }
 #endif
