@@ -16,12 +16,15 @@ namespace splat {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
+constexpr int kMaxSplits = 512;
 
 struct Attn {
   splat_attention a;
   int rep, R;            // query heads per key head; rows per (image, key head)
+  FastDiv by_rep;
   int tiles, splits;     // workgroups per (image, key head) along the rows (or keys), and along the other axis
   int per;               // tiles of the other axis that a split takes
+  bool chunked;          // heads are whole chunks, and offsets within a tile are 31-bit
 };
 
 template <typename T, int DP>
@@ -50,12 +53,16 @@ __device__ __forceinline__ int key_count(const splat_attention& a, int b) {
   return n < 0 ? 0 : n > (int)a.Lk ? (int)a.Lk : n;
 }
 
-// Bit i: key k0 + i is valid (i < 64), the same in every lane.
-__device__ __forceinline__ unsigned long long valid_keys(const splat_attention& a, int b, int k0, int len) {
+// Bit i: key k0 + i counts (i < 64), the same in every lane. mask: the image's row, or null.
+__device__ __forceinline__ unsigned long long valid_keys(const unsigned char* mask, long long ml, int k0, int len) {
   const int k = k0 + (threadIdx.x & 63);
   bool in = k < len;
-  if (a.key_mask && in) in = a.key_mask[(long long)b * a.mb + (long long)k * a.ml] != 0;
+  if (mask && in) in = mask[(long long)k * ml] != 0;
   return __ballot(in);
+}
+
+__device__ __forceinline__ const unsigned char* mask_row(const splat_attention& a, int b) {
+  return a.key_mask ? a.key_mask + b * a.mb : nullptr;
 }
 
 // Adds 32 x 32 scores: acc = rows of `t` (LDS) times the lanes' register rows.
@@ -81,25 +88,127 @@ __device__ __forceinline__ void gather(RowAcc<T, DP>& acc, const T* t, const f32
   }
 }
 
-// N rows of an LDS tile: global -> registers -> LDS, zeros for rows whose bit is off and columns past D.
+struct Work {
+  int tile, split, b, hk, bh;
+};
+
+// Workgroup -> (image, key head), tile and split: a head's tiles follow each other on one XCD, whose L2 then holds the
+// other side of them.
+__device__ __forceinline__ Work work_of(const Attn& n) {
+  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  Work w;
+  w.tile = id % n.tiles;
+  w.split = id / n.tiles % n.splits;
+  w.bh = id / (n.tiles * n.splits);
+  w.b = w.bh / n.a.Hk;
+  w.hk = w.bh % n.a.Hk;
+  return w;
+}
+
+// Address of row r's head vector in a tensor of strides (sb, sl, sh).
+template <typename T>
+__device__ __forceinline__ const T* head_row(const void* p, const Attn& n, const Work& w, int r, long long sb, long long sl,
+                                             long long sh) {
+  const int q = r / n.by_rep, j = r - q * n.rep;
+  return (const T*)p + w.b * sb + q * sl + (long long)(w.hk * n.rep + j) * sh;
+}
+
+// N rows of an LDS tile: global -> registers -> LDS. A thread has one column of chunks and every RS-th row, so that whole
+// tiles load from scalar bases and one offset that stays, without address arithmetic per tile. Heads that are not whole
+// chunks (D no multiple of V) are copied value by value when the tile is written.
 template <typename T, int DP, int N>
 struct Rows {
-  static constexpr int V = kV<T>, chunks = N * (DP / V), per = (chunks + kThreads - 1) / kThreads;
-  template <typename F>
-  __device__ static void load(Chunk<T> (&c)[per], int D, F&& row) {   // row(i): pointer of row i, or null
+  static constexpr int V = kV<T>, CP = DP == 96 ? 128 / V : DP / V;   // chunks of a row, a power of two
+  static constexpr int RS = kThreads / CP, per = N > RS ? N / RS : 1;
+  Chunk<T> c[per];
+  unsigned off;   // the thread's elements from the tile's base
+  bool on;        // its column holds values
+
+  __device__ static int row0() { return threadIdx.x / CP; }
+  __device__ static int col() { return threadIdx.x % CP * V; }
+  __device__ static T* place(T* t, int i) { return t + (row0() + i * RS) * Shape<T, DP>::ld + col(); }
+  __device__ static bool holds() { return (N >= RS || row0() < N) && (DP != 96 || col() < DP); }
+  // offset: elements from a tile's base to the thread's row row0().
+  __device__ void init(int D, int offset) {
+    off = offset + col();
+    on = col() < D && (N >= RS || row0() < N);
+  }
+  __device__ void load(const T* base, long long step) {   // step: elements from row to row + RS
 #pragma unroll
     for (int i = 0; i < per; ++i) {
-      const int e = threadIdx.x + i * kThreads, col = e % (DP / V) * V;
-      const T* p = chunks % kThreads == 0 || e < chunks ? row(e / (DP / V)) : nullptr;
-      c[i] = load_chunk(p + col, p ? D - col : 0);
+      c[i] = Chunk<T>{};
+      if (on) __builtin_memcpy(c[i].v, base + i * step + off, 16);
     }
   }
-  __device__ static void put(const Chunk<T> (&c)[per], T* t) {
+  template <typename F>
+  __device__ void load(F&& row) {   // row(i): pointer of row i, or null for zeros
 #pragma unroll
     for (int i = 0; i < per; ++i) {
-      const int e = threadIdx.x + i * kThreads;
-      if (chunks % kThreads == 0 || e < chunks)
-        *(f32x4*)(t + e / (DP / V) * Shape<T, DP>::ld + e % (DP / V) * V) = *(const f32x4*)c[i].v;
+      const T* p = on ? row(row0() + i * RS) : nullptr;
+      c[i] = Chunk<T>{};
+      if (p) __builtin_memcpy(c[i].v, p + col(), 16);
+    }
+  }
+  __device__ void put(T* t) const {
+#pragma unroll
+    for (int i = 0; i < per; ++i)
+      if (holds()) *(f32x4*)place(t, i) = *(const f32x4*)c[i].v;
+  }
+  template <typename F>
+  __device__ static void copy(T* t, int D, F&& row) {
+#pragma unroll 1
+    for (int i = 0; i < per; ++i) {
+      if (!holds()) continue;
+      const T* p = row(row0() + i * RS);
+      const Chunk<T> x = load_chunk(p + col(), p ? D - col() : 0);
+      *(f32x4*)place(t, i) = *(const f32x4*)x.v;
+    }
+  }
+};
+
+// Tiles of N keys and values in turn: fetch(t) loads tile t to registers and says which of its keys count, put() writes it.
+template <typename T, int DP, int N>
+struct KeyTiles {
+  const T *k, *v;               // the head's first key and value
+  long long kl, vl, ml;
+  const unsigned char* mask;
+  int D, len;
+  bool chunked;                 // rows are whole chunks
+  Rows<T, DP, N> rk, rv;
+  unsigned long long ok0, ok1;  // the fetched tile's keys that count: the first 64, the others
+  int k0;
+
+  __device__ KeyTiles(const Attn& n, const Work& w, const T* kp, const T* vp)
+      : k(kp + w.b * n.a.kb + w.hk * n.a.kh), v(vp + w.b * n.a.vb + w.hk * n.a.vh), kl(n.a.kl), vl(n.a.vl), ml(n.a.ml),
+        mask(mask_row(n.a, w.b)), D(n.a.D), len(key_count(n.a, w.b)), chunked(n.chunked), ok0(0), ok1(0), k0(0) {
+    rk.init(D, rk.row0() * (int)kl);
+    rv.init(D, rv.row0() * (int)vl);
+  }
+  __device__ __forceinline__ const T* row(const T* p, long long l, int i) const {
+    return ((N > 64 && i >= 64 ? ok1 : ok0) >> (i & 63)) & 1 ? p + (k0 + i) * l : nullptr;
+  }
+  __device__ __forceinline__ void fetch(int t) {
+    k0 = t * N;
+    if (chunked && !mask && k0 + N <= len) {
+      ok0 = ok1 = ~0ull;
+      rk.load(k + k0 * kl, rk.RS * kl);
+      rv.load(v + k0 * vl, rv.RS * vl);
+      return;
+    }
+    ok0 = valid_keys(mask, ml, k0, len);
+    ok1 = N > 64 ? valid_keys(mask, ml, k0 + 64, len) : 0;
+    if (chunked) {
+      rk.load([&](int i) { return row(k, kl, i); });
+      rv.load([&](int i) { return row(v, vl, i); });
+    }
+  }
+  __device__ __forceinline__ void put(T* tk, T* tv) const {
+    if (chunked) {
+      rk.put(tk);
+      rv.put(tv);
+    } else {
+      Rows<T, DP, N>::copy(tk, D, [&](int i) { return row(k, kl, i); });
+      Rows<T, DP, N>::copy(tv, D, [&](int i) { return row(v, vl, i); });
     }
   }
 };
@@ -122,115 +231,144 @@ __device__ __forceinline__ void store_row(O* row, const RowAcc<T, DP>& acc, floa
   }
 }
 
-struct Work {
-  int tile, split, b, hk, bh;
+// ------------------------------------------------------------------------------------------------ forward
+// Of the workgroup's four waves QW take 32 rows each and 4 / QW share the keys of a tile between them: few rows would
+// leave waves idle otherwise. A wave's 32-key blocks of a tile (two for bf16, one for float) are one softmax step. Key and
+// value tiles go through registers into two LDS buffers in turn: the next tile's loads are in flight during a step, and
+// one barrier a tile suffices (where only one buffer fits, two). Waves that shared keys join their results in LDS, splits
+// of the key axis in k_attn_join.
+template <typename T, int DP, int QW>
+struct FwdShape {
+  static constexpr int KW = kWaves / QW;
+  static constexpr int KB = sizeof(T) == 2 && QW > 1 ? 2 : 1;   // 32-key blocks of a wave
+  static constexpr int KT = 32 * KB * KW;
+  static constexpr int tile = KT * Shape<T, DP>::ld;
+  static constexpr int buffers = 4 * tile * (int)sizeof(T) <= 140 * 1024 ? 2 : 1;
+  static constexpr int lds = 2 * buffers * tile;                // elements: keys and values
+  static_assert(lds * sizeof(T) >= sizeof(float) * (kWaves - QW) * 64 * (DP / 2 + 2), "the join's values fit");
 };
 
-// Workgroup -> (image, key head), tile and split: a head's tiles follow each other on one XCD, whose L2 then holds the
-// other side of them.
-__device__ __forceinline__ Work work_of(const Attn& n) {
-  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
-  Work w;
-  w.tile = id % n.tiles;
-  w.split = id / n.tiles % n.splits;
-  w.bh = id / (n.tiles * n.splits);
-  w.b = w.bh / n.a.Hk;
-  w.hk = w.bh % n.a.Hk;
-  return w;
+// Adds to the running softmax of the lane's row the scores s of a step, `live` the keys that count (0 .. 32 KB - 1): m the
+// maximum that l and acc are scaled by, in units of the raw scores; c > 0 turns those into exponents of two. The maximum
+// is only raised when it grew by more than 2^8 in the result: l and acc are scaled by 2^-m either way.
+template <typename T, int DP, int KB>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[KB], unsigned long long live, float c, float& m, float& l,
+                                             RowAcc<T, DP>& acc, int h) {
+  if (live != (KB == 2 ? ~0ull : 0xffffffffull)) {
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      const unsigned bits = (unsigned)(live >> (32 * b)) >> (4 * h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[b][i] = (bits >> acc_row(i, 0)) & 1 ? s[b][i] : -INFINITY;
+    }
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int b = 0; b < KB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+  const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+  mx = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
+  if (__any(mx > m + fminf(8.f / c, 1e30f))) {
+    const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
+    const float al = hw_exp2((m - mu) * c);
+    m = mn;
+    l *= al;
+#pragma unroll
+    for (int d = 0; d < Shape<T, DP>::nd; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] *= al;
+  }
+  const float mc = m == -INFINITY ? 0.f : m * c;
+  float sum = 0.f;
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[b][i] = hw_exp2(fmaf(s[b][i], c, -mc));
+      sum += s[b][i];
+    }
+  }
+  l += sum;
 }
 
-// Address of row r's head vector in a tensor of strides (sb, sl, sh).
-template <typename T>
-__device__ __forceinline__ const T* head_row(const void* p, const Attn& n, const Work& w, int r, long long sb, long long sl,
-                                             long long sh) {
-  const int q = r / n.rep, j = r - q * n.rep;
-  return (const T*)p + w.b * sb + q * sl + (long long)(w.hk * n.rep + j) * sh;
-}
-
-// ------------------------------------------------------------------------------------------------ forward
-// QW = 4: the workgroup's waves take 32 rows each and share every key tile. QW = 1: they share 32 rows and take a quarter
-// of every key tile each, ending in four partial results. Partial results (maximum, sum, unscaled output) of splits and
-// waves are joined by k_attn_join; without any the output is final.
 template <typename T, int DP, int QW>
 __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restrict__ q, const T* __restrict__ k,
                                                        const T* __restrict__ v, T* __restrict__ o, float* __restrict__ lse,
                                                        float* __restrict__ part, float* __restrict__ stat) {
   using S = Shape<T, DP>;
-  constexpr int KB = QW == 4 ? 64 / (int)sizeof(T) / 16 : 1;   // 32-key blocks a wave takes of a tile: 2 bf16, 1 float
-  constexpr int KT = QW == 4 ? 32 * KB : 128;
-  __shared__ __align__(16) T tk[KT * S::ld];
-  __shared__ __align__(16) T tv[KT * S::ld];
+  using F = FwdShape<T, DP, QW>;
+  __shared__ __align__(16) T tiles[F::lds];
   const splat_attention& a = n.a;
   const Work w = work_of(n);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int r = w.tile * 32 * QW + (QW == 4 ? wave * 32 : 0) + (lane & 31);
+  const int wq = wave % QW, wk = wave / QW;
+  const int r = (w.tile * QW + wq) * 32 + (lane & 31);
   const bool in = r < n.R;
-  const int kw = QW == 4 ? 0 : wave * 32;   // the wave's first key of a tile
+  const int kw = wk * 32 * F::KB;   // the wave's first key of a tile
   Chunk<T> fq[S::nc];
   load_rows<T, DP>(fq, head_row<T>(q, n, w, in ? r : 0, a.qb, a.ql, a.qh), in, a.D, h);
-  const int len = key_count(a, w.b);
-  const int t0 = w.split * n.per, t1 = min((len + KT - 1) / KT, t0 + n.per);
-  const float c = a.scale * kLog2e;
+  if (a.scale < 0.f) {   // the running maximum is of raw scores: their sign goes to the queries
+#pragma unroll
+    for (int i = 0; i < S::nc; ++i)
+#pragma unroll
+      for (int j = 0; j < S::V; ++j) fq[i].v[j] = -fq[i].v[j];
+  }
+  const float c = fmaxf(fabsf(a.scale) * kLog2e, 1.17549435e-38f);
+  KeyTiles<T, DP, F::KT> kt(n, w, k, v);
+  const int t0 = w.split * n.per, t1 = min((kt.len + F::KT - 1) / F::KT, t0 + n.per);
   f32x16 acc[S::nd] = {};
   float m = -INFINITY, l = 0.f;
-  using R = Rows<T, DP, KT>;
-  Chunk<T> ck[R::per], cv[R::per];
-  unsigned long long ok[2] = {};   // valid keys of the tile (128 at most)
-  const T* kb = k + w.b * a.kb + w.hk * a.kh;
-  const T* vb = v + w.b * a.vb + w.hk * a.vh;
-  auto fetch = [&](int t) {
-    const int k0 = t * KT;
-    ok[0] = valid_keys(a, w.b, k0, len);
-    if (KT > 64) ok[1] = valid_keys(a, w.b, k0 + 64, len);
-    auto bit = [&](int i) { return (ok[KT > 64 ? i >> 6 : 0] >> (i & 63)) & 1; };
-    R::load(ck, a.D, [&](int i) { return bit(i) ? kb + (long long)(k0 + i) * a.kl : nullptr; });
-    R::load(cv, a.D, [&](int i) { return bit(i) ? vb + (long long)(k0 + i) * a.vl : nullptr; });
-  };
-  if (t0 < t1) fetch(t0);
+  if (t0 < t1) kt.fetch(t0);
   for (int t = t0; t < t1; ++t) {
-    const unsigned long long good = KT > 64 && kw >= 64 ? ok[1] : ok[0];
+    unsigned long long live = F::KT > 64 && kw >= 64 ? kt.ok1 : kt.ok0;
+    live >>= kw & 63;
+    if (F::KB == 1) live &= 0xffffffffull;
+    T* tk = tiles + (F::buffers == 2 ? (t & 1) * 2 * F::tile : 0);
+    T* tv = tk + F::tile;
+    if (F::buffers == 1) __syncthreads();
+    kt.put(tk, tv);
     __syncthreads();
-    R::put(ck, tk);
-    R::put(cv, tv);
-    __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
-    f32x16 s[KB] = {};
-    float mx = -INFINITY;
+    if (t + 1 < t1) kt.fetch(t + 1);
+    if (!live) continue;
+    f32x16 s[F::KB] = {};
 #pragma unroll
-    for (int kb2 = 0; kb2 < KB; ++kb2) {
-      scores<T, DP>(s[kb2], tk + (kw + 32 * kb2) * S::ld, fq, lane);
-      const unsigned bits = (unsigned)(good >> ((kw & 63) + 32 * kb2)) >> (4 * h);
+    for (int b = 0; b < F::KB; ++b) scores<T, DP>(s[b], tk + (kw + 32 * b) * S::ld, fq, lane);
+    softmax_step<T, DP, F::KB>(s, live, c, m, l, acc, h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kb2][i] = (bits >> acc_row(i, 0)) & 1 ? s[kb2][i] * c : -INFINITY;
-        mx = fmaxf(mx, s[kb2][i]);
-      }
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
-    const float al = hw_exp2(m - mu);
-    m = mn;
-    float sum = 0.f;
-#pragma unroll
-    for (int kb2 = 0; kb2 < KB; ++kb2) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kb2][i] = hw_exp2(s[kb2][i] - mu);
-        sum += s[kb2][i];
-      }
-    }
-    l = fmaf(l, al, sum);
-#pragma unroll
-    for (int d = 0; d < S::nd; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[d][i] *= al;
-#pragma unroll
-    for (int kb2 = 0; kb2 < KB; ++kb2) gather<T, DP>(acc, tv + (kw + 32 * kb2) * S::ld, s[kb2], lane);
+    for (int b = 0; b < F::KB; ++b) gather<T, DP>(acc, tv + (kw + 32 * b) * S::ld, s[b], lane);
   }
   l += __shfl_xor(l, 32, 64);
+  if (QW < kWaves) {   // the waves of the same rows: the first one adds the others' results in their order
+    __syncthreads();
+    float* join = (float*)tiles;
+    constexpr int per = 64 * (DP / 2 + 2);   // a wave's values
+    if (wk > 0) {
+      float* p = join + ((wk - 1) * QW + wq) * per + lane;
+      p[0] = m;
+      p[64] = l;
+#pragma unroll
+      for (int d = 0; d < S::nd; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[64 * (2 + 16 * d + i)] = acc[d][i];
+    }
+    __syncthreads();
+    if (wk > 0) return;
+    for (int j = 1; j < F::KW; ++j) {
+      const float* p = join + ((j - 1) * QW + wq) * per + lane;
+      const float mo = p[0], mn = fmaxf(m, mo), mu = mn == -INFINITY ? 0.f : mn;
+      const float x = hw_exp2((m - mu) * c), y = hw_exp2((mo - mu) * c);
+      m = mn;
+      l = fmaf(l, x, p[64] * y);
+#pragma unroll
+      for (int d = 0; d < S::nd; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = fmaf(acc[d][i], x, p[64 * (2 + 16 * d + i)] * y);
+    }
+  }
+  m *= c;   // from here in exponents of two
   if (part) {
-    const int slot = QW == 4 ? w.split : w.split * kWaves + wave;
-    const long long at = ((long long)slot * n.a.B * n.a.Hk + w.bh) * n.R + r;
+    const long long at = ((long long)w.split * n.a.B * n.a.Hk + w.bh) * n.R + r;
     if (in && h == 0) {
       stat[2 * at] = m;
       stat[2 * at + 1] = l;
@@ -239,41 +377,82 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restri
   } else {
     const float inv = l > 0.f ? 1.f / l : l;   // 0 for a row without keys, NaN stays
     if (lse && in && h == 0) lse[(long long)w.bh * n.R + r] = l == 0.f ? INFINITY : m + hw_log2(l);
-    const int qi = r / n.rep, j = r - qi * n.rep;
+    const int qi = r / n.by_rep, j = r - qi * n.rep;
     store_row<T, T, DP>(o + ((w.b * a.Lq + qi) * a.H + w.hk * n.rep + j) * a.D, acc, inv, a.D, in, h);
   }
 }
 
-// Joins the partial results of a row: one wave a row, lanes over the head's values.
-template <typename T>
+// Joins the splits' partial results of a row, one workgroup a row: lanes over the head's values, 256 / DP groups of lanes
+// over the splits, whose sums are added in LDS in their order.
+template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void k_attn_join(Attn n, const float* __restrict__ part, const float* __restrict__ stat,
-                                                        int slots, T* __restrict__ o, float* __restrict__ lse) {
+                                                        T* __restrict__ o, float* __restrict__ lse) {
+  constexpr int GS = DP == 96 ? 2 : kThreads / DP;   // groups
+  __shared__ float weight[kMaxSplits], sums[GS * DP], wred[2];
   const splat_attention& a = n.a;
-  const long long rows = (long long)a.B * a.Hk * n.R;
-  const long long row = (long long)blockIdx.x * kWaves + (threadIdx.x >> 6);
-  if (row >= rows) return;
+  const long long rows = (long long)a.B * a.Hk * n.R, row = blockIdx.x;
   const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  for (int s = lane; s < slots; s += 64) m = fmaxf(m, stat[2 * (s * rows + row)]);
+  if (threadIdx.x < 64) {
+    float m = -INFINITY;
+    for (int s = lane; s < n.splits; s += 64) m = fmaxf(m, stat[2 * (s * rows + row)]);
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-  const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int s = lane; s < slots; s += 64) l = fmaf(stat[2 * (s * rows + row) + 1], hw_exp2(stat[2 * (s * rows + row)] - mu), l);
-  l = wave_sum(l);
-  const float inv = l > 0.f ? 1.f / l : l;
-  const int bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
-  const int qi = r / n.rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
-  T* op = o + (((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D;
-  for (int d = lane; d < a.D; d += 64) {
-    float s = 0.f;
-    for (int i = 0; i < slots; ++i) {
-      const long long at = i * rows + row;
-      s = fmaf(part[at * a.D + d], hw_exp2(stat[2 * at] - mu), s);
+    for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    const float mu = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int s = lane; s < n.splits; s += 64) {
+      const float e = hw_exp2(stat[2 * (s * rows + row)] - mu);
+      weight[s] = e;
+      l = fmaf(stat[2 * (s * rows + row) + 1], e, l);
     }
-    op[d] = (T)(s * inv);
+    l = wave_sum(l);
+    if (lane == 0) {
+      wred[0] = l > 0.f ? 1.f / l : l;
+      if (lse) lse[row] = l == 0.f ? INFINITY : m + hw_log2(l);
+    }
   }
-  if (lse && lane == 0) lse[row] = l == 0.f ? INFINITY : m + hw_log2(l);
+  __syncthreads();
+  const int d = threadIdx.x % DP, g = threadIdx.x / DP;
+  if (g < GS) {
+    float s = 0.f;
+    if (d < a.D) {
+#pragma unroll 8
+      for (int i = g; i < n.splits; i += GS) s = fmaf(part[(i * rows + row) * a.D + d], weight[i], s);
+    }
+    sums[g * DP + d] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x < a.D) {
+    float s = sums[threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < GS; ++i) s += sums[i * DP + threadIdx.x];
+    const int bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
+    const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
+    o[(((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + threadIdx.x] = (T)(s * wred[0]);
+  }
+}
+
+// The same for few splits: a thread per value.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, const float* __restrict__ part,
+                                                            const float* __restrict__ stat, T* __restrict__ o,
+                                                            float* __restrict__ lse) {
+  const splat_attention& a = n.a;
+  const long long rows = (long long)a.B * a.Hk * n.R, i = (long long)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= rows * a.D) return;
+  const long long row = i / a.D;
+  const int d = (int)(i - row * a.D);
+  float m = stat[2 * row], l = stat[2 * row + 1], s = part[i];
+  for (int k = 1; k < n.splits; ++k) {
+    const float mo = stat[2 * (k * rows + row)], mn = fmaxf(m, mo), mu = mn == -INFINITY ? 0.f : mn;
+    const float x = hw_exp2(m - mu), y = hw_exp2(mo - mu);
+    m = mn;
+    l = fmaf(l, x, stat[2 * (k * rows + row) + 1] * y);
+    s = fmaf(s, x, part[k * rows * a.D + i] * y);
+  }
+  const int bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
+  const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
+  o[(((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + d] = (T)(s * (l > 0.f ? 1.f / l : l));
+  if (lse && d == 0) lse[row] = l == 0.f ? INFINITY : m + hw_log2(l);
 }
 
 // ----------------------------------------------------------------------------------------------- backward
@@ -286,7 +465,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_delta(Attn n, const T* __rest
   const long long row = ((long long)blockIdx.x * kThreads + threadIdx.x) >> 3;
   if (row >= (long long)a.B * a.Hk * n.R) return;
   const int bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
-  const int qi = r / n.rep, j = r - qi * n.rep, b = bh / a.Hk, hq = bh % a.Hk * n.rep + j;
+  const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hq = bh % a.Hk * n.rep + j;
   const T* op = o + (((long long)b * a.Lq + qi) * a.H + hq) * a.D;
   const T* gp = g + b * a.gb + qi * a.gl + hq * a.gh;
   float s = 0.f;
@@ -301,6 +480,9 @@ __global__ __launch_bounds__(kThreads) void k_attn_delta(Attn n, const T* __rest
   if ((threadIdx.x & 7) == 0) delta[row] = s;
 }
 
+// Rows (dk, dv) or keys (dq) of an LDS tile of the backward; two of them in turn, as in the forward.
+template <typename T> constexpr int kBwdTile = sizeof(T) == 2 ? 64 : 32;
+
 // dk and dv: a wave holds 32 keys and values, the workgroup's four share tiles of query rows. With s = q k^T a lane is a
 // key: p and ds are the operands of dv = p^T do and dk = ds^T q as they are.
 template <typename T, int DP>
@@ -309,16 +491,15 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
                                                           const float* __restrict__ lse, const float* __restrict__ delta,
                                                           T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
   using S = Shape<T, DP>;
-  constexpr int QT = 32;
-  __shared__ __align__(16) T tq[QT * S::ld];
-  __shared__ __align__(16) T tg[QT * S::ld];
-  __shared__ __align__(16) float tl[QT], td[QT];
+  constexpr int QT = kBwdTile<T>, tile = QT * S::ld;
+  __shared__ __align__(16) T tiles[4 * tile];
+  __shared__ __align__(16) float stats[4 * QT];
   const splat_attention& a = n.a;
   const Work w = work_of(n);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int len = key_count(a, w.b);
   const int k0 = w.tile * 128 + (wave & 2) * 32;
-  const unsigned long long ok = valid_keys(a, w.b, k0, len);
+  const unsigned long long ok = valid_keys(mask_row(a, w.b), a.ml, k0, len);
   const int ki = w.tile * 128 + wave * 32 + (lane & 31);
   const bool good = (ok >> ((wave & 1) * 32 + (lane & 31))) & 1;
   Chunk<T> fk[S::nc], fv[S::nc];
@@ -328,45 +509,82 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
   const int t0 = w.split * n.per, t1 = any ? min((n.R + QT - 1) / QT, t0 + n.per) : t0;
   const float c = a.scale * kLog2e;
   f32x16 ak[S::nd] = {}, av[S::nd] = {};
-  using R = Rows<T, DP, QT>;
-  Chunk<T> cq[R::per], cg[R::per];
+  Rows<T, DP, QT> rq, rg;
+  // tiles, and a thread's rows of one, are whole queries apart where their row counts are multiples of rep
+  const bool whole = n.chunked && QT % n.rep == 0 && (rq.per == 1 || rq.RS % n.rep == 0);
+  const int qi0 = rq.row0() / n.by_rep, j0 = rq.row0() - qi0 * n.rep, qs = rq.RS / n.by_rep;
+  rq.init(a.D, qi0 * (int)a.ql + j0 * (int)a.qh);
+  rg.init(a.D, qi0 * (int)a.gl + j0 * (int)a.gh);
+  const T* qp = head_row<T>(q, n, w, 0, a.qb, a.ql, a.qh);
+  const T* gp = head_row<T>(g, n, w, 0, a.gb, a.gl, a.gh);
+  const float* lp = lse + (long long)w.bh * n.R;
+  const float* dp0 = delta + (long long)w.bh * n.R;
   float sl = 0.f, sd = 0.f;
+  int r0 = 0;
+  auto qrow = [&](int i) { return r0 + i < n.R ? head_row<T>(q, n, w, r0 + i, a.qb, a.ql, a.qh) : nullptr; };
+  auto grow = [&](int i) { return r0 + i < n.R ? head_row<T>(g, n, w, r0 + i, a.gb, a.gl, a.gh) : nullptr; };
   auto fetch = [&](int t) {
-    const int r0 = t * QT;
-    R::load(cq, a.D, [&](int i) { return r0 + i < n.R ? head_row<T>(q, n, w, r0 + i, a.qb, a.ql, a.qh) : nullptr; });
-    R::load(cg, a.D, [&](int i) { return r0 + i < n.R ? head_row<T>(g, n, w, r0 + i, a.gb, a.gl, a.gh) : nullptr; });
+    r0 = t * QT;
+    if (whole && r0 + QT <= n.R) {
+      const int q0 = r0 / n.by_rep;
+      rq.load(qp + q0 * a.ql, qs * a.ql);
+      rg.load(gp + q0 * a.gl, qs * a.gl);
+    } else if (n.chunked) {
+      rq.load(qrow);
+      rg.load(grow);
+    }
     if (threadIdx.x < QT) {
       const int r = r0 + threadIdx.x;
-      sl = r < n.R ? lse[(long long)w.bh * n.R + r] : INFINITY;
-      sd = r < n.R ? delta[(long long)w.bh * n.R + r] : 0.f;
+      sl = r < n.R ? -lp[r] : -INFINITY;
+      sd = r < n.R ? -dp0[r] : 0.f;
     }
   };
   if (t0 < t1) fetch(t0);
   for (int t = t0; t < t1; ++t) {
-    __syncthreads();
-    R::put(cq, tq);
-    R::put(cg, tg);
+    T* tq = tiles + (t & 1) * 2 * tile;
+    T* tg = tq + tile;
+    float* tl = stats + (t & 1) * 2 * QT;
+    float* td = tl + QT;
+    if (n.chunked) {
+      rq.put(tq);
+      rg.put(tg);
+    } else {
+      Rows<T, DP, QT>::copy(tq, a.D, qrow);
+      Rows<T, DP, QT>::copy(tg, a.D, grow);
+    }
     if (threadIdx.x < QT) {
       tl[threadIdx.x] = sl;
       td[threadIdx.x] = sd;
     }
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
-    f32x16 s = {}, dp = {};
-    scores<T, DP>(s, tq, fk, lane);
-    scores<T, DP>(dp, tg, fv, lane);
+#pragma unroll 1
+    for (int rb = 0; rb < QT; rb += 32) {
+      f32x16 s = {}, dp;
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const f32x4 L = *(const f32x4*)(tl + acc_row(i, h)), D = *(const f32x4*)(td + acc_row(i, h));
+      for (int i = 0; i < 16; i += 4) {   // dp starts at -delta
+        const f32x4 D = *(const f32x4*)(td + rb + acc_row(i, h));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = good ? hw_exp2(fmaf(s[i + e], c, -L[e])) : 0.f;
-        s[i + e] = p;
-        dp[i + e] = p * (dp[i + e] - D[e]);
+        for (int e = 0; e < 4; ++e) dp[i + e] = D[e];
       }
+      scores<T, DP>(s, tq + rb * S::ld, fk, lane);
+      scores<T, DP>(dp, tg + rb * S::ld, fv, lane);
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 L = *(const f32x4*)(tl + rb + acc_row(i, h));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[i + e] = hw_exp2(fmaf(s[i + e], c, L[e]));
+          dp[i + e] *= s[i + e];
+        }
+      }
+      gather<T, DP>(av, tg + rb * S::ld, s, lane);
+      gather<T, DP>(ak, tq + rb * S::ld, dp, lane);
     }
-    gather<T, DP>(av, tg, s, lane);
-    gather<T, DP>(ak, tq, dp, lane);
+  }
+  if (!good) {   // the lane gathered what a key of zeros would get (infinite where the rows' scores are far below zero)
+#pragma unroll
+    for (int d = 0; d < S::nd; ++d) ak[d] = av[d] = f32x16{};
   }
   const bool in = ki < a.Lk;
   if (part) {
@@ -388,9 +606,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_q(Attn n, const T* __rest
                                                          const float* __restrict__ lse, const float* __restrict__ delta,
                                                          T* __restrict__ dq, float* __restrict__ part) {
   using S = Shape<T, DP>;
-  constexpr int KT = 32;
-  __shared__ __align__(16) T tk[KT * S::ld];
-  __shared__ __align__(16) T tv[KT * S::ld];
+  constexpr int KT = kBwdTile<T>, tile = KT * S::ld;
+  __shared__ __align__(16) T tiles[4 * tile];
   const splat_attention& a = n.a;
   const Work w = work_of(n);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
@@ -399,46 +616,43 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_q(Attn n, const T* __rest
   Chunk<T> fq[S::nc], fg[S::nc];
   load_rows<T, DP>(fq, head_row<T>(q, n, w, in ? r : 0, a.qb, a.ql, a.qh), in, a.D, h);
   load_rows<T, DP>(fg, head_row<T>(g, n, w, in ? r : 0, a.gb, a.gl, a.gh), in, a.D, h);
-  const float L = in ? lse[(long long)w.bh * n.R + r] : INFINITY;
-  const float dl = in ? delta[(long long)w.bh * n.R + r] : 0.f;
-  const int len = key_count(a, w.b);
-  const int t0 = w.split * n.per, t1 = min((len + KT - 1) / KT, t0 + n.per);
+  const float L = in ? -lse[(long long)w.bh * n.R + r] : -INFINITY;
+  const float dl = in ? -delta[(long long)w.bh * n.R + r] : 0.f;
+  KeyTiles<T, DP, KT> kt(n, w, k, v);
+  const int t0 = w.split * n.per, t1 = min((kt.len + KT - 1) / KT, t0 + n.per);
   const float c = a.scale * kLog2e;
   f32x16 acc[S::nd] = {};
-  using R = Rows<T, DP, KT>;
-  Chunk<T> ck[R::per], cv[R::per];
-  unsigned ok = 0;
-  const T* kb = k + w.b * a.kb + w.hk * a.kh;
-  const T* vb = v + w.b * a.vb + w.hk * a.vh;
-  auto fetch = [&](int t) {
-    const int k0 = t * KT;
-    ok = (unsigned)valid_keys(a, w.b, k0, len);
-    R::load(ck, a.D, [&](int i) { return (ok >> i) & 1 ? kb + (long long)(k0 + i) * a.kl : nullptr; });
-    R::load(cv, a.D, [&](int i) { return (ok >> i) & 1 ? vb + (long long)(k0 + i) * a.vl : nullptr; });
-  };
-  if (t0 < t1) fetch(t0);
+  if (t0 < t1) kt.fetch(t0);
   for (int t = t0; t < t1; ++t) {
-    const unsigned bits = ok >> (4 * h);
+    const unsigned long long live = KT == 64 ? kt.ok0 : kt.ok0 & 0xffffffffull;
+    T* tk = tiles + (t & 1) * 2 * tile;
+    T* tv = tk + tile;
+    kt.put(tk, tv);
     __syncthreads();
-    R::put(ck, tk);
-    R::put(cv, tv);
-    __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
-    f32x16 s = {}, dp = {};
-    scores<T, DP>(s, tk, fq, lane);
-    scores<T, DP>(dp, tv, fg, lane);
+    if (t + 1 < t1) kt.fetch(t + 1);
+    if (!live) continue;
+#pragma unroll 1
+    for (int k0 = 0; k0 < KT; k0 += 32) {
+      f32x16 s = {}, dp;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float p = (bits >> acc_row(i, 0)) & 1 ? hw_exp2(fmaf(s[i], c, -L)) : 0.f;
-      dp[i] = p * (dp[i] - dl);
+      for (int i = 0; i < 16; ++i) dp[i] = dl;   // dp starts at -delta
+      scores<T, DP>(s, tk + k0 * S::ld, fq, lane);
+      scores<T, DP>(dp, tv + k0 * S::ld, fg, lane);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[i] *= hw_exp2(fmaf(s[i], c, L));
+      if (live != (KT == 64 ? ~0ull : 0xffffffffull)) {
+        const unsigned bits = (unsigned)(live >> k0) >> (4 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] = (bits >> acc_row(i, 0)) & 1 ? dp[i] : 0.f;
+      }
+      gather<T, DP>(acc, tk + k0 * S::ld, dp, lane);
     }
-    gather<T, DP>(acc, tk, dp, lane);
   }
   if (part) {
     const long long rows = (long long)a.B * a.Hk * n.R;
     store_row<T, float, DP>(part + (w.split * rows + (long long)w.bh * n.R + r) * a.D, acc, a.scale, a.D, in, h);
   } else {
-    const int qi = r / n.rep, j = r - qi * n.rep;
+    const int qi = r / n.by_rep, j = r - qi * n.rep;
     store_row<T, T, DP>(dq + ((w.b * a.Lq + qi) * a.H + w.hk * n.rep + j) * a.D, acc, a.scale, a.D, in, h);
   }
 }
@@ -457,7 +671,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_add(Attn n, const float* __re
     const splat_attention& a = n.a;
     const long long row = i / a.D;
     const int d = (int)(i - row * a.D), bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
-    const int qi = r / n.rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
+    const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
     at = (((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + d;
   }
   out[at] = (T)s;
@@ -490,45 +704,66 @@ int with_shape(const splat_attention& a, F&& f) {
   return a.dtype == kF32 ? go(float{}) : go(bf16{});
 }
 
-// Splits of an axis of `tiles` tiles where `groups` workgroups would run: as many as make about 512, of at least `least`
-// tiles each.
-void split(Attn& n, long long groups, int tiles, int least) {
-  long long s = groups >= 256 || groups == 0 ? 1 : 512 / groups;
-  if (s > (tiles + least - 1) / least) s = (tiles + least - 1) / least;
-  if (s < 1) s = 1;
-  n.per = (int)((tiles + s - 1) / s);
-  if (n.per < 1) n.per = 1;
-  n.splits = tiles > 0 ? (tiles + n.per - 1) / n.per : 1;
+// Splits of an axis of `tiles` tiles for `groups` workgroups of which `slots` run at a time: the number with the least
+// estimated time, in tiles, of the rounds that the card takes (a last round that is not full runs faster, by about half of
+// what it lacks) where writing and joining partial results costs a split about as much as six tiles. At least four tiles
+// a split.
+void split(Attn& n, long long groups, int tiles, int slots) {
+  n.splits = 1;
+  n.per = tiles < 1 ? 1 : tiles;
+  if (groups == 0) return;
+  double best = 0;
+  for (int s = 1; s <= kMaxSplits && (s == 1 || tiles / s >= 4); ++s) {
+    const int per = (tiles + s - 1) / s;
+    const double r = (double)groups * s / slots, whole = (double)((groups * s + slots - 1) / slots);
+    const double cost = (r < 1 ? 1 : 0.5 * (r + whole)) * (per + (s > 1 ? 6 : 0));
+    if (s == 1 || cost < 0.97 * best) {
+      best = cost;
+      n.per = per < 1 ? 1 : per;
+      n.splits = tiles > 0 ? (tiles + n.per - 1) / n.per : 1;
+    }
+    if (r > 8) break;
+  }
 }
+
+// Workgroups that the card's 256 CUs hold at a time, from the kernels' registers and (few rows) their LDS.
+int slots_rows(const splat_attention& a, int qw) {
+  return 256 * (qw < 4 ? (a.D <= 64 ? 2 : 1) : a.D <= 64 ? 3 : a.dtype == kBf16 ? 2 : 1);
+}
+int slots_keys(const splat_attention& a) { return 256 * (a.D <= 64 ? 2 : 1); }
 
 Attn base(const splat_attention& a) {
   Attn n{};
   n.a = a;
   n.rep = a.H / a.Hk;
+  n.by_rep = fast_div(n.rep);
   n.R = (int)(a.Lq * n.rep);
+  n.chunked = a.D % (a.dtype == kF32 ? 4 : 8) == 0;
+  for (const long long s : {a.ql, a.qh, a.kl, a.vl, a.gl, a.gh}) n.chunked = n.chunked && s >= 0 && s < (1 << 22);
   return n;
 }
 
-Attn plan_fwd(const splat_attention& a, bool* shared) {
+// qw: waves along the rows, as few as the rows need (the others share the keys).
+Attn plan_fwd(const splat_attention& a, int* qw) {
   Attn n = base(a);
-  *shared = n.R <= 32;   // few rows: the waves split the keys
-  n.tiles = *shared ? 1 : div_up(n.R, 128);
-  const int kt = *shared ? 128 : a.dtype == kF32 ? 32 : 64;
-  split(n, (long long)n.tiles * a.B * a.Hk, div_up(a.Lk, kt), 4);
+  *qw = n.R <= 32 ? 1 : n.R <= 64 ? 2 : 4;
+  n.tiles = div_up(n.R, 32 * *qw);
+  const int kt = 32 * (kWaves / *qw) * (a.dtype == kBf16 && *qw > 1 ? 2 : 1);
+  split(n, (long long)n.tiles * a.B * a.Hk, div_up(a.Lk, kt), slots_rows(a, *qw));
   return n;
 }
 
 Attn plan_kv(const splat_attention& a) {
   Attn n = base(a);
   n.tiles = div_up(a.Lk, 128);
-  split(n, (long long)n.tiles * a.B * a.Hk, div_up(n.R, 32), 8);
+  split(n, (long long)n.tiles * a.B * a.Hk, div_up(n.R, a.dtype == kBf16 ? 64 : 32), slots_keys(a));
   return n;
 }
 
 Attn plan_q(const splat_attention& a) {
   Attn n = base(a);
   n.tiles = div_up(n.R, 128);
-  split(n, (long long)n.tiles * a.B * a.Hk, div_up(a.Lk, 32), 8);
+  split(n, (long long)n.tiles * a.B * a.Hk, div_up(a.Lk, a.dtype == kBf16 ? 64 : 32), slots_rows(a, 4));
   return n;
 }
 
@@ -543,10 +778,9 @@ extern "C" {
 
 size_t splat_attention_workspace_bytes(const splat_attention* a) {
   if (check_attn("splat_attention_workspace_bytes", a) || a->B == 0 || a->Lq == 0) return 0;
-  bool shared;
-  const Attn n = plan_fwd(*a, &shared);
-  if (!shared && n.splits == 1) return 0;
-  return sizeof(float) * (size_t)n.splits * (shared ? kWaves : 1) * a->B * a->Hk * n.R * (a->D + 2);
+  int qw;
+  const Attn n = plan_fwd(*a, &qw);
+  return n.splits == 1 ? 0 : sizeof(float) * (size_t)n.splits * a->B * a->Hk * n.R * (a->D + 2);
 }
 
 int splat_attention_fwd(const splat_attention* a, const void* q, const void* k, const void* v, void* o, float* lse,
@@ -554,25 +788,30 @@ int splat_attention_fwd(const splat_attention* a, const void* q, const void* k, 
   if (const int rc = check_attn("splat_attention_fwd", a)) return rc;
   if (a->B == 0 || a->Lq == 0) return kOk;
   if (!q || !o || (a->Lk > 0 && (!k || !v))) return set_error(kInvalid, "splat_attention_fwd: null pointer");
-  bool shared;
-  const Attn n = plan_fwd(*a, &shared);
+  int qw;
+  const Attn n = plan_fwd(*a, &qw);
   const size_t need = splat_attention_workspace_bytes(a);
   if (need && (!ws || ws_bytes < need))
     return set_error(kWorkspace, "splat_attention_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
-  const int slots = n.splits * (shared ? kWaves : 1);
   const long long rows = (long long)a->B * a->Hk * n.R;
   float* part = need ? (float*)ws : nullptr;
-  float* stat = need ? part + (size_t)slots * rows * a->D : nullptr;
+  float* stat = need ? part + (size_t)n.splits * rows * a->D : nullptr;
   const hipStream_t st = (hipStream_t)stream;
   return with_shape(*a, [&](auto t, auto dp) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     const int grid = n.tiles * n.splits * a->B * a->Hk;
-    if (shared)
-      k_attn_fwd<T, DP, 1><<<grid, kThreads, 0, st>>>(n, (const T*)q, (const T*)k, (const T*)v, (T*)o, lse, part, stat);
-    else
-      k_attn_fwd<T, DP, 4><<<grid, kThreads, 0, st>>>(n, (const T*)q, (const T*)k, (const T*)v, (T*)o, lse, part, stat);
-    if (need) k_attn_join<T><<<div_up(rows, kWaves), kThreads, 0, st>>>(n, part, stat, slots, (T*)o, lse);
+    auto go = [&](auto w) {
+      k_attn_fwd<T, DP, decltype(w)::value><<<grid, kThreads, 0, st>>>(n, (const T*)q, (const T*)k, (const T*)v, (T*)o, lse,
+                                                                       part, stat);
+    };
+    if (qw == 1) go(std::integral_constant<int, 1>{});
+    else if (qw == 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 4>{});
+    if (need && n.splits <= 8)
+      k_attn_join_few<T><<<div_up(rows * a->D, kThreads), kThreads, 0, st>>>(n, part, stat, (T*)o, lse);
+    else if (need)
+      k_attn_join<T, DP><<<(unsigned)rows, kThreads, 0, st>>>(n, part, stat, (T*)o, lse);
     return check_launch("splat_attention_fwd");
   });
 }

@@ -153,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
               store_chunk((T*)g.z + (long long)q * g.P + p, o, n);
             }
 #pragma unroll
-            for (int e = 0; e < V; ++e) run[t][e] = act_fwd<A>(run[t][e]);
+            for (int e = 0; e < V; ++e) run[t][e] = act_fwd<A, T>(run[t][e]);
             if (g.res) {
               const Chunk<T> r = load_chunk((const T*)g.res + q * g.ldr + p, n);
 #pragma unroll
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
   const Chunk<T> d = load_chunk(dy + i, n - i), c = load_chunk(z + i, n - i);
   Chunk<T> o;
 #pragma unroll
-  for (int j = 0; j < kV<T>; ++j) o.v[j] = (T)((float)d.v[j] * act_grad<A>((float)c.v[j]));
+  for (int j = 0; j < kV<T>; ++j) o.v[j] = (T)((float)d.v[j] * act_grad<A, T>((float)c.v[j]));
   store_chunk(g + i, o, n - i);
 }
 

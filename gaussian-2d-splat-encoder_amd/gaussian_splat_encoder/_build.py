@@ -24,14 +24,17 @@ HIP_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wno-unused-result",
 ]
-# Per-source extra flags: the binning must round every fp32 op separately (no FMA contraction).
+# Per-source extra flags: the binning must round every fp32 op separately (no FMA contraction); matrix instructions of
+# the products and the attention keep their accumulators in vector registers (in accumulation registers the compiler moves
+# them to vector registers and back around every softmax step).
+_VGPR_ACC = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 SOURCES = {
     "capi.hip": [],
     "bin.hip": ["-ffp-contract=off"],
     "render.hip": [],
     "norm.hip": [],
-    "linear.hip": [],
-    "attend.hip": [],
+    "linear.hip": _VGPR_ACC,
+    "attend.hip": _VGPR_ACC,
 }
 
 
