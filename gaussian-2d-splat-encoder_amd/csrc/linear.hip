@@ -27,35 +27,51 @@ struct Gemm {
 
 enum Epilogue { kOut, kForward, kPartial };
 
-// One operand's tile in LDS: R operand rows by KE contraction indices. Stored along k as R rows of KE, across it as KE
-// rows of R; 16 bytes of padding a row keep the reads of neighbouring rows on different banks.
+// One operand's tile: R operand rows by KE contraction indices, global -> registers -> LDS. Stored along k it is R rows of
+// KE in LDS, across it KE rows of R; 16 bytes of padding a row keep the reads of neighbouring rows on different banks.
+// A thread's chunks keep their places from tile to tile. Operand rows past the matrix are read from its last row (their
+// results are not stored); contraction indices past the end have to be zeros.
 template <typename T, int R, bool Col>
 struct Stage {
   static constexpr int V = kV<T>, KE = kBytesK / (int)sizeof(T);
   static constexpr int rows = Col ? KE : R, cols = Col ? R : KE;
-  static constexpr int ld = cols + V;
-  static constexpr int chunks = rows * cols / V, per = chunks / kThreads;
-  static_assert(chunks % kThreads == 0, "every thread stages the same number of chunks");
+  static constexpr int ld = cols + V, cc = cols / V;                 // chunks of an LDS row
+  static constexpr int RS = kThreads / cc, per = rows / RS;          // rows from chunk to chunk of a thread
+  static_assert(kThreads % cc == 0 && rows % RS == 0, "every thread stages the same number of chunks");
+  Chunk<T> c[per];
+  const T* p[per];   // the chunks of the next tile
+  long long step;    // elements from tile to tile
+  int in;            // Col: operand rows that the thread's chunk holds
 
-  // The thread's chunks of the tile at operand row r0 (of R_all) and contraction index k0 (up to k1).
-  __device__ static void load(Chunk<T> (&c)[per], const T* m, long long ldm, int r0, int R_all, long long k0, long long k1) {
+  __device__ static int row0() { return threadIdx.x / cc; }
+  __device__ static int col() { return threadIdx.x % cc * V; }
+  __device__ void init(const T* m, long long ldm, int r0, int R_all, long long k0) {
 #pragma unroll
     for (int i = 0; i < per; ++i) {
-      const int e = threadIdx.x + i * kThreads, row = e / (cols / V), col = e % (cols / V) * V;
-      if constexpr (Col) {
-        const long long k = k0 + row;
-        c[i] = load_chunk(m + k * ldm + r0 + col, k < k1 ? (long long)R_all - r0 - col : 0);
-      } else {
-        c[i] = load_chunk(m + (long long)(r0 + row) * ldm + k0 + col, r0 + row < R_all ? k1 - k0 - col : 0);
+      const int row = row0() + i * RS;
+      p[i] = Col ? m + (k0 + row) * ldm + r0 + col() : m + (long long)min(r0 + row, R_all - 1) * ldm + k0 + col();
+    }
+    step = Col ? KE * ldm : KE;
+    in = R_all - r0 - col();
+  }
+  // left: contraction indices from the tile's first one to the end.
+  __device__ __forceinline__ void load(long long left) {
+    if (left >= KE && (!Col || in >= V)) {
+#pragma unroll
+      for (int i = 0; i < per; ++i) __builtin_memcpy(c[i].v, p[i], 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < per; ++i) {
+        if constexpr (Col) c[i] = load_chunk(p[i], row0() + i * RS < left ? in : 0);
+        else c[i] = load_chunk(p[i], left - col());
       }
     }
-  }
-  __device__ static void put(const Chunk<T> (&c)[per], T* t) {
 #pragma unroll
-    for (int i = 0; i < per; ++i) {
-      const int e = threadIdx.x + i * kThreads, row = e / (cols / V), col = e % (cols / V) * V;
-      *(f32x4*)(t + row * ld + col) = *(const f32x4*)c[i].v;
-    }
+    for (int i = 0; i < per; ++i) p[i] += step;
+  }
+  __device__ void put(T* t) const {
+#pragma unroll
+    for (int i = 0; i < per; ++i) *(f32x4*)(t + (row0() + i * RS) * ld + col()) = *(const f32x4*)c[i].v;
   }
   // Operand chunk of the 32 rows from r at the contraction index k.
   __device__ static Chunk<T> frag(const T* t, int r, int k, int lane) {
@@ -64,20 +80,26 @@ struct Stage {
   }
 };
 
-// A workgroup's WP x WQ waves take PB x QB blocks of 32 x 32 each.
+// A workgroup's WP x WQ waves take PB x QB blocks of 32 x 32 each. The epilogue passes the results through LDS, 32 WQ rows
+// of the output at a time, so that every load and store of it is a run of whole rows (stored straight from the matrix
+// instructions' layout, 32 bytes a row at a time, the writes were 1.5 times the output).
 template <typename T, int PB, int QB, int WP, int WQ, bool ACol, bool BCol, int Epi, int A>
 __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
   static_assert(WP * WQ * 64 == kThreads, "four waves");
   constexpr int V = kV<T>;
-  using SA = Stage<T, PB * WP * 32, ACol>;
-  using SB = Stage<T, QB * WQ * 32, BCol>;
-  __shared__ __align__(16) T ta[SA::rows * SA::ld];
-  __shared__ __align__(16) T tb[SB::rows * SB::ld];
+  constexpr int TP = PB * WP * 32, TQ = QB * WQ * 32;
+  using SA = Stage<T, TP, ACol>;
+  using SB = Stage<T, TQ, BCol>;
+  constexpr int na = SA::rows * SA::ld, nb = SB::rows * SB::ld, ldo = TP + 4;
+  constexpr int bytes = (na + nb) * (int)sizeof(T) > WQ * 32 * ldo * 4 ? (na + nb) * (int)sizeof(T) : WQ * 32 * ldo * 4;
+  __shared__ __align__(16) char lds[bytes];
+  T* ta = (T*)lds;
+  T* tb = ta + na;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   // neighbouring workgroups of an XCD share rows of B
   const int tile = xcd_swizzle(blockIdx.x, gridDim.x);
-  const int p0 = tile % g.tp * (PB * WP * 32), q0 = tile / g.tp * (QB * WQ * 32);
-  const int wp = wave % WP * PB * 32, wq = wave / WP * QB * 32;
+  const int p0 = tile % g.tp * TP, q0 = tile / g.tp * TQ;
+  const int wp = wave % WP * PB * 32, wq = wave / WP * 32;   // block j of a wave: rows q0 + 32 WQ j + wq ..
   const long long k0 = (long long)blockIdx.y * g.kper, k1 = min(g.K, k0 + g.kper);
   f32x16 acc[PB][QB] = {};
   f32x16 bsum[QB] = {};
@@ -85,17 +107,20 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
 #pragma unroll
   for (int j = 0; j < V; ++j) one.v[j] = (T)1.f;
   const bool sums = Epi == kPartial && g.bpart && p0 == 0 && wp == 0;
-  Chunk<T> ca[SA::per], cb[SB::per];
-  SA::load(ca, (const T*)g.A, g.lda, p0, g.P, k0, k1);
-  SB::load(cb, (const T*)g.B, g.ldb, q0, g.Q, k0, k1);
+  SA sa;
+  SB sb;
+  sa.init((const T*)g.A, g.lda, p0, g.P, k0);
+  sb.init((const T*)g.B, g.ldb, q0, g.Q, k0);
+  sa.load(k1 - k0);
+  sb.load(k1 - k0);
   for (long long k = k0; k < k1; k += SA::KE) {
     __syncthreads();
-    SA::put(ca, ta);
-    SB::put(cb, tb);
+    sa.put(ta);
+    sb.put(tb);
     __syncthreads();
     if (k + SA::KE < k1) {
-      SA::load(ca, (const T*)g.A, g.lda, p0, g.P, k + SA::KE, k1);
-      SB::load(cb, (const T*)g.B, g.ldb, q0, g.Q, k + SA::KE, k1);
+      sa.load(k1 - k - SA::KE);
+      sb.load(k1 - k - SA::KE);
     }
 #pragma unroll
     for (int s = 0; s < SA::KE; s += 2 * V) {
@@ -103,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
 #pragma unroll
       for (int i = 0; i < PB; ++i) a[i] = SA::frag(ta, wp + 32 * i, s, lane);
 #pragma unroll
-      for (int i = 0; i < QB; ++i) b[i] = SB::frag(tb, wq + 32 * i, s, lane);
+      for (int i = 0; i < QB; ++i) b[i] = SB::frag(tb, 32 * WQ * i + wq, s, lane);
 #pragma unroll
       for (int i = 0; i < PB; ++i)
 #pragma unroll
@@ -114,68 +139,79 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
       }
     }
   }
+  float* to = (float*)lds;
+  constexpr int VO = Epi == kPartial ? 4 : V, cc = TP / VO;   // values a thread writes at a time
+  const int p = p0 + threadIdx.x % cc * VO, n = g.P - p;
+  Chunk<T> bias{};
+  if (Epi == kForward && g.bias) bias = load_chunk((const T*)g.bias + p, n);
 #pragma unroll
   for (int j = 0; j < QB; ++j) {
-    const int q = q0 + wq + 32 * j + (lane & 31);
-    if (q >= g.Q) continue;
-    if (sums && h == 0) g.bpart[(long long)blockIdx.y * g.Q + q] = bsum[j][0];
+    const int qj = q0 + 32 * WQ * j;
+    if (sums && h == 0 && qj + wq + lane < g.Q) g.bpart[(long long)blockIdx.y * g.Q + qj + wq + lane] = bsum[j][0];
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < PB; ++i) {
+    for (int i = 0; i < PB; ++i)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 run = {acc[i][j][4 * t], acc[i][j][4 * t + 1], acc[i][j][4 * t + 2], acc[i][j][4 * t + 3]};
+        *(f32x4*)(to + (wq + (lane & 31)) * ldo + wp + 32 * i + acc_row(4 * t, h)) = run;
+      }
+    __syncthreads();
+    if (n <= 0) continue;
+#pragma unroll
+    for (int r = threadIdx.x / cc; r < 32 * WQ; r += kThreads / cc) {
+      const int q = qj + r;
+      if (q >= g.Q) break;
+      float x[VO];
+#pragma unroll
+      for (int e = 0; e < VO; e += 4) {
+        const f32x4 run = *(const f32x4*)(to + r * ldo + (p - p0) + e);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) x[e + f] = run[f];
+      }
       if constexpr (Epi == kPartial) {
-        float run[4][4];
-        acc_runs<float>(acc[i][j], run);
+        Chunk<float> o;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int p = p0 + wp + 32 * i + run_row<float>(t, h);
-          Chunk<float> o;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o.v[e] = run[t][e];
-          store_chunk(g.part + ((long long)blockIdx.y * g.Q + q) * g.P + p, o, g.P - p);
-        }
+        for (int e = 0; e < 4; ++e) o.v[e] = x[e];
+        store_chunk(g.part + ((long long)blockIdx.y * g.Q + q) * g.P + p, o, n);
       } else {
-        float run[16 / V][V];
-        acc_runs<T>(acc[i][j], run);
+        Chunk<T> o;
+        if constexpr (Epi == kForward) {
 #pragma unroll
-        for (int t = 0; t < 16 / V; ++t) {
-          const int p = p0 + wp + 32 * i + run_row<T>(t, h);
-          const int n = g.P - p;
-          if (n <= 0) continue;
-          Chunk<T> o;
-          if constexpr (Epi == kForward) {
-            if (g.bias) {
-              const Chunk<T> b = load_chunk((const T*)g.bias + p, n);
+          for (int e = 0; e < V; ++e) x[e] += (float)bias.v[e];
+          if (g.z) {
 #pragma unroll
-              for (int e = 0; e < V; ++e) run[t][e] += (float)b.v[e];
-            }
-            if (g.z) {
-#pragma unroll
-              for (int e = 0; e < V; ++e) o.v[e] = (T)run[t][e];
-              store_chunk((T*)g.z + (long long)q * g.P + p, o, n);
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) run[t][e] = act_fwd<A, T>(run[t][e]);
-            if (g.res) {
-              const Chunk<T> r = load_chunk((const T*)g.res + q * g.ldr + p, n);
-#pragma unroll
-              for (int e = 0; e < V; ++e) run[t][e] += (float)r.v[e];
-            }
+            for (int e = 0; e < V; ++e) o.v[e] = (T)x[e];
+            store_chunk((T*)g.z + (long long)q * g.P + p, o, n);
           }
 #pragma unroll
-          for (int e = 0; e < V; ++e) o.v[e] = (T)run[t][e];
-          store_chunk((T*)g.out + (long long)q * g.P + p, o, n);
+          for (int e = 0; e < V; ++e) x[e] = act_fwd<A, T>(x[e]);
+          if (g.res) {
+            const Chunk<T> rs = load_chunk((const T*)g.res + q * g.ldr + p, n);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] += (float)rs.v[e];
+          }
         }
+#pragma unroll
+        for (int e = 0; e < V; ++e) o.v[e] = (T)x[e];
+        store_chunk((T*)g.out + (long long)q * g.P + p, o, n);
       }
     }
   }
 }
 
-// out[i] = sum over the slices, in their order, of part[slice][i].
+// out[i] = sum over the slices, in their order, of part[slice][i]; in the workgroups from `wgs` on the same for the bias,
+// 32 columns each, 8 groups of threads over its slices.
 template <typename T>
 __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, int slices, long long n, T* __restrict__ out,
-                                              const float* __restrict__ bpart, long long nb, T* __restrict__ bout) {
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i < n) {
+                                              unsigned wgs, const float* __restrict__ bpart, int bslices, int nb,
+                                              T* __restrict__ bout) {
+  __shared__ float red[8][32];
+  if (blockIdx.x < wgs) {
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
     f32x4 s = {};
+#pragma unroll 8
     for (int k = 0; k < slices; ++k) {
       const Chunk<float> c = load_chunk(part + k * n + i, n - i);
 #pragma unroll
@@ -184,27 +220,55 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (i + j < n) out[i + j] = (T)s[j];
-  } else {
-    for (long long e = i - (n + 3) / 4 * 4; e < i - (n + 3) / 4 * 4 + 4; ++e) {
-      if (e >= nb) return;
-      float s = 0.f;
-      for (int k = 0; k < slices; ++k) s += bpart[k * nb + e];
-      bout[e] = (T)s;
-    }
+    return;
+  }
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, c = (blockIdx.x - wgs) * 32 + lane;
+  float s = 0.f;
+  if (c < nb) {
+#pragma unroll 8
+    for (int k = grp; k < bslices; k += 8) s += bpart[(long long)k * nb + c];
+  }
+  red[grp][lane] = s;
+  __syncthreads();
+  if (grp == 0 && c < nb) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += red[k][lane];
+    bout[c] = (T)s;
   }
 }
 
-// g = dy act'(z)
+// g = dy act'(z) over `per` rows a workgroup, 64 chunks of columns wide, and the rows' sums of g before its rounding.
 template <typename T, int A>
 __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ g,
-                                                  long long n) {
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * kV<T>;
-  if (i >= n) return;
-  const Chunk<T> d = load_chunk(dy + i, n - i), c = load_chunk(z + i, n - i);
-  Chunk<T> o;
+                                                  long long M, int N, int per, float* __restrict__ bpart) {
+  constexpr int V = kV<T>;
+  __shared__ float red[4][64 * V];
+  const int col = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
+  const long long r0 = (long long)blockIdx.y * per, r1 = min(M, r0 + per);
+  float s[V] = {};
+  if (col < N) {
+#pragma unroll 4
+    for (long long r = r0 + (threadIdx.x >> 6); r < r1; r += 4) {
+      const long long i = r * N + col;
+      const Chunk<T> d = load_chunk(dy + i, N - col), c = load_chunk(z + i, N - col);
+      Chunk<T> o;
 #pragma unroll
-  for (int j = 0; j < kV<T>; ++j) o.v[j] = (T)((float)d.v[j] * act_grad<A, T>((float)c.v[j]));
-  store_chunk(g + i, o, n - i);
+      for (int j = 0; j < V; ++j) {
+        const float x = (float)d.v[j] * act_grad<A, T>((float)c.v[j]);
+        s[j] += x;
+        o.v[j] = (T)x;
+      }
+      store_chunk(g + i, o, N - col);
+    }
+  }
+  if (!bpart) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) red[threadIdx.x >> 6][(threadIdx.x & 63) * V + j] = s[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 64 * V; c += 256) {
+    const int n = blockIdx.x * 64 * V + c;
+    if (n < N) bpart[(long long)blockIdx.y * N + n] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+  }
 }
 
 template <typename T, int PB, int QB, int WP, int WQ, bool ACol, bool BCol, int Epi, int A>
@@ -225,14 +289,24 @@ void gemm(const Gemm& g, int slices, hipStream_t st) {
   else launch<T, 1, 1, 2, 2, ACol, BCol, Epi, A>(g, slices, st);
 }
 
-// Slices of the contraction over M rows for a weight gradient [N, K].
+// Slices of the contraction over M rows for a weight gradient [N, K]: about 512 workgroups, of at least 256 rows each.
 int weight_slices(long long M, int N, int K) {
-  const long long tiles = (long long)div_up(N, 64) * div_up(K, 64);
-  const long long want = 512 / tiles > 0 ? 512 / tiles : 1;
+  const int t = N >= 128 && K >= 128 ? 128 : 64;
+  const long long tiles = (long long)div_up(N, t) * div_up(K, t);
+  const long long want = (512 + tiles - 1) / tiles;
   const long long room = (M + 255) / 256;
   const long long s = want < room ? want : room;
   return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
 }
+
+// Rows of a workgroup of k_act_grad: about 1024 workgroups, of at least 16 rows each.
+int grad_rows(int dtype, long long M, int N) {
+  const long long wide = div_up(N, 64 * (dtype == kF32 ? 4 : 8)), want = (1024 + wide - 1) / wide;
+  const long long per = (M + want - 1) / want;
+  return (int)(per < 16 ? 16 : per);
+}
+
+size_t grad_bytes(int dtype, long long M, int N) { return ((size_t)M * N * (dtype == kF32 ? 4 : 2) + 255) & ~(size_t)255; }
 
 int check_linear(const char* what, int dtype, long long M, int N, int K, int act) {
   if (dtype != kF32 && dtype != kBf16) return set_error(kInvalid, "%s: unknown element type %d", what, dtype);
@@ -277,9 +351,9 @@ int splat_linear_fwd(const void* x, long long ldx, const void* weight, const voi
 
 size_t splat_linear_bwd_workspace_bytes(int dtype, long long M, int N, int K, int act) {
   if (check_linear("splat_linear_bwd_workspace_bytes", dtype, M, N, K, act) || M == 0) return 0;
-  const int s = weight_slices(M, N, K);
-  const size_t grad = act == kActNone ? 0 : ((size_t)M * N * (dtype == kF32 ? 4 : 2) + 255) & ~(size_t)255;
-  return grad + sizeof(float) * (size_t)s * ((size_t)N * K + N);
+  const size_t slices = weight_slices(M, N, K);
+  if (act == kActNone) return sizeof(float) * slices * ((size_t)N * K + N);
+  return grad_bytes(dtype, M, N) + sizeof(float) * (slices * N * K + (size_t)div_up(M, grad_rows(dtype, M, N)) * N);
 }
 
 int splat_linear_bwd(const void* x, long long ldx, const void* weight, const void* dy, const void* z, int dtype,
@@ -295,12 +369,17 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
   const hipStream_t st = (hipStream_t)stream;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const size_t grad = act == kActNone ? 0 : ((size_t)M * N * sizeof(T) + 255) & ~(size_t)255;
+    const int s = weight_slices(M, N, K);
     const T* gr = (const T*)dy;
+    float* part = (float*)((char*)ws + (act == kActNone ? 0 : grad_bytes(dtype, M, N)));
+    float* bpart = dbias ? part + (size_t)s * N * K : nullptr;
+    int bslices = s;
     if (act != kActNone) {
+      const int per = grad_rows(dtype, M, N);
+      bslices = div_up(M, per);
       with_act(act, [&](auto a) {
-        const long long n = M * N;
-        k_act_grad<T, decltype(a)::value><<<div_up(n, 256 * kV<T>), 256, 0, st>>>((const T*)dy, (const T*)z, (T*)ws, n);
+        k_act_grad<T, decltype(a)::value><<<dim3(div_up(N, 64 * kV<T>), bslices), 256, 0, st>>>(
+            (const T*)dy, (const T*)z, (T*)ws, M, N, per, bpart);
         return kOk;
       });
       gr = (const T*)ws;
@@ -314,18 +393,19 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
       gemm<T, true, false, kOut, 0>(g, 1, st);
     }
     if (dweight || dbias) {
-      const int s = weight_slices(M, N, K);
-      Gemm g{};
-      // dbias alone: one column of products, with the gradient itself for want of x
-      g.A = dweight ? x : gr; g.lda = dweight ? ldx : N; g.P = dweight ? K : 1;
-      g.B = gr; g.ldb = N; g.Q = N;
-      g.K = M; g.kper = (M + s - 1) / s;
-      g.part = (float*)((char*)ws + grad);
-      g.bpart = dbias ? g.part + (size_t)s * N * K : nullptr;
-      gemm<T, true, true, kPartial, 0>(g, s, st);
+      if (dweight || act == kActNone) {
+        Gemm g{};
+        // dbias alone: one column of products, with the gradient itself for want of x
+        g.A = dweight ? x : gr; g.lda = dweight ? ldx : N; g.P = dweight ? K : 1;
+        g.B = gr; g.ldb = N; g.Q = N;
+        g.K = M; g.kper = (M + s - 1) / s;
+        g.part = part;
+        g.bpart = act == kActNone ? bpart : nullptr;
+        gemm<T, true, true, kPartial, 0>(g, s, st);
+      }
       const long long n = dweight ? (long long)N * K : 0;
-      k_join<T><<<div_up((n + 3) / 4 + (dbias ? (N + 3) / 4 : 0), 256), 256, 0, st>>>(g.part, s, n, (T*)dweight, g.bpart,
-                                                                                     dbias ? N : 0, (T*)dbias);
+      const unsigned wgs = div_up(n, 1024), bwgs = dbias ? div_up(N, 32) : 0;
+      k_join<T><<<wgs + bwgs, 256, 0, st>>>(part, s, n, (T*)dweight, wgs, bpart, bslices, N, (T*)dbias);
     }
     return check_launch("splat_linear_bwd");
   });
