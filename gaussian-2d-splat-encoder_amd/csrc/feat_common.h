@@ -21,18 +21,16 @@ enum Act : int { kActNone = 0, kActGelu = 1, kActSilu = 2, kActRelu = 3, kActTan
 // ------------------------------------------------------------------------------------------ activations
 // T is the type that the result is rounded to: for bf16 (2^-9 of a value) shorter polynomials do.
 
-// Phi(x), the normal distribution's integral (gelu(x) = x Phi(x)), and its density *pdf. With a = |x| and t = 1 / (1 + p a),
-// Phi(-a) = exp(-a^2 / 2) t P(t), P fitted for the least relative error over a in [0, 16] (beyond it the exponential is
-// zero): 8e-8 with 9 coefficients (3e-7 evaluated in float32), 4e-5 with 5. About 20 instructions; erfc takes about 60, and
-// the group norm's passes were then bound by them (stats of a bf16 map of 37.7M values: 63 us, 23 us with this).
+// Phi(x), the normal distribution's integral (gelu(x) = x Phi(x)).
+// float: with a = |x| and t = 1 / (1 + 0.33 a), Phi(-a) = exp(-a^2 / 2) t P(t), P of degree 8 fitted for the least relative
+// error over a in [0, 16] (beyond it the exponential is zero): 8e-8, 3e-7 evaluated in float32. About 20 instructions.
+// bf16: the logistic function of an odd polynomial of degree 5, fitted for the least error of x Phi(x): 2.5e-5. About 11.
+// erfc takes about 60, and the group norm's passes were then bound by them (statistics of a bf16 map of 37.7M values 63 us).
 template <typename T>
-__device__ __forceinline__ float normal_cdf(float x, float* pdf) {
-  const float e = hw_exp2(-0.5f * kLog2e * x * x);
-  float p;
-  float t;
+__device__ __forceinline__ float normal_cdf(float x) {
   if constexpr (sizeof(T) == 4) {
-    t = hw_rcp(fmaf(0.33f, fabsf(x), 1.f));
-    p = fmaf(-0.01941489987075329f, t, 0.11651250720024109f);
+    const float e = hw_exp2(-0.5f * kLog2e * x * x), t = hw_rcp(fmaf(0.33f, fabsf(x), 1.f));
+    float p = fmaf(-0.01941489987075329f, t, 0.11651250720024109f);
     p = fmaf(p, t, -0.25408560037612915f);
     p = fmaf(p, t, 0.21024172008037567f);
     p = fmaf(p, t, -0.04704420268535614f);
@@ -40,17 +38,17 @@ __device__ __forceinline__ float normal_cdf(float x, float* pdf) {
     p = fmaf(p, t, 0.1119847446680069f);
     p = fmaf(p, t, 0.1321829855442047f);
     p = fmaf(p, t, 0.1316286325454712f);
+    const float q = e * (p * t);
+    return x > 0.f ? 1.f - q : q;
   } else {
-    t = hw_rcp(fmaf(0.375f, fabsf(x), 1.f));
-    p = fmaf(-0.08943793922662735f, t, 0.19760045409202576f);
-    p = fmaf(p, t, 0.08563226461410522f);
-    p = fmaf(p, t, 0.15708869695663452f);
-    p = fmaf(p, t, 0.14912866055965424f);
+    const float s = fminf(x * x, 30.25f);
+    float p = fmaf(0.0007030339911580086f * kLog2e, s, -0.07401129603385925f * kLog2e);
+    p = fmaf(p, s, -1.5950157642364502f * kLog2e);
+    return hw_rcp(1.f + hw_exp2(p * x));
   }
-  const float q = e * (p * t);
-  *pdf = 0.39894228040143268f * e;
-  return x > 0.f ? 1.f - q : q;
 }
+// The normal distribution's density.
+__device__ __forceinline__ float normal_pdf(float x) { return 0.39894228040143268f * hw_exp2(-0.5f * kLog2e * x * x); }
 __device__ __forceinline__ float sigmoidf(float x) { return hw_rcp(1.f + hw_exp2(-kLog2e * x)); }
 
 // Odd series to x^9 (fitted, 8e-8 relative) up to 0.6, beyond it 1 - 2 / (e^2|x| + 1), which loses no digits there.
@@ -67,8 +65,7 @@ __device__ __forceinline__ float tanh_of(float x) {
 template <int A, typename T>
 __device__ __forceinline__ float act_fwd(float x) {
   if constexpr (A == kActGelu) {
-    float pdf;
-    return x * normal_cdf<T>(x, &pdf);
+    return x * normal_cdf<T>(x);
   } else if constexpr (A == kActSilu) {
     return x * sigmoidf(x);
   } else if constexpr (A == kActRelu) {
@@ -86,9 +83,7 @@ __device__ __forceinline__ float act_fwd(float x) {
 template <int A, typename T>
 __device__ __forceinline__ float act_grad(float x) {
   if constexpr (A == kActGelu) {
-    float pdf;
-    const float cdf = normal_cdf<T>(x, &pdf);
-    return fmaf(x, pdf, cdf);
+    return fmaf(x, normal_pdf(x), normal_cdf<T>(x));
   } else if constexpr (A == kActSilu) {
     const float s = sigmoidf(x);
     return fmaf(x * s, 1.f - s, s);

@@ -5,17 +5,19 @@
 // with mean and rstd = 1 / sqrt(var + eps) over the C / G channels of a group and all positions of an image.
 //
 // A workgroup covers a channel tile (whole groups, or a part of one group wider than a tile) and a range of positions:
-// thread (rt, cc) holds the 16-byte chunk cc of the tile's channels at the positions rt, rt + RT, ... Both directions are
-// bound by memory. Where one workgroup's registers hold a group, everything is one launch that reads x once; otherwise
-// one launch reduces each range to partial sums and a second one joins them and writes the result, x coming from
-// the caches the second time where it fits them.
+// thread (rt, cc) holds the 16-byte chunk cc of the tile's channels at the positions rt, rt + RT, ... Where one workgroup's
+// registers hold a group, everything is one launch that reads x once; otherwise one launch reduces each range to partial
+// sums and a second one joins them and writes the result, x coming from the caches the second time where it fits them.
+// Both directions are bound by memory, and maps of a few megabytes by the chain of loads, reductions and barriers of a
+// workgroup: x's first rows are requested before anything else, and a reduction is one exchange through LDS.
 #include "feat_common.h"
 
 namespace splat {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kKeep = 16;   // chunks of x that a thread keeps in registers in the one-launch forward
+constexpr int kTile = 2048;   // channels of a tile at most
+constexpr int kKeep = 16;     // chunks of x that a thread keeps in registers in the one-launch forward, at most
 
 struct Norm {
   long long L, xsb, xsl, gsb, gsl;   // positions; strides of x and of dy per image and position (channels are dense)
@@ -27,14 +29,21 @@ struct Norm {
   float eps;
 };
 
-// A thread's place: its channels [c, c + nv) of the map and its first position rt.
+// A thread's place: its channels [c, c + nv) of the map, its first position rt and its positions of the range [lo, hi).
 struct Place {
   int rt, cc, c, nv, c0, ct;   // c0, ct: the tile's first channel and its channels
-  bool on;
+  int g0, ng;                  // the tile's groups: the first one and how many (1 where the tile is a part of a group)
+  long long lo, hi;
+  int rows;
 };
 
+__device__ __forceinline__ int rows_of(long long lo, long long hi, int rt, int RT) {
+  const long long r = hi - lo - rt;
+  return r <= 0 ? 0 : (int)((r + RT - 1) / RT);
+}
+
 template <typename T>
-__device__ __forceinline__ Place place(const Norm& n, int tile) {
+__device__ __forceinline__ Place place(const Norm& n, int tile, int split) {
   Place p;
   if (n.tpg == 1) {
     p.c0 = tile * n.Ct;
@@ -44,18 +53,16 @@ __device__ __forceinline__ Place place(const Norm& n, int tile) {
     p.c0 = g * n.Cg + k * n.Ct;
     p.ct = min(n.Ct, n.Cg - k * n.Ct);
   }
+  p.g0 = p.c0 / n.Cg;
+  p.ng = n.tpg == 1 ? p.ct / n.Cg : 1;
   p.rt = threadIdx.x / n.nch;
   p.cc = threadIdx.x % n.nch;
   p.c = p.c0 + p.cc * kV<T>;
-  p.nv = min(kV<T>, p.ct - p.cc * kV<T>);
-  p.on = p.rt < n.RT && p.nv > 0;
+  p.nv = p.rt < n.RT ? max(0, min(kV<T>, p.ct - p.cc * kV<T>)) : 0;
+  p.lo = (long long)split * n.per;
+  p.hi = min(n.L, p.lo + n.per);
+  p.rows = p.nv > 0 ? rows_of(p.lo, p.hi, p.rt, n.RT) : 0;
   return p;
-}
-
-// The tile's groups: the first one and how many (1 where the tile is a part of one group).
-__device__ __forceinline__ int tile_groups(const Norm& n, const Place& p, int* g0) {
-  *g0 = p.c0 / n.Cg;
-  return n.tpg == 1 ? p.ct / n.Cg : 1;
 }
 
 // Group of the thread's channel j within the tile.
@@ -63,39 +70,106 @@ __device__ __forceinline__ int group_of(const Norm& n, const Place& p, int j) {
   return n.tpg == 1 ? (p.c - p.c0 + j) / n.Cg : 0;
 }
 
-// out[g] = sum over the workgroup's threads and the channels of group g of v. One value per thread goes through LDS
-// where no chunk meets two groups, one per channel otherwise; either way a group's values lie next to each other
-// (channel-major), and one wave adds them in a fixed order. `red` holds kThreads * kV floats.
-template <typename T>
-__device__ __forceinline__ void group_sums(const Norm& n, const Place& p, int ng, const float* v, float* red, float* out) {
-  const bool whole = n.Cg % kV<T> == 0 || n.tpg > 1;
-  __syncthreads();
-  if (threadIdx.x < (unsigned)(n.RT * n.nch)) {
-    if (whole) {
-      float s = 0.f;
+// The thread's rows of one or two tensors, U at a time: begin() requests the first U, run() hands every row's chunks to
+// f(chunk of a, chunk of b, row) with the next U in flight. Whole chunks load without conditions, so that all U can be
+// issued before the first is needed; a last chunk with fewer channels goes row by row.
+template <typename T, int U, bool Two>
+struct RowStream {
+  const T *a, *b;
+  long long sa, sb;
+  int rows, nv, batches;
+  Chunk<T> ca[U], cb[U];
+
+  __device__ __forceinline__ void get(const T* pa, const T* pb, Chunk<T>& x, Chunk<T>& y) const {
+    __builtin_memcpy(x.v, pa, 16);
+    if (Two) __builtin_memcpy(y.v, pb, 16);
+  }
+  __device__ __forceinline__ void begin(const T* a_, long long sa_, const T* b_, long long sb_, int rows_, int nv_) {
+    a = a_; sa = sa_; b = b_; sb = sb_; rows = rows_; nv = nv_;
+    batches = nv == kV<T> ? rows / U : 0;
+    if (batches > 0) {
 #pragma unroll
-      for (int j = 0; j < kV<T>; ++j) s += v[j];
-      red[p.cc * n.RT + p.rt] = s;
+      for (int u = 0; u < U; ++u) get(a + u * sa, b + u * sb, ca[u], cb[u]);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void run(F&& f) {
+    for (int i = 0; i < batches; ++i) {
+      Chunk<T> na[U], nb[U];
+      a += U * sa;
+      if (Two) b += U * sb;
+      if (i + 1 < batches) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) get(a + u * sa, b + u * sb, na[u], nb[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(ca[u], cb[u], i * U + u);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        ca[u] = na[u];
+        if (Two) cb[u] = nb[u];
+      }
+    }
+#pragma unroll 1
+    for (int i = batches * U; i < rows; ++i, a += sa, b += Two ? sb : 0)
+      f(load_chunk(a, nv), Two ? load_chunk(b, nv) : Chunk<T>{}, i);
+  }
+};
+
+// Entries of a group in LDS, one after another: (chunk, rt) where no chunk meets two groups, else (channel, rt).
+struct Entries {
+  bool whole;
+  int per, n;   // entries of a chunk (1 or V); of a group
+};
+template <typename T>
+__device__ __forceinline__ Entries entries(const Norm& n) {
+  const bool whole = n.Cg % kV<T> == 0 || n.tpg > 1;
+  return {whole, whole ? 1 : kV<T>, n.tpg > 1 ? n.nch * n.RT : (whole ? n.Cg / kV<T> : n.Cg) * n.RT};
+}
+
+// f(g, mean, m2) in one lane for each group of the tile, from every thread's mean m and squared deviations q of each of its
+// channels over its `rows` positions. m2 = sum q + sum count (m - mean)^2, both sums over positive terms.
+template <typename T, typename F>
+__device__ __forceinline__ void group_stats(const Norm& n, const Place& p, float (&m)[kV<T>], float (&q)[kV<T>],
+                                            float2* red, F&& f) {
+  const Entries e = entries<T>(n);
+  if (threadIdx.x < (unsigned)(n.RT * n.nch)) {
+    if (e.whole) {
+      float s = 0.f, v = 0.f;
+#pragma unroll
+      for (int j = 0; j < kV<T>; ++j) s += j < p.nv ? m[j] : 0.f;
+      s = p.nv > 0 ? s / p.nv : 0.f;
+#pragma unroll
+      for (int j = 0; j < kV<T>; ++j) {
+        const float d = m[j] - s;
+        v += j < p.nv ? fmaf((float)p.rows * d, d, q[j]) : 0.f;
+      }
+      red[p.cc * n.RT + p.rt] = make_float2(s, v);
     } else {
 #pragma unroll
-      for (int j = 0; j < kV<T>; ++j) red[(p.cc * kV<T> + j) * n.RT + p.rt] = v[j];
+      for (int j = 0; j < kV<T>; ++j) red[(p.cc * kV<T> + j) * n.RT + p.rt] = make_float2(m[j], q[j]);
     }
   }
   __syncthreads();
-  const int seg = n.tpg > 1 ? n.nch * n.RT : (whole ? n.Cg / kV<T> : n.Cg) * n.RT;
+  const float inv = 1.f / ((float)(p.hi - p.lo) * (float)(n.tpg == 1 ? n.Cg : p.ct));
   const int lane = threadIdx.x & 63;
-  for (int g = threadIdx.x >> 6; g < ng; g += kThreads / 64) {
+  for (int g = threadIdx.x >> 6; g < p.ng; g += kThreads / 64) {
+    // an entry's values: its row count times its channels
+    auto count = [&](int k) {
+      const int at = k / n.RT, rows = rows_of(p.lo, p.hi, k - at * n.RT, n.RT);
+      return (float)rows * (float)(e.whole ? max(0, min(kV<T>, p.ct - at * kV<T>)) : 1);
+    };
     float s = 0.f;
-    for (int e = lane; e < seg; e += 64) s += red[g * seg + e];
-    s = wave_sum(s);
-    if (lane == 0) out[g] = s;
+    for (int k = g * e.n + lane; k < (g + 1) * e.n; k += 64) s = fmaf(count(k), red[k].x, s);
+    const float mean = wave_sum(s) * inv;
+    float v = 0.f;
+    for (int k = g * e.n + lane; k < (g + 1) * e.n; k += 64) {
+      const float d = red[k].x - mean;
+      v += fmaf(count(k) * d, d, red[k].y);
+    }
+    v = wave_sum(v);
+    if (lane == 0) f(g, mean, v);
   }
-  __syncthreads();
-}
-
-__device__ __forceinline__ long long rows_of(long long lo, long long hi, int rt, int RT) {
-  const long long r = hi - lo - rt;
-  return r <= 0 ? 0 : (r + RT - 1) / RT;
 }
 
 template <typename T, int A, bool First>
@@ -109,146 +183,123 @@ __device__ __forceinline__ T post(float u, float mean, float a, float b) {
   return (T)(First ? z : act_fwd<A, T>(z));
 }
 
-// Per-channel scale (rstd w) and shift of a thread's chunk, and its groups' means.
+// Parameters of the thread's channels, `none` where there are none.
 template <typename T>
-__device__ __forceinline__ void affine(const Norm& n, const Place& p, const float* gmean, const float* grstd,
-                                       const float* w, const float* b, float* m, float* a, float* s) {
+__device__ __forceinline__ void params(const float* w, const Place& p, float none, float (&o)[kV<T>]) {
 #pragma unroll
-  for (int j = 0; j < kV<T>; ++j) {
-    const bool in = p.on && j < p.nv;
-    const int g = in ? group_of(n, p, j) : 0;
-    m[j] = gmean[g];
-    a[j] = in ? (w ? w[p.c + j] : 1.f) * grstd[g] : 0.f;
-    s[j] = in && b ? b[p.c + j] : 0.f;
+  for (int j = 0; j < kV<T>; ++j) o[j] = none;
+  if (w && p.nv == kV<T>) {
+    __builtin_memcpy(o, w + p.c, sizeof(o));
+  } else if (w) {
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j)
+      if (j < p.nv) o[j] = w[p.c + j];
   }
 }
 
-// Statistics and result in one launch, one workgroup per image and tile of whole groups: x stays in registers between
-// the two sums (the mean, then the squared deviations from it) and the result.
-template <typename T, int A, bool First>
+// Statistics and result in one launch, one workgroup per image and tile of whole groups: x stays in registers between the
+// statistics (each thread's own mean and deviations, joined per group) and the result.
+template <typename T, int A, bool First, int Keep>
 __global__ __launch_bounds__(kThreads) void k_norm_whole(Norm n, const T* __restrict__ x, const float* __restrict__ w,
                                                          const float* __restrict__ b, T* __restrict__ y,
                                                          float* __restrict__ mean, float* __restrict__ rstd) {
-  __shared__ float red[kThreads * kV<T>], gm[kThreads * kV<T>], gr[kThreads * kV<T>];
+  __shared__ float2 red[kThreads * kV<T>];
+  __shared__ float gm[kTile], gr[kTile];
   const int img = blockIdx.y;
-  const Place p = place<T>(n, blockIdx.x);
-  int g0;
-  const int ng = tile_groups(n, p, &g0);
-  const int rows = p.on ? (int)rows_of(0, n.L, p.rt, n.RT) : 0;
+  const Place p = place<T>(n, blockIdx.x, 0);
   const T* xp = x + (long long)img * n.xsb + (long long)p.rt * n.xsl + p.c;
-  Chunk<T> keep[kKeep];
-  float v[kV<T>] = {};
+  Chunk<T> keep[Keep];
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    if (i < rows) keep[i] = load_chunk(xp + (long long)i * n.RT * n.xsl, p.nv);
-  }
+  for (int i = 0; i < Keep; ++i)
+    if (i < p.rows) keep[i] = load_chunk(xp + (long long)i * n.RT * n.xsl, p.nv);
+  float wj[kV<T>], bj[kV<T>], m[kV<T>] = {}, q[kV<T>] = {};
+  params<T>(w, p, 1.f, wj);
+  params<T>(b, p, 0.f, bj);
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    if (i < rows) {
+  for (int i = 0; i < Keep; ++i) {
+    if (i < p.rows) {
 #pragma unroll
-      for (int j = 0; j < kV<T>; ++j)
-        if (j < p.nv) v[j] += pre<T, A, First>(keep[i].v[j]);
+      for (int j = 0; j < kV<T>; ++j) m[j] += pre<T, A, First>(keep[i].v[j]);
     }
   }
-  const float inv = 1.f / ((float)n.L * (float)n.Cg);
-  group_sums<T>(n, p, ng, v, red, gm);
-  for (int g = threadIdx.x; g < ng; g += kThreads) gm[g] *= inv;
-  __syncthreads();
+  const float inv = p.rows > 0 ? 1.f / (float)p.rows : 0.f;
 #pragma unroll
-  for (int j = 0; j < kV<T>; ++j) v[j] = 0.f;
+  for (int j = 0; j < kV<T>; ++j) m[j] *= inv;
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    if (i < rows) {
+  for (int i = 0; i < Keep; ++i) {
+    if (i < p.rows) {
 #pragma unroll
       for (int j = 0; j < kV<T>; ++j) {
-        if (j < p.nv) {
-          const float d = pre<T, A, First>(keep[i].v[j]) - gm[group_of(n, p, j)];
-          v[j] = fmaf(d, d, v[j]);
-        }
+        const float d = pre<T, A, First>(keep[i].v[j]) - m[j];
+        q[j] = fmaf(d, d, q[j]);
       }
     }
   }
-  group_sums<T>(n, p, ng, v, red, gr);
-  for (int g = threadIdx.x; g < ng; g += kThreads) {
-    const float r = 1.f / sqrtf(gr[g] * inv + n.eps);
+  const float ivar = 1.f / ((float)n.L * (float)n.Cg);
+  group_stats<T>(n, p, m, q, red, [&](int g, float mu, float m2) {
+    const float r = 1.f / sqrtf(fmaf(m2, ivar, n.eps));
+    gm[g] = mu;
     gr[g] = r;
     if (mean) {
-      mean[(long long)img * n.G + g0 + g] = gm[g];
-      rstd[(long long)img * n.G + g0 + g] = r;
+      mean[(long long)img * n.G + p.g0 + g] = mu;
+      rstd[(long long)img * n.G + p.g0 + g] = r;
     }
-  }
+  });
   __syncthreads();
-  float m[kV<T>], a[kV<T>], s[kV<T>];
-  affine<T>(n, p, gm, gr, w, b, m, a, s);
+#pragma unroll
+  for (int j = 0; j < kV<T>; ++j) {
+    const int g = j < p.nv ? group_of(n, p, j) : 0;
+    m[j] = gm[g];
+    wj[j] *= gr[g];
+  }
   T* yp = y + ((long long)img * n.L + p.rt) * n.C + p.c;
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    if (i < rows) {
+  for (int i = 0; i < Keep; ++i) {
+    if (i < p.rows) {
       Chunk<T> o;
 #pragma unroll
-      for (int j = 0; j < kV<T>; ++j) o.v[j] = post<T, A, First>(pre<T, A, First>(keep[i].v[j]), m[j], a[j], s[j]);
+      for (int j = 0; j < kV<T>; ++j) o.v[j] = post<T, A, First>(pre<T, A, First>(keep[i].v[j]), m[j], wj[j], bj[j]);
       store_chunk(yp + (long long)i * n.RT * n.C, o, p.nv);
     }
   }
 }
 
-// Partial statistics of one range: (count, mean, squared deviations from it) per group. Each thread's sums are taken
-// about its own first value of the channel, so that a mean far from zero costs no digits.
+// Partial statistics of one range: (count, mean, squared deviations from it) per group. Each thread's sums are taken about
+// its own first value of the channel, so that a mean far from zero costs no digits.
 template <typename T, int A, bool First>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(Norm n, const T* __restrict__ x, float* __restrict__ part) {
-  __shared__ float red[kThreads * kV<T>], gm[kThreads * kV<T>], gq[kThreads * kV<T>];
+  __shared__ float2 red[kThreads * kV<T>];
   const int img = blockIdx.z, split = blockIdx.x;
-  const Place p = place<T>(n, blockIdx.y);
-  int g0;
-  const int ng = tile_groups(n, p, &g0);
-  const long long lo = (long long)split * n.per, hi = min(n.L, lo + n.per);
-  const int rows = p.on ? (int)rows_of(lo, hi, p.rt, n.RT) : 0;
-  const T* xp = x + (long long)img * n.xsb + (lo + p.rt) * n.xsl + p.c;
-  const long long step = (long long)n.RT * n.xsl;
-  float k0[kV<T>], s[kV<T>] = {}, q[kV<T>] = {};
-  if (rows > 0) {
-    const Chunk<T> c = load_chunk(xp, p.nv);
+  const Place p = place<T>(n, blockIdx.y, split);
+  RowStream<T, 4, false> xs;
+  xs.begin(x + (long long)img * n.xsb + (p.lo + p.rt) * n.xsl + p.c, n.RT * n.xsl, nullptr, 0, p.rows, p.nv);
+  float k0[kV<T>] = {}, s[kV<T>] = {}, q[kV<T>] = {};
+  xs.run([&](const Chunk<T>& d, const Chunk<T>&, int i) {
+    if (i == 0) {
 #pragma unroll
-    for (int j = 0; j < kV<T>; ++j) k0[j] = pre<T, A, First>(c.v[j]);
-#pragma unroll 4
-    for (int i = 1; i < rows; ++i) {
-      const Chunk<T> d = load_chunk(xp + i * step, p.nv);
-#pragma unroll
-      for (int j = 0; j < kV<T>; ++j) {
-        const float u = pre<T, A, First>(d.v[j]) - k0[j];
-        s[j] += u;
-        q[j] = fmaf(u, u, q[j]);
-      }
+      for (int j = 0; j < kV<T>; ++j) k0[j] = pre<T, A, First>(d.v[j]);
     }
-  }
-  const float cnt = (float)rows, icnt = rows > 0 ? 1.f / cnt : 0.f;
-  float v[kV<T>];
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j) {
+      const float u = pre<T, A, First>(d.v[j]) - k0[j];
+      s[j] += u;
+      q[j] = fmaf(u, u, q[j]);
+    }
+  });
+  const float inv = p.rows > 0 ? 1.f / (float)p.rows : 0.f;
 #pragma unroll
   for (int j = 0; j < kV<T>; ++j) {
-    const bool in = rows > 0 && j < p.nv;
-    k0[j] = in ? fmaf(s[j], icnt, k0[j]) : 0.f;                // the thread's mean
-    q[j] = in ? fmaxf(q[j] - s[j] * s[j] * icnt, 0.f) : 0.f;   // its squared deviations (NaN: below)
-    if (in && s[j] != s[j]) q[j] = s[j];
-    v[j] = in ? cnt * k0[j] : 0.f;
+    const float d = fmaf(-s[j] * inv, s[j], q[j]);
+    q[j] = d > 0.f || d != d ? d : 0.f;   // rounding may leave less than zero; NaN stays
+    k0[j] = fmaf(s[j], inv, k0[j]);
   }
-  group_sums<T>(n, p, ng, v, red, gm);
-  const float total = (float)(hi - lo) * (float)(n.tpg == 1 ? n.Cg : p.ct);
-  for (int g = threadIdx.x; g < ng; g += kThreads) gm[g] /= total;
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kV<T>; ++j) {
-    const bool in = rows > 0 && j < p.nv;
-    const float d = in ? k0[j] - gm[group_of(n, p, j)] : 0.f;
-    v[j] = in ? fmaf(cnt * d, d, q[j]) : 0.f;
-  }
-  group_sums<T>(n, p, ng, v, red, gq);
   const int slots = n.splits * n.tpg, slot = split * n.tpg + (n.tpg > 1 ? blockIdx.y % n.tpg : 0);
-  for (int g = threadIdx.x; g < ng; g += kThreads) {
-    float* o = part + 3 * (((long long)img * n.G + g0 + g) * slots + slot);
-    o[0] = total;
-    o[1] = gm[g];
-    o[2] = gq[g];
-  }
+  group_stats<T>(n, p, k0, q, red, [&](int g, float mu, float m2) {
+    float* o = part + 3 * (((long long)img * n.G + p.g0 + g) * slots + slot);
+    o[0] = (float)(p.hi - p.lo) * (float)(n.tpg == 1 ? n.Cg : p.ct);
+    o[1] = mu;
+    o[2] = m2;
+  });
 }
 
 // Joins the partial statistics of the tile's groups (one wave a group), then writes the result of one range.
@@ -257,50 +308,54 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(Norm n, const T* __rest
                                                          const float* __restrict__ b, const float* __restrict__ part,
                                                          T* __restrict__ y, float* __restrict__ mean,
                                                          float* __restrict__ rstd) {
-  __shared__ float gm[kThreads * kV<T>], gr[kThreads * kV<T>];
+  __shared__ float gm[kTile], gr[kTile];
   const int img = blockIdx.z, split = blockIdx.x;
-  const Place p = place<T>(n, blockIdx.y);
-  int g0;
-  const int ng = tile_groups(n, p, &g0);
+  const Place p = place<T>(n, blockIdx.y, split);
+  RowStream<T, 4, false> xs;
+  xs.begin(x + (long long)img * n.xsb + (p.lo + p.rt) * n.xsl + p.c, n.RT * n.xsl, nullptr, 0, p.rows, p.nv);
+  float wj[kV<T>], bj[kV<T>], m[kV<T>];
+  params<T>(w, p, 1.f, wj);
+  params<T>(b, p, 0.f, bj);
   const int slots = n.splits * n.tpg;
   const int lane = threadIdx.x & 63;
   const float inv = 1.f / ((float)n.L * (float)n.Cg);
-  for (int g = threadIdx.x >> 6; g < ng; g += kThreads / 64) {
-    const float* o = part + 3 * ((long long)img * n.G + g0 + g) * slots;
+  for (int g = threadIdx.x >> 6; g < p.ng; g += kThreads / 64) {
+    const float* o = part + 3 * ((long long)img * n.G + p.g0 + g) * slots;
     float s = 0.f;
+#pragma unroll 4
     for (int e = lane; e < slots; e += 64) s = fmaf(o[3 * e], o[3 * e + 1], s);
-    const float m = wave_sum(s) * inv;
+    const float mu = wave_sum(s) * inv;
     float q = 0.f;
+#pragma unroll 4
     for (int e = lane; e < slots; e += 64) {
-      const float d = o[3 * e + 1] - m;
+      const float d = o[3 * e + 1] - mu;
       q += fmaf(o[3 * e] * d, d, o[3 * e + 2]);
     }
-    const float r = 1.f / sqrtf(wave_sum(q) * inv + n.eps);
+    const float r = 1.f / sqrtf(fmaf(wave_sum(q), inv, n.eps));
     if (lane == 0) {
-      gm[g] = m;
+      gm[g] = mu;
       gr[g] = r;
       if (mean && split == 0 && (n.tpg == 1 || blockIdx.y % n.tpg == 0)) {
-        mean[(long long)img * n.G + g0 + g] = m;
-        rstd[(long long)img * n.G + g0 + g] = r;
+        mean[(long long)img * n.G + p.g0 + g] = mu;
+        rstd[(long long)img * n.G + p.g0 + g] = r;
       }
     }
   }
   __syncthreads();
-  const long long lo = (long long)split * n.per, hi = min(n.L, lo + n.per);
-  const int rows = p.on ? (int)rows_of(lo, hi, p.rt, n.RT) : 0;
-  float m[kV<T>], a[kV<T>], s[kV<T>];
-  affine<T>(n, p, gm, gr, w, b, m, a, s);
-  const T* xp = x + (long long)img * n.xsb + (lo + p.rt) * n.xsl + p.c;
-  T* yp = y + ((long long)img * n.L + lo + p.rt) * n.C + p.c;
-  const long long step = (long long)n.RT * n.xsl, ystep = (long long)n.RT * n.C;
-#pragma unroll 4
-  for (int i = 0; i < rows; ++i) {
-    const Chunk<T> c = load_chunk(xp + i * step, p.nv);
+#pragma unroll
+  for (int j = 0; j < kV<T>; ++j) {
+    const int g = j < p.nv ? group_of(n, p, j) : 0;
+    m[j] = gm[g];
+    wj[j] *= gr[g];
+  }
+  T* yp = y + ((long long)img * n.L + p.lo + p.rt) * n.C + p.c;
+  const long long ystep = (long long)n.RT * n.C;
+  xs.run([&](const Chunk<T>& c, const Chunk<T>&, int i) {
     Chunk<T> o;
 #pragma unroll
-    for (int j = 0; j < kV<T>; ++j) o.v[j] = post<T, A, First>(pre<T, A, First>(c.v[j]), m[j], a[j], s[j]);
+    for (int j = 0; j < kV<T>; ++j) o.v[j] = post<T, A, First>(pre<T, A, First>(c.v[j]), m[j], wj[j], bj[j]);
     store_chunk(yp + i * ystep, o, p.nv);
-  }
+  });
 }
 
 // g = dL/dz at the norm's output z (before the activation where that comes after), and the normalised input.
@@ -316,6 +371,18 @@ __device__ __forceinline__ float rounded_product_less(float a, float b, float c)
   return p - c;
 }
 
+// Means and inverse deviations of the groups of the thread's channels.
+template <typename T>
+__device__ __forceinline__ void group_params(const Norm& n, const Place& p, int img, const float* mean, const float* rstd,
+                                             float (&m)[kV<T>], float (&r)[kV<T>]) {
+#pragma unroll
+  for (int j = 0; j < kV<T>; ++j) {
+    const long long g = (long long)img * n.G + p.g0 + (j < p.nv ? group_of(n, p, j) : 0);
+    m[j] = mean[g];
+    r[j] = rstd[g];
+  }
+}
+
 // Backward sums of one range: per channel sum g and sum g uhat (`cpart`, for the parameters), per group the same weighted
 // by w (`gpart`, for dx).
 template <typename T, int A, bool First>
@@ -324,75 +391,73 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_sums(Norm n, const T* __r
                                                             const float* __restrict__ mean,
                                                             const float* __restrict__ rstd, float* __restrict__ cpart,
                                                             float* __restrict__ gpart) {
-  __shared__ float red[kThreads * kV<T>], ga[kThreads * kV<T>], gb[kThreads * kV<T>];
+  __shared__ float2 red[kThreads * kV<T>], chan[kTile];
   const int img = blockIdx.z, split = blockIdx.x;
-  const Place p = place<T>(n, blockIdx.y);
-  int g0;
-  const int ng = tile_groups(n, p, &g0);
-  const long long lo = (long long)split * n.per, hi = min(n.L, lo + n.per);
-  const int rows = p.on ? (int)rows_of(lo, hi, p.rt, n.RT) : 0;
+  const Place p = place<T>(n, blockIdx.y, split);
+  RowStream<T, 2, true> xs;
+  xs.begin(x + (long long)img * n.xsb + (p.lo + p.rt) * n.xsl + p.c, n.RT * n.xsl,
+           dy + (long long)img * n.gsb + (p.lo + p.rt) * n.gsl + p.c, n.RT * n.gsl, p.rows, p.nv);
   float m[kV<T>], r[kV<T>], wj[kV<T>], bj[kV<T>], sa[kV<T>] = {}, sb[kV<T>] = {};
-#pragma unroll
-  for (int j = 0; j < kV<T>; ++j) {
-    const bool in = p.on && j < p.nv;
-    const long long g = (long long)img * n.G + g0 + (in ? group_of(n, p, j) : 0);
-    m[j] = mean[g];
-    r[j] = rstd[g];
-    wj[j] = in && w ? w[p.c + j] : 1.f;
-    bj[j] = in && b ? b[p.c + j] : 0.f;
-  }
-  const T* xp = x + (long long)img * n.xsb + (lo + p.rt) * n.xsl + p.c;
-  const T* gp = dy + (long long)img * n.gsb + (lo + p.rt) * n.gsl + p.c;
-  const long long step = (long long)n.RT * n.xsl, gstep = (long long)n.RT * n.gsl;
-#pragma unroll 2
-  for (int i = 0; i < rows; ++i) {
-    const Chunk<T> c = load_chunk(xp + i * step, p.nv), d = load_chunk(gp + i * gstep, p.nv);
+  group_params<T>(n, p, img, mean, rstd, m, r);
+  params<T>(w, p, 1.f, wj);
+  params<T>(b, p, 0.f, bj);
+  xs.run([&](const Chunk<T>& c, const Chunk<T>& d, int) {
 #pragma unroll
     for (int j = 0; j < kV<T>; ++j) {
-      if (j < p.nv) {
-        const float uh = (pre<T, A, First>(c.v[j]) - m[j]) * r[j];
-        const float g = grad_at<T, A, First>((float)d.v[j], uh, wj[j], bj[j]);
-        sa[j] += g;
-        sb[j] = fmaf(g, uh, sb[j]);
+      const float uh = (pre<T, A, First>(c.v[j]) - m[j]) * r[j];
+      const float g = grad_at<T, A, First>((float)d.v[j], uh, wj[j], bj[j]);
+      sa[j] += g;
+      sb[j] = fmaf(g, uh, sb[j]);
+    }
+  });
+  // per channel over the workgroup's positions (channel-major in LDS, 8 lanes a channel where they suffice), then per group
+  if (threadIdx.x < (unsigned)(n.RT * n.nch)) {
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j) red[(p.cc * kV<T> + j) * n.RT + p.rt] = make_float2(sa[j], sb[j]);
+  }
+  __syncthreads();
+  const int lanes = n.RT >= 8 ? 8 : 1;
+  for (int e = threadIdx.x; e < (p.ct * lanes + 63) / 64 * 64; e += kThreads) {
+    const int c = e / lanes;
+    float2 s = make_float2(0.f, 0.f);
+    if (c < p.ct) {
+      for (int k = e % lanes; k < n.RT; k += lanes) {
+        const float2 v = red[c * n.RT + k];
+        s.x += v.x;
+        s.y += v.y;
       }
     }
-  }
-  // per channel, over the workgroup's positions: channel-major in LDS, a few lanes a channel
-  const int lanes = p.ct * 8 <= kThreads ? 8 : 1;
+    if (lanes == 8) {
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {
-    __syncthreads();
-    if (threadIdx.x < (unsigned)(n.RT * n.nch)) {
-#pragma unroll
-      for (int j = 0; j < kV<T>; ++j) red[(p.cc * kV<T> + j) * n.RT + p.rt] = pass ? sb[j] : sa[j];
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < (p.ct * lanes + 63) / 64 * 64; e += kThreads) {
-      const int c = e / lanes;
-      float s = 0.f;
-      if (c < p.ct)
-        for (int k = e % lanes; k < n.RT; k += lanes) s += red[c * n.RT + k];
-      if (lanes == 8) {
-        s += __shfl_xor(s, 1, 64);
-        s += __shfl_xor(s, 2, 64);
-        s += __shfl_xor(s, 4, 64);
+      for (int d = 1; d < 8; d <<= 1) {
+        s.x += __shfl_xor(s.x, d, 64);
+        s.y += __shfl_xor(s.y, d, 64);
       }
-      if (c < p.ct && e % lanes == 0)
-        cpart[(((long long)img * n.splits + split) * 2 + pass) * n.C + p.c0 + c] = s;
+    }
+    if (c < p.ct && e % lanes == 0) {
+      float* o = cpart + ((long long)img * n.splits + split) * 2 * n.C + p.c0 + c;
+      o[0] = s.x;
+      o[n.C] = s.y;
+      const float wc = w ? w[p.c0 + c] : 1.f;
+      chan[c] = make_float2(wc * s.x, wc * s.y);
     }
   }
-  float v[kV<T>];
-#pragma unroll
-  for (int j = 0; j < kV<T>; ++j) v[j] = wj[j] * sa[j];
-  group_sums<T>(n, p, ng, v, red, ga);
-#pragma unroll
-  for (int j = 0; j < kV<T>; ++j) v[j] = wj[j] * sb[j];
-  group_sums<T>(n, p, ng, v, red, gb);
+  __syncthreads();
   const int slots = n.splits * n.tpg, slot = split * n.tpg + (n.tpg > 1 ? blockIdx.y % n.tpg : 0);
-  for (int g = threadIdx.x; g < ng; g += kThreads) {
-    float* o = gpart + 2 * (((long long)img * n.G + g0 + g) * slots + slot);
-    o[0] = ga[g];
-    o[1] = gb[g];
+  const int wide = n.tpg > 1 ? p.ct : n.Cg, lane = threadIdx.x & 63;
+  for (int g = threadIdx.x >> 6; g < p.ng; g += kThreads / 64) {
+    float a = 0.f, q = 0.f;
+    for (int c = lane; c < wide; c += 64) {
+      a += chan[g * wide + c].x;
+      q += chan[g * wide + c].y;
+    }
+    a = wave_sum(a);
+    q = wave_sum(q);
+    if (lane == 0) {
+      float* o = gpart + 2 * (((long long)img * n.G + p.g0 + g) * slots + slot);
+      o[0] = a;
+      o[1] = q;
+    }
   }
 }
 
@@ -405,7 +470,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
                                                              const float* __restrict__ cpart,
                                                              const float* __restrict__ gpart, T* __restrict__ dx,
                                                              float* __restrict__ dw, float* __restrict__ db) {
-  __shared__ float ga[kThreads * kV<T>], gb[kThreads * kV<T>];
+  __shared__ float ga[kTile], gb[kTile];
   const int img = blockIdx.z;
   if (img == n.B) {
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, nrow = kThreads / 32;
@@ -414,6 +479,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
       float a = 0.f, q = 0.f;
       if (c < n.C) {
         const long long R = (long long)n.B * n.splits;
+#pragma unroll 4
         for (long long i = row; i < R; i += nrow) {
           a += cpart[2 * i * n.C + c];
           q += cpart[(2 * i + 1) * n.C + c];
@@ -435,15 +501,21 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
     return;
   }
   const int split = blockIdx.x;
-  const Place p = place<T>(n, blockIdx.y);
-  int g0;
-  const int ng = tile_groups(n, p, &g0);
+  const Place p = place<T>(n, blockIdx.y, split);
+  RowStream<T, 2, true> xs;
+  xs.begin(x + (long long)img * n.xsb + (p.lo + p.rt) * n.xsl + p.c, n.RT * n.xsl,
+           dy + (long long)img * n.gsb + (p.lo + p.rt) * n.gsl + p.c, n.RT * n.gsl, p.rows, p.nv);
+  float m[kV<T>], r[kV<T>], wj[kV<T>], bj[kV<T>], s1[kV<T>], s2[kV<T>];
+  group_params<T>(n, p, img, mean, rstd, m, r);
+  params<T>(w, p, 1.f, wj);
+  params<T>(b, p, 0.f, bj);
   const int slots = n.splits * n.tpg;
   const int lane = threadIdx.x & 63;
   const float inv = 1.f / ((float)n.L * (float)n.Cg);
-  for (int g = threadIdx.x >> 6; g < ng; g += kThreads / 64) {
-    const float* o = gpart + 2 * ((long long)img * n.G + g0 + g) * slots;
+  for (int g = threadIdx.x >> 6; g < p.ng; g += kThreads / 64) {
+    const float* o = gpart + 2 * ((long long)img * n.G + p.g0 + g) * slots;
     float s = 0.f, q = 0.f;
+#pragma unroll 4
     for (int e = lane; e < slots; e += 64) {
       s += o[2 * e];
       q += o[2 * e + 1];
@@ -456,39 +528,25 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
     }
   }
   __syncthreads();
-  const long long lo = (long long)split * n.per, hi = min(n.L, lo + n.per);
-  const int rows = p.on ? (int)rows_of(lo, hi, p.rt, n.RT) : 0;
-  float m[kV<T>], r[kV<T>], wj[kV<T>], bj[kV<T>], s1[kV<T>], s2[kV<T>];
 #pragma unroll
   for (int j = 0; j < kV<T>; ++j) {
-    const bool in = p.on && j < p.nv;
-    const int gl = in ? group_of(n, p, j) : 0;
-    const long long g = (long long)img * n.G + g0 + gl;
-    m[j] = mean[g];
-    r[j] = rstd[g];
-    wj[j] = in && w ? w[p.c + j] : 1.f;
-    bj[j] = in && b ? b[p.c + j] : 0.f;
-    s1[j] = ga[gl];
-    s2[j] = gb[gl];
+    const int g = j < p.nv ? group_of(n, p, j) : 0;
+    s1[j] = ga[g];
+    s2[j] = gb[g];
   }
-  const T* xp = x + (long long)img * n.xsb + (lo + p.rt) * n.xsl + p.c;
-  const T* gp = dy + (long long)img * n.gsb + (lo + p.rt) * n.gsl + p.c;
-  T* op = dx + ((long long)img * n.L + lo + p.rt) * n.C + p.c;
-  const long long step = (long long)n.RT * n.xsl, gstep = (long long)n.RT * n.gsl, ostep = (long long)n.RT * n.C;
-#pragma unroll 2
-  for (int i = 0; i < rows; ++i) {
-    const Chunk<T> c = load_chunk(xp + i * step, p.nv), d = load_chunk(gp + i * gstep, p.nv);
+  T* op = dx + ((long long)img * n.L + p.lo + p.rt) * n.C + p.c;
+  const long long ostep = (long long)n.RT * n.C;
+  xs.run([&](const Chunk<T>& c, const Chunk<T>& d, int i) {
     Chunk<T> o;
 #pragma unroll
     for (int j = 0; j < kV<T>; ++j) {
-      const float xv = (float)c.v[j];
       const float uh = (pre<T, A, First>(c.v[j]) - m[j]) * r[j];
       const float du = r[j] * (rounded_product_less(grad_at<T, A, First>((float)d.v[j], uh, wj[j], bj[j]), wj[j], s1[j]) -
                                uh * s2[j]);
-      o.v[j] = (T)(First ? du * act_grad<A, T>(xv) : du);
+      o.v[j] = (T)(First ? du * act_grad<A, T>((float)c.v[j]) : du);
     }
     store_chunk(op + i * ostep, o, p.nv);
-  }
+  });
 }
 
 // The launch geometry of a call. whole: one workgroup holds its groups' values in registers.
@@ -497,7 +555,7 @@ Norm plan(int B, long long L, int C, int G, bool want_whole, bool* whole) {
   Norm n{};
   constexpr int V = kV<T>;
   n.B = B; n.L = L; n.C = C; n.G = G; n.Cg = C / G;
-  const int most = kThreads * V;   // channels that the threads of a workgroup hold at one position
+  const int most = kThreads * V < kTile ? kThreads * V : kTile;   // channels of a tile
   *whole = false;
   if (want_whole && n.Cg <= most) {
     // as few groups a workgroup as make 64-byte runs of a position's channels, for the most workgroups
@@ -527,6 +585,7 @@ Norm plan(int B, long long L, int C, int G, bool want_whole, bool* whole) {
   n.splits = (int)(want < room ? want : room);
   if (n.splits < 1) n.splits = 1;
   n.per = (L + n.splits - 1) / n.splits;
+  n.per = (n.per + 4LL * n.RT - 1) / (4LL * n.RT) * (4LL * n.RT);   // whole batches of rows
   n.splits = (int)((L + n.per - 1) / n.per);
   return n;
 }
@@ -583,7 +642,13 @@ int splat_group_norm_fwd(const void* x, long long xsb, long long xsl, const floa
       auto go = [&](auto f) {
         constexpr bool First = decltype(f)::value;
         if (whole) {
-          k_norm_whole<T, A, First><<<dim3(n.tiles, B), kThreads, 0, st>>>(n, (const T*)x, weight, bias, (T*)y, mean, rstd);
+          auto whole_of = [&](auto keep) {
+            k_norm_whole<T, A, First, decltype(keep)::value><<<dim3(n.tiles, B), kThreads, 0, st>>>(
+                n, (const T*)x, weight, bias, (T*)y, mean, rstd);
+          };
+          if (L <= 4LL * n.RT) whole_of(std::integral_constant<int, 4>{});
+          else if (L <= 8LL * n.RT) whole_of(std::integral_constant<int, 8>{});
+          else whole_of(std::integral_constant<int, kKeep>{});
         } else {
           const dim3 grid(n.splits, n.tiles, B);
           k_norm_stats<T, A, First><<<grid, kThreads, 0, st>>>(n, (const T*)x, (float*)ws);

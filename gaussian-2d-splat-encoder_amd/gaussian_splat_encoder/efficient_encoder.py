@@ -14,6 +14,10 @@ reference's, because checkpoints trained there must load strictly and produce th
   decoder of the backbone skips at fine_stride (:326-378);
 * a per-image background from the pooled stride-8 features (:272-273).
 
+Two options have no counterpart in the reference and are off by default: `channels_last` runs every stage's GELU and
+norm as one kernel and the heads' 1x1 convolutions as products with their activation, on channels-last features;
+`fine_reader_heads` lets the fine cells read the deepest map (cell_reader.py).
+
 All rendering goes through this package's HIP renderer. `stage_marks` (optional callable taking a stage name)
 is called at the stage boundaries of `forward` so a harness can time backbone / coarse render / fine head.
 """
@@ -26,6 +30,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .cell_reader import CellReader
+from .feature_ops import group_norm_act, linear_act
 from .render import render_alpha_full  # noqa: F401  (re-exported like the reference module)
 from .render_hip import render_alpha_full_triton, render_alpha_octave  # noqa: F401
 
@@ -54,6 +60,16 @@ def _conv_stage(cin: int, cout: int, k: int, norm_type: str) -> nn.Sequential:
     return nn.Sequential(nn.Conv2d(cin, cout, k, stride=2, padding=k // 2), nn.GELU(), _norm(cout, norm_type))
 
 
+def _run_stage(stage: nn.Sequential, x, channels_last: bool):
+    """A conv -> GELU -> norm stage; with channels_last the GELU and the norm are one kernel."""
+    if not channels_last:
+        return stage(x)
+    conv, _, norm = stage
+    y = conv(x).permute(0, 2, 3, 1)
+    return group_norm_act(y, norm.num_groups, norm.weight, norm.bias, norm.eps, act="gelu",
+                          act_first=True).permute(0, 3, 1, 2)
+
+
 class _Backbone(nn.Module):
     """Strided CNN returning its deepest map and the intermediate maps by stride (the fine decoder's skips)."""
 
@@ -62,6 +78,7 @@ class _Backbone(nn.Module):
         if stride not in (8, 16):
             raise ValueError(f"stride must be 8 or 16, got {stride}")
         self.stride = stride
+        self.channels_last = False
         self.stage_s2 = _conv_stage(in_ch, d // 4, 7, norm_type)
         self.stage_s4 = _conv_stage(d // 4, d // 2, 3, norm_type)
         self.stage_s8 = _conv_stage(d // 2, d, 3, norm_type)
@@ -73,7 +90,7 @@ class _Backbone(nn.Module):
         for s in (2, 4, 8, 16):
             if s > self.stride:
                 break
-            x = getattr(self, f"stage_s{s}")(x)
+            x = _run_stage(getattr(self, f"stage_s{s}"), x, self.channels_last)
             skips[s] = x
         return x, skips
 
@@ -87,12 +104,13 @@ class _UpBlock(nn.Module):
 
     def __init__(self, in_ch: int, skip_ch: int, out_ch: int, norm_type: str):
         super().__init__()
+        self.channels_last = False
         self.fuse = nn.Sequential(nn.Conv2d(in_ch + skip_ch, out_ch, 3, stride=1, padding=1), nn.GELU(),
                                   _norm(out_ch, norm_type))
 
     def forward(self, x, skip):
         up = F.interpolate(x, size=skip.shape[2:], mode="bilinear", align_corners=False)
-        return self.fuse(torch.cat([up, skip], dim=1))
+        return _run_stage(self.fuse, torch.cat([up, skip], dim=1), self.channels_last)
 
 
 class _FineDecoder(nn.Module):
@@ -151,6 +169,7 @@ class _SplatHead(nn.Module):
         self.M, self.color_dim, self.use_rotation = M, color_dim, use_rotation
         self.offset_cells = offset_cells
         self.min_opacity = min_opacity
+        self.channels_last = False
         self.mu_head = nn.Conv2d(in_ch, 2 * M, 1)
         self.scale_head = nn.Conv2d(in_ch, 2 * M, 1)
         self.color_head = nn.Conv2d(in_ch, color_dim * M, 1)
@@ -167,7 +186,35 @@ class _SplatHead(nn.Module):
         """[B, M*k, fH, fW] conv output -> [B, fH*fW*M, k] (cell-major, then slot)."""
         return t.reshape(B, M, k, fH, fW).permute(0, 3, 4, 1, 2).reshape(B, fH * fW * M, k)
 
+    @staticmethod
+    def _product(cells, conv, act):
+        """act(conv(cells)) of a 1x1 convolution on channels-last cells [B, fH, fW, C]."""
+        return linear_act(cells, conv.weight.flatten(1), conv.bias, act=act)
+
+    def _forward_channels_last(self, feat):
+        """forward on channels-last cells: an output's channels are (slot, value), so that a cell's values already lie in
+        the splats' order."""
+        B, _, fH, fW = feat.shape
+        M, n = self.M, fH * fW * self.M
+        cells = feat.permute(0, 2, 3, 1)
+        ys = torch.linspace(0.5 / fH, 1 - 0.5 / fH, fH, device=feat.device, dtype=feat.dtype)
+        xs = torch.linspace(0.5 / fW, 1 - 0.5 / fW, fW, device=feat.device, dtype=feat.dtype)
+        base = torch.stack(torch.meshgrid(ys, xs, indexing="ij"), -1).reshape(1, fH * fW, 1, 2)
+        off = self._product(cells, self.mu_head, "tanh").reshape(B, fH * fW, M, 2)
+        mu = (base + off * (self.offset_cells / max(fH, fW))).reshape(B, n, 2).clamp(0.005, 0.995)
+        ls = self._product(cells, self.scale_head, "none").reshape(B, n, 2)
+        col = self._product(cells, self.color_head, "sigmoid").reshape(B, n, self.color_dim)
+        op = self._product(cells, self.opacity_head, "sigmoid").reshape(B, n)
+        if self.min_opacity > 0.0:
+            op = self.min_opacity + (1.0 - self.min_opacity) * op
+        th = None
+        if self.use_rotation:
+            th = self._product(cells, self.theta_head, "tanh").reshape(B, n) * (math.pi / 2)
+        return {"mu": mu, "log_scale": ls, "color": col, "opacity": op, "theta": th}
+
     def forward(self, feat):
+        if self.channels_last:
+            return self._forward_channels_last(feat)
         B, _, fH, fW = feat.shape
         M = self.M
         ys = torch.linspace(0.5 / fH, 1 - 0.5 / fH, fH, device=feat.device, dtype=feat.dtype)
@@ -197,13 +244,20 @@ class EfficientGaussianEncoder(nn.Module):
                  use_grad_input=True, gaussians_per_cell=2, fine_per_cell=2, free_offset_cells=4.0,
                  coarse_scale_bias=-1.5, coarse_min_scale=0.04, fine_scale_bias=-4.0, free_scale_bias=-3.0,
                  opacity_bias=2.0, residual_grid=64, fine_stride=None, coarse_min_opacity=0.0,
-                 coarse_offset_cells=2.0, fine_offset_cells=2.0, odds=False):
+                 coarse_offset_cells=2.0, fine_offset_cells=2.0, odds=False, channels_last=False,
+                 fine_reader_heads=0):
+        """channels_last, fine_reader_heads (adaptive variant): see the module's text; both need a HIP device."""
         super().__init__()
         if variant not in ("free", "adaptive"):
             raise ValueError(f"variant must be 'free' or 'adaptive', got {variant!r}")
         if stride not in (8, 16):
             raise ValueError("the encoder supports stride 8 or 16")
+        if channels_last and norm_type != "group":
+            raise ValueError(f"channels_last needs norm_type 'group', got {norm_type!r}")
+        if fine_reader_heads and variant != "adaptive":
+            raise ValueError("fine_reader_heads needs the adaptive variant")
         self.variant = variant
+        self.channels_last = channels_last
         self.stride = stride
         self.fine_stride = fine_stride if fine_stride is not None else stride
         self.odds = odds
@@ -230,6 +284,12 @@ class EfficientGaussianEncoder(nn.Module):
             self.fine_head = _SplatHead(self.fine_decoder.out_ch + g_ch + 4, self.Mf, scale_bias=fine_scale_bias,
                                         opacity_bias=opacity_bias, offset_cells=fine_offset_cells,
                                         use_rotation=use_rotation)
+            if fine_reader_heads:
+                self.fine_reader = CellReader(self.fine_decoder.out_ch, d_feature, heads=fine_reader_heads)
+        self.reads = bool(fine_reader_heads)
+        for m in self.modules():
+            if isinstance(m, (_Backbone, _UpBlock, _SplatHead)):
+                m.channels_last = channels_last
 
     def _mark(self, name):
         if self.stage_marks is not None:
@@ -261,9 +321,15 @@ class EfficientGaussianEncoder(nn.Module):
 
     def forward(self, image, return_latents: bool = False):
         x = torch.cat([image, sobel_gradmag(image)], dim=1) if self.use_grad_input else image
+        if self.channels_last:
+            x = x.contiguous(memory_format=torch.channels_last)
         feat, skips = self.backbone(x)
         fused = self._with_grad(feat, image)
-        bg = torch.sigmoid(self.bg_head(feat.mean(dim=(2, 3))))
+        pooled = feat.mean(dim=(2, 3))
+        if self.channels_last:
+            bg = linear_act(pooled, self.bg_head.weight, self.bg_head.bias, act="sigmoid")
+        else:
+            bg = torch.sigmoid(self.bg_head(pooled))
         self._mark("backbone")
         if self.variant == "free":
             out = self.head(fused)
@@ -284,6 +350,8 @@ class EfficientGaussianEncoder(nn.Module):
         target_small = F.interpolate(image, size=(rg, rg), mode="bilinear", align_corners=False)
         cond = torch.cat([(target_small - c_render).abs(), c_render.mean(1, keepdim=True)], dim=1)
         fine_feat = self.fine_decoder(feat, skips)
+        if self.reads:
+            fine_feat = self.fine_reader(fine_feat.permute(0, 2, 3, 1), feat.permute(0, 2, 3, 1)).permute(0, 3, 1, 2)
         fsz = fine_feat.shape[2:]
         cond_fine = F.interpolate(cond, size=fsz, mode="bilinear", align_corners=False)
         fine_in = torch.cat([self._with_grad(fine_feat, image, fsz), cond_fine], dim=1)

@@ -72,7 +72,7 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lin(M=1 << 33) == 3
     assert lib.splat_linear_bwd(256, 8, 256, 256, None, 0, 4, 8, 8, 1, 256, None, None, 256, 1 << 20, None) == 1   # no z
     assert lib.splat_linear_bwd(256, 8, 256, 256, None, 0, 4, 8, 8, 0, 256, 256, None, 256, 8, None) == 5
-    a = _lib.SplatAttention(0, 1, 4, 2, 64, 0.125, 2, 3)
+    a = _lib.SplatAttention(0, 1, 4, 2, 64, 0.125, 2, 5000)   # few rows, many keys: split, so a workspace is due
     fwd = lambda: lib.splat_attention_fwd(ctypes.byref(a), 256, 256, 256, 256, None, None, 0, None)  # noqa: E731
     assert fwd() == 5
     for field, value, rc in (("H", 3, 1), ("D", 129, 3), ("D", 0, 1), ("dtype", 7, 1), ("Lk", 1 << 33, 3), ("Lq", -1, 1)):
@@ -91,7 +91,7 @@ def test_workspaces_are_what_the_plans_need():
     assert lib.splat_group_norm_workspace_bytes(0, 1, 576, 64, 8) == 0          # one launch, no partial sums
     assert lib.splat_group_norm_workspace_bytes(1, 1, 384 * 384, 64, 8) > 0
     assert lib.splat_group_norm_workspace_bytes(1, 0, 5, 64, 8) == 0
-    a = _lib.SplatAttention(1, 1, 4, 4, 64, 0.125, 36864, 9216)
-    assert lib.splat_attention_workspace_bytes(ctypes.byref(a)) == 0            # enough rows: no split
-    a.Lq = 1
+    a = _lib.SplatAttention(1, 1, 4, 4, 64, 0.125, 36864, 100)
+    assert lib.splat_attention_workspace_bytes(ctypes.byref(a)) == 0            # few keys: no split
+    a.Lq, a.Lk = 1, 92160
     assert lib.splat_attention_workspace_bytes(ctypes.byref(a)) > 0
