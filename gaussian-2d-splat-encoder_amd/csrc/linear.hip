@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
             store_chunk((T*)g.z + (long long)q * g.P + p, o, n);
           }
 #pragma unroll
-          for (int e = 0; e < V; ++e) x[e] = act_fwd<A, T>(x[e]);
+          for (int e = 0; e < V; ++e) x[e] = act_fwd<A>(x[e]);
           if (g.res) {
             const Chunk<T> rs = load_chunk((const T*)g.res + q * g.ldr + p, n);
 #pragma unroll
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
       Chunk<T> o;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float x = (float)d.v[j] * act_grad<A, T>((float)c.v[j]);
+        const float x = (float)d.v[j] * act_grad<A>((float)c.v[j]);
         s[j] += x;
         o.v[j] = (T)x;
       }

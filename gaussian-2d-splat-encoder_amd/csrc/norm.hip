@@ -174,13 +174,13 @@ __device__ __forceinline__ void group_stats(const Norm& n, const Place& p, float
 
 template <typename T, int A, bool First>
 __device__ __forceinline__ float pre(T x) {
-  return First ? act_fwd<A, T>((float)x) : (float)x;
+  return First ? act_fwd<A>((float)x) : (float)x;
 }
 
 template <typename T, int A, bool First>
 __device__ __forceinline__ T post(float u, float mean, float a, float b) {
   const float z = fmaf(u - mean, a, b);
-  return (T)(First ? z : act_fwd<A, T>(z));
+  return (T)(First ? z : act_fwd<A>(z));
 }
 
 // Parameters of the thread's channels, `none` where there are none.
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(Norm n, const T* __rest
 // g = dL/dz at the norm's output z (before the activation where that comes after), and the normalised input.
 template <typename T, int A, bool First>
 __device__ __forceinline__ float grad_at(float dy, float uhat, float wj, float bj) {
-  return First ? dy : dy * act_grad<A, T>(fmaf(uhat, wj, bj));
+  return First ? dy : dy * act_grad<A>(fmaf(uhat, wj, bj));
 }
 
 // a b - c with the product rounded by itself: a group of one value has c = round(a b), and a zero difference.
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
       const float uh = (pre<T, A, First>(c.v[j]) - m[j]) * r[j];
       const float du = r[j] * (rounded_product_less(grad_at<T, A, First>((float)d.v[j], uh, wj[j], bj[j]), wj[j], s1[j]) -
                                uh * s2[j]);
-      o.v[j] = (T)(First ? du * act_grad<A, T>((float)c.v[j]) : du);
+      o.v[j] = (T)(First ? du * act_grad<A>((float)c.v[j]) : du);
     }
     store_chunk(op + i * ostep, o, p.nv);
   });
