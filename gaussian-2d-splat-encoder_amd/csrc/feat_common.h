@@ -101,6 +101,22 @@ inline int with_act(int act, F&& f) {
   return set_error(kInvalid, "unknown activation %d", act);
 }
 
+// Sum over a wave's 64 lanes, the same in every lane, without LDS: two exchanges within four lanes, mirrors within 8 and
+// 16, swaps of rows of 16 and 32.
+__device__ __forceinline__ float wave_add(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v += dpp(v, std::integral_constant<int, 0xb1>{});    // lanes 1 0 3 2
+  v += dpp(v, std::integral_constant<int, 0x4e>{});    // lanes 2 3 0 1
+  v += dpp(v, std::integral_constant<int, 0x141>{});   // mirror within 8
+  v += dpp(v, std::integral_constant<int, 0x140>{});   // mirror within 16
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // n / d for 0 <= n < 2^31 by a multiplication, d >= 1 fixed on the host.
 struct FastDiv {
   unsigned mul, shift;

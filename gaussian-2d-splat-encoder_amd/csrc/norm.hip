@@ -26,6 +26,7 @@ struct Norm {
   int nch, RT;                       // chunks of a tile; positions a workgroup takes at a time
   int splits;                        // ranges of positions
   long long per;                     // positions of a range
+  FastDiv by_nch, by_RT, by_Cg;
   float eps;
 };
 
@@ -37,9 +38,8 @@ struct Place {
   int rows;
 };
 
-__device__ __forceinline__ int rows_of(long long lo, long long hi, int rt, int RT) {
-  const long long r = hi - lo - rt;
-  return r <= 0 ? 0 : (int)((r + RT - 1) / RT);
+__device__ __forceinline__ int rows_of(const Norm& n, int range, int rt) {
+  return range <= rt ? 0 : (range - rt + n.RT - 1) / n.by_RT;
 }
 
 template <typename T>
@@ -53,66 +53,76 @@ __device__ __forceinline__ Place place(const Norm& n, int tile, int split) {
     p.c0 = g * n.Cg + k * n.Ct;
     p.ct = min(n.Ct, n.Cg - k * n.Ct);
   }
-  p.g0 = p.c0 / n.Cg;
-  p.ng = n.tpg == 1 ? p.ct / n.Cg : 1;
-  p.rt = threadIdx.x / n.nch;
-  p.cc = threadIdx.x % n.nch;
+  p.g0 = p.c0 / n.by_Cg;
+  p.ng = n.tpg == 1 ? p.ct / n.by_Cg : 1;
+  p.rt = (int)threadIdx.x / n.by_nch;
+  p.cc = threadIdx.x - p.rt * n.nch;
   p.c = p.c0 + p.cc * kV<T>;
   p.nv = p.rt < n.RT ? max(0, min(kV<T>, p.ct - p.cc * kV<T>)) : 0;
   p.lo = (long long)split * n.per;
   p.hi = min(n.L, p.lo + n.per);
-  p.rows = p.nv > 0 ? rows_of(p.lo, p.hi, p.rt, n.RT) : 0;
+  p.rows = p.nv > 0 ? rows_of(n, (int)(p.hi - p.lo), p.rt) : 0;
   return p;
 }
 
 // Group of the thread's channel j within the tile.
 __device__ __forceinline__ int group_of(const Norm& n, const Place& p, int j) {
-  return n.tpg == 1 ? (p.c - p.c0 + j) / n.Cg : 0;
+  return n.tpg == 1 ? (p.c - p.c0 + j) / n.by_Cg : 0;
 }
 
 // The thread's rows of one or two tensors, U at a time: begin() requests the first U, run() hands every row's chunks to
-// f(chunk of a, chunk of b, row) with the next U in flight. Whole chunks load without conditions, so that all U can be
-// issued before the first is needed; a last chunk with fewer channels goes row by row.
+// f(chunk of a, chunk of b, row) with the next U in flight. Whole chunks load without conditions (the last U repeat the
+// last row where there are fewer), so that all are issued before the first is needed; a last chunk with fewer channels goes
+// row by row.
 template <typename T, int U, bool Two>
 struct RowStream {
   const T *a, *b;
   long long sa, sb;
-  int rows, nv, batches;
+  int rows, nv;
   Chunk<T> ca[U], cb[U];
 
-  __device__ __forceinline__ void get(const T* pa, const T* pb, Chunk<T>& x, Chunk<T>& y) const {
-    __builtin_memcpy(x.v, pa, 16);
-    if (Two) __builtin_memcpy(y.v, pb, 16);
+  __device__ __forceinline__ void get(int i, Chunk<T> (&x)[U], Chunk<T> (&y)[U]) const {   // rows i .. i + U - 1
+    if (i + U <= rows) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        __builtin_memcpy(x[u].v, a + (i + u) * sa, 16);
+        if (Two) __builtin_memcpy(y[u].v, b + (i + u) * sb, 16);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        __builtin_memcpy(x[u].v, a + min(i + u, rows - 1) * sa, 16);
+        if (Two) __builtin_memcpy(y[u].v, b + min(i + u, rows - 1) * sb, 16);
+      }
+    }
   }
   __device__ __forceinline__ void begin(const T* a_, long long sa_, const T* b_, long long sb_, int rows_, int nv_) {
     a = a_; sa = sa_; b = b_; sb = sb_; rows = rows_; nv = nv_;
-    batches = nv == kV<T> ? rows / U : 0;
-    if (batches > 0) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) get(a + u * sa, b + u * sb, ca[u], cb[u]);
-    }
+    if (rows > 0 && nv == kV<T>) get(0, ca, cb);
   }
   template <typename F>
   __device__ __forceinline__ void run(F&& f) {
-    for (int i = 0; i < batches; ++i) {
-      Chunk<T> na[U], nb[U];
-      a += U * sa;
-      if (Two) b += U * sb;
-      if (i + 1 < batches) {
+    if (nv == kV<T>) {
+      int i = 0;
+      for (; i + U < rows; i += U) {
+        Chunk<T> na[U], nb[U];
+        get(i + U, na, nb);
 #pragma unroll
-        for (int u = 0; u < U; ++u) get(a + u * sa, b + u * sb, na[u], nb[u]);
+        for (int u = 0; u < U; ++u) f(ca[u], cb[u], i + u);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          ca[u] = na[u];
+          if (Two) cb[u] = nb[u];
+        }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) f(ca[u], cb[u], i * U + u);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        ca[u] = na[u];
-        if (Two) cb[u] = nb[u];
-      }
-    }
+      for (int u = 0; u < U; ++u)
+        if (i + u < rows) f(ca[u], cb[u], i + u);
+    } else {
 #pragma unroll 1
-    for (int i = batches * U; i < rows; ++i, a += sa, b += Two ? sb : 0)
-      f(load_chunk(a, nv), Two ? load_chunk(b, nv) : Chunk<T>{}, i);
+      for (int i = 0; i < rows; ++i, a += sa, b += Two ? sb : 0)
+        f(load_chunk(a, nv), Two ? load_chunk(b, nv) : Chunk<T>{}, i);
+    }
   }
 };
 
@@ -156,18 +166,18 @@ __device__ __forceinline__ void group_stats(const Norm& n, const Place& p, float
   for (int g = threadIdx.x >> 6; g < p.ng; g += kThreads / 64) {
     // an entry's values: its row count times its channels
     auto count = [&](int k) {
-      const int at = k / n.RT, rows = rows_of(p.lo, p.hi, k - at * n.RT, n.RT);
+      const int at = k / n.by_RT, rows = rows_of(n, (int)(p.hi - p.lo), k - at * n.RT);
       return (float)rows * (float)(e.whole ? max(0, min(kV<T>, p.ct - at * kV<T>)) : 1);
     };
     float s = 0.f;
     for (int k = g * e.n + lane; k < (g + 1) * e.n; k += 64) s = fmaf(count(k), red[k].x, s);
-    const float mean = wave_sum(s) * inv;
+    const float mean = wave_add(s) * inv;
     float v = 0.f;
     for (int k = g * e.n + lane; k < (g + 1) * e.n; k += 64) {
       const float d = red[k].x - mean;
       v += fmaf(count(k) * d, d, red[k].y);
     }
-    v = wave_sum(v);
+    v = wave_add(v);
     if (lane == 0) f(g, mean, v);
   }
 }
@@ -267,7 +277,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_whole(Norm n, const T* __rest
 // Partial statistics of one range: (count, mean, squared deviations from it) per group. Each thread's sums are taken about
 // its own first value of the channel, so that a mean far from zero costs no digits.
 template <typename T, int A, bool First>
-__global__ __launch_bounds__(kThreads) void k_norm_stats(Norm n, const T* __restrict__ x, float* __restrict__ part) {
+__global__ __launch_bounds__(kThreads) void k_norm_stats(Norm n, const T* __restrict__ x, float4* __restrict__ part) {
   __shared__ float2 red[kThreads * kV<T>];
   const int img = blockIdx.z, split = blockIdx.x;
   const Place p = place<T>(n, blockIdx.y, split);
@@ -295,17 +305,15 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(Norm n, const T* __rest
   }
   const int slots = n.splits * n.tpg, slot = split * n.tpg + (n.tpg > 1 ? blockIdx.y % n.tpg : 0);
   group_stats<T>(n, p, k0, q, red, [&](int g, float mu, float m2) {
-    float* o = part + 3 * (((long long)img * n.G + p.g0 + g) * slots + slot);
-    o[0] = (float)(p.hi - p.lo) * (float)(n.tpg == 1 ? n.Cg : p.ct);
-    o[1] = mu;
-    o[2] = m2;
+    part[((long long)img * n.G + p.g0 + g) * slots + slot] =
+        make_float4((float)(p.hi - p.lo) * (float)(n.tpg == 1 ? n.Cg : p.ct), mu, m2, 0.f);
   });
 }
 
 // Joins the partial statistics of the tile's groups (one wave a group), then writes the result of one range.
 template <typename T, int A, bool First>
 __global__ __launch_bounds__(kThreads) void k_norm_apply(Norm n, const T* __restrict__ x, const float* __restrict__ w,
-                                                         const float* __restrict__ b, const float* __restrict__ part,
+                                                         const float* __restrict__ b, const float4* __restrict__ part,
                                                          T* __restrict__ y, float* __restrict__ mean,
                                                          float* __restrict__ rstd) {
   __shared__ float gm[kTile], gr[kTile];
@@ -320,18 +328,20 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(Norm n, const T* __rest
   const int lane = threadIdx.x & 63;
   const float inv = 1.f / ((float)n.L * (float)n.Cg);
   for (int g = threadIdx.x >> 6; g < p.ng; g += kThreads / 64) {
-    const float* o = part + 3 * ((long long)img * n.G + p.g0 + g) * slots;
-    float s = 0.f;
-#pragma unroll 4
-    for (int e = lane; e < slots; e += 64) s = fmaf(o[3 * e], o[3 * e + 1], s);
-    const float mu = wave_sum(s) * inv;
-    float q = 0.f;
+    const float4* o = part + ((long long)img * n.G + p.g0 + g) * slots;
+    float cnt = 0.f, mu = 0.f, q = 0.f;   // the lane's ranges so far
 #pragma unroll 4
     for (int e = lane; e < slots; e += 64) {
-      const float d = o[3 * e + 1] - mu;
-      q += fmaf(o[3 * e] * d, d, o[3 * e + 2]);
+      const float4 v = o[e];
+      const float d = v.y - mu, r = v.x * hw_rcp(cnt + v.x);
+      mu = fmaf(d, r, mu);
+      q += fmaf(d * d, cnt * r, v.z);
+      cnt += v.x;
     }
-    const float r = 1.f / sqrtf(fmaf(wave_sum(q), inv, n.eps));
+    const float lm = mu;
+    mu = wave_add(cnt * lm) * inv;
+    const float d = lm - mu;
+    const float r = 1.f / sqrtf(fmaf(wave_add(fmaf(cnt * d, d, q)), inv, n.eps));
     if (lane == 0) {
       gm[g] = mu;
       gr[g] = r;
@@ -451,8 +461,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_sums(Norm n, const T* __r
       a += chan[g * wide + c].x;
       q += chan[g * wide + c].y;
     }
-    a = wave_sum(a);
-    q = wave_sum(q);
+    a = wave_add(a);
+    q = wave_add(q);
     if (lane == 0) {
       float* o = gpart + 2 * (((long long)img * n.G + p.g0 + g) * slots + slot);
       o[0] = a;
@@ -520,8 +530,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
       s += o[2 * e];
       q += o[2 * e + 1];
     }
-    s = wave_sum(s);
-    q = wave_sum(q);
+    s = wave_add(s);
+    q = wave_add(q);
     if (lane == 0) {
       ga[g] = s * inv;
       gb[g] = q * inv;
@@ -555,37 +565,38 @@ Norm plan(int B, long long L, int C, int G, bool want_whole, bool* whole) {
   Norm n{};
   constexpr int V = kV<T>;
   n.B = B; n.L = L; n.C = C; n.G = G; n.Cg = C / G;
+  n.by_Cg = fast_div(n.Cg);
   const int most = kThreads * V < kTile ? kThreads * V : kTile;   // channels of a tile
+  auto tile = [&](int gpt) {   // whole groups
+    n.Ct = gpt * n.Cg; n.tpg = 1; n.tiles = (G + gpt - 1) / gpt;
+    n.nch = (n.Ct + V - 1) / V;
+    n.RT = kThreads / n.nch;
+  };
   *whole = false;
-  if (want_whole && n.Cg <= most) {
-    // as few groups a workgroup as make 64-byte runs of a position's channels, for the most workgroups
-    const int run = 64 / (int)sizeof(T);
-    const int gpt = n.Cg >= run ? 1 : (run + n.Cg - 1) / n.Cg < G ? (run + n.Cg - 1) / n.Cg : G;
-    const int nch = (gpt * n.Cg + V - 1) / V;
-    const int RT = nch <= kThreads ? kThreads / nch : 0;
-    if (RT > 0 && L <= (long long)RT * kKeep) {
-      n.Ct = gpt * n.Cg; n.tpg = 1; n.tiles = (G + gpt - 1) / gpt; n.nch = nch; n.RT = RT;
+  if (n.Cg <= most) {
+    // one launch: as few groups a workgroup as make 64-byte runs of a position's channels, for the most workgroups
+    const int run = 64 / (int)sizeof(T), gpt = (run + n.Cg - 1) / n.Cg;
+    tile(gpt < G ? gpt : G);
+    if (want_whole && L <= (long long)n.RT * kKeep) {
       n.splits = 1; n.per = L;
       *whole = true;
-      return n;
+    } else {
+      tile(most / n.Cg < G ? most / n.Cg : G);
     }
-  }
-  if (n.Cg <= most) {
-    int gpt = most / n.Cg < G ? most / n.Cg : G;
-    while (gpt > 1 && (gpt * n.Cg + V - 1) / V > kThreads) --gpt;
-    n.Ct = gpt * n.Cg; n.tpg = 1; n.tiles = (G + gpt - 1) / gpt;
   } else {
     n.Ct = most; n.tpg = (n.Cg + most - 1) / most; n.tiles = G * n.tpg;
+    n.nch = n.Ct / V;
+    n.RT = kThreads / n.nch;
   }
-  n.nch = (n.Ct + V - 1) / V;
-  n.RT = kThreads / n.nch;
-  // about 512 workgroups, two per CU, of at least four passes over their threads' positions each
+  n.by_nch = fast_div(n.nch);
+  n.by_RT = fast_div(n.RT);
+  if (*whole) return n;
+  // 512 workgroups, the two per CU that registers allow at a time, of at least a batch of rows of their threads
   const long long want = 512 / ((long long)B * n.tiles) > 0 ? 512 / ((long long)B * n.tiles) : 1;
-  const long long room = (L + 4LL * n.RT - 1) / (4LL * n.RT);
-  n.splits = (int)(want < room ? want : room);
-  if (n.splits < 1) n.splits = 1;
-  n.per = (L + n.splits - 1) / n.splits;
-  n.per = (n.per + 4LL * n.RT - 1) / (4LL * n.RT) * (4LL * n.RT);   // whole batches of rows
+  const long long batch = 4LL * n.RT;
+  n.per = (L + want - 1) / want;
+  if (n.per < batch) n.per = batch;
+  if (n.per > (1LL << 30)) n.per = 1LL << 30;   // a range's rows are counted in 32 bits
   n.splits = (int)((L + n.per - 1) / n.per);
   return n;
 }
@@ -618,7 +629,7 @@ size_t splat_group_norm_workspace_bytes(int dtype, int B, long long L, int C, in
   if (check_norm("splat_group_norm_workspace_bytes", dtype, B, L, C, G, 0) || B == 0 || L == 0) return 0;
   bool whole;
   const Norm n = plan_of(dtype, B, L, C, G, true, &whole);
-  return whole ? 0 : 3 * sizeof(float) * (size_t)B * G * n.splits * n.tpg;
+  return whole ? 0 : sizeof(float4) * (size_t)B * G * n.splits * n.tpg;
 }
 
 int splat_group_norm_fwd(const void* x, long long xsb, long long xsl, const float* weight, const float* bias, int dtype,
@@ -630,7 +641,7 @@ int splat_group_norm_fwd(const void* x, long long xsb, long long xsl, const floa
   bool whole;
   Norm n = plan_of(dtype, B, L, C, G, true, &whole);
   n.xsb = xsb; n.xsl = xsl; n.eps = eps;
-  const size_t need = whole ? 0 : 3 * sizeof(float) * (size_t)B * G * n.splits * n.tpg;
+  const size_t need = whole ? 0 : sizeof(float4) * (size_t)B * G * n.splits * n.tpg;
   if (need && (!ws || ws_bytes < need))
     return set_error(kWorkspace, "splat_group_norm_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
   if (n.tiles > 65535) return set_error(kUnsupported, "splat_group_norm_fwd: %d channel tiles", n.tiles);
@@ -651,8 +662,8 @@ int splat_group_norm_fwd(const void* x, long long xsb, long long xsl, const floa
           else whole_of(std::integral_constant<int, kKeep>{});
         } else {
           const dim3 grid(n.splits, n.tiles, B);
-          k_norm_stats<T, A, First><<<grid, kThreads, 0, st>>>(n, (const T*)x, (float*)ws);
-          k_norm_apply<T, A, First><<<grid, kThreads, 0, st>>>(n, (const T*)x, weight, bias, (const float*)ws, (T*)y, mean,
+          k_norm_stats<T, A, First><<<grid, kThreads, 0, st>>>(n, (const T*)x, (float4*)ws);
+          k_norm_apply<T, A, First><<<grid, kThreads, 0, st>>>(n, (const T*)x, weight, bias, (const float4*)ws, (T*)y, mean,
                                                                rstd);
         }
         return check_launch("splat_group_norm_fwd");
