@@ -25,19 +25,22 @@ MAX_HEAD = 128   # values of a head at most
 
 
 def _args(act, x, *others):
-    """Type and activation codes of a call; x's type is every other tensor's too."""
-    for t in (x, *others):
+    """Type and activation codes of a call; x's type and device are every other tensor's too."""
+    if not x.is_cuda:
+        raise RuntimeError("the HIP feature operators need device tensors (got a CPU tensor)")
+    dtype, dev = x.dtype, x.get_device()
+    for t in others:
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError("the HIP feature operators need device tensors (got a CPU tensor)")
-        if t.dtype is not x.dtype:
-            raise ValueError(f"tensors of one type are needed, got {x.dtype} and {t.dtype}")
-        if t.device != x.device:
+        if t.dtype is not dtype:
+            raise ValueError(f"tensors of one type are needed, got {dtype} and {t.dtype}")
+        if t.get_device() != dev:
             raise ValueError(f"tensors of one device are needed, got {x.device} and {t.device}")
-    dt = _DTYPES.get(x.dtype)
+    dt = _DTYPES.get(dtype)
     if dt is None:
-        raise ValueError(f"float32 or bfloat16 is needed, got {x.dtype}")
+        raise ValueError(f"float32 or bfloat16 is needed, got {dtype}")
     code = _ACTS.get(act)
     if code is None:
         raise ValueError(f"unknown activation {act!r}: one of {sorted(_ACTS)}")
@@ -56,22 +59,17 @@ def _scratch(nbytes, x):
     return t, t.data_ptr()
 
 
-class _On:
-    """Makes x's device current for a call where it is not (the library launches on the current device)."""
-
-    def __init__(self, x):
-        i = x.device.index
-        self.guard = None if i == torch.cuda.current_device() else torch.cuda.device(i)
-        self.index = i
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return _lib.stream_ptr(self.index)
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _launch(x, name, *args):
+    """Calls the library's entry point on the current stream of x's device (the library launches on the current device,
+    which is made x's where it is another)."""
+    fn, i = getattr(_lib.load(), name), x.get_device()
+    if i == torch._C._cuda_getDevice():
+        rc = fn(*args, _lib.stream_ptr(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, _lib.stream_ptr(i))
+    if rc:
+        check(rc, name)
 
 
 def _wants_grad(*ts):
@@ -86,30 +84,29 @@ def _positions(x):
     return x if C == 1 or x.stride(2) == 1 else x.contiguous()
 
 
-def _norm_fwd(x3, weight, bias, G, eps, dt, act, first, save):
+def _norm_fwd(x, weight, bias, G, eps, dt, act, first, save):
+    """(result like x, x as [B, L, C], statistics or None)"""
+    x3 = _positions(x)
     B, L, C = x3.shape
-    lib = _lib.load()
-    y = torch.empty((B, L, C), dtype=x3.dtype, device=x3.device)
-    stat = torch.empty((2, B, G), dtype=torch.float32, device=x3.device) if save else None
-    if y.numel():
-        with _On(x3) as stream:
-            n = lib.splat_group_norm_workspace_bytes(dt, B, L, C, G)
-            keep, ws = _scratch(n, x3)
-            sp = _ptr(stat)
-            check(lib.splat_group_norm_fwd(x3.data_ptr(), x3.stride(0), x3.stride(1), _ptr(weight), _ptr(bias), dt, B, L, C, G,
-                                           eps, act, first, y.data_ptr(), sp, sp + 4 * B * G if save else None, ws, n,
-                                           stream), "splat_group_norm_fwd")
-    return y, stat
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stat = torch.empty((2, B, G), dtype=torch.float32, device=x.device) if save else None
+    if B and L:
+        n = _lib.load().splat_group_norm_workspace_bytes(dt, B, L, C, G)
+        keep, ws = _scratch(n, x)
+        sb, sl, _ = x3.stride()
+        sp = _ptr(stat)
+        _launch(x, "splat_group_norm_fwd", x3.data_ptr(), sb, sl, _ptr(weight), _ptr(bias), dt, B, L, C, G, eps, act, first,
+                y.data_ptr(), sp, sp + 4 * B * G if save else None, ws, n)
+    return y, x3, stat
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, G, eps, dt, act, first):
-        x3 = _positions(x)
-        y, stat = _norm_fwd(x3, weight, bias, G, eps, dt, act, first, True)
+        y, x3, stat = _norm_fwd(x, weight, bias, G, eps, dt, act, first, True)
         ctx.save_for_backward(x3, weight, bias, stat)
         ctx.args = (x.shape, G, dt, act, first)
-        return y.view(x.shape)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -117,22 +114,21 @@ class _GroupNormAct(torch.autograd.Function):
         x3, weight, bias, stat = ctx.saved_tensors
         shape, G, dt, act, first = ctx.args
         B, L, C = x3.shape
-        lib = _lib.load()
-        new = torch.empty if x3.numel() else torch.zeros
-        dx = torch.empty((B, L, C), dtype=x3.dtype, device=x3.device)
-        dw = new(C, dtype=torch.float32, device=x3.device) if ctx.needs_input_grad[1] else None
-        db = new(C, dtype=torch.float32, device=x3.device) if ctx.needs_input_grad[2] else None
-        if x3.numel():
+        need = ctx.needs_input_grad
+        new = torch.empty if B and L else torch.zeros
+        dx = torch.empty(shape, dtype=x3.dtype, device=x3.device)
+        dw = new(C, dtype=torch.float32, device=x3.device) if need[1] else None
+        db = new(C, dtype=torch.float32, device=x3.device) if need[2] else None
+        if B and L:
             g3 = _positions(dy)
-            with _On(x3) as stream:
-                n = lib.splat_group_norm_bwd_workspace_bytes(dt, B, L, C, G)
-                keep, ws = _scratch(n, x3)
-                sp = stat.data_ptr()
-                check(lib.splat_group_norm_bwd(x3.data_ptr(), x3.stride(0), x3.stride(1), g3.data_ptr(), g3.stride(0),
-                                               g3.stride(1), _ptr(weight), _ptr(bias), sp, sp + 4 * B * G, dt, B, L, C, G,
-                                               act, first, dx.data_ptr(), _ptr(dw), _ptr(db), ws, n, stream),
-                      "splat_group_norm_bwd")
-        return dx.view(shape) if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None, None
+            n = _lib.load().splat_group_norm_bwd_workspace_bytes(dt, B, L, C, G)
+            keep, ws = _scratch(n, x3)
+            sp = stat.data_ptr()
+            xb, xl, _ = x3.stride()
+            gb, gl, _ = g3.stride()
+            _launch(x3, "splat_group_norm_bwd", x3.data_ptr(), xb, xl, g3.data_ptr(), gb, gl, _ptr(weight), _ptr(bias), sp,
+                    sp + 4 * B * G, dt, B, L, C, G, act, first, dx.data_ptr(), _ptr(dw), _ptr(db), ws, n)
+        return dx if need[0] else None, dw, db, None, None, None, None, None
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="gelu", act_first=False):
@@ -153,14 +149,14 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="gelu", 
         if t is not None:
             if t.shape != (C,):
                 raise ValueError(f"{name} must be [{C}], got {list(t.shape)}")
-            if t.device != x.device:
+            if t.get_device() != x.get_device():
                 raise ValueError(f"{name} is on {t.device}, x on {x.device}")
     weight = None if weight is None else weight.float().contiguous()
     bias = None if bias is None else bias.float().contiguous()
     first = 1 if act_first else 0
     if _wants_grad(x, weight, bias):
         return _GroupNormAct.apply(x, weight, bias, G, float(eps), dt, code, first)
-    return _norm_fwd(_positions(x), weight, bias, G, float(eps), dt, code, first, False)[0].view(x.shape)
+    return _norm_fwd(x, weight, bias, G, float(eps), dt, code, first, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ products
@@ -171,49 +167,47 @@ def _rows(x):
     return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
 
 
-def _linear_fwd(x2, weight, bias, r2, dt, act, save):
+def _linear_fwd(x, weight, bias, residual, dt, act, save):
+    """(result [..., N], x as [M, K], the activation's input or None)"""
+    x2 = _rows(x)
     M, K = x2.shape
     N = weight.shape[0]
-    y = torch.empty((M, N), dtype=x2.dtype, device=x2.device)
-    z = torch.empty_like(y) if save and act else None
+    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
+    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if save and act else None
     if M:
-        with _On(x2) as stream:
-            check(_lib.load().splat_linear_fwd(x2.data_ptr(), x2.stride(0), weight.data_ptr(), _ptr(bias), _ptr(r2),
-                                               0 if r2 is None else r2.stride(0), dt, M, N, K, act, y.data_ptr(), _ptr(z),
-                                               stream), "splat_linear_fwd")
-    return y, z
+        r2 = None if residual is None else _rows(residual)
+        _launch(x, "splat_linear_fwd", x2.data_ptr(), x2.stride(0), weight.data_ptr(), _ptr(bias), _ptr(r2),
+                0 if r2 is None else r2.stride(0), dt, M, N, K, act, y.data_ptr(), _ptr(z))
+    return y, x2, z
 
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, dt, act):
-        x2 = _rows(x)
-        y, z = _linear_fwd(x2, weight, bias, None if residual is None else _rows(residual), dt, act, True)
+        y, x2, z = _linear_fwd(x, weight, bias, residual, dt, act, True)
         ctx.save_for_backward(x2, weight, z)
-        ctx.args = (x.shape, dt, act, bias is not None)
-        return y.view(x.shape[:-1] + (weight.shape[0],))
+        ctx.args = (x.shape, dt, act)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x2, weight, z = ctx.saved_tensors
-        shape, dt, act, has_bias = ctx.args
+        shape, dt, act = ctx.args
         need = ctx.needs_input_grad
         M, K = x2.shape
         N = weight.shape[0]
         new = torch.empty if M else torch.zeros
-        dx = torch.empty((M, K), dtype=x2.dtype, device=x2.device) if need[0] else None
+        dx = torch.empty(shape, dtype=x2.dtype, device=x2.device) if need[0] else None
         dw = new((N, K), dtype=x2.dtype, device=x2.device) if need[1] else None
-        db = new(N, dtype=x2.dtype, device=x2.device) if need[2] and has_bias else None
-        if M and (need[0] or need[1] or db is not None):
+        db = new(N, dtype=x2.dtype, device=x2.device) if need[2] else None
+        if M and (need[0] or need[1] or need[2]):
             g = dy.contiguous()
-            lib = _lib.load()
-            with _On(x2) as stream:
-                n = lib.splat_linear_bwd_workspace_bytes(dt, M, N, K, act)
-                keep, ws = _scratch(n, x2)
-                check(lib.splat_linear_bwd(x2.data_ptr(), x2.stride(0), weight.data_ptr(), g.data_ptr(), _ptr(z), dt, M, N, K,
-                                           act, _ptr(dx), _ptr(dw), _ptr(db), ws, n, stream), "splat_linear_bwd")
-        return None if dx is None else dx.view(shape), dw, db, dy if need[3] else None, None, None
+            n = _lib.load().splat_linear_bwd_workspace_bytes(dt, M, N, K, act)
+            keep, ws = _scratch(n, x2)
+            _launch(x2, "splat_linear_bwd", x2.data_ptr(), x2.stride(0), weight.data_ptr(), g.data_ptr(), _ptr(z), dt, M, N,
+                    K, act, _ptr(dx), _ptr(dw), _ptr(db), ws, n)
+        return dx, dw, db, dy if need[3] else None, None, None
 
 
 def linear_act(x, weight, bias=None, act="none", residual=None):
@@ -237,7 +231,7 @@ def linear_act(x, weight, bias=None, act="none", residual=None):
         bias = bias.contiguous()
     if _wants_grad(x, weight, bias, residual):
         return _LinearAct.apply(x, weight, bias, residual, dt, code)
-    return _linear_fwd(_rows(x), weight, bias, None if residual is None else _rows(residual), dt, code, False)[0].view(out)
+    return _linear_fwd(x, weight, bias, residual, dt, code, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ cross attention
@@ -258,17 +252,13 @@ def _describe(q, k, v, lengths, mask, scale, dt):
 
 def _attention_fwd(q, k, v, lengths, mask, scale, dt, save):
     B, Lq, H, D = q.shape
-    lib = _lib.load()
     o = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
     lse = torch.empty(B * Lq * H, dtype=torch.float32, device=q.device) if save else None
     if o.numel():
-        a = _describe(q, k, v, lengths, mask, scale, dt)
-        ref = ctypes.byref(a)
-        with _On(q) as stream:
-            n = lib.splat_attention_workspace_bytes(ref)
-            keep, ws = _scratch(n, q)
-            check(lib.splat_attention_fwd(ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), ws, n,
-                                          stream), "splat_attention_fwd")
+        ref = ctypes.byref(_describe(q, k, v, lengths, mask, scale, dt))
+        n = _lib.load().splat_attention_workspace_bytes(ref)
+        keep, ws = _scratch(n, q)
+        _launch(q, "splat_attention_fwd", ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), ws, n)
     return o, lse
 
 
@@ -286,19 +276,16 @@ class _CrossAttention(torch.autograd.Function):
     def backward(ctx, g):
         q, k, v, o, lse, lengths, mask = ctx.saved_tensors
         scale, dt = ctx.args
-        lib = _lib.load()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         if dq.numel() or dk.numel():
             g = _dense(g)
             a = _describe(q, k, v, lengths, mask, scale, dt)
             a.gb, a.gl, a.gh = g.stride()[:3]
             ref = ctypes.byref(a)
-            with _On(q) as stream:
-                n = lib.splat_attention_bwd_workspace_bytes(ref)
-                keep, ws = _scratch(n, q)
-                check(lib.splat_attention_bwd(ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
-                                              g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws, n, stream),
-                      "splat_attention_bwd")
+            n = _lib.load().splat_attention_bwd_workspace_bytes(ref)
+            keep, ws = _scratch(n, q)
+            _launch(q, "splat_attention_bwd", ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+                    g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws, n)
         need = ctx.needs_input_grad
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
