@@ -245,22 +245,21 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
   __shared__ float red[4][64 * V];
   const int col = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
   const long long r0 = (long long)blockIdx.y * per, r1 = min(M, r0 + per);
+  const long long r = r0 + (threadIdx.x >> 6);
+  const int rows = col < N && r < r1 ? (int)((r1 - r + 3) / 4) : 0;
   float s[V] = {};
-  if (col < N) {
-#pragma unroll 4
-    for (long long r = r0 + (threadIdx.x >> 6); r < r1; r += 4) {
-      const long long i = r * N + col;
-      const Chunk<T> d = load_chunk(dy + i, N - col), c = load_chunk(z + i, N - col);
-      Chunk<T> o;
+  RowStream<T, 4, true> in;
+  in.begin(dy + r * N + col, 4LL * N, z + r * N + col, 4LL * N, rows, min(V, N - col));
+  in.run([&](const Chunk<T>& d, const Chunk<T>& c, int i) {
+    Chunk<T> o;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float x = (float)d.v[j] * act_grad<A>((float)c.v[j]);
-        s[j] += x;
-        o.v[j] = (T)x;
-      }
-      store_chunk(g + i, o, N - col);
+    for (int j = 0; j < V; ++j) {
+      const float x = (float)d.v[j] * act_grad<A>((float)c.v[j]);
+      s[j] += x;
+      o.v[j] = (T)x;
     }
-  }
+    store_chunk(g + (r + 4LL * i) * N + col, o, N - col);
+  });
   if (!bpart) return;
 #pragma unroll
   for (int j = 0; j < V; ++j) red[threadIdx.x >> 6][(threadIdx.x & 63) * V + j] = s[j];

@@ -70,62 +70,6 @@ __device__ __forceinline__ int group_of(const Norm& n, const Place& p, int j) {
   return n.tpg == 1 ? (p.c - p.c0 + j) / n.by_Cg : 0;
 }
 
-// The thread's rows of one or two tensors, U at a time: begin() requests the first U, run() hands every row's chunks to
-// f(chunk of a, chunk of b, row) with the next U in flight. Whole chunks load without conditions (the last U repeat the
-// last row where there are fewer), so that all are issued before the first is needed; a last chunk with fewer channels goes
-// row by row.
-template <typename T, int U, bool Two>
-struct RowStream {
-  const T *a, *b;
-  long long sa, sb;
-  int rows, nv;
-  Chunk<T> ca[U], cb[U];
-
-  __device__ __forceinline__ void get(int i, Chunk<T> (&x)[U], Chunk<T> (&y)[U]) const {   // rows i .. i + U - 1
-    if (i + U <= rows) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        __builtin_memcpy(x[u].v, a + (i + u) * sa, 16);
-        if (Two) __builtin_memcpy(y[u].v, b + (i + u) * sb, 16);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        __builtin_memcpy(x[u].v, a + min(i + u, rows - 1) * sa, 16);
-        if (Two) __builtin_memcpy(y[u].v, b + min(i + u, rows - 1) * sb, 16);
-      }
-    }
-  }
-  __device__ __forceinline__ void begin(const T* a_, long long sa_, const T* b_, long long sb_, int rows_, int nv_) {
-    a = a_; sa = sa_; b = b_; sb = sb_; rows = rows_; nv = nv_;
-    if (rows > 0 && nv == kV<T>) get(0, ca, cb);
-  }
-  template <typename F>
-  __device__ __forceinline__ void run(F&& f) {
-    if (nv == kV<T>) {
-      int i = 0;
-      for (; i + U < rows; i += U) {
-        Chunk<T> na[U], nb[U];
-        get(i + U, na, nb);
-#pragma unroll
-        for (int u = 0; u < U; ++u) f(ca[u], cb[u], i + u);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          ca[u] = na[u];
-          if (Two) cb[u] = nb[u];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u < rows) f(ca[u], cb[u], i + u);
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < rows; ++i, a += sa, b += Two ? sb : 0)
-        f(load_chunk(a, nv), Two ? load_chunk(b, nv) : Chunk<T>{}, i);
-    }
-  }
-};
-
 // Entries of a group in LDS, one after another: (chunk, rt) where no chunk meets two groups, else (channel, rt).
 struct Entries {
   bool whole;
