@@ -176,13 +176,24 @@ struct KeyTiles {
   bool chunked;                 // rows are whole chunks
   Rows<T, DP, N> rk, rv;
   unsigned long long ok0, ok1;  // the fetched tile's keys that count: the first 64, the others
+  unsigned char m0, m1;         // the lane's mask bytes of the tile to be fetched next
   int k0;
 
   __device__ KeyTiles(const Attn& n, const Work& w, const T* kp, const T* vp)
       : k(kp + w.b * n.a.kb + w.hk * n.a.kh), v(vp + w.b * n.a.vb + w.hk * n.a.vh), kl(n.a.kl), vl(n.a.vl), ml(n.a.ml),
-        mask(mask_row(n.a, w.b)), D(n.a.D), len(key_count(n.a, w.b)), chunked(n.chunked), ok0(0), ok1(0), k0(0) {
+        mask(mask_row(n.a, w.b)), D(n.a.D), len(key_count(n.a, w.b)), chunked(n.chunked), ok0(0), ok1(0), m0(0), m1(0), k0(0) {
     rk.init(D, rk.row0() * (int)kl);
     rv.init(D, rv.row0() * (int)vl);
+  }
+  // Requests the mask of tile t: before its keys are, which wait for it.
+  __device__ __forceinline__ void peek(int t) {
+    const int i = t * N + (threadIdx.x & 63);
+    m0 = i < len && (!mask || mask[(long long)i * ml] != 0);
+    m1 = N > 64 && i + 64 < len && (!mask || mask[(long long)(i + 64) * ml] != 0);
+  }
+  __device__ __forceinline__ void begin(int t) {
+    peek(t);
+    fetch(t);
   }
   __device__ __forceinline__ const T* row(const T* p, long long l, int i) const {
     return ((N > 64 && i >= 64 ? ok1 : ok0) >> (i & 63)) & 1 ? p + (k0 + i) * l : nullptr;
@@ -195,12 +206,14 @@ struct KeyTiles {
       rv.load(v + k0 * vl, rv.RS * vl);
       return;
     }
-    ok0 = valid_keys(mask, ml, k0, len);
-    ok1 = N > 64 ? valid_keys(mask, ml, k0 + 64, len) : 0;
+    if (!mask) peek(t);
+    ok0 = __ballot(m0);
+    ok1 = N > 64 ? __ballot(m1) : 0;
     if (chunked) {
       rk.load([&](int i) { return row(k, kl, i); });
       rv.load([&](int i) { return row(v, vl, i); });
     }
+    if (mask) peek(t + 1);
   }
   __device__ __forceinline__ void put(T* tk, T* tv) const {
     if (chunked) {
@@ -319,7 +332,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restri
   const int t0 = w.split * n.per, t1 = min((kt.len + F::KT - 1) / F::KT, t0 + n.per);
   f32x16 acc[S::nd] = {};
   float m = -INFINITY, l = 0.f;
-  if (t0 < t1) kt.fetch(t0);
+  if (t0 < t1) kt.begin(t0);
   for (int t = t0; t < t1; ++t) {
     unsigned long long live = F::KT > 64 && kw >= 64 ? kt.ok1 : kt.ok0;
     live >>= kw & 63;
@@ -382,21 +395,27 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restri
   }
 }
 
-// Joins the splits' partial results of a row, one workgroup a row: lanes over the head's values, 256 / DP groups of lanes
-// over the splits, whose sums are added in LDS in their order.
+// Joins the splits' partial results of a row, one workgroup a row: lanes over the head's values, groups of lanes over the
+// splits, whose sums are added in LDS in their order. The first values are on their way while the statistics are joined.
+constexpr int kJoinThreads = 1024;
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void k_attn_join(Attn n, const float* __restrict__ part, const float* __restrict__ stat,
-                                                        T* __restrict__ o, float* __restrict__ lse) {
-  constexpr int GS = DP == 96 ? 2 : kThreads / DP;   // groups
-  __shared__ float weight[kMaxSplits], sums[GS * DP], wred[2];
+__global__ __launch_bounds__(kJoinThreads) void k_attn_join(Attn n, const float* __restrict__ part,
+                                                            const float* __restrict__ stat, T* __restrict__ o,
+                                                            float* __restrict__ lse) {
+  constexpr int W = DP == 96 ? 128 : DP, GS = kJoinThreads / W, U = 8;   // groups; splits that a lane asks for at a time
+  __shared__ float weight[kMaxSplits], sums[GS * W], total;
   const splat_attention& a = n.a;
   const long long rows = (long long)a.B * a.Hk * n.R, row = blockIdx.x;
-  const int lane = threadIdx.x & 63;
+  const int d = threadIdx.x % W, g = threadIdx.x / W, lane = threadIdx.x & 63;
+  const float* p = part + row * a.D + d;
+  float v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) v[u] = d < a.D && g + u * GS < n.splits ? p[(g + u * GS) * rows * a.D] : 0.f;
   if (threadIdx.x < 64) {
     float m = -INFINITY;
     for (int s = lane; s < n.splits; s += 64) m = fmaxf(m, stat[2 * (s * rows + row)]);
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    for (int e = 32; e >= 1; e >>= 1) m = fmaxf(m, __shfl_xor(m, e, 64));
     const float mu = m == -INFINITY ? 0.f : m;
     float l = 0.f;
     for (int s = lane; s < n.splits; s += 64) {
@@ -404,55 +423,68 @@ __global__ __launch_bounds__(kThreads) void k_attn_join(Attn n, const float* __r
       weight[s] = e;
       l = fmaf(stat[2 * (s * rows + row) + 1], e, l);
     }
-    l = wave_sum(l);
+    l = wave_add(l);
     if (lane == 0) {
-      wred[0] = l > 0.f ? 1.f / l : l;
+      total = l > 0.f ? 1.f / l : l;
       if (lse) lse[row] = l == 0.f ? INFINITY : m + hw_log2(l);
     }
   }
   __syncthreads();
-  const int d = threadIdx.x % DP, g = threadIdx.x / DP;
-  if (g < GS) {
-    float s = 0.f;
-    if (d < a.D) {
-#pragma unroll 8
-      for (int i = g; i < n.splits; i += GS) s = fmaf(part[(i * rows + row) * a.D + d], weight[i], s);
-    }
-    sums[g * DP + d] = s;
+  float s = 0.f;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (g + u * GS < n.splits) s = fmaf(v[u], weight[g + u * GS], s);
+  if (d < a.D) {
+    for (int i = g + U * GS; i < n.splits; i += GS) s = fmaf(p[i * rows * a.D], weight[i], s);
   }
+  sums[g * W + d] = s;
   __syncthreads();
   if (threadIdx.x < a.D) {
-    float s = sums[threadIdx.x];
+    s = sums[threadIdx.x];
 #pragma unroll
-    for (int i = 1; i < GS; ++i) s += sums[i * DP + threadIdx.x];
+    for (int i = 1; i < GS; ++i) s += sums[i * W + threadIdx.x];
     const int bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
     const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
-    o[(((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + threadIdx.x] = (T)(s * wred[0]);
+    o[(((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + threadIdx.x] = (T)(s * total);
   }
 }
 
-// The same for few splits: a thread per value.
+// The same for few splits (rows are many then): a thread per four values of a row.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, const float* __restrict__ part,
+__global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, FastDiv by_quads, int quads, const float* __restrict__ part,
                                                             const float* __restrict__ stat, T* __restrict__ o,
                                                             float* __restrict__ lse) {
   const splat_attention& a = n.a;
-  const long long rows = (long long)a.B * a.Hk * n.R, i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= rows * a.D) return;
-  const long long row = i / a.D;
-  const int d = (int)(i - row * a.D);
-  float m = stat[2 * row], l = stat[2 * row + 1], s = part[i];
+  const int rows = a.B * a.Hk * n.R, i = blockIdx.x * kThreads + threadIdx.x;
+  const int row = i / by_quads, d = (i - row * quads) * 4;
+  if (row >= rows) return;
+  Chunk<float> s = load_chunk(part + (long long)row * a.D + d, a.D - d);
+  float2 ml = *(const float2*)(stat + 2LL * row);
   for (int k = 1; k < n.splits; ++k) {
-    const float mo = stat[2 * (k * rows + row)], mn = fmaxf(m, mo), mu = mn == -INFINITY ? 0.f : mn;
-    const float x = hw_exp2(m - mu), y = hw_exp2(mo - mu);
-    m = mn;
-    l = fmaf(l, x, stat[2 * (k * rows + row) + 1] * y);
-    s = fmaf(s, x, part[k * rows * a.D + i] * y);
+    const long long at = (long long)k * rows + row;
+    const Chunk<float> x = load_chunk(part + at * a.D + d, a.D - d);
+    const float2 mo = *(const float2*)(stat + 2 * at);
+    const float mn = fmaxf(ml.x, mo.x), mu = mn == -INFINITY ? 0.f : mn;
+    const float e = hw_exp2(ml.x - mu), f = hw_exp2(mo.x - mu);
+    ml = make_float2(mn, fmaf(ml.y, e, mo.y * f));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s.v[j] = fmaf(s.v[j], e, x.v[j] * f);
   }
-  const int bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
+  const float inv = ml.y > 0.f ? 1.f / ml.y : ml.y;
+  const int bh = row / n.R, r = row - bh * n.R;
   const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
-  o[(((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + d] = (T)(s * (l > 0.f ? 1.f / l : l));
-  if (lse && d == 0) lse[row] = l == 0.f ? INFINITY : m + hw_log2(l);
+  T* op = o + (((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + d;
+  T x[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = (T)(s.v[e] * inv);
+  if (d + 4 <= a.D) {
+    __builtin_memcpy(op, x, sizeof(x));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d + e < a.D) op[e] = x[e];
+  }
+  if (lse && d == 0) lse[row] = ml.y == 0.f ? INFINITY : ml.x + hw_log2(ml.y);
 }
 
 // ----------------------------------------------------------------------------------------------- backward
@@ -600,8 +632,10 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
 }
 
 // dq: as the forward, a lane per query row; ds^T is the operand of dq^T = k^T ds^T as it is.
+// Three waves a SIMD for bf16 heads of 64 (with a few registers more there are two: 646 us instead of 578 at 36,864 rows
+// and 9,216 keys of 4 heads).
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void k_attn_bwd_q(Attn n, const T* __restrict__ q, const T* __restrict__ k,
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 ? 3 : 1) void k_attn_bwd_q(Attn n, const T* __restrict__ q, const T* __restrict__ k,
                                                          const T* __restrict__ v, const T* __restrict__ g,
                                                          const float* __restrict__ lse, const float* __restrict__ delta,
                                                          T* __restrict__ dq, float* __restrict__ part) {
@@ -622,7 +656,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_q(Attn n, const T* __rest
   const int t0 = w.split * n.per, t1 = min((kt.len + KT - 1) / KT, t0 + n.per);
   const float c = a.scale * kLog2e;
   f32x16 acc[S::nd] = {};
-  if (t0 < t1) kt.fetch(t0);
+  if (t0 < t1) kt.begin(t0);
   for (int t = t0; t < t1; ++t) {
     const unsigned long long live = KT == 64 ? kt.ok0 : kt.ok0 & 0xffffffffull;
     T* tk = tiles + (t & 1) * 2 * tile;
@@ -706,14 +740,14 @@ int with_shape(const splat_attention& a, F&& f) {
 
 // Splits of an axis of `tiles` tiles for `groups` workgroups of which `slots` run at a time: the number with the least
 // estimated time, in tiles, of the rounds that the card takes (a last round that is not full runs faster, by about half of
-// what it lacks) where writing and joining partial results costs a split about as much as six tiles. At least four tiles
-// a split.
+// what it lacks) where writing and joining partial results costs a split about as much as six tiles. At least three tiles a
+// split (attend of 64 rows and 18,432 masked keys: 16 us; 18 with four, 23 with eight).
 void split(Attn& n, long long groups, int tiles, int slots) {
   n.splits = 1;
   n.per = tiles < 1 ? 1 : tiles;
   if (groups == 0) return;
   double best = 0;
-  for (int s = 1; s <= kMaxSplits && (s == 1 || tiles / s >= 4); ++s) {
+  for (int s = 1; s <= kMaxSplits && (s == 1 || tiles / s >= 3); ++s) {
     const int per = (tiles + s - 1) / s;
     const double r = (double)groups * s / slots, whole = (double)((groups * s + slots - 1) / slots);
     const double cost = (r < 1 ? 1 : 0.5 * (r + whole)) * (per + (s > 1 ? 6 : 0));
@@ -808,10 +842,12 @@ int splat_attention_fwd(const splat_attention* a, const void* q, const void* k, 
     if (qw == 1) go(std::integral_constant<int, 1>{});
     else if (qw == 2) go(std::integral_constant<int, 2>{});
     else go(std::integral_constant<int, 4>{});
-    if (need && n.splits <= 8)
-      k_attn_join_few<T><<<div_up(rows * a->D, kThreads), kThreads, 0, st>>>(n, part, stat, (T*)o, lse);
+    const int quads = (a->D + 3) / 4;
+    if (need && n.splits <= 8 && rows * quads < 0x7fffff00LL)
+      k_attn_join_few<T><<<div_up(rows * quads, kThreads), kThreads, 0, st>>>(n, fast_div(quads), quads, part, stat, (T*)o,
+                                                                             lse);
     else if (need)
-      k_attn_join<T, DP><<<(unsigned)rows, kThreads, 0, st>>>(n, part, stat, (T*)o, lse);
+      k_attn_join<T, DP><<<(unsigned)rows, kJoinThreads, 0, st>>>(n, part, stat, (T*)o, lse);
     return check_launch("splat_attention_fwd");
   });
 }

@@ -271,21 +271,24 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
 }
 
 template <typename T, int PB, int QB, int WP, int WQ, bool ACol, bool BCol, int Epi, int A>
-void launch(Gemm g, int slices, hipStream_t st) {
+int launch(Gemm g, int slices, hipStream_t st) {
   g.tp = div_up(g.P, PB * WP * 32);
   g.tq = div_up(g.Q, QB * WQ * 32);
+  if ((long long)g.tp * g.tq >= 1 << 24)   // a launch holds 2^32 threads
+    return set_error(kUnsupported, "product of %d x %d outputs", g.Q, g.P);
   k_gemm<T, PB, QB, WP, WQ, ACol, BCol, Epi, A><<<dim3(g.tp * g.tq, slices), kThreads, 0, st>>>(g);
+  return kOk;
 }
 
 // Tiles of 128 x 128 where they fill the card, otherwise the smaller ones whose workgroups are more; 32 along an
 // output dimension that is no longer.
 template <typename T, bool ACol, bool BCol, int Epi, int A>
-void gemm(const Gemm& g, int slices, hipStream_t st) {
+int gemm(const Gemm& g, int slices, hipStream_t st) {
   const long long big = (long long)div_up(g.P, 128) * div_up(g.Q, 128) * slices;
-  if (g.P <= 32) launch<T, 1, 1, 1, 4, ACol, BCol, Epi, A>(g, slices, st);
-  else if (g.Q <= 32) launch<T, 1, 1, 4, 1, ACol, BCol, Epi, A>(g, slices, st);
-  else if (big >= 256) launch<T, 2, 2, 2, 2, ACol, BCol, Epi, A>(g, slices, st);
-  else launch<T, 1, 1, 2, 2, ACol, BCol, Epi, A>(g, slices, st);
+  if (g.P <= 32) return launch<T, 1, 1, 1, 4, ACol, BCol, Epi, A>(g, slices, st);
+  if (g.Q <= 32) return launch<T, 1, 1, 4, 1, ACol, BCol, Epi, A>(g, slices, st);
+  if (big >= 256) return launch<T, 2, 2, 2, 2, ACol, BCol, Epi, A>(g, slices, st);
+  return launch<T, 1, 1, 2, 2, ACol, BCol, Epi, A>(g, slices, st);
 }
 
 // Slices of the contraction over M rows for a weight gradient [N, K]: about 512 workgroups, of at least 256 rows each.
@@ -311,8 +314,7 @@ int check_linear(const char* what, int dtype, long long M, int N, int K, int act
   if (dtype != kF32 && dtype != kBf16) return set_error(kInvalid, "%s: unknown element type %d", what, dtype);
   if (M < 0 || N < 1 || K < 1) return set_error(kInvalid, "%s: M %lld, N %d, K %d", what, M, N, K);
   if (act < 0 || act >= kActCount) return set_error(kInvalid, "%s: unknown activation %d", what, act);
-  const long long tiles = ((M + 31) / 32) * (((long long)N + 31) / 32);
-  if (M > 0x7fffff00LL || N > 0x7fffff00 || K > 0x7fffff00 || tiles > 0x7fffff00LL || ((M + 31) / 32) * (((long long)K + 31) / 32) > 0x7fffff00LL)
+  if (M > 0x7fffff00LL || N > 0x7fffff00 || K > 0x7fffff00)
     return set_error(kUnsupported, "%s: M %lld, N %d, K %d", what, M, N, K);
   return kOk;
 }
@@ -342,8 +344,8 @@ int splat_linear_fwd(const void* x, long long ldx, const void* weight, const voi
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_act(act, [&](auto a) {
-      gemm<T, false, false, kForward, decltype(a)::value>(g, 1, (hipStream_t)stream);
-      return check_launch("splat_linear_fwd");
+      const int rc = gemm<T, false, false, kForward, decltype(a)::value>(g, 1, (hipStream_t)stream);
+      return rc ? rc : check_launch("splat_linear_fwd");
     });
   });
 }
@@ -377,8 +379,9 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
       const int per = grad_rows(dtype, M, N);
       bslices = div_up(M, per);
       with_act(act, [&](auto a) {
-        k_act_grad<T, decltype(a)::value><<<dim3(div_up(N, 64 * kV<T>), bslices), 256, 0, st>>>(
-            (const T*)dy, (const T*)z, (T*)ws, M, N, per, bpart);
+        if constexpr (decltype(a)::value != kActNone)
+          k_act_grad<T, decltype(a)::value><<<dim3(div_up(N, 64 * kV<T>), bslices), 256, 0, st>>>(
+              (const T*)dy, (const T*)z, (T*)ws, M, N, per, bpart);
         return kOk;
       });
       gr = (const T*)ws;
@@ -389,7 +392,7 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
       g.B = gr; g.ldb = N; g.Q = (int)M;
       g.K = g.kper = N;
       g.out = dx;
-      gemm<T, true, false, kOut, 0>(g, 1, st);
+      if (const int rc = gemm<T, true, false, kOut, 0>(g, 1, st)) return rc;
     }
     if (dweight || dbias) {
       if (dweight || act == kActNone) {
@@ -400,7 +403,7 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
         g.K = M; g.kper = (M + s - 1) / s;
         g.part = part;
         g.bpart = act == kActNone ? bpart : nullptr;
-        gemm<T, true, true, kPartial, 0>(g, s, st);
+        if (const int rc = gemm<T, true, true, kPartial, 0>(g, s, st)) return rc;
       }
       const long long n = dweight ? (long long)N * K : 0;
       const unsigned wgs = div_up(n, 1024), bwgs = dbias ? div_up(N, 32) : 0;

@@ -319,3 +319,56 @@ def test_another_stream():
                F.linear_act(x.clone(), w.clone(), act="gelu")]
     torch.cuda.current_stream().wait_stream(s)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: their far ends give what the same rows give alone."""
+    M = 2 ** 31 // 32 + 4099
+    x = torch.empty(M, 32, device="cuda", dtype=torch.bfloat16)
+    x.copy_(rand(1, 32, dt=torch.bfloat16).expand(M, 32))
+    tail = rand(300, 32, dt=torch.bfloat16, seed=3)
+    x[-300:] = tail
+    w = rand(40, 32, dt=torch.bfloat16, seed=1)
+    y = F.linear_act(x, w, act="gelu")
+    assert torch.equal(y[-300:], F.linear_act(tail, w, act="gelu")) and torch.equal(y[:1], F.linear_act(x[:1], w, act="gelu"))
+    del y
+    # one image whose far half is the near one negated: the mean is zero, and the far end is the near one negated
+    half = M // 2
+    x[half:2 * half] = -x[:half]
+    x[2 * half:] = 0
+    y = F.group_norm_act(x[None, :2 * half], 1, act="none")[0]
+    assert torch.isfinite(y[-1]).all() and (y[half:half + 100].float() + y[:100].float()).abs().max() <= 2.0 ** -6
+    del x, y
+    # a cache whose keys lie 40,000 elements apart
+    big = torch.zeros(60000, 40000, device="cuda", dtype=torch.bfloat16)
+    big[:, :128] = rand(60000, 128, dt=torch.bfloat16, seed=5)
+    k, v = big[None, :, None, :64], big[None, :, None, 64:128]
+    q = rand(1, 2, 1, 64, dt=torch.bfloat16)
+    assert torch.equal(F.cross_attention(q, k, v), F.cross_attention(q, k.contiguous(), v.contiguous()))
+
+
+def test_graph_replays():
+    """A captured chain of the operators gives the eager result on every replay, with eager work in between."""
+    q, k, v = qkv(2, 40, 3000, 4, 2, 64, torch.bfloat16)
+    w = rand(256, 256, dt=torch.bfloat16, seed=4, scale=0.1)
+    mask = torch.rand(2, 3000, generator=torch.Generator("cuda").manual_seed(3), device="cuda") < 0.5
+
+    def chain():
+        a = F.cross_attention(q, k, v, key_mask=mask).reshape(2, 40, 256)
+        return F.linear_act(F.group_norm_act(a, 8, act="silu"), w, act="gelu", residual=a)
+
+    want = chain()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        chain()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = chain()
+    for _ in range(4):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(chain(), want)
