@@ -200,6 +200,61 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
   }
 }
 
+// The forward for at most 32 rows (tokens): bound by reading the weight, and for a small one by the chain of its loads. A
+// workgroup makes 32 outputs of every row; its eight waves share the contraction and load their operands straight from
+// memory in the matrix instructions' layout, four steps in flight, and their sums meet in LDS once. x of one row of 256,
+// 1,024 outputs: 3.4 us, 7.8 through k_gemm's staged tiles (eight workgroups, four barriers in a row).
+constexpr int kFewThreads = 512, kFewRows = 32;
+template <typename T, int A>
+__global__ __launch_bounds__(kFewThreads) void k_few_rows(Gemm g) {
+  constexpr int V = kV<T>, S = 2 * V, U = 4, W = kFewThreads / 64;
+  __shared__ __align__(16) float sums[W][32][36];   // [wave][row][output]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int p0 = blockIdx.x * 32;
+  // lanes past the last output or row read the last one's values; what they make is not stored
+  const T* a = (const T*)g.A + (long long)min(p0 + (lane & 31), g.P - 1) * g.lda;
+  const T* b = (const T*)g.B + (long long)min(lane & 31, g.Q - 1) * g.ldb;
+  const int steps = (int)((g.K + S - 1) / S), whole = (int)(g.K / S);
+  f32x16 acc = {};
+  for (int s0 = wave * U; s0 < steps; s0 += W * U) {
+    Chunk<T> ca[U], cb[U];
+    if (s0 + U <= whole) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        __builtin_memcpy(ca[u].v, a + (s0 + u) * S + h * V, 16);
+        __builtin_memcpy(cb[u].v, b + (s0 + u) * S + h * V, 16);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long k = (long long)(s0 + u) * S + h * V;
+        ca[u] = load_chunk(a + k, g.K - k);
+        cb[u] = load_chunk(b + k, g.K - k);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) mma(acc, ca[u], cb[u]);
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const f32x4 run = {acc[4 * t], acc[4 * t + 1], acc[4 * t + 2], acc[4 * t + 3]};
+    *(f32x4*)&sums[wave][lane & 31][acc_row(4 * t, h)] = run;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < g.Q * 32; e += kFewThreads) {
+    const int q = e >> 5, c = e & 31, p = p0 + c;
+    if (p >= g.P) continue;
+    float x = sums[0][q][c];
+#pragma unroll
+    for (int w = 1; w < W; ++w) x += sums[w][q][c];
+    if (g.bias) x += (float)((const T*)g.bias)[p];
+    if (g.z) ((T*)g.z)[(long long)q * g.P + p] = (T)x;
+    x = act_fwd<A>(x);
+    if (g.res) x += (float)((const T*)g.res)[q * g.ldr + p];
+    ((T*)g.out)[(long long)q * g.P + p] = (T)x;
+  }
+}
+
 // out[i] = sum over the slices, in their order, of part[slice][i]; in the workgroups from `wgs` on the same for the bias,
 // 32 columns each, 8 groups of threads over its slices.
 template <typename T>
@@ -286,7 +341,7 @@ template <typename T, bool ACol, bool BCol, int Epi, int A>
 int gemm(const Gemm& g, int slices, hipStream_t st) {
   const long long big = (long long)div_up(g.P, 128) * div_up(g.Q, 128) * slices;
   if (g.P <= 32) return launch<T, 1, 1, 1, 4, ACol, BCol, Epi, A>(g, slices, st);
-  if (g.Q <= 32) return launch<T, 1, 1, 4, 1, ACol, BCol, Epi, A>(g, slices, st);
+  if (Epi != kForward && g.Q <= 32) return launch<T, 1, 1, 4, 1, ACol, BCol, Epi, A>(g, slices, st);
   if (big >= 256) return launch<T, 2, 2, 2, 2, ACol, BCol, Epi, A>(g, slices, st);
   return launch<T, 1, 1, 2, 2, ACol, BCol, Epi, A>(g, slices, st);
 }
@@ -344,7 +399,12 @@ int splat_linear_fwd(const void* x, long long ldx, const void* weight, const voi
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_act(act, [&](auto a) {
-      const int rc = gemm<T, false, false, kForward, decltype(a)::value>(g, 1, (hipStream_t)stream);
+      constexpr int A = decltype(a)::value;
+      if (M <= kFewRows) {
+        k_few_rows<T, A><<<div_up(N, 32), kFewThreads, 0, (hipStream_t)stream>>>(g);
+        return check_launch("splat_linear_fwd");
+      }
+      const int rc = gemm<T, false, false, kForward, A>(g, 1, (hipStream_t)stream);
       return rc ? rc : check_launch("splat_linear_fwd");
     });
   });
