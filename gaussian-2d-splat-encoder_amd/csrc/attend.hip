@@ -92,14 +92,15 @@ struct Work {
   int tile, split, b, hk, bh;
 };
 
-// Workgroup -> (image, key head), tile and split: a head's tiles follow each other on one XCD, whose L2 then holds the
-// other side of them.
+// Workgroup -> (image, key head), tile and split. The card works on one head's workgroups after the other, each XCD on a
+// band of them: its L2 holds the other side's head, and images without keys leave no XCD idle (with a band of heads each,
+// a third of the XCDs had nothing to do where one image of three was empty: 55 us instead of 40).
 __device__ __forceinline__ Work work_of(const Attn& n) {
-  const int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int per = n.tiles * n.splits, bh = blockIdx.x / per, id = xcd_swizzle(blockIdx.x - bh * per, per);
   Work w;
   w.tile = id % n.tiles;
-  w.split = id / n.tiles % n.splits;
-  w.bh = id / (n.tiles * n.splits);
+  w.split = id / n.tiles;
+  w.bh = bh;
   w.b = w.bh / n.a.Hk;
   w.hk = w.bh % n.a.Hk;
   return w;
@@ -741,16 +742,22 @@ int with_shape(const splat_attention& a, F&& f) {
 // Splits of an axis of `tiles` tiles for `groups` workgroups of which `slots` run at a time: the number with the least
 // estimated time, in tiles, of the rounds that the card takes (a last round that is not full runs faster, by about half of
 // what it lacks) where writing and joining partial results costs a split about as much as six tiles. At least three tiles a
-// split (attend of 64 rows and 18,432 masked keys: 16 us; 18 with four, 23 with eight).
+// split (64 rows and 18,432 masked bf16 keys: 16 us; 18 with four, 23 with eight).
+// A float tile takes sixteen times the matrix instructions' time: one workgroup a CU is a round there, and a split costs
+// about one tile. Where lengths or a mask, which only the device knows, may leave workgroups idle, more of them even out
+// what is left: two rounds are added to the estimate (dk and dv of 3 x 1,201 x 777, two heads of 40, one image empty: 67 us;
+// 97 with half the splits).
 void split(Attn& n, long long groups, int tiles, int slots) {
   n.splits = 1;
   n.per = tiles < 1 ? 1 : tiles;
   if (groups == 0) return;
+  const bool f32 = n.a.dtype == kF32, masked = f32 && (n.a.kv_lengths || n.a.key_mask);
+  if (f32) slots = 256;
   double best = 0;
   for (int s = 1; s <= kMaxSplits && (s == 1 || tiles / s >= 3); ++s) {
     const int per = (tiles + s - 1) / s;
     const double r = (double)groups * s / slots, whole = (double)((groups * s + slots - 1) / slots);
-    const double cost = (r < 1 ? 1 : 0.5 * (r + whole)) * (per + (s > 1 ? 6 : 0));
+    const double cost = (masked ? r + 2 : r < 1 ? 1 : 0.5 * (r + whole)) * (per + (s == 1 ? 0 : f32 ? 1 : 6));
     if (s == 1 || cost < 0.97 * best) {
       best = cost;
       n.per = per < 1 ? 1 : per;
@@ -760,9 +767,9 @@ void split(Attn& n, long long groups, int tiles, int slots) {
   }
 }
 
-// Workgroups that the card's 256 CUs hold at a time, from the kernels' registers and (few rows) their LDS.
+// Workgroups that the card's 256 CUs hold at a time (bf16), from the kernels' registers and (few rows) their LDS.
 int slots_rows(const splat_attention& a, int qw) {
-  return 256 * (qw < 4 ? (a.D <= 64 ? 2 : 1) : a.D <= 64 ? 3 : a.dtype == kBf16 ? 2 : 1);
+  return 256 * (qw < 4 ? (a.D <= 64 ? 2 : 1) : a.D <= 64 ? 3 : 2);
 }
 int slots_keys(const splat_attention& a) { return 256 * (a.D <= 64 ? 2 : 1); }
 
