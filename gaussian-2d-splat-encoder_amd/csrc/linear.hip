@@ -12,6 +12,26 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBytesK = 128;   // bytes of contraction indices staged at a time
 
+// The activation's input, kept for its backward: float, or for bf16 a half of the same size. Its rounding, 2^-12 of the
+// value, moves act' by an eighth of what bf16's would (which cost tanh's gradients half as much again as their own
+// roundings); past +-65504 every act' is constant, and a positive value stays positive, which relu's needs.
+template <typename T>
+struct Kept;
+template <>
+struct Kept<float> {
+  __device__ static float pack(float z) { return z; }
+  __device__ static float unpack(float z) { return z; }
+};
+template <>
+struct Kept<bf16> {
+  __device__ static bf16 pack(float z) {
+    const _Float16 h = (_Float16)(z > 65504.f ? 65504.f : z < -65504.f ? -65504.f : z);   // NaN stays
+    const unsigned short b = __builtin_bit_cast(unsigned short, h);
+    return __builtin_bit_cast(bf16, (unsigned short)(z > 0.f && b == 0 ? 1 : b));
+  }
+  __device__ static float unpack(bf16 z) { return (float)__builtin_bit_cast(_Float16, z); }
+};
+
 struct Gemm {
   const void *A, *B;       // A(p, k), B(q, k)
   long long lda, ldb;      // elements from row to row of the stored matrices
@@ -181,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
           for (int e = 0; e < V; ++e) x[e] += (float)bias.v[e];
           if (g.z) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) o.v[e] = (T)x[e];
+            for (int e = 0; e < V; ++e) o.v[e] = Kept<T>::pack(x[e]);
             store_chunk((T*)g.z + (long long)q * g.P + p, o, n);
           }
 #pragma unroll
@@ -248,7 +268,7 @@ __global__ __launch_bounds__(kFewThreads) void k_few_rows(Gemm g) {
 #pragma unroll
     for (int w = 1; w < W; ++w) x += sums[w][q][c];
     if (g.bias) x += (float)((const T*)g.bias)[p];
-    if (g.z) ((T*)g.z)[(long long)q * g.P + p] = (T)x;
+    if (g.z) ((T*)g.z)[(long long)q * g.P + p] = Kept<T>::pack(x);
     x = act_fwd<A>(x);
     if (g.res) x += (float)((const T*)g.res)[q * g.ldr + p];
     ((T*)g.out)[(long long)q * g.P + p] = (T)x;
@@ -292,7 +312,7 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
   }
 }
 
-// g = dy act'(z) over `per` rows a workgroup, 64 chunks of columns wide, and the rows' sums of g before its rounding.
+// g = dy act'(z) (z as Kept has it) over `per` rows a workgroup, 64 chunks of columns wide, and the rows' sums of g before its rounding.
 template <typename T, int A>
 __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ g,
                                                   long long M, int N, int per, float* __restrict__ bpart) {
@@ -309,7 +329,7 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
     Chunk<T> o;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float x = (float)d.v[j] * act_grad<A>((float)c.v[j]);
+      const float x = (float)d.v[j] * act_grad<A>(Kept<T>::unpack(c.v[j]));
       s[j] += x;
       o.v[j] = (T)x;
     }

@@ -20,6 +20,7 @@ from . import _lib
 from ._lib import SplatAttention, check
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_KEPT = {torch.float32: torch.float32, torch.bfloat16: torch.float16}   # type of an activation's input for its backward
 _ACTS = {"none": 0, "gelu": 1, "silu": 2, "relu": 3, "tanh": 4, "sigmoid": 5}
 MAX_HEAD = 128   # values of a head at most
 
@@ -173,7 +174,7 @@ def _linear_fwd(x, weight, bias, residual, dt, act, save):
     M, K = x2.shape
     N = weight.shape[0]
     y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
-    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if save and act else None
+    z = torch.empty((M, N), dtype=_KEPT[x.dtype], device=x.device) if save and act else None
     if M:
         r2 = None if residual is None else _rows(residual)
         _launch(x, "splat_linear_fwd", x2.data_ptr(), x2.stride(0), weight.data_ptr(), _ptr(bias), _ptr(r2),

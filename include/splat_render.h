@@ -324,7 +324,8 @@ int splat_group_norm_bwd(const void *x, long long xsb, long long xsl, const void
                          void *ws, size_t ws_bytes, void *stream);
 
 /* y[M, N] = act(x[M, K] weight[N, K]^T + bias[N]) + residual[M, N]; bias and residual may be NULL; ldx, ldr: elements from
- * row to row. z[M, N] (or NULL) receives the activation's input, which the backward of act != 0 takes.
+ * row to row. z[M, N] (or NULL) receives the activation's input, which the backward of act != 0 takes: float32, or IEEE
+ * half for bfloat16 rows (the same size, a finer rounding).
  * Backward from dy[M, N]: dx[M, K], dweight[N, K], dbias[N] (NULL skips). */
 int splat_linear_fwd(const void *x, long long ldx, const void *weight, const void *bias, const void *residual,
                      long long ldr, int dtype, long long M, int N, int K, int act, void *y, void *z, void *stream);

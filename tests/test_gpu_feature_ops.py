@@ -185,6 +185,18 @@ def test_linear_empty_and_nan(dt):
     assert torch.isnan(y[7]).all() and torch.isnan(y).sum() == 5
 
 
+def test_linear_activation_inputs_out_of_the_kept_range():
+    """Inputs of the activation past a half's range, and positive ones below it: the slopes are the limits', 1 for a relu of
+    any positive value."""
+    w = torch.eye(8, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    x = torch.tensor([[1e30, -1e30, 1e5, -1e5, 1e-30, -1e-30, 3.0, -3.0]], device="cuda").bfloat16().requires_grad_(True)
+    for name, want in (("relu", [1, 0, 1, 0, 1, 0, 1, 0]), ("gelu", [1, 0, 1, 0, 0.5, 0.5, 1.0119, -0.0119]),
+                       ("sigmoid", [0, 0, 0, 0, 0.25, 0.25, 0.0452, 0.0452])):
+        y = F.linear_act(x, w, act=name)
+        g, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert torch.allclose(g.float()[0], torch.tensor(want, device="cuda", dtype=torch.float32), atol=2.0 ** -8), name
+
+
 # ------------------------------------------------------------------------------------------------ cross attention
 def qkv(B, Lq, Lk, H, Hk, D, dt, scale=1.5):
     kv = rand(B, Lk, 2, Hk, D, dt=dt, seed=1)
