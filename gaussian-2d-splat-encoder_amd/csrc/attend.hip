@@ -9,6 +9,12 @@
 //
 // Keys that a length or a mask leaves out are replaced by zeros as they are loaded, so that nothing they hold (NaN
 // included) reaches a product; a row without valid keys gives zeros, and zero gradients.
+//
+// Measured on 36,864 rows and 9,216 keys of four heads of 64, bf16 (174 GFLOP a product; a large library
+// product reaches 1,394 TFLOP/s here): forward 460 us (755 TFLOP/s), dk and dv 780 us (890), dq 545 us (955). Matrix and
+// vector instructions take about the same time and overlap only in part: matrix units 36 to 47% busy, vector units 42 to
+// 63%, LDS 36 to 49%. One pass for all three gradients would do with five products instead of seven, but dq would need
+// atomics (whose order changes results) or 2.7 GB of partial sums.
 #include "feat_common.h"
 #include "splat_attention.h"
 
@@ -250,7 +256,8 @@ __device__ __forceinline__ void store_row(O* row, const RowAcc<T, DP>& acc, floa
 // leave waves idle otherwise. A wave's 32-key blocks of a tile (two for bf16, one for float) are one softmax step. Key and
 // value tiles go through registers into two LDS buffers in turn: the next tile's loads are in flight during a step, and
 // one barrier a tile suffices (where only one buffer fits, two). Waves that shared keys join their results in LDS, splits
-// of the key axis in k_attn_join.
+// of the key axis in k_attn_join. Few rows are bound by reading keys and values: one token, 92,160 keys of four heads of 64
+// in bf16 (94 MB) 21 us, 4.5 TB/s, and 4 us to join.
 template <typename T, int DP, int QW>
 struct FwdShape {
   static constexpr int KW = kWaves / QW;
@@ -397,7 +404,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restri
 }
 
 // Joins the splits' partial results of a row, one workgroup a row: lanes over the head's values, groups of lanes over the
-// splits, whose sums are added in LDS in their order. The first values are on their way while the statistics are joined.
+// splits, whose sums are added in LDS in their order. The first values are on their way while the statistics are joined:
+// 4 us for 120 splits of four rows, 6 with them asked for afterwards.
 constexpr int kJoinThreads = 1024;
 template <typename T, int DP>
 __global__ __launch_bounds__(kJoinThreads) void k_attn_join(Attn n, const float* __restrict__ part,
@@ -450,7 +458,8 @@ __global__ __launch_bounds__(kJoinThreads) void k_attn_join(Attn n, const float*
   }
 }
 
-// The same for few splits (rows are many then): a thread per four values of a row.
+// The same for few splits (rows are many then): a thread per four values of a row. Two splits of 147,456 rows of 64: 17 us
+// (5.5 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, FastDiv by_quads, int quads, const float* __restrict__ part,
                                                             const float* __restrict__ stat, T* __restrict__ o,
@@ -489,7 +498,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, FastDiv by_q
 }
 
 // ----------------------------------------------------------------------------------------------- backward
-// delta[row] = sum over d of do * o.
+// delta[row] = sum over d of do * o, which the score gradients p (dp - delta) take. Bound by memory: 147,456 rows of 64 bf16
+// 12 us (3.2 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_attn_delta(Attn n, const T* __restrict__ o, const T* __restrict__ g,
                                                          float* __restrict__ delta) {
@@ -517,7 +527,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_delta(Attn n, const T* __rest
 template <typename T> constexpr int kBwdTile = sizeof(T) == 2 ? 64 : 32;
 
 // dk and dv: a wave holds 32 keys and values, the workgroup's four share tiles of query rows. With s = q k^T a lane is a
-// key: p and ds are the operands of dv = p^T do and dk = ds^T q as they are.
+// key: p and ds are the operands of dv = p^T do and dk = ds^T q as they are. 64 keys a wave would halve the LDS reads but
+// leave one wave a SIMD (1,014 us instead of 793).
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __restrict__ q, const T* __restrict__ k,
                                                           const T* __restrict__ v, const T* __restrict__ g,
@@ -692,7 +703,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 ? 3 : 1) void 
   }
 }
 
-// Adds the splits' partial gradients in their order. Rows of `part` are the output's own order, or (heads) the rows of
+// Adds the splits' partial gradients in their order (seven of 9,216 keys of four heads of 64: 17 us, 4.2 TB/s). Rows of `part` are the output's own order, or (heads) the rows of
 // (image, key head) problems.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_attn_add(Attn n, const float* __restrict__ part, int splits, long long stride,

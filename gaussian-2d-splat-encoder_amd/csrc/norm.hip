@@ -10,6 +10,10 @@
 // sums and a second one joins them and writes the result, x coming from the caches the second time where it fits them.
 // Both directions are bound by memory, and maps of a few megabytes by the chain of loads, reductions and barriers of a
 // workgroup: x's first rows are requested before anything else, and a reduction is one exchange through LDS.
+//
+// Measured at 8 x 192 x 192 x 128 bf16, gelu first (37.7M values, 75 MB a tensor; a large copy moves 4.9 TB/s here):
+// statistics 32 us, result 30 us (5.0 TB/s), backward sums 32 us (4.7), dx 41 us (5.5). The vector unit is busy 60 to 80%
+// of that time, half of it with gelu (15 instructions a value, once per pass).
 #include "feat_common.h"
 
 namespace splat {
@@ -152,7 +156,8 @@ __device__ __forceinline__ void params(const float* w, const Place& p, float non
 }
 
 // Statistics and result in one launch, one workgroup per image and tile of whole groups: x stays in registers between the
-// statistics (each thread's own mean and deviations, joined per group) and the result.
+// statistics (each thread's own mean and deviations, joined per group) and the result. 24 x 24 x 64 float: 8 us, the chain
+// of a load, the reduction and a store.
 template <typename T, int A, bool First, int Keep>
 __global__ __launch_bounds__(kThreads) void k_norm_whole(Norm n, const T* __restrict__ x, const float* __restrict__ w,
                                                          const float* __restrict__ b, T* __restrict__ y,
