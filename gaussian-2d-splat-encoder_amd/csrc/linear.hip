@@ -226,20 +226,23 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
   }
 }
 
-// The forward for at most 32 rows (tokens): bound by reading the weight, and for a small one by the chain of its loads. A
-// workgroup makes 32 outputs of every row; its eight waves share the contraction and load their operands straight from
-// memory in the matrix instructions' layout, four steps in flight, and their sums meet in LDS once. x of one row of 256,
-// 1,024 outputs: 3.4 us, 7.8 through k_gemm's staged tiles (eight workgroups, four barriers in a row).
-constexpr int kFewThreads = 512, kFewRows = 32;
+// The forward where outputs are few (tokens, small maps): bound by reading the weight, and for a small one by the chain of
+// its loads. A workgroup makes 32 outputs of 32 rows; its eight waves share the contraction and load their operands straight
+// from memory in the matrix instructions' layout, four steps in flight, and their sums meet in LDS once. Every 32 rows read
+// the weight and every 32 outputs the rows again, so it pays up to `few_tiles` workgroups. bf16, through k_gemm's staged
+// tiles after it: 1 x 256 -> 1,024 3.4 us (7.8), 256 x 1,024 -> 1,024 6.3 (9.2), 512 x 1,024 -> 1,024 9.9 (9.4); float:
+// 512 x 1,024 -> 1,024 19.5 (27.3), 1,024 x 1,024 -> 1,024 36 (28).
+constexpr int kFewThreads = 512;
+template <typename T> constexpr long long few_tiles = sizeof(T) == 4 ? 512 : 256;
 template <typename T, int A>
 __global__ __launch_bounds__(kFewThreads) void k_few_rows(Gemm g) {
   constexpr int V = kV<T>, S = 2 * V, U = 4, W = kFewThreads / 64;
   __shared__ __align__(16) float sums[W][32][36];   // [wave][row][output]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int p0 = blockIdx.x * 32;
+  const int p0 = blockIdx.x * 32, q0 = blockIdx.y * 32, nq = min(32, g.Q - q0);
   // lanes past the last output or row read the last one's values; what they make is not stored
   const T* a = (const T*)g.A + (long long)min(p0 + (lane & 31), g.P - 1) * g.lda;
-  const T* b = (const T*)g.B + (long long)min(lane & 31, g.Q - 1) * g.ldb;
+  const T* b = (const T*)g.B + (long long)min(q0 + (lane & 31), g.Q - 1) * g.ldb;
   const int steps = (int)((g.K + S - 1) / S), whole = (int)(g.K / S);
   f32x16 acc = {};
   for (int s0 = wave * U; s0 < steps; s0 += W * U) {
@@ -267,12 +270,12 @@ __global__ __launch_bounds__(kFewThreads) void k_few_rows(Gemm g) {
     *(f32x4*)&sums[wave][lane & 31][acc_row(4 * t, h)] = run;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < g.Q * 32; e += kFewThreads) {
-    const int q = e >> 5, c = e & 31, p = p0 + c;
+  for (int e = threadIdx.x; e < nq * 32; e += kFewThreads) {
+    const int c = e & 31, p = p0 + c, q = q0 + (e >> 5);
     if (p >= g.P) continue;
-    float x = sums[0][q][c];
+    float x = sums[0][e >> 5][c];
 #pragma unroll
-    for (int w = 1; w < W; ++w) x += sums[w][q][c];
+    for (int w = 1; w < W; ++w) x += sums[w][e >> 5][c];
     if (g.bias) x += (float)((const T*)g.bias)[p];
     if (g.z) ((T*)g.z)[(long long)q * g.P + p] = Kept<T>::pack(x);
     x = act_fwd<A>(x);
@@ -427,8 +430,8 @@ int splat_linear_fwd(const void* x, long long ldx, const void* weight, const voi
     using T = decltype(t);
     return with_act(act, [&](auto a) {
       constexpr int A = decltype(a)::value;
-      if (M <= kFewRows) {
-        k_few_rows<T, A><<<div_up(N, 32), kFewThreads, 0, (hipStream_t)stream>>>(g);
+      if (M <= 32 || (long long)div_up(N, 32) * div_up(M, 32) <= few_tiles<T>) {
+        k_few_rows<T, A><<<dim3(div_up(N, 32), div_up(M, 32)), kFewThreads, 0, (hipStream_t)stream>>>(g);
         return check_launch("splat_linear_fwd");
       }
       const int rc = gemm<T, false, false, kForward, A>(g, 1, (hipStream_t)stream);

@@ -62,6 +62,8 @@ class CellReader(nn.Module):
     def forward(self, x, states=None, kv_lengths=None, key_mask=None, kv=None):
         """x [B, ..., channels], states [B, ..., state_channels] (or kv from keys_values) -> like x. kv_lengths [B] and
         key_mask [B, Lk] leave states out; where none is left the attention adds its projection's bias alone."""
+        if (states is None) == (kv is None):
+            raise ValueError("either states or kv is needed")
         if kv is None:
             kv = self.keys_values(states)
         q = self._product(self._norm(x, self.norm1), self.to_q)

@@ -188,8 +188,8 @@ class _SplatHead(nn.Module):
 
     @staticmethod
     def _product(cells, conv, act):
-        """act(conv(cells)) of a 1x1 convolution on channels-last cells [B, fH, fW, C]."""
-        return linear_act(cells, conv.weight.flatten(1), conv.bias, act=act)
+        """act(conv(cells)) of a 1x1 convolution on channels-last cells [B, fH, fW, C], in the cells' type."""
+        return linear_act(cells, conv.weight.flatten(1).to(cells.dtype), conv.bias.to(cells.dtype), act=act)
 
     def _forward_channels_last(self, feat):
         """forward on channels-last cells: an output's channels are (slot, value), so that a cell's values already lie in
@@ -327,7 +327,8 @@ class EfficientGaussianEncoder(nn.Module):
         fused = self._with_grad(feat, image)
         pooled = feat.mean(dim=(2, 3))
         if self.channels_last:
-            bg = linear_act(pooled, self.bg_head.weight, self.bg_head.bias, act="sigmoid")
+            bg = linear_act(pooled, self.bg_head.weight.to(pooled.dtype), self.bg_head.bias.to(pooled.dtype),
+                            act="sigmoid")
         else:
             bg = torch.sigmoid(self.bg_head(pooled))
         self._mark("backbone")

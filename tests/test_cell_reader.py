@@ -32,6 +32,11 @@ def test_reader_refuses(a, kw):
         CellReader(*a, **kw)
 
 
+def test_reader_needs_states():
+    with pytest.raises(ValueError, match="states or kv"):
+        CellReader(32, 16)(torch.zeros(1, 4, 32))
+
+
 def test_host_tensors_are_refused():
     with pytest.raises(RuntimeError, match="device tensors"):
         CellReader(32, 16)(torch.zeros(1, 4, 32), torch.zeros(1, 3, 16))

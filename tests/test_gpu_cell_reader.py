@@ -109,3 +109,15 @@ def test_channels_last_encoder_is_the_same_encoder(variant, kw):
         b.zero_grad()
         TF.mse_loss(r, img).backward()
         assert all(torch.isfinite(p.grad).all() for p in b.parameters() if p.grad is not None)
+
+
+def test_channels_last_encoder_under_autocast():
+    """bfloat16 convolutions feed bfloat16 operators; parameters stay float32 and get finite gradients."""
+    torch.manual_seed(2)
+    enc = EE.EfficientGaussianEncoder(d_feature=32, variant="free", channels_last=True).cuda()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = enc(torch.rand(1, 3, 64, 64, device="cuda"))
+    ref = enc(torch.rand(1, 3, 64, 64, device="cuda"))
+    assert out["log_scale"].dtype is torch.bfloat16 and out["mu"].shape == ref["mu"].shape
+    sum(out[k].float().sum() for k in ("mu", "log_scale", "color", "opacity", "bg")).backward()
+    assert all(p.grad is None or (p.grad.dtype is torch.float32 and torch.isfinite(p.grad).all()) for p in enc.parameters())

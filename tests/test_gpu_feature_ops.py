@@ -295,6 +295,27 @@ def test_attention_large_scores(dt):
     assert torch.isfinite(y).all() and R.rel(y, ref) <= (4e-3 if dt is torch.float32 else 8e-3)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-30])
+def test_attention_scales(dt, scale):
+    """A negative scale turns the order of the scores round; zero weighs all keys alike."""
+    q, k, v = qkv(2, 70, 333, 4, 2, 40, dt)
+    ins = [q, k, v]
+    if scale == -0.3:
+        compare(lambda *t: F.cross_attention(*t, scale=scale), lambda *t: R.cross_attention(*t, None, None, scale), ins, dt)
+    else:   # the gradients of q and k vanish with the scale
+        y = F.cross_attention(*ins, scale=scale)
+        assert R.rel(y, v.double().mean(1, keepdim=True).repeat_interleave(2, 2).expand(q.shape)) <= R.BOUND[dt]
+
+
+def test_second_derivatives_are_refused():
+    x = rand(4, 8).requires_grad_(True)
+    w = rand(8, 8, seed=1).requires_grad_(True)
+    g, = torch.autograd.grad(F.linear_act(x, w, act="gelu").sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_gradients_against_differences():
     """Directional differences of the float32 kernels' own outputs, in the middle of their precision: a step of 2^-9 leaves
     an error of order 2^-18 from the curvature and 2^-24 * 2^9 from rounding, relative to the output's norm."""
