@@ -18,25 +18,28 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBytesK = 128;   // bytes of contraction indices staged at a time
 
-// The activation's input, kept for its backward: float, or for bf16 a half of the same size. Its rounding, 2^-12 of the
-// value, moves act' by an eighth of what bf16's would (which cost tanh's gradients half as much again as their own
-// roundings); past +-65504 every act' is constant, and a positive value stays positive, which relu's needs.
-template <typename T>
-struct Kept;
-template <>
-struct Kept<float> {
-  __device__ static float pack(float z) { return z; }
-  __device__ static float unpack(float z) { return z; }
-};
-template <>
-struct Kept<bf16> {
-  __device__ static bf16 pack(float z) {
-    const _Float16 h = (_Float16)(z > 65504.f ? 65504.f : z < -65504.f ? -65504.f : z);   // NaN stays
-    const unsigned short b = __builtin_bit_cast(unsigned short, h);
-    return __builtin_bit_cast(bf16, (unsigned short)(z > 0.f && b == 0 ? 1 : b));
+// The activation's input, kept for its backward: float, or for bf16 a half of the same size. Its rounding (towards zero,
+// 2^-11 of the value at most, one instruction for two values, finite past +-65504 where every act' is constant) moves act'
+// by a quarter of what bf16's would, which cost tanh's gradients half as much again as their own roundings.
+template <int A>
+__device__ __forceinline__ float keep(float z) {   // a positive value stays positive, which relu's slope needs
+  return A == kActRelu && z > 0.f ? fmaxf(z, 5.9604645e-8f) : z;
+}
+template <int A>
+__device__ __forceinline__ void keep(const float (&z)[4], Chunk<float>& c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c.v[e] = z[e];
+}
+template <int A>
+__device__ __forceinline__ void keep(const float (&z)[8], Chunk<bf16>& c) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(keep<A>(z[e]), keep<A>(z[e + 1]));
+    __builtin_memcpy(c.v + e, &h, 4);
   }
-  __device__ static float unpack(bf16 z) { return (float)__builtin_bit_cast(_Float16, z); }
-};
+}
+__device__ __forceinline__ float kept(float z) { return z; }
+__device__ __forceinline__ float kept(bf16 z) { return (float)__builtin_bit_cast(_Float16, z); }
 
 struct Gemm {
   const void *A, *B;       // A(p, k), B(q, k)
@@ -54,14 +57,17 @@ struct Gemm {
 enum Epilogue { kOut, kForward, kPartial };
 
 // One operand's tile: R operand rows by KE contraction indices, global -> registers -> LDS. Stored along k it is R rows of
-// KE in LDS, across it KE rows of R; 16 bytes of padding a row keep the reads of neighbouring rows on different banks.
+// KE in LDS, across it KE rows of R. Padding keeps the reads on different banks (of 64 words): 16 bytes where 16 rows are read
+// at the same column; across k, where a read takes 4 rows of 16 words (bf16), rows lie 16 words apart or as much before
+// the next multiple of 64, and where it takes rows k and k + 4 of 32 words (float), four rows lie 32 apart.
 // A thread's chunks keep their places from tile to tile. Operand rows past the matrix are read from its last row (their
 // results are not stored); contraction indices past the end have to be zeros.
 template <typename T, int R, bool Col>
 struct Stage {
   static constexpr int V = kV<T>, KE = kBytesK / (int)sizeof(T);
   static constexpr int rows = Col ? KE : R, cols = Col ? R : KE;
-  static constexpr int ld = cols + V, cc = cols / V;                 // chunks of an LDS row
+  static constexpr int ld = !Col ? cols + V : sizeof(T) == 4 ? cols + 8 : cols % 64 == 0 ? cols + 32 : cols;
+  static constexpr int cc = cols / V;                                // chunks of an LDS row
   static constexpr int RS = kThreads / cc, per = rows / RS;          // rows from chunk to chunk of a thread
   static_assert(kThreads % cc == 0 && rows % RS == 0, "every thread stages the same number of chunks");
   Chunk<T> c[per];
@@ -206,8 +212,7 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
 #pragma unroll
           for (int e = 0; e < V; ++e) x[e] += (float)bias.v[e];
           if (g.z) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) o.v[e] = Kept<T>::pack(x[e]);
+            keep<A>(x, o);
             store_chunk((T*)g.z + (long long)q * g.P + p, o, n);
           }
 #pragma unroll
@@ -277,7 +282,12 @@ __global__ __launch_bounds__(kFewThreads) void k_few_rows(Gemm g) {
 #pragma unroll
     for (int w = 1; w < W; ++w) x += sums[w][e >> 5][c];
     if (g.bias) x += (float)((const T*)g.bias)[p];
-    if (g.z) ((T*)g.z)[(long long)q * g.P + p] = Kept<T>::pack(x);
+    if (g.z) {
+      float z[V] = {x};
+      Chunk<T> c;
+      keep<A>(z, c);
+      ((T*)g.z)[(long long)q * g.P + p] = c.v[0];
+    }
     x = act_fwd<A>(x);
     if (g.res) x += (float)((const T*)g.res)[q * g.ldr + p];
     ((T*)g.out)[(long long)q * g.P + p] = (T)x;
@@ -321,7 +331,7 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
   }
 }
 
-// g = dy act'(z) (z as Kept has it) over `per` rows a workgroup, 64 chunks of columns wide, and the rows' sums of g before
+// g = dy act'(z) (z as it was kept) over `per` rows a workgroup, 64 chunks of columns wide, and the rows' sums of g before
 // its rounding. Bound by memory: 36,864 x 1,024 bf16 with gelu 43 us (5.2 TB/s).
 template <typename T, int A>
 __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ g,
@@ -339,7 +349,7 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
     Chunk<T> o;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float x = (float)d.v[j] * act_grad<A>(Kept<T>::unpack(c.v[j]));
+      const float x = (float)d.v[j] * act_grad<A>(kept(c.v[j]));
       s[j] += x;
       o.v[j] = (T)x;
     }
