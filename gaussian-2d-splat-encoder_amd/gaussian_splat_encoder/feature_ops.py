@@ -65,71 +65,91 @@ def _launch(x, name, *args):
     which is made x's where it is another)."""
     fn, i = getattr(_lib.load(), name), x.get_device()
     if i == torch._C._cuda_getDevice():
-        rc = fn(*args, _lib.stream_ptr(i))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(i):
-            rc = fn(*args, _lib.stream_ptr(i))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     if rc:
         check(rc, name)
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ------------------------------------------------------------------------------------------------ group norm
 def _positions(x):
-    """x [B, ..., C] as [B, L, C] with dense channels (a view where the strides allow it)."""
-    B, C = x.shape[0], x.shape[-1]
-    x = x.reshape(B, math.prod(x.shape[1:-1]), C)
-    return x if C == 1 or x.stride(2) == 1 else x.contiguous()
+    """x [B, ..., C] with dense channels and positions at one distance (itself where its strides allow that), and B, L, C and
+    the distances of images and positions."""
+    shape = x.shape
+    B, C = shape[0], shape[-1]
+    L = math.prod(shape[1:-1])
+    if x.is_contiguous():
+        return x, B, L, C, L * C, C
+    x = x.reshape(B, L, C)
+    if C != 1 and x.stride(2) != 1:
+        x = x.contiguous()
+    return x, B, L, C, x.stride(0), x.stride(1)
 
 
 def _norm_fwd(x, weight, bias, G, eps, dt, act, first, save):
-    """(result like x, x as [B, L, C], statistics or None)"""
-    x3 = _positions(x)
-    B, L, C = x3.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stat = torch.empty((2, B, G), dtype=torch.float32, device=x.device) if save else None
+    """(result like x, x as _positions has it, statistics or None)"""
+    at = xp, B, L, C, sb, sl = _positions(x)
+    y = x.new_empty(x.shape)
+    stat = x.new_empty((2, B, G), dtype=torch.float32) if save else None
     if B and L:
         n = _lib.load().splat_group_norm_workspace_bytes(dt, B, L, C, G)
         keep, ws = _scratch(n, x)
-        sb, sl, _ = x3.stride()
         sp = _ptr(stat)
-        _launch(x, "splat_group_norm_fwd", x3.data_ptr(), sb, sl, _ptr(weight), _ptr(bias), dt, B, L, C, G, eps, act, first,
+        _launch(x, "splat_group_norm_fwd", xp.data_ptr(), sb, sl, _ptr(weight), _ptr(bias), dt, B, L, C, G, eps, act, first,
                 y.data_ptr(), sp, sp + 4 * B * G if save else None, ws, n)
-    return y, x3, stat
+    return y, at, stat
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, G, eps, dt, act, first):
-        y, x3, stat = _norm_fwd(x, weight, bias, G, eps, dt, act, first, True)
-        ctx.save_for_backward(x3, weight, bias, stat)
+        y, at, stat = _norm_fwd(x, weight, bias, G, eps, dt, act, first, True)
+        ctx.save_for_backward(at[0], weight, bias, stat)
         ctx.args = (x.shape, G, dt, act, first)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x3, weight, bias, stat = ctx.saved_tensors
+        x, weight, bias, stat = ctx.saved_tensors
         shape, G, dt, act, first = ctx.args
-        B, L, C = x3.shape
+        x, B, L, C, xb, xl = _positions(x)          # what a saved-tensor hook gives back may lie differently
         need = ctx.needs_input_grad
-        new = torch.empty if B and L else torch.zeros
-        dx = torch.empty(shape, dtype=x3.dtype, device=x3.device)
-        dw = new(C, dtype=torch.float32, device=x3.device) if need[1] else None
-        db = new(C, dtype=torch.float32, device=x3.device) if need[2] else None
+        new = x.new_empty if B and L else x.new_zeros
+        dx = x.new_empty(shape)
+        dw = new(C, dtype=torch.float32) if need[1] else None
+        db = new(C, dtype=torch.float32) if need[2] else None
         if B and L:
-            g3 = _positions(dy)
+            g, _, _, _, gb, gl = _positions(dy)
             n = _lib.load().splat_group_norm_bwd_workspace_bytes(dt, B, L, C, G)
-            keep, ws = _scratch(n, x3)
+            keep, ws = _scratch(n, x)
             sp = stat.data_ptr()
-            xb, xl, _ = x3.stride()
-            gb, gl, _ = g3.stride()
-            _launch(x3, "splat_group_norm_bwd", x3.data_ptr(), xb, xl, g3.data_ptr(), gb, gl, _ptr(weight), _ptr(bias), sp,
+            _launch(x, "splat_group_norm_bwd", x.data_ptr(), xb, xl, g.data_ptr(), gb, gl, _ptr(weight), _ptr(bias), sp,
                     sp + 4 * B * G, dt, B, L, C, G, act, first, dx.data_ptr(), _ptr(dw), _ptr(db), ws, n)
         return dx if need[0] else None, dw, db, None, None, None, None, None
+
+
+def _norm_param(name, t, C, x):
+    """A norm parameter as dense float32 (itself where it is that)."""
+    if t is None:
+        return None
+    if t.shape != (C,):
+        raise ValueError(f"{name} must be [{C}], got {list(t.shape)}")
+    if t.get_device() != x.get_device():
+        raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    if t.dtype is not torch.float32:
+        t = t.float()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="gelu", act_first=False):
@@ -146,14 +166,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="gelu", 
         raise ValueError(f"{C} channels do not divide into {num_groups} groups")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            if t.shape != (C,):
-                raise ValueError(f"{name} must be [{C}], got {list(t.shape)}")
-            if t.get_device() != x.get_device():
-                raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-    weight = None if weight is None else weight.float().contiguous()
-    bias = None if bias is None else bias.float().contiguous()
+    weight, bias = _norm_param("weight", weight, C, x), _norm_param("bias", bias, C, x)
     first = 1 if act_first else 0
     if _wants_grad(x, weight, bias):
         return _GroupNormAct.apply(x, weight, bias, G, float(eps), dt, code, first)
@@ -168,13 +181,13 @@ def _rows(x):
     return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
 
 
-def _linear_fwd(x, weight, bias, residual, dt, act, save):
-    """(result [..., N], x as [M, K], the activation's input or None)"""
+def _linear_fwd(x, weight, bias, residual, out, dt, act, save):
+    """(result of shape `out`, x as [M, K], the activation's input or None)"""
     x2 = _rows(x)
     M, K = x2.shape
-    N = weight.shape[0]
-    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=x.device)
-    z = torch.empty((M, N), dtype=_KEPT[x.dtype], device=x.device) if save and act else None
+    N = out[-1]
+    y = x.new_empty(out)
+    z = x.new_empty((M, N), dtype=_KEPT[x.dtype]) if save and act else None
     if M:
         r2 = None if residual is None else _rows(residual)
         _launch(x, "splat_linear_fwd", x2.data_ptr(), x2.stride(0), weight.data_ptr(), _ptr(bias), _ptr(r2),
@@ -184,8 +197,8 @@ def _linear_fwd(x, weight, bias, residual, dt, act, save):
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, dt, act):
-        y, x2, z = _linear_fwd(x, weight, bias, residual, dt, act, True)
+    def forward(ctx, x, weight, bias, residual, out, dt, act):
+        y, x2, z = _linear_fwd(x, weight, bias, residual, out, dt, act, True)
         ctx.save_for_backward(x2, weight, z)
         ctx.args = (x.shape, dt, act)
         return y
@@ -198,17 +211,17 @@ class _LinearAct(torch.autograd.Function):
         need = ctx.needs_input_grad
         M, K = x2.shape
         N = weight.shape[0]
-        new = torch.empty if M else torch.zeros
-        dx = torch.empty(shape, dtype=x2.dtype, device=x2.device) if need[0] else None
-        dw = new((N, K), dtype=x2.dtype, device=x2.device) if need[1] else None
-        db = new(N, dtype=x2.dtype, device=x2.device) if need[2] else None
+        new = x2.new_empty if M else x2.new_zeros
+        dx = x2.new_empty(shape) if need[0] else None
+        dw = new((N, K)) if need[1] else None
+        db = new(N) if need[2] else None
         if M and (need[0] or need[1] or need[2]):
             g = dy.contiguous()
             n = _lib.load().splat_linear_bwd_workspace_bytes(dt, M, N, K, act)
             keep, ws = _scratch(n, x2)
             _launch(x2, "splat_linear_bwd", x2.data_ptr(), x2.stride(0), weight.data_ptr(), g.data_ptr(), _ptr(z), dt, M, N,
                     K, act, _ptr(dx), _ptr(dw), _ptr(db), ws, n)
-        return dx, dw, db, dy if need[3] else None, None, None
+        return dx, dw, db, dy if need[3] else None, None, None, None
 
 
 def linear_act(x, weight, bias=None, act="none", residual=None):
@@ -216,14 +229,15 @@ def linear_act(x, weight, bias=None, act="none", residual=None):
     flattened), bias [N] or None, residual [..., N] or None -> [..., N]. All of one type; the product, the bias, the
     activation and the residual are added in float32 and rounded once."""
     dt, code = _args(act, x, weight, bias, residual)
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"x [..., K] and weight [N, K] are needed, got {list(x.shape)} and {list(weight.shape)}")
-    N, K = weight.shape
+    xs, ws = x.shape, weight.shape
+    if len(xs) < 1 or len(ws) != 2 or xs[-1] != ws[1]:
+        raise ValueError(f"x [..., K] and weight [N, K] are needed, got {list(xs)} and {list(ws)}")
+    N, K = ws
     if N < 1 or K < 1:
-        raise ValueError(f"weight must not be empty, got {list(weight.shape)}")
+        raise ValueError(f"weight must not be empty, got {list(ws)}")
     if bias is not None and bias.shape != (N,):
         raise ValueError(f"bias must be [{N}], got {list(bias.shape)}")
-    out = x.shape[:-1] + (N,)
+    out = xs[:-1] + (N,)
     if residual is not None and residual.shape != out:
         raise ValueError(f"residual must be {list(out)}, got {list(residual.shape)}")
     if not weight.is_contiguous():
@@ -231,8 +245,8 @@ def linear_act(x, weight, bias=None, act="none", residual=None):
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     if _wants_grad(x, weight, bias, residual):
-        return _LinearAct.apply(x, weight, bias, residual, dt, code)
-    return _linear_fwd(x, weight, bias, residual, dt, code, False)[0]
+        return _LinearAct.apply(x, weight, bias, residual, out, dt, code)
+    return _linear_fwd(x, weight, bias, residual, out, dt, code, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ cross attention
@@ -253,8 +267,8 @@ def _describe(q, k, v, lengths, mask, scale, dt):
 
 def _attention_fwd(q, k, v, lengths, mask, scale, dt, save):
     B, Lq, H, D = q.shape
-    o = torch.empty((B, Lq, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty(B * Lq * H, dtype=torch.float32, device=q.device) if save else None
+    o = q.new_empty((B, Lq, H, D))
+    lse = q.new_empty(B * Lq * H, dtype=torch.float32) if save else None
     if o.numel():
         ref = ctypes.byref(_describe(q, k, v, lengths, mask, scale, dt))
         n = _lib.load().splat_attention_workspace_bytes(ref)

@@ -316,6 +316,24 @@ def test_second_derivatives_are_refused():
         g.sum().backward()
 
 
+def test_saved_tensors_that_come_back_dense():
+    """Hooks that move what a backward keeps may give strided views back as dense tensors; the gradients stay the same."""
+    big = rand(2, 10, 12, 40)
+    calls = {"norm": (lambda v: F.group_norm_act(v, 4, act="gelu"), big[:, 1:9, 2:7, 3:27]),
+             "linear": (lambda v: F.linear_act(v, rand(8, 24, seed=1), act="silu"), big[:, :, 3, 3:27]),
+             "attention": (lambda v: F.cross_attention(rand(2, 7, 4, 24, seed=2), v, v), big[:, :, 2:4, 3:27])}
+    for name, (fn, view) in calls.items():
+        v = view.detach().requires_grad_(True)
+        assert not v.is_contiguous(), name
+        y = fn(v)
+        up = rand(*y.shape, seed=3)
+        want, = torch.autograd.grad(y, v, up)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu().contiguous(), lambda t: t.cuda()):
+            y = fn(v)
+        got, = torch.autograd.grad(y, v, up)
+        assert torch.equal(got, want), name
+
+
 def test_gradients_against_differences():
     """Directional differences of the float32 kernels' own outputs, in the middle of their precision: a step of 2^-9 leaves
     an error of order 2^-18 from the curvature and 2^-24 * 2^9 from rounding, relative to the output's norm."""
