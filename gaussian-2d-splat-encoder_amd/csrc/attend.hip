@@ -71,12 +71,17 @@ __device__ __forceinline__ const unsigned char* mask_row(const splat_attention& 
   return a.key_mask ? a.key_mask + b * a.mb : nullptr;
 }
 
-// Adds 32 x 32 scores: acc = rows of `t` (LDS) times the lanes' register rows.
-template <typename T, int DP>
-__device__ __forceinline__ void scores(f32x16& acc, const T* t, const RowFrag<T, DP>& f, int lane) {
+// Adds 32 x 32 scores: acc = rows of `t` (LDS) times the lanes' register rows. Part: D leaves the last of a row's chunks
+// empty, and the empty ones are skipped (forward and backward of 4,096 x 4,096, four heads of 40, float: 613 us instead of
+// 711; 8,192 x 8,192, heads of 80, bf16: 640 instead of 671). Kernels of their own: the branches cost heads of 64 2%.
+template <typename T, int DP, bool Part>
+__device__ __forceinline__ void scores(f32x16& acc, const T* t, const RowFrag<T, DP>& f, int D, int lane) {
+  constexpr int nc = Shape<T, DP>::nc, last = nc - 16 / kV<T>;   // the first chunk of the last 32 values holds some
 #pragma unroll
-  for (int c = 0; c < Shape<T, DP>::nc; ++c)
+  for (int c = 0; c < nc; ++c) {
+    if (Part && c > last && (c == nc - 1 || 2 * c * kV<T> >= D)) break;
     mma(acc, row_frag(t + 2 * c * kV<T>, Shape<T, DP>::ld, lane), f[c]);
+  }
 }
 
 // acc[d][lane] += sum over the 32 LDS rows from t of row[d] * p[row][lane], p as the results of scores().
@@ -313,7 +318,7 @@ __device__ __forceinline__ void softmax_step(f32x16 (&s)[KB], unsigned long long
   l += sum;
 }
 
-template <typename T, int DP, int QW>
+template <typename T, int DP, bool Part, int QW>
 __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restrict__ q, const T* __restrict__ k,
                                                        const T* __restrict__ v, T* __restrict__ o, float* __restrict__ lse,
                                                        float* __restrict__ part, float* __restrict__ stat) {
@@ -354,7 +359,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restri
     if (!live) continue;
     f32x16 s[F::KB] = {};
 #pragma unroll
-    for (int b = 0; b < F::KB; ++b) scores<T, DP>(s[b], tk + (kw + 32 * b) * S::ld, fq, lane);
+    for (int b = 0; b < F::KB; ++b) scores<T, DP, Part>(s[b], tk + (kw + 32 * b) * S::ld, fq, a.D, lane);
     softmax_step<T, DP, F::KB>(s, live, c, m, l, acc, h);
 #pragma unroll
     for (int b = 0; b < F::KB; ++b) gather<T, DP>(acc, tv + (kw + 32 * b) * S::ld, s[b], lane);
@@ -458,6 +463,21 @@ __global__ __launch_bounds__(kJoinThreads) void k_attn_join(Attn n, const float*
   }
 }
 
+// Four values of a row to its place, of which `left` are the row's.
+template <typename T>
+__device__ __forceinline__ void store_head(T* p, const float (&s)[4], int left) {
+  T x[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = (T)s[e];
+  if (left >= 4) {
+    __builtin_memcpy(p, x, sizeof(x));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) p[e] = x[e];
+  }
+}
+
 // The same for few splits (rows are many then): a thread per four values of a row. Two splits of 147,456 rows of 64: 17 us
 // (5.5 TB/s).
 template <typename T>
@@ -484,16 +504,9 @@ __global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, FastDiv by_q
   const int bh = row / n.R, r = row - bh * n.R;
   const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
   T* op = o + (((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + d;
-  T x[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = (T)(s.v[e] * inv);
-  if (d + 4 <= a.D) {
-    __builtin_memcpy(op, x, sizeof(x));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (d + e < a.D) op[e] = x[e];
-  }
+  for (int e = 0; e < 4; ++e) s.v[e] *= inv;
+  store_head(op, s.v, a.D - d);
   if (lse && d == 0) lse[row] = ml.y == 0.f ? INFINITY : ml.x + hw_log2(ml.y);
 }
 
@@ -529,7 +542,7 @@ template <typename T> constexpr int kBwdTile = sizeof(T) == 2 ? 64 : 32;
 // dk and dv: a wave holds 32 keys and values, the workgroup's four share tiles of query rows. With s = q k^T a lane is a
 // key: p and ds are the operands of dv = p^T do and dk = ds^T q as they are. 64 keys a wave would halve the LDS reads but
 // leave one wave a SIMD (1,014 us instead of 793).
-template <typename T, int DP>
+template <typename T, int DP, bool Part>
 __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __restrict__ q, const T* __restrict__ k,
                                                           const T* __restrict__ v, const T* __restrict__ g,
                                                           const float* __restrict__ lse, const float* __restrict__ delta,
@@ -611,8 +624,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
 #pragma unroll
         for (int e = 0; e < 4; ++e) dp[i + e] = D[e];
       }
-      scores<T, DP>(s, tq + rb * S::ld, fk, lane);
-      scores<T, DP>(dp, tg + rb * S::ld, fv, lane);
+      scores<T, DP, Part>(s, tq + rb * S::ld, fk, a.D, lane);
+      scores<T, DP, Part>(dp, tg + rb * S::ld, fv, a.D, lane);
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const f32x4 L = *(const f32x4*)(tl + rb + acc_row(i, h));
@@ -646,7 +659,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
 // dq: as the forward, a lane per query row; ds^T is the operand of dq^T = k^T ds^T as it is.
 // Three waves a SIMD for bf16 heads of 64 (with a few registers more there are two: 646 us instead of 578 at 36,864 rows
 // and 9,216 keys of 4 heads).
-template <typename T, int DP>
+template <typename T, int DP, bool Part>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 ? 3 : 1) void k_attn_bwd_q(Attn n, const T* __restrict__ q, const T* __restrict__ k,
                                                          const T* __restrict__ v, const T* __restrict__ g,
                                                          const float* __restrict__ lse, const float* __restrict__ delta,
@@ -682,8 +695,8 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 ? 3 : 1) void 
       f32x16 s = {}, dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] = dl;   // dp starts at -delta
-      scores<T, DP>(s, tk + k0 * S::ld, fq, lane);
-      scores<T, DP>(dp, tv + k0 * S::ld, fg, lane);
+      scores<T, DP, Part>(s, tk + k0 * S::ld, fq, a.D, lane);
+      scores<T, DP, Part>(dp, tv + k0 * S::ld, fg, a.D, lane);
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[i] *= hw_exp2(fmaf(s[i], c, L));
       if (live != (KT == 64 ? ~0ull : 0xffffffffull)) {
@@ -703,24 +716,42 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 ? 3 : 1) void 
   }
 }
 
-// Adds the splits' partial gradients in their order (seven of 9,216 keys of four heads of 64: 17 us, 4.2 TB/s). Rows of `part` are the output's own order, or (heads) the rows of
-// (image, key head) problems.
+// Adds the splits' partial gradients in their order, a thread per four values of a row, four splits asked for at a time.
+// Rows of `part` are the output's own order, or (heads) the rows of (image, key head) problems; the grid's second half in y
+// adds the rows behind them to out1. Bound by memory: two splits of 147,456 rows of 64 to bf16 15.5 us (6.1 TB/s, part of
+// it still cached; 34 with a thread a value), seven splits of twice 36,864 rows 22 us (two launches: 33).
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_attn_add(Attn n, const float* __restrict__ part, int splits, long long stride,
-                                                       long long count, bool heads, T* __restrict__ out) {
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= count) return;
-  float s = 0.f;
-  for (int k = 0; k < splits; ++k) s += part[k * stride + i];
-  long long at = i;
-  if (heads) {
-    const splat_attention& a = n.a;
-    const long long row = i / a.D;
-    const int d = (int)(i - row * a.D), bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
-    const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
-    at = (((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + d;
+__global__ __launch_bounds__(kThreads) void k_attn_add(Attn n, FastDiv by_quads, int quads, const float* __restrict__ part,
+                                                       int splits, long long stride, int rows, bool heads,
+                                                       T* __restrict__ out0, T* __restrict__ out1) {
+  const splat_attention& a = n.a;
+  const int i = blockIdx.x * kThreads + threadIdx.x, row = i / by_quads, d = (i - row * quads) * 4;
+  if (row >= rows) return;
+  const float* p = part + ((long long)blockIdx.y * rows + row) * a.D + d;
+  float s[4] = {};
+  auto add = [&](auto m, int k) {
+    constexpr int M = decltype(m)::value;
+    Chunk<float> v[M];
+#pragma unroll
+    for (int j = 0; j < M; ++j) v[j] = load_chunk(p + (k + j) * stride, a.D - d);
+#pragma unroll
+    for (int j = 0; j < M; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += v[j].v[e];
+  };
+  int k = 0;
+  for (; k + 4 <= splits; k += 4) add(std::integral_constant<int, 4>{}, k);
+  if (k + 2 <= splits) {
+    add(std::integral_constant<int, 2>{}, k);
+    k += 2;
   }
-  out[at] = (T)s;
+  if (k < splits) add(std::integral_constant<int, 1>{}, k);
+  long long at = row;
+  if (heads) {
+    const int bh = row / n.R, r = row - bh * n.R, qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
+    at = ((long long)b * a.Lq + qi) * a.H + hk * n.rep + j;
+  }
+  store_head((blockIdx.y ? out1 : out0) + at * a.D + d, s, a.D - d);
 }
 
 // ---------------------------------------------------------------------------------------------- launches
@@ -742,10 +773,14 @@ template <typename F>
 int with_shape(const splat_attention& a, F&& f) {
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (a.D <= 32) return f(T{}, std::integral_constant<int, 32>{});
-    if (a.D <= 64) return f(T{}, std::integral_constant<int, 64>{});
-    if (a.D <= 96) return f(T{}, std::integral_constant<int, 96>{});
-    return f(T{}, std::integral_constant<int, 128>{});
+    auto width = [&](auto dp) {
+      constexpr int DP = decltype(dp)::value;
+      return a.D <= DP - 2 * kV<T> ? f(t, dp, std::true_type{}) : f(t, dp, std::false_type{});
+    };
+    if (a.D <= 32) return width(std::integral_constant<int, 32>{});
+    if (a.D <= 64) return width(std::integral_constant<int, 64>{});
+    if (a.D <= 96) return width(std::integral_constant<int, 96>{});
+    return width(std::integral_constant<int, 128>{});
   };
   return a.dtype == kF32 ? go(float{}) : go(bf16{});
 }
@@ -756,8 +791,8 @@ int with_shape(const splat_attention& a, F&& f) {
 // split (64 rows and 18,432 masked bf16 keys: 16 us; 18 with four, 23 with eight).
 // A float tile takes sixteen times the matrix instructions' time: one workgroup a CU is a round there, and a split costs
 // about one tile. Where lengths or a mask, which only the device knows, may leave workgroups idle, more of them even out
-// what is left: two rounds are added to the estimate (dk and dv of 3 x 1,201 x 777, two heads of 40, one image empty: 67 us;
-// 97 with half the splits).
+// what is left: two rounds are added to the estimate (dk and dv of 3 x 1,201 x 777, two heads of 40, one image empty, took
+// 97 us with half the splits and 67 with these; 59 since empty chunks are skipped).
 void split(Attn& n, long long groups, int tiles, int slots) {
   n.splits = 1;
   n.per = tiles < 1 ? 1 : tiles;
@@ -849,12 +884,13 @@ int splat_attention_fwd(const splat_attention* a, const void* q, const void* k, 
   float* part = need ? (float*)ws : nullptr;
   float* stat = need ? part + (size_t)n.splits * rows * a->D : nullptr;
   const hipStream_t st = (hipStream_t)stream;
-  return with_shape(*a, [&](auto t, auto dp) {
+  return with_shape(*a, [&](auto t, auto dp, auto some) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
+    constexpr bool Part = decltype(some)::value;
     const int grid = n.tiles * n.splits * a->B * a->Hk;
     auto go = [&](auto w) {
-      k_attn_fwd<T, DP, decltype(w)::value><<<grid, kThreads, 0, st>>>(n, (const T*)q, (const T*)k, (const T*)v, (T*)o, lse,
+      k_attn_fwd<T, DP, Part, decltype(w)::value><<<grid, kThreads, 0, st>>>(n, (const T*)q, (const T*)k, (const T*)v, (T*)o, lse,
                                                                        part, stat);
     };
     if (qw == 1) go(std::integral_constant<int, 1>{});
@@ -895,27 +931,31 @@ int splat_attention_bwd(const splat_attention* a, const void* q, const void* k, 
   float* delta = (float*)ws;
   float* part = (float*)((char*)ws + up(sizeof(float) * rows));
   const hipStream_t st = (hipStream_t)stream;
-  return with_shape(*a, [&](auto t, auto dp) {
+  return with_shape(*a, [&](auto t, auto dp, auto some) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
+    constexpr bool Part = decltype(some)::value;
     const T *tq = (const T*)q, *tk = (const T*)k, *tv = (const T*)v, *tg = (const T*)g;
     if (rows) k_attn_delta<T><<<div_up(rows, kThreads / 8), kThreads, 0, st>>>(nk, (const T*)o, tg, delta);
+    // rows that are split fill the card a few times at most: their values' quads are 32-bit
+    const int quads = (a->D + 3) / 4;
+    auto wgs = [&](long long r) { return (unsigned)div_up(r * quads, kThreads); };
     if (a->Lk > 0) {
-      const long long cnt = (long long)a->B * a->Lk * a->Hk * a->D;
+      const long long keys = (long long)a->B * a->Lk * a->Hk;
       float* pk = nk.splits > 1 ? part : nullptr;
-      k_attn_bwd_kv<T, DP><<<nk.tiles * nk.splits * a->B * a->Hk, kThreads, 0, st>>>(nk, tq, tk, tv, tg, lse, delta, (T*)dk,
-                                                                                     (T*)dv, pk);
-      if (pk) {
-        k_attn_add<T><<<div_up(cnt, kThreads), kThreads, 0, st>>>(nk, pk, nk.splits, 2 * cnt, cnt, false, (T*)dk);
-        k_attn_add<T><<<div_up(cnt, kThreads), kThreads, 0, st>>>(nk, pk + cnt, nk.splits, 2 * cnt, cnt, false, (T*)dv);
-      }
+      k_attn_bwd_kv<T, DP, Part><<<nk.tiles * nk.splits * a->B * a->Hk, kThreads, 0, st>>>(nk, tq, tk, tv, tg, lse, delta,
+                                                                                           (T*)dk, (T*)dv, pk);
+      if (pk)
+        k_attn_add<T><<<dim3(wgs(keys), 2), kThreads, 0, st>>>(nk, fast_div(quads), quads, pk, nk.splits, 2 * keys * a->D,
+                                                               (int)keys, false, (T*)dk, (T*)dv);
     }
     if (a->Lq > 0) {
-      const long long cnt = rows * a->D;
       float* pq = nq.splits > 1 ? part : nullptr;
-      k_attn_bwd_q<T, DP><<<nq.tiles * nq.splits * a->B * a->Hk, kThreads, 0, st>>>(nq, tq, tk, tv, tg, lse, delta, (T*)dq,
-                                                                                    pq);
-      if (pq) k_attn_add<T><<<div_up(cnt, kThreads), kThreads, 0, st>>>(nq, pq, nq.splits, cnt, cnt, true, (T*)dq);
+      k_attn_bwd_q<T, DP, Part><<<nq.tiles * nq.splits * a->B * a->Hk, kThreads, 0, st>>>(nq, tq, tk, tv, tg, lse, delta,
+                                                                                          (T*)dq, pq);
+      if (pq)
+        k_attn_add<T><<<wgs(rows), kThreads, 0, st>>>(nq, fast_div(quads), quads, pq, nq.splits, rows * a->D, (int)rows, true,
+                                                      (T*)dq, (T*)nullptr);
     }
     return check_launch("splat_attention_bwd");
   });
