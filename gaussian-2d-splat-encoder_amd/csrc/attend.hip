@@ -660,10 +660,10 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
 // Three waves a SIMD for bf16 heads of 64 (with a few registers more there are two: 646 us instead of 578 at 36,864 rows
 // and 9,216 keys of 4 heads).
 template <typename T, int DP, bool Part>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 ? 3 : 1) void k_attn_bwd_q(Attn n, const T* __restrict__ q, const T* __restrict__ k,
-                                                         const T* __restrict__ v, const T* __restrict__ g,
-                                                         const float* __restrict__ lse, const float* __restrict__ delta,
-                                                         T* __restrict__ dq, float* __restrict__ part) {
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 ? 3 : 1)
+void k_attn_bwd_q(Attn n, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ g,
+                  const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dq,
+                  float* __restrict__ part) {
   using S = Shape<T, DP>;
   constexpr int KT = kBwdTile<T>, tile = KT * S::ld;
   __shared__ __align__(16) T tiles[4 * tile];
