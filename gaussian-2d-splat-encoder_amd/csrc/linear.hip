@@ -6,7 +6,7 @@
 // floats. A long contraction with few outputs (dW) is cut into slices whose partial sums a second launch adds in order.
 //
 // Measured at 36,864 rows, bf16 (a large library product reaches 1,394 TFLOP/s here, a large copy 4.9 TB/s): 256 -> 1,024
-// 42 us (460 TFLOP/s, 2.2 TB/s), 64 us with gelu and its input kept; its dx 38 us (510), dW 40 us (480) and 10 us to join 32
+// 42 us (460 TFLOP/s, 2.2 TB/s), 50 us with gelu and its input kept; its dx 36 us (535), dW 39 us (490) and 10 us to join 32
 // slices. 1,024 -> 1,024: 105 us (735). float, 1,024 -> 1,024: 594 us (130 of 153). Operands reach the matrix units through
 // one LDS buffer and registers: three workgroups a CU hide the barriers better than two buffers with two workgroups (117 us
 // instead of 105) or smaller tiles (124 us).
