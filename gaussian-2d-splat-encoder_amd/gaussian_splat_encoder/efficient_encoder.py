@@ -16,7 +16,9 @@ reference's, because checkpoints trained there must load strictly and produce th
 
 Two options have no counterpart in the reference and are off by default: `channels_last` runs every stage's GELU and
 norm as one kernel and the heads' 1x1 convolutions as products with their activation, on channels-last features;
-`fine_reader_heads` lets the fine cells read the deepest map (cell_reader.py).
+`fine_reader_heads` lets the fine cells read the deepest map (cell_reader.py). Under bfloat16 autocast channels-last
+features stay bfloat16 between the stages, where torch's own norms would return float32; under float16 autocast they are
+float32. Positions, the background's mean and its product are float32 either way.
 
 All rendering goes through this package's HIP renderer. `stage_marks` (optional callable taking a stage name)
 is called at the stage boundaries of `forward` so a harness can time backbone / coarse render / fine head.
@@ -61,11 +63,14 @@ def _conv_stage(cin: int, cout: int, k: int, norm_type: str) -> nn.Sequential:
 
 
 def _run_stage(stage: nn.Sequential, x, channels_last: bool):
-    """A conv -> GELU -> norm stage; with channels_last the GELU and the norm are one kernel."""
+    """A conv -> GELU -> norm stage; with channels_last the GELU and the norm are one kernel, in the convolution's type
+    (under float16 autocast, a type that the kernels do not have, in float32)."""
     if not channels_last:
         return stage(x)
     conv, _, norm = stage
     y = conv(x).permute(0, 2, 3, 1)
+    if y.dtype is torch.float16 and norm.weight.dtype is torch.float32:
+        y = y.float()
     return group_norm_act(y, norm.num_groups, norm.weight, norm.bias, norm.eps, act="gelu",
                           act_first=True).permute(0, 3, 1, 2)
 
@@ -193,14 +198,15 @@ class _SplatHead(nn.Module):
 
     def _forward_channels_last(self, feat):
         """forward on channels-last cells: an output's channels are (slot, value), so that a cell's values already lie in
-        the splats' order."""
+        the splats' order. Positions are float32 whatever the features' type: bfloat16 centres of 96 cells in a row would
+        be off by up to two pixels of 768."""
         B, _, fH, fW = feat.shape
         M, n = self.M, fH * fW * self.M
         cells = feat.permute(0, 2, 3, 1)
-        ys = torch.linspace(0.5 / fH, 1 - 0.5 / fH, fH, device=feat.device, dtype=feat.dtype)
-        xs = torch.linspace(0.5 / fW, 1 - 0.5 / fW, fW, device=feat.device, dtype=feat.dtype)
+        ys = torch.linspace(0.5 / fH, 1 - 0.5 / fH, fH, device=feat.device, dtype=torch.float32)
+        xs = torch.linspace(0.5 / fW, 1 - 0.5 / fW, fW, device=feat.device, dtype=torch.float32)
         base = torch.stack(torch.meshgrid(ys, xs, indexing="ij"), -1).reshape(1, fH * fW, 1, 2)
-        off = self._product(cells, self.mu_head, "tanh").reshape(B, fH * fW, M, 2)
+        off = self._product(cells, self.mu_head, "tanh").float().reshape(B, fH * fW, M, 2)
         mu = (base + off * (self.offset_cells / max(fH, fW))).reshape(B, n, 2).clamp(0.005, 0.995)
         ls = self._product(cells, self.scale_head, "none").reshape(B, n, 2)
         col = self._product(cells, self.color_head, "sigmoid").reshape(B, n, self.color_dim)
@@ -325,7 +331,7 @@ class EfficientGaussianEncoder(nn.Module):
             x = x.contiguous(memory_format=torch.channels_last)
         feat, skips = self.backbone(x)
         fused = self._with_grad(feat, image)
-        pooled = feat.mean(dim=(2, 3))
+        pooled = feat.mean(dim=(2, 3), dtype=torch.float32 if self.channels_last else None)
         if self.channels_last:
             bg = linear_act(pooled, self.bg_head.weight.to(pooled.dtype), self.bg_head.bias.to(pooled.dtype),
                             act="sigmoid")
