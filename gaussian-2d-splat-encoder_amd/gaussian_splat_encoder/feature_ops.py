@@ -3,8 +3,9 @@ backward: group norm with an activation, products with an epilogue, cross attent
 
 Tensors are float32 or bfloat16 on a HIP device, the last dimension dense (anything else is copied first); sums, softmax
 statistics and norms are float32 whatever the type. Results are deterministic: no atomics, fixed orders of summation.
-Everything runs on the current stream and returns without waiting. Device work goes through libsplat_hip.so
-(include/splat_render.h). The reference has no counterpart: its network runs on stock torch operations.
+Everything runs on the current stream and returns without waiting. Gradients are reverse-mode, of first order (forward-mode
+and second derivatives are refused). Device work goes through libsplat_hip.so (include/splat_render.h). The reference has
+no counterpart: its network runs on stock torch operations.
 
 Activations: "none", "gelu" (x Phi(x)), "silu", "relu", "tanh", "sigmoid".
 """
@@ -15,6 +16,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import SplatAttention, check
@@ -74,6 +76,11 @@ def _launch(x, name, *args):
 
 
 def _wants_grad(*ts):
+    """Whether a backward may follow. Tangents, which say nothing in requires_grad, are refused."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the HIP feature operators have no forward-mode derivatives")
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:

@@ -1,0 +1,35 @@
+"""Calls that the feature operators refuse, and layouts that they promise, at the edges (CPU; no kernel runs)."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from gaussian_splat_encoder import feature_ops as F
+
+
+class Dev(torch.Tensor):
+    """A host tensor that says it is on a device: the checks before any launch are what is tested."""
+    is_cuda = True
+
+
+def t(*shape):
+    return torch.zeros(*shape).as_subclass(Dev)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("call,n", [
+    (lambda *a: F.group_norm_act(a[0], 2, a[1], a[2]), 3),
+    (lambda *a: F.linear_act(a[0], a[1], a[2], residual=a[3]), 4),
+    (lambda *a: F.cross_attention(*a), 3)])
+def test_forward_mode_is_refused(call, n, grad):
+    """A tangent on any input: a result without one would be a wrong derivative."""
+    norm = call.__code__.co_names[1] == "group_norm_act"
+    shapes = ([(1, 4, 8), (8,), (8,)] if norm else [(2, 4), (3, 4), (3,), (2, 3)] if n == 4 else
+              [(1, 2, 1, 8), (1, 3, 1, 8), (1, 3, 1, 8)])
+    for i in range(n):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            a = [t(*s) for s in shapes]
+            a[i] = forward_ad.make_dual(a[i], torch.ones_like(a[i])).as_subclass(Dev)
+            assert forward_ad.unpack_dual(a[i]).tangent is not None
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(*a)
