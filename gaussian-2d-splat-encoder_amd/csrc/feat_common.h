@@ -66,14 +66,14 @@ __device__ __forceinline__ float act_fwd(float x) {
   }
 }
 
-// d act / dx at x.
+// d act / dx at x; `factor` is x, or a finite value in the place of an infinite one.
 template <int A>
-__device__ __forceinline__ float act_grad(float x) {
+__device__ __forceinline__ float act_grad(float x, float factor) {
   if constexpr (A == kActGelu) {
-    return fmaf(x, normal_pdf(x), normal_cdf(x));
+    return fmaf(factor, normal_pdf(x), normal_cdf(x));
   } else if constexpr (A == kActSilu) {
     const float s = sigmoidf(x);
-    return fmaf(x * s, 1.f - s, s);
+    return fmaf(factor * s, 1.f - s, s);
   } else if constexpr (A == kActRelu) {
     return x > 0.f ? 1.f : 0.f;
   } else if constexpr (A == kActTanh) {
@@ -86,6 +86,8 @@ __device__ __forceinline__ float act_grad(float x) {
     return 1.f;
   }
 }
+template <int A>
+__device__ __forceinline__ float act_grad(float x) { return act_grad<A>(x, x); }
 
 // Calls f with the activation as a compile-time constant.
 template <typename F>

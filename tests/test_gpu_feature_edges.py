@@ -1,0 +1,47 @@
+"""The feature operators on the GPU where sizes, types and values are at an end of their range."""
+
+import math
+
+import pytest
+import torch
+
+from gaussian_splat_encoder import feature_ops as F
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.mark.parametrize("M", [4096, 16384])
+def test_slopes_keep_their_mean(M):
+    """The bias gradient of tanh over bfloat16 rows, against its formula, in the mean over 1,024 columns of different sizes.
+    Rounding the kept input to the nearest half goes either way and leaves that mean; the results' own rounding to bfloat16
+    moves it by 2^-8 / sqrt(12) / sqrt(1024) = 3.5e-5 of standard deviation at most, and 1.5e-4 is four times that. Cutting
+    bits of the input off would move every slope one way, by 2 tanh(z) 2^-12 = 3e-4 for inputs from 0.5 to 1."""
+    z = torch.rand(M, 1024, generator=torch.Generator("cuda").manual_seed(4), device="cuda") * 0.5 + 0.5
+    hi = z.bfloat16()
+    lo = (z - hi.float()).bfloat16()   # the product adds the two exactly: inputs of more bits than a half's 11
+    w = torch.eye(64, device="cuda", dtype=torch.bfloat16).repeat(1, 2)
+    up = (1 + torch.arange(1024, device="cuda") % 128 / 128).bfloat16()
+    got = []
+    for c in range(0, 1024, 64):
+        b = torch.zeros(64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        y = F.linear_act(torch.cat([hi[:, c:c + 64], lo[:, c:c + 64]], 1), w, b, act="tanh")
+        got.append(torch.autograd.grad(y, b, up[c:c + 64].expand_as(y))[0].double())
+    want = (up.double() * (1 - torch.tanh(hi.double() + lo.double()) ** 2)).sum(0)
+    off = (torch.cat(got) / want - 1).mean().abs().item()
+    print(f"mean error of the slopes {off:.1e}", flush=True)
+    assert off < 1.5e-4
+
+
+def test_kept_inputs_hold_nan_and_infinities():
+    """NaN in a row reaches its gradient; infinite inputs of gelu and silu have the limits' slopes, past a half's range too."""
+    w = torch.eye(4, device="cuda", dtype=torch.bfloat16)
+    for name, want in (("gelu", (1, 0)), ("silu", (1, 0)), ("relu", (1, 0)), ("tanh", (0, 0)), ("sigmoid", (0, 0))):
+        for dt in TYPES:
+            x = torch.tensor([[7e4, -7e4, 3e38, -3e38], [0, 0, math.nan, 0]], device="cuda", dtype=dt).requires_grad_(True)
+            y = F.linear_act(x, w.to(dt), act=name)
+            g, = torch.autograd.grad(y, x, torch.ones_like(y))
+            assert g[0].tolist() == [want[0], want[1]] * 2, (name, dt, g)
+            if name != "relu":
+                assert torch.isnan(g[1]).all(), (name, dt, g)
