@@ -30,9 +30,19 @@ struct Norm {
   int nch, RT;                       // chunks of a tile; positions a workgroup takes at a time
   int splits;                        // ranges of positions
   long long per;                     // positions of a range
-  FastDiv by_nch, by_RT, by_Cg;
+  FastDiv by_nch, by_RT, by_Cg, by_splits, by_tiles;
   float eps;
 };
+
+// A workgroup's work: ranges of a tile follow each other, tiles of an image, images. (One grid dimension: the others hold
+// 65,535, fewer than the images of a norm per token.)
+struct Unit {
+  int img, tile, split;
+};
+__device__ __forceinline__ Unit unit(const Norm& n) {
+  const int id = blockIdx.x, u = id / n.by_splits, img = u / n.by_tiles;
+  return {img, u - img * n.tiles, id - u * n.splits};
+}
 
 // A thread's place: its channels [c, c + nv) of the map, its first position rt and its positions of the range [lo, hi).
 struct Place {
@@ -164,8 +174,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_whole(Norm n, const T* __rest
                                                          float* __restrict__ mean, float* __restrict__ rstd) {
   __shared__ float2 red[kThreads * kV<T>];
   __shared__ float gm[kTile], gr[kTile];
-  const int img = blockIdx.y;
-  const Place p = place<T>(n, blockIdx.x, 0);
+  const Unit u = unit(n);
+  const int img = u.img, tile = u.tile, split = u.split;
+  const Place p = place<T>(n, tile, split);
   const T* xp = x + (long long)img * n.xsb + (long long)p.rt * n.xsl + p.c;
   Chunk<T> keep[Keep];
 #pragma unroll
@@ -228,8 +239,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_whole(Norm n, const T* __rest
 template <typename T, int A, bool First>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(Norm n, const T* __restrict__ x, float4* __restrict__ part) {
   __shared__ float2 red[kThreads * kV<T>];
-  const int img = blockIdx.z, split = blockIdx.x;
-  const Place p = place<T>(n, blockIdx.y, split);
+  const Unit u = unit(n);
+  const int img = u.img, tile = u.tile, split = u.split;
+  const Place p = place<T>(n, tile, split);
   RowStream<T, 4, false> xs;
   xs.begin(x + (long long)img * n.xsb + (p.lo + p.rt) * n.xsl + p.c, n.RT * n.xsl, nullptr, 0, p.rows, p.nv);
   float k0[kV<T>] = {}, s[kV<T>] = {}, q[kV<T>] = {};
@@ -252,7 +264,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(Norm n, const T* __rest
     q[j] = d > 0.f || d != d ? d : 0.f;   // rounding may leave less than zero; NaN stays
     k0[j] = fmaf(s[j], inv, k0[j]);
   }
-  const int slots = n.splits * n.tpg, slot = split * n.tpg + (n.tpg > 1 ? blockIdx.y % n.tpg : 0);
+  const int slots = n.splits * n.tpg, slot = split * n.tpg + (n.tpg > 1 ? tile % n.tpg : 0);
   group_stats<T>(n, p, k0, q, red, [&](int g, float mu, float m2) {
     part[((long long)img * n.G + p.g0 + g) * slots + slot] =
         make_float4((float)(p.hi - p.lo) * (float)(n.tpg == 1 ? n.Cg : p.ct), mu, m2, 0.f);
@@ -266,8 +278,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(Norm n, const T* __rest
                                                          T* __restrict__ y, float* __restrict__ mean,
                                                          float* __restrict__ rstd) {
   __shared__ float gm[kTile], gr[kTile];
-  const int img = blockIdx.z, split = blockIdx.x;
-  const Place p = place<T>(n, blockIdx.y, split);
+  const Unit u = unit(n);
+  const int img = u.img, tile = u.tile, split = u.split;
+  const Place p = place<T>(n, tile, split);
   RowStream<T, 4, false> xs;
   xs.begin(x + (long long)img * n.xsb + (p.lo + p.rt) * n.xsl + p.c, n.RT * n.xsl, nullptr, 0, p.rows, p.nv);
   float wj[kV<T>], bj[kV<T>], m[kV<T>];
@@ -294,7 +307,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(Norm n, const T* __rest
     if (lane == 0) {
       gm[g] = mu;
       gr[g] = r;
-      if (mean && split == 0 && (n.tpg == 1 || blockIdx.y % n.tpg == 0)) {
+      if (mean && split == 0 && (n.tpg == 1 || tile % n.tpg == 0)) {
         mean[(long long)img * n.G + p.g0 + g] = mu;
         rstd[(long long)img * n.G + p.g0 + g] = r;
       }
@@ -351,8 +364,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_sums(Norm n, const T* __r
                                                             const float* __restrict__ rstd, float* __restrict__ cpart,
                                                             float* __restrict__ gpart) {
   __shared__ float2 red[kThreads * kV<T>], chan[kTile];
-  const int img = blockIdx.z, split = blockIdx.x;
-  const Place p = place<T>(n, blockIdx.y, split);
+  const Unit u = unit(n);
+  const int img = u.img, tile = u.tile, split = u.split;
+  const Place p = place<T>(n, tile, split);
   RowStream<T, 2, true> xs;
   xs.begin(x + (long long)img * n.xsb + (p.lo + p.rt) * n.xsl + p.c, n.RT * n.xsl,
            dy + (long long)img * n.gsb + (p.lo + p.rt) * n.gsl + p.c, n.RT * n.gsl, p.rows, p.nv);
@@ -402,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_sums(Norm n, const T* __r
     }
   }
   __syncthreads();
-  const int slots = n.splits * n.tpg, slot = split * n.tpg + (n.tpg > 1 ? blockIdx.y % n.tpg : 0);
+  const int slots = n.splits * n.tpg, slot = split * n.tpg + (n.tpg > 1 ? tile % n.tpg : 0);
   const int wide = n.tpg > 1 ? p.ct : n.Cg, lane = threadIdx.x & 63;
   for (int g = threadIdx.x >> 6; g < p.ng; g += kThreads / 64) {
     float a = 0.f, q = 0.f;
@@ -420,7 +434,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_sums(Norm n, const T* __r
   }
 }
 
-// dx of one range; in the workgroups past the maps' (blockIdx.z == B) the parameters' gradients, 32 channels each.
+// dx of one range; in the workgroups past the maps' (image B) the parameters' gradients, 32 channels each.
 template <typename T, int A, bool First>
 __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __restrict__ x, const T* __restrict__ dy,
                                                              const float* __restrict__ w, const float* __restrict__ b,
@@ -430,10 +444,11 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
                                                              const float* __restrict__ gpart, T* __restrict__ dx,
                                                              float* __restrict__ dw, float* __restrict__ db) {
   __shared__ float ga[kTile], gb[kTile];
-  const int img = blockIdx.z;
+  const Unit u = unit(n);
+  const int img = u.img, tile = u.tile, split = u.split;
   if (img == n.B) {
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, nrow = kThreads / 32;
-    for (int c0 = (blockIdx.y * gridDim.x + blockIdx.x) * 32; c0 < n.C; c0 += 32 * gridDim.x * gridDim.y) {
+    for (int c0 = (tile * n.splits + split) * 32; c0 < n.C; c0 += 32 * n.tiles * n.splits) {
       const int c = c0 + lane;
       float a = 0.f, q = 0.f;
       if (c < n.C) {
@@ -459,8 +474,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
     }
     return;
   }
-  const int split = blockIdx.x;
-  const Place p = place<T>(n, blockIdx.y, split);
+  const Place p = place<T>(n, tile, split);
   RowStream<T, 2, true> xs;
   xs.begin(x + (long long)img * n.xsb + (p.lo + p.rt) * n.xsl + p.c, n.RT * n.xsl,
            dy + (long long)img * n.gsb + (p.lo + p.rt) * n.gsl + p.c, n.RT * n.gsl, p.rows, p.nv);
@@ -539,6 +553,8 @@ Norm plan(int B, long long L, int C, int G, bool want_whole, bool* whole) {
   }
   n.by_nch = fast_div(n.nch);
   n.by_RT = fast_div(n.RT);
+  n.by_tiles = fast_div(n.tiles);
+  n.by_splits = fast_div(1);
   if (*whole) return n;
   // 512 workgroups, the two per CU that registers allow at a time, of at least a batch of rows of their threads
   const long long want = 512 / ((long long)B * n.tiles) > 0 ? 512 / ((long long)B * n.tiles) : 1;
@@ -547,14 +563,21 @@ Norm plan(int B, long long L, int C, int G, bool want_whole, bool* whole) {
   if (n.per < batch) n.per = batch;
   if (n.per > (1LL << 30)) n.per = 1LL << 30;   // a range's rows are counted in 32 bits
   n.splits = (int)((L + n.per - 1) / n.per);
+  n.by_splits = fast_div(n.splits);
   return n;
+}
+
+// Workgroups of `images` images, 0 where a launch (2^32 threads) does not hold them.
+unsigned grid_of(const Norm& n, long long images) {
+  const long long per = (long long)n.tiles * n.splits;
+  return per < (1 << 23) && images * per < (1 << 23) ? (unsigned)(images * per) : 0;
 }
 
 int check_norm(const char* what, int dtype, int B, long long L, int C, int G, int act) {
   if (dtype != kF32 && dtype != kBf16) return set_error(kInvalid, "%s: unknown element type %d", what, dtype);
   if (B < 0 || L < 0 || C < 1 || G < 1 || C % G) return set_error(kInvalid, "%s: B %d, L %lld, C %d, G %d", what, B, L, C, G);
   if (act < 0 || act >= kActCount) return set_error(kInvalid, "%s: unknown activation %d", what, act);
-  if (B > 65534 || L > 0x7fffffffLL * 4) return set_error(kUnsupported, "%s: %d images of %lld positions", what, B, L);
+  if (L > 0x7fffffffLL * 4) return set_error(kUnsupported, "%s: %d images of %lld positions", what, B, L);
   return kOk;
 }
 
@@ -593,7 +616,8 @@ int splat_group_norm_fwd(const void* x, long long xsb, long long xsl, const floa
   const size_t need = whole ? 0 : sizeof(float4) * (size_t)B * G * n.splits * n.tpg;
   if (need && (!ws || ws_bytes < need))
     return set_error(kWorkspace, "splat_group_norm_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
-  if (n.tiles > 65535) return set_error(kUnsupported, "splat_group_norm_fwd: %d channel tiles", n.tiles);
+  const unsigned grid = grid_of(n, B);
+  if (!grid) return set_error(kUnsupported, "splat_group_norm_fwd: %d images of %d channel tiles", B, n.tiles);
   const hipStream_t st = (hipStream_t)stream;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -603,14 +627,13 @@ int splat_group_norm_fwd(const void* x, long long xsb, long long xsl, const floa
         constexpr bool First = decltype(f)::value;
         if (whole) {
           auto whole_of = [&](auto keep) {
-            k_norm_whole<T, A, First, decltype(keep)::value><<<dim3(n.tiles, B), kThreads, 0, st>>>(
+            k_norm_whole<T, A, First, decltype(keep)::value><<<grid, kThreads, 0, st>>>(
                 n, (const T*)x, weight, bias, (T*)y, mean, rstd);
           };
           if (L <= 4LL * n.RT) whole_of(std::integral_constant<int, 4>{});
           else if (L <= 8LL * n.RT) whole_of(std::integral_constant<int, 8>{});
           else whole_of(std::integral_constant<int, kKeep>{});
         } else {
-          const dim3 grid(n.splits, n.tiles, B);
           k_norm_stats<T, A, First><<<grid, kThreads, 0, st>>>(n, (const T*)x, (float4*)ws);
           k_norm_apply<T, A, First><<<grid, kThreads, 0, st>>>(n, (const T*)x, weight, bias, (const float4*)ws, (T*)y, mean,
                                                                rstd);
@@ -642,7 +665,8 @@ int splat_group_norm_bwd(const void* x, long long xsb, long long xsl, const void
   const size_t need = splat_group_norm_bwd_workspace_bytes(dtype, B, L, C, G);
   if (!ws || ws_bytes < need)
     return set_error(kWorkspace, "splat_group_norm_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
-  if (n.tiles > 65535) return set_error(kUnsupported, "splat_group_norm_bwd: %d channel tiles", n.tiles);
+  const unsigned maps = grid_of(n, B), all = grid_of(n, B + (dweight || dbias ? 1LL : 0));   // parameters come last
+  if (!all) return set_error(kUnsupported, "splat_group_norm_bwd: %d images of %d channel tiles", B, n.tiles);
   float* cpart = (float*)ws;
   float* gpart = cpart + 2 * (size_t)B * n.splits * C;
   const hipStream_t st = (hipStream_t)stream;
@@ -652,9 +676,9 @@ int splat_group_norm_bwd(const void* x, long long xsb, long long xsl, const void
       constexpr int A = decltype(a)::value;
       auto go = [&](auto f) {
         constexpr bool First = decltype(f)::value;
-        k_norm_bwd_sums<T, A, First><<<dim3(n.splits, n.tiles, B), kThreads, 0, st>>>(
+        k_norm_bwd_sums<T, A, First><<<maps, kThreads, 0, st>>>(
             n, (const T*)x, (const T*)dy, weight, bias, mean, rstd, cpart, gpart);
-        k_norm_bwd_apply<T, A, First><<<dim3(n.splits, n.tiles, B + (dweight || dbias ? 1 : 0)), kThreads, 0, st>>>(
+        k_norm_bwd_apply<T, A, First><<<all, kThreads, 0, st>>>(
             n, (const T*)x, (const T*)dy, weight, bias, mean, rstd, cpart, gpart, (T*)dx, dweight, dbias);
         return check_launch("splat_group_norm_bwd");
       };

@@ -164,7 +164,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="gelu", 
 
     act_first=False: act(weight * norm(x) + bias). act_first=True: weight * norm(act(x)) + bias, the order of the encoder's
     stages (conv -> GELU -> norm). The mean and the biased variance run over the C / num_groups channels of a group and all
-    positions of an image. weight and bias [C] may be None; they are used, and their gradients returned, in float32."""
+    positions of an image (a norm per token: B tokens of no positions, [B, C]; millions of images fit a launch). weight and
+    bias [C] may be None; they are used, and their gradients returned, in float32."""
     dt, code = _args(act, x)
     if x.dim() < 2:
         raise ValueError(f"x must be [B, ..., C], got {list(x.shape)}")

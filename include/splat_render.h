@@ -311,7 +311,8 @@ int splat_exact_render_bwd(const float *rec, const float *reach, int N, int C, c
 
 /* y[B, L, C] = group norm over G groups of C / G channels and all L positions of an image, then act (act_first = 0), or
  * of act(x) (act_first = 1). x has strides xsb (images) and xsl (positions), dense channels; y is contiguous; weight[C] and
- * bias[C] may be NULL. mean[B, G] and rstd[B, G] (both or neither) are what the backward takes.
+ * bias[C] may be NULL. mean[B, G] and rstd[B, G] (both or neither) are what the backward takes. An image takes one workgroup or
+ * more, a launch holds fewer than 2^23 (status 3 beyond).
  * Backward: dx contiguous, dweight[C], dbias[C] (NULL skips), dy with strides gsb, gsl. */
 size_t splat_group_norm_workspace_bytes(int dtype, int B, long long L, int C, int G);
 int splat_group_norm_fwd(const void *x, long long xsb, long long xsl, const float *weight, const float *bias, int dtype,

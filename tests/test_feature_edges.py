@@ -4,6 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from gaussian_splat_encoder import _lib
 from gaussian_splat_encoder import feature_ops as F
 
 
@@ -33,3 +34,12 @@ def test_forward_mode_is_refused(call, n, grad):
             assert forward_ad.unpack_dual(a[i]).tangent is not None
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call(*a)
+
+
+def test_norm_of_many_images():
+    """An image per token: 92,160 splat latents, and as many as a launch holds."""
+    lib = _lib.load()
+    assert lib.splat_group_norm_bwd_workspace_bytes(0, 92160, 1, 64, 8) > 0
+    norm = lambda B, C: lib.splat_group_norm_fwd(256, C, C, None, None, 0, B, 1, C, 1, 1e-5, 0, 0, 256, None,  # noqa: E731
+                                                 None, None, 0, None)
+    assert norm(1 << 23, 8) == 3 and norm((1 << 31) - 1, 8) == 3

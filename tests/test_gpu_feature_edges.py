@@ -5,11 +5,33 @@ import math
 import pytest
 import torch
 
+import _feature_ref as R
 from gaussian_splat_encoder import feature_ops as F
 
 pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float32, torch.bfloat16]
+
+
+def rand(*shape, dt=torch.float32, seed=0, scale=1.0, shift=0.0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale + shift).to(dt)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape,G", [((70000, 24), 4), ((65536, 3, 16), 2), ((92160, 1, 20), 20)])
+def test_norm_of_many_images(dt, shape, G):
+    """More images than a grid's second and third dimensions hold: one norm per token."""
+    x, w, b = rand(*shape, dt=dt, shift=0.2), rand(shape[-1], seed=1, scale=0.3, shift=1.0), rand(shape[-1], seed=2)
+    a = [t.requires_grad_(True) for t in (x, w, b)]
+    d = [t.detach().double().requires_grad_(True) for t in (x, w, b)]
+    y, z = F.group_norm_act(a[0], G, a[1], a[2], act="gelu"), R.group_norm_act(*d[:1], G, *d[1:], 1e-5, "gelu", False)
+    g = rand(*shape, dt=dt, seed=3)
+    got, want = torch.autograd.grad(y, a, g), torch.autograd.grad(z, d, g.double())
+    errs = [R.rel(p, q) for p, q in zip((y, *got), (z, *want))]
+    assert all(e <= R.BOUND[dt] for e in errs), errs
+    if dt is torch.float32:   # the far end, element by element
+        assert torch.allclose(y[-5:].double(), z[-5:], atol=1e-5)
 
 
 @pytest.mark.parametrize("M", [4096, 16384])
