@@ -19,6 +19,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
+constexpr long long kMaxThreads = 1LL << 32;   // a launch holds fewer
 constexpr int kBytesK = 128;   // bytes of contraction indices staged at a time
 
 // The activation's input, kept for its backward: float, or for bf16 a half of the same size. Its rounding (to the nearest,
@@ -380,7 +381,7 @@ template <typename T, int PB, int QB, int WP, int WQ, bool ACol, bool BCol, int 
 int launch(Gemm g, int slices, hipStream_t st) {
   g.tp = div_up(g.P, PB * WP * 32);
   g.tq = div_up(g.Q, QB * WQ * 32);
-  if ((long long)g.tp * g.tq >= 1 << 24)   // a launch holds 2^32 threads
+  if ((long long)g.tp * g.tq >= kMaxThreads / kThreads)
     return set_error(kUnsupported, "product of %d x %d outputs", g.Q, g.P);
   k_gemm<T, PB, QB, WP, WQ, ACol, BCol, Epi, A><<<dim3(g.tp * g.tq, slices), kThreads, 0, st>>>(g);
   return kOk;
@@ -452,6 +453,8 @@ int splat_linear_fwd(const void* x, long long ldx, const void* weight, const voi
     return with_act(act, [&](auto a) {
       constexpr int A = decltype(a)::value;
       if (M <= 32 || (long long)div_up(N, 32) * div_up(M, 32) <= few_tiles<T>) {
+        if (div_up(N, 32) >= kMaxThreads / kFewThreads)
+          return set_error(kUnsupported, "splat_linear_fwd: %d outputs of %lld rows", N, M);
         k_few_rows<T, A><<<dim3(div_up(N, 32), div_up(M, 32)), kFewThreads, 0, (hipStream_t)stream>>>(g);
         return check_launch("splat_linear_fwd");
       }
@@ -478,6 +481,9 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
   const size_t need = splat_linear_bwd_workspace_bytes(dtype, M, N, K, act);
   if (need && (!ws || ws_bytes < need))
     return set_error(kWorkspace, "splat_linear_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  // the join of a weight gradient: four values a thread
+  const long long n = dweight ? (long long)N * K : 0, wgs = (n + 1023) / 1024, bwgs = dbias ? div_up(N, 32) : 0;
+  if (wgs + bwgs >= kMaxThreads / 256) return set_error(kUnsupported, "splat_linear_bwd: a weight of %d x %d", N, K);
   const hipStream_t st = (hipStream_t)stream;
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -516,9 +522,7 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
         g.bpart = act == kActNone ? bpart : nullptr;
         if (const int rc = gemm<T, true, true, kPartial, 0>(g, s, st)) return rc;
       }
-      const long long n = dweight ? (long long)N * K : 0;
-      const unsigned wgs = div_up(n, 1024), bwgs = dbias ? div_up(N, 32) : 0;
-      k_join<T><<<wgs + bwgs, 256, 0, st>>>(part, s, n, (T*)dweight, wgs, bpart, bslices, N, (T*)dbias);
+      k_join<T><<<(unsigned)(wgs + bwgs), 256, 0, st>>>(part, s, n, (T*)dweight, (unsigned)wgs, bpart, bslices, N, (T*)dbias);
     }
     return check_launch("splat_linear_bwd");
   });

@@ -36,6 +36,16 @@ def test_forward_mode_is_refused(call, n, grad):
                 call(*a)
 
 
+def test_products_that_a_launch_cannot_hold():
+    """2^32 threads and more: an answer before any launch."""
+    lib = _lib.load()
+    lin = lambda M, N, K: lib.splat_linear_fwd(256, K, 256, None, None, 0, 1, M, N, K, 0, 256, None, None)  # noqa: E731
+    assert lin(1, 1 << 28, 1) == 3 and lin(32, 1 << 30, 8) == 3
+    bwd = lambda M, N, K: lib.splat_linear_bwd(256, K, 256, 256, None, 1, M, N, K, 0, None, 256, None, 256,  # noqa: E731
+                                               1 << 60, None)
+    assert bwd(1, 1 << 18, 1 << 17) == 3
+
+
 def test_norm_of_many_images():
     """An image per token: 92,160 splat latents, and as many as a launch holds."""
     lib = _lib.load()
