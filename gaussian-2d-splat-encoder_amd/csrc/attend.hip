@@ -856,6 +856,9 @@ Attn plan_q(const splat_attention& a) {
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// A split forward's workspace: two statistics of every split and row, then the partial rows.
+size_t stat_bytes(const Attn& n) { return up(2 * sizeof(float) * (size_t)n.splits * n.a.B * n.a.Hk * n.R); }
+
 }  // namespace
 }  // namespace splat
 
@@ -867,7 +870,7 @@ size_t splat_attention_workspace_bytes(const splat_attention* a) {
   if (check_attn("splat_attention_workspace_bytes", a) || a->B == 0 || a->Lq == 0) return 0;
   int qw;
   const Attn n = plan_fwd(*a, &qw);
-  return n.splits == 1 ? 0 : sizeof(float) * (size_t)n.splits * a->B * a->Hk * n.R * (a->D + 2);
+  return n.splits == 1 ? 0 : stat_bytes(n) + sizeof(float) * (size_t)n.splits * a->B * a->Hk * n.R * a->D;
 }
 
 int splat_attention_fwd(const splat_attention* a, const void* q, const void* k, const void* v, void* o, float* lse,
@@ -881,8 +884,8 @@ int splat_attention_fwd(const splat_attention* a, const void* q, const void* k, 
   if (need && (!ws || ws_bytes < need))
     return set_error(kWorkspace, "splat_attention_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
   const long long rows = (long long)a->B * a->Hk * n.R;
-  float* part = need ? (float*)ws : nullptr;
-  float* stat = need ? part + (size_t)n.splits * rows * a->D : nullptr;
+  float* stat = need ? (float*)ws : nullptr;
+  float* part = need ? (float*)((char*)ws + stat_bytes(n)) : nullptr;
   const hipStream_t st = (hipStream_t)stream;
   return with_shape(*a, [&](auto t, auto dp, auto some) {
     using T = decltype(t);

@@ -1,5 +1,7 @@
 """Calls that the feature operators refuse, and layouts that they promise, at the edges (CPU; no kernel runs)."""
 
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -44,6 +46,17 @@ def test_products_that_a_launch_cannot_hold():
     bwd = lambda M, N, K: lib.splat_linear_bwd(256, K, 256, 256, None, 1, M, N, K, 0, None, 256, None, 256,  # noqa: E731
                                                1 << 60, None)
     assert bwd(1, 1 << 18, 1 << 17) == 3
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("D,Lq", [(33, 77), (1, 301), (127, 3), (64, 16)])
+def test_attention_statistics_are_aligned(dtype, D, Lq):
+    """The workspace holds two statistics of every split and row, then (from a multiple of 256 bytes) D values of each:
+    neither depends on how the other divides."""
+    a = _lib.SplatAttention(dtype, 1, 1, 1, D, 0.125, Lq, 20001)
+    n = _lib.load().splat_attention_workspace_bytes(ctypes.byref(a))
+    splits = [s for s in range(2, 513) if n == (8 * s * Lq + 255) // 256 * 256 + 4 * s * Lq * D]
+    assert len(splits) == 1
 
 
 def test_norm_of_many_images():
