@@ -72,14 +72,20 @@ __device__ __forceinline__ const unsigned char* mask_row(const splat_attention& 
 }
 
 // Adds 32 x 32 scores: acc = rows of `t` (LDS) times the lanes' register rows. Part: D leaves the last of a row's chunks
-// empty, and the empty ones are skipped (forward and backward of 4,096 x 4,096, four heads of 40, float: 613 us instead of
-// 711; 8,192 x 8,192, heads of 80, bf16: 640 instead of 671). Kernels of their own: the branches cost heads of 64 2%.
+// empty, and the empty ones are skipped (4,096 x 4,096, four heads, forward and backward, float: heads of 40 617 us instead
+// of 714, of 112 1,246 instead of 1,301; bf16: of 80 204 instead of 211, of 112 249 instead of 285). Kernels of their own:
+// the branches cost heads of 64 2%. The loop has to unroll, as the rows' registers have no addresses: with more than eight
+// chunks a row a way out of it keeps it rolled and the rows in memory (heads of 112, float: 2,432 us), so those are skipped
+// one by one; the way out is 1% faster where it does unroll.
 template <typename T, int DP, bool Part>
 __device__ __forceinline__ void scores(f32x16& acc, const T* t, const RowFrag<T, DP>& f, int D, int lane) {
   constexpr int nc = Shape<T, DP>::nc, last = nc - 16 / kV<T>;   // the first chunk of the last 32 values holds some
 #pragma unroll
   for (int c = 0; c < nc; ++c) {
-    if (Part && c > last && (c == nc - 1 || 2 * c * kV<T> >= D)) break;
+    if (Part && c > last && (c == nc - 1 || 2 * c * kV<T> >= D)) {
+      if constexpr (nc <= 8) break;
+      else continue;
+    }
     mma(acc, row_frag(t + 2 * c * kV<T>, Shape<T, DP>::ld, lane), f[c]);
   }
 }
