@@ -766,6 +766,7 @@ int check_attn(const char* what, const splat_attention* a) {
   if (a->dtype != kF32 && a->dtype != kBf16) return set_error(kInvalid, "%s: unknown element type %d", what, a->dtype);
   if (a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->H < 1 || a->Hk < 1 || a->H % a->Hk || a->D < 1)
     return set_error(kInvalid, "%s: B %d, Lq %lld, Lk %lld, H %d, Hk %d, D %d", what, a->B, a->Lq, a->Lk, a->H, a->Hk, a->D);
+  if (!(fabsf(a->scale) <= 3.40282347e+38f)) return set_error(kInvalid, "%s: scale %g", what, (double)a->scale);
   if (a->D > 128) return set_error(kUnsupported, "%s: heads of %d values (128 at most)", what, a->D);
   // rows and keys are 32-bit within a head, workgroups 32-bit in all
   const long long heads = (long long)a->B * a->Hk, rows = a->Lq * (a->H / a->Hk);

@@ -25,6 +25,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _KEPT = {torch.float32: torch.float32, torch.bfloat16: torch.float16}   # type of an activation's input for its backward
 _ACTS = {"none": 0, "gelu": 1, "silu": 2, "relu": 3, "tanh": 4, "sigmoid": 5}
 MAX_HEAD = 128   # values of a head at most
+_MAX_FLOAT = torch.finfo(torch.float32).max
 
 
 def _args(act, x, *others):
@@ -343,6 +344,8 @@ def cross_attention(q, k, v, kv_lengths=None, key_mask=None, scale=None):
         raise ValueError(f"key_mask must be [{B}, {Lk}] bool on {q.device}, got {list(key_mask.shape)} {key_mask.dtype} on "
                          f"{key_mask.device}")
     scale = D ** -0.5 if scale is None else float(scale)
+    if not abs(scale) <= _MAX_FLOAT:
+        raise ValueError(f"scale must be a finite float32, got {scale}")
     if _wants_grad(q, k, v):
         return _CrossAttention.apply(q, k, v, kv_lengths, key_mask, scale, dt)
     return _attention_fwd(_dense(q), _dense(k), _dense(v), kv_lengths, key_mask, scale, dt, False)[0]

@@ -340,7 +340,7 @@ int splat_linear_bwd(const void *x, long long ldx, const void *weight, const voi
  * [B, Hk, Lq H / Hk] (or NULL) is what the backward takes; dq, dk and dv are contiguous. */
 typedef struct splat_attention {
   int dtype, B, H, Hk, D;                          /* element type; images; query heads; key heads; values per head */
-  float scale;                                     /* of the scores */
+  float scale;                                     /* of the scores, finite */
   long long Lq, Lk;                                /* queries and keys of an image */
   long long qb, ql, qh, kb, kl, kh, vb, vl, vh;    /* elements from image to image, token to token, head to head */
   long long gb, gl, gh;                            /* the same of the output's gradient (backward) */

@@ -1,6 +1,7 @@
 """Calls that the feature operators refuse, and layouts that they promise, at the edges (CPU; no kernel runs)."""
 
 import ctypes
+import math
 
 import pytest
 import torch
@@ -36,6 +37,16 @@ def test_forward_mode_is_refused(call, n, grad):
             assert forward_ad.unpack_dual(a[i]).tangent is not None
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call(*a)
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 1e39])
+def test_attention_scale_has_to_be_finite(scale):
+    with pytest.raises(ValueError, match="scale"):
+        F.cross_attention(t(1, 2, 1, 8), t(1, 3, 1, 8), t(1, 3, 1, 8), scale=scale)
+    a = _lib.SplatAttention(0, 1, 1, 1, 8, scale, 2, 3)
+    lib = _lib.load()
+    assert lib.splat_attention_fwd(ctypes.byref(a), 256, 256, 256, 256, None, None, 0, None) == 1
+    assert b"scale" in lib.splat_last_error()
 
 
 def test_products_that_a_launch_cannot_hold():
