@@ -10,6 +10,8 @@ all splats of an image (EfficientGaussianEncoder.gather_splat_latents). The refe
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn as nn
 
@@ -52,12 +54,16 @@ class CellReader(nn.Module):
         """The layer's product in x's type (float32 weights are rounded for bfloat16 features)."""
         return linear_act(x, layer.weight.to(x.dtype), layer.bias.to(x.dtype), act=act, residual=residual)
 
+    @staticmethod
+    def _tokens(t):
+        """Images and tokens of an image of t [B, ..., C]."""
+        return t.shape[0], math.prod(t.shape[1:-1])
+
     def keys_values(self, states):
         """[B, Lk, 2, kv_heads, head_dim] of states [B, ..., state_channels]: what a program keeps where many calls read
         the same states (forward's `kv`)."""
-        B = states.shape[0]
         kv = self._product(states, self.to_kv)
-        return kv.reshape(B, -1, 2, self.kv_heads, self.head_dim)
+        return kv.reshape(self._tokens(states) + (2, self.kv_heads, self.head_dim))
 
     def forward(self, x, states=None, kv_lengths=None, key_mask=None, kv=None):
         """x [B, ..., channels], states [B, ..., state_channels] (or kv from keys_values) -> like x. kv_lengths [B] and
@@ -67,7 +73,7 @@ class CellReader(nn.Module):
         if kv is None:
             kv = self.keys_values(states)
         q = self._product(self._norm(x, self.norm1), self.to_q)
-        q = q.reshape(x.shape[0], -1, self.heads, self.head_dim)
+        q = q.reshape(self._tokens(x) + (self.heads, self.head_dim))
         a = cross_attention(q, kv[:, :, 0], kv[:, :, 1], kv_lengths=kv_lengths, key_mask=key_mask)
         x = self._product(a.reshape(x.shape[:-1] + (self.heads * self.head_dim,)), self.to_out, residual=x)
         return self._product(self._product(self._norm(x, self.norm2), self.fc1, act="gelu"), self.fc2, residual=x)

@@ -7,6 +7,7 @@ import torch
 
 import _feature_ref as R
 from gaussian_splat_encoder import feature_ops as F
+from gaussian_splat_encoder.cell_reader import CellReader
 
 pytestmark = pytest.mark.gpu
 
@@ -32,6 +33,18 @@ def test_norm_of_many_images(dt, shape, G):
     assert all(e <= R.BOUND[dt] for e in errs), errs
     if dt is torch.float32:   # the far end, element by element
         assert torch.allclose(y[-5:].double(), z[-5:], atol=1e-5)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_reader_of_no_images(dt):
+    """An empty batch gives an empty batch, forward and backward, as the operators do."""
+    m = CellReader(32, 16).cuda()
+    x = torch.zeros(0, 4, 5, 32, device="cuda", dtype=dt, requires_grad=True)
+    y = m(x, torch.zeros(0, 3, 16, device="cuda", dtype=dt))
+    gx, = torch.autograd.grad(y.sum(), x)
+    assert y.shape == x.shape and y.dtype is dt and gx.shape == x.shape
+    none = m(torch.randn(2, 0, 32, device="cuda").to(dt), torch.randn(2, 0, 16, device="cuda").to(dt))
+    assert none.shape == (2, 0, 32)
 
 
 @pytest.mark.parametrize("M", [4096, 16384])
