@@ -82,6 +82,80 @@ def test_kept_inputs_hold_nan_and_infinities():
                 assert torch.isnan(g[1]).all(), (name, dt, g)
 
 
+@pytest.mark.parametrize("name", ["gelu", "silu", "relu", "tanh", "sigmoid"])
+def test_activations_point_by_point(name):
+    """float32 activations over a fine grid, the product being the value itself. An error of 2^-20 (9.5e-7) at most: half a
+    unit of results up to 8 (2.4e-7), a unit of the reciprocal times x (6e-8 * 8), half of one of its argument, and 7e-8 of
+    gelu's fit."""
+    x = torch.linspace(-8, 8, 1 << 20, device="cuda")[:, None]
+    y = F.linear_act(x, torch.ones(1, 1, device="cuda"), act=name)
+    err = (y.double() - R.act(x.double(), name)).abs()
+    print(f"{name}: {err.max().item():.2e} at x = {x[err.argmax()].item():.3f}", flush=True)
+    assert err.max().item() <= 2.0 ** -20
+
+
+def test_norm_offsets_past_32_bits():
+    """One image of more than 2^31 values, whose last 4,000 rows are values of their own and, negated, the rows of the first
+    half's end: outputs and gradients there are the negated ones exactly, as the mean is zero and all sums are alike."""
+    M = 2 ** 31 // 32 + 4099
+    half = M // 2 + 1
+    x = torch.empty(1, 2 * half, 32, device="cuda", dtype=torch.bfloat16)
+    x[0, :half] = rand(1, 32, dt=torch.bfloat16)
+    x[0, half - 4000:half] = rand(4000, 32, dt=torch.bfloat16, seed=1)
+    x[0, half:] = -x[0, :half]
+    assert (2 * half - 4000) * 32 > 2 ** 31
+    x.requires_grad_(True)
+    y = F.group_norm_act(x, 1, act="none")
+    far, near = y[0, -4000:].float(), y[0, half - 4000:half].float()
+    # the sums of the two halves come in other orders: a mean of 2^-24 of the deviation may be left
+    ref = rand(4000, 32, dt=torch.bfloat16, seed=1).float() / x.detach()[0, :half].float().square().mean().sqrt()
+    assert (far + near).abs().max() <= 2.0 ** -7 * near.abs().max() and R.rel(near, ref) <= R.BOUND[torch.bfloat16]
+    assert R.rel(far, -ref) <= R.BOUND[torch.bfloat16]
+    g = torch.zeros_like(y)
+    g[0, -4000:] = rand(4000, 32, dt=torch.bfloat16, seed=2)
+    g[0, half - 4000:half] = -g[0, -4000:]
+    dx, = torch.autograd.grad(y, x, g)
+    # the gradient's sums vanish against 2^31 values: dx is g / deviation but for 4,000 * 32 terms over them
+    rstd = 1 / x.detach()[0, :half].float().square().mean().sqrt()
+    want = g[0, -4000:].float() * rstd
+    assert R.rel(dx[0, -4000:], want) <= R.BOUND[torch.bfloat16]
+    assert R.rel(dx[0, half - 4000:half], -want) <= R.BOUND[torch.bfloat16]
+    assert dx[0, :half - 4000].abs().max() <= 1e-3
+
+
+def test_linear_gradient_offsets_past_32_bits():
+    """Rows and their gradients of more than 2^31 values: the far end gives what the same rows give alone."""
+    M = 2 ** 31 // 32 + 4099
+    x = torch.zeros(M, 32, device="cuda", dtype=torch.bfloat16)
+    x[-300:] = rand(300, 32, dt=torch.bfloat16, seed=3)
+    w = rand(32, 32, dt=torch.bfloat16, seed=1, scale=0.2)
+    g = torch.zeros(M, 32, device="cuda", dtype=torch.bfloat16)
+    g[-300:] = rand(300, 32, dt=torch.bfloat16, seed=5)
+
+    def grads(x, g):
+        a = [x.detach().requires_grad_(True), w.detach().requires_grad_(True)]
+        return torch.autograd.grad(F.linear_act(*a, act="gelu"), a, g)
+
+    (dx, dw), (tx, tw) = grads(x, g), grads(x[-300:].clone(), g[-300:].clone())
+    bound = R.BOUND[torch.bfloat16]
+    assert R.rel(dx[-300:], tx) <= bound and R.rel(dw, tw) <= bound and not dx[:-300].any()
+
+
+def test_attention_gradient_offsets_past_32_bits():
+    """Queries, keys, values and the output's gradient whose rows lie 40,000 values apart, over 2^31 values in all: the bits
+    of dense copies, forward and backward."""
+    big = torch.zeros(60000, 40000, device="cuda", dtype=torch.bfloat16)
+    big[:, :256] = rand(60000, 256, dt=torch.bfloat16, seed=5)
+    views = [big[None, :, None, i:i + 64] for i in (0, 64, 128, 192)]
+
+    def grads(q, k, v, g):
+        a = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        y = F.cross_attention(*a)
+        return [y, *torch.autograd.grad(y, a, g)]
+
+    assert all(torch.equal(a, b) for a, b in zip(grads(*views), grads(*[t.contiguous() for t in views])))
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("D,full", [(80, 96), (88, 96), (112, 128), (120, 128)])
 def test_attention_of_part_heads_costs_no_more(dt, D, full):
