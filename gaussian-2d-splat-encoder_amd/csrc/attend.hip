@@ -123,6 +123,12 @@ __device__ __forceinline__ Work work_of(const Attn& n) {
   return w;
 }
 
+// Place `at` of what the outputs' rounding left, null where that is not kept (floats, inference).
+template <typename T>
+__device__ __forceinline__ T* rest_of(const splat_attention& a, long long at) {
+  return sizeof(T) == 2 && a.rest ? (T*)a.rest + at : nullptr;
+}
+
 // Address of row r's head vector in a tensor of strides (sb, sl, sh).
 template <typename T>
 __device__ __forceinline__ const T* head_row(const void* p, const Attn& n, const Work& w, int r, long long sb, long long sl,
@@ -244,9 +250,14 @@ struct KeyTiles {
   }
 };
 
-// Writes the lane's row of DP values, scaled, from the accumulators.
+// What rounding x to o leaves.
+template <typename O>
+__device__ __forceinline__ O left_of(float x, O o) { return (O)(x - (float)o); }
+
+// Writes the lane's row of DP values, scaled, from the accumulators; to `rest`, unless null, what rounding them leaves.
 template <typename T, typename O, int DP>
-__device__ __forceinline__ void store_row(O* row, const RowAcc<T, DP>& acc, float s, int D, bool in, int h) {
+__device__ __forceinline__ void store_row(O* row, const RowAcc<T, DP>& acc, float s, int D, bool in, int h,
+                                          O* rest = nullptr) {
 #pragma unroll
   for (int d = 0; d < Shape<T, DP>::nd; ++d) {
     float run[16 / kV<O>][kV<O>];
@@ -258,6 +269,12 @@ __device__ __forceinline__ void store_row(O* row, const RowAcc<T, DP>& acc, floa
 #pragma unroll
       for (int e = 0; e < kV<O>; ++e) o.v[e] = (O)(run[t][e] * s);
       if (in) store_chunk(row + c, o, D - c);
+      if (in && rest) {
+        Chunk<O> r;
+#pragma unroll
+        for (int e = 0; e < kV<O>; ++e) r.v[e] = left_of(run[t][e] * s, o.v[e]);
+        store_chunk(rest + c, r, D - c);
+      }
     }
   }
 }
@@ -410,7 +427,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restri
     const float inv = l > 0.f ? 1.f / l : l;   // 0 for a row without keys, NaN stays
     if (lse && in && h == 0) lse[(long long)w.bh * n.R + r] = l == 0.f ? INFINITY : m + hw_log2(l);
     const int qi = r / n.by_rep, j = r - qi * n.rep;
-    store_row<T, T, DP>(o + ((w.b * a.Lq + qi) * a.H + w.hk * n.rep + j) * a.D, acc, inv, a.D, in, h);
+    const long long at = ((w.b * a.Lq + qi) * a.H + w.hk * n.rep + j) * a.D;
+    store_row<T, T, DP>(o + at, acc, inv, a.D, in, h, rest_of<T>(a, at));
   }
 }
 
@@ -465,7 +483,9 @@ __global__ __launch_bounds__(kJoinThreads) void k_attn_join(Attn n, const float*
     for (int i = 1; i < GS; ++i) s += sums[i * W + threadIdx.x];
     const int bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
     const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
-    o[(((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + threadIdx.x] = (T)(s * total);
+    const long long at = (((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + threadIdx.x;
+    o[at] = (T)(s * total);
+    if (T* r = rest_of<T>(a, at)) *r = left_of(s * total, o[at]);
   }
 }
 
@@ -509,15 +529,23 @@ __global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, FastDiv by_q
   const float inv = ml.y > 0.f ? 1.f / ml.y : ml.y;
   const int bh = row / n.R, r = row - bh * n.R;
   const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hk = bh % a.Hk;
-  T* op = o + (((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + d;
+  const long long at = (((long long)b * a.Lq + qi) * a.H + hk * n.rep + j) * a.D + d;
 #pragma unroll
   for (int e = 0; e < 4; ++e) s.v[e] *= inv;
-  store_head(op, s.v, a.D - d);
+  store_head(o + at, s.v, a.D - d);
+  if (T* r = rest_of<T>(a, at)) {
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = s.v[e] - (float)(T)s.v[e];
+    store_head(r, x, a.D - d);
+  }
   if (lse && d == 0) lse[row] = ml.y == 0.f ? INFINITY : ml.x + hw_log2(ml.y);
 }
 
 // ----------------------------------------------------------------------------------------------- backward
-// delta[row] = sum over d of do * o, which the score gradients p (dp - delta) take. Bound by memory: 147,456 rows of 64 bf16
+// delta[row] = sum over d of do * o, which the score gradients p (dp - delta) take, o with what its rounding left: where a few
+// keys hold most of a row's weight, dp - delta is far smaller than either, and a bf16 output's rounding four times the
+// gradients' own (8 keys, heads of 32: dq 5.9e-3 off instead of 2.3e-3). Bound by memory: 147,456 rows of 64 bf16
 // 12 us (3.2 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_attn_delta(Attn n, const T* __restrict__ o, const T* __restrict__ g,
@@ -528,13 +556,19 @@ __global__ __launch_bounds__(kThreads) void k_attn_delta(Attn n, const T* __rest
   if (row >= (long long)a.B * a.Hk * n.R) return;
   const int bh = (int)(row / n.R), r = (int)(row - (long long)bh * n.R);
   const int qi = r / n.by_rep, j = r - qi * n.rep, b = bh / a.Hk, hq = bh % a.Hk * n.rep + j;
-  const T* op = o + (((long long)b * a.Lq + qi) * a.H + hq) * a.D;
+  const long long at = (((long long)b * a.Lq + qi) * a.H + hq) * a.D;
+  const T *op = o + at, *rp = rest_of<T>(a, at);
   const T* gp = g + b * a.gb + qi * a.gl + hq * a.gh;
   float s = 0.f;
   for (int d = (threadIdx.x & 7) * kV<T>; d < a.D; d += 8 * kV<T>) {
     const Chunk<T> x = load_chunk(op + d, a.D - d), y = load_chunk(gp + d, a.D - d);
 #pragma unroll
     for (int e = 0; e < kV<T>; ++e) s = fmaf((float)x.v[e], (float)y.v[e], s);
+    if (rp) {
+      const Chunk<T> r = load_chunk(rp + d, a.D - d);
+#pragma unroll
+      for (int e = 0; e < kV<T>; ++e) s = fmaf((float)r.v[e], (float)y.v[e], s);
+    }
   }
   s += __shfl_xor(s, 1, 64);
   s += __shfl_xor(s, 2, 64);

@@ -11,5 +11,6 @@ typedef struct splat_attention {
   long long mb, ml;                                // key_mask: bytes from image to image and from key to key
   const int* kv_lengths;                           // [B] keys of each image that count, the first ones; or NULL
   const unsigned char* key_mask;                   // [B, Lk], 0: the key is left out; or NULL
+  void* rest;                                      // bfloat16: what the outputs' rounding left, [B, Lq, H, D]; or NULL
 } splat_attention;
 }

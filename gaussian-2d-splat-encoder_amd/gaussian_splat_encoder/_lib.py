@@ -34,7 +34,7 @@ class SplatAttention(ctypes.Structure):
     _fields_ = [("dtype", _I), ("B", _I), ("H", _I), ("Hk", _I), ("D", _I), ("scale", _F), ("Lq", _LL), ("Lk", _LL),
                 ("qb", _LL), ("ql", _LL), ("qh", _LL), ("kb", _LL), ("kl", _LL), ("kh", _LL),
                 ("vb", _LL), ("vl", _LL), ("vh", _LL), ("gb", _LL), ("gl", _LL), ("gh", _LL),
-                ("mb", _LL), ("ml", _LL), ("kv_lengths", _VP), ("key_mask", _VP)]
+                ("mb", _LL), ("ml", _LL), ("kv_lengths", _VP), ("key_mask", _VP), ("rest", _VP)]
 
 
 _LV = ctypes.POINTER(SplatLevels)

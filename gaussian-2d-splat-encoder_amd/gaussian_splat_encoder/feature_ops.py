@@ -275,36 +275,41 @@ def _describe(q, k, v, lengths, mask, scale, dt):
 
 
 def _attention_fwd(q, k, v, lengths, mask, scale, dt, save):
+    """(result, log sums, what the rounding to bfloat16 left of the result; the two None where no backward follows)"""
     B, Lq, H, D = q.shape
     o = q.new_empty((B, Lq, H, D))
     lse = q.new_empty(B * Lq * H, dtype=torch.float32) if save else None
+    rest = torch.empty_like(o) if save and dt else None
     if o.numel():
-        ref = ctypes.byref(_describe(q, k, v, lengths, mask, scale, dt))
+        a = _describe(q, k, v, lengths, mask, scale, dt)
+        a.rest = _ptr(rest)
+        ref = ctypes.byref(a)
         n = _lib.load().splat_attention_workspace_bytes(ref)
         keep, ws = _scratch(n, q)
         _launch(q, "splat_attention_fwd", ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), ws, n)
-    return o, lse
+    return o, lse, rest
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, mask, scale, dt):
         q, k, v = _dense(q), _dense(k), _dense(v)
-        o, lse = _attention_fwd(q, k, v, lengths, mask, scale, dt, True)
-        ctx.save_for_backward(q, k, v, o, lse, lengths, mask)
+        o, lse, rest = _attention_fwd(q, k, v, lengths, mask, scale, dt, True)
+        ctx.save_for_backward(q, k, v, o, lse, rest, lengths, mask)
         ctx.args = (scale, dt)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        q, k, v, o, lse, lengths, mask = ctx.saved_tensors
+        q, k, v, o, lse, rest, lengths, mask = ctx.saved_tensors
         scale, dt = ctx.args
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         if dq.numel() or dk.numel():
             g = _dense(g)
             a = _describe(q, k, v, lengths, mask, scale, dt)
             a.gb, a.gl, a.gh = g.stride()[:3]
+            a.rest = _ptr(rest)
             ref = ctypes.byref(a)
             n = _lib.load().splat_attention_bwd_workspace_bytes(ref)
             keep, ws = _scratch(n, q)

@@ -181,3 +181,19 @@ def test_attention_of_part_heads_costs_no_more(dt, D, full):
     part, whole = min(times[D]), min(times[full])
     print(f"{dt}: heads of {D} {part / 4:.3f} ms, of {full} {whole / 4:.3f} ms", flush=True)
     assert part < 1.5 * whole
+
+
+@pytest.mark.parametrize("B,Lq,Lk,H,Hk,D,scale", [(2, 300, 8, 4, 4, 32, 1.5), (3, 600, 71, 4, 2, 40, 1.5)])
+def test_attention_gradients_round_twice(B, Lq, Lk, H, Hk, D, scale):
+    """bfloat16 results carry two roundings: the probabilities' or score gradients' before the second product, and their
+    own. A rounding is 1.66e-3 in the 2-norm of normal values, two are 2.35e-3, three (the output's, which the score
+    gradients are taken against) 2.9e-3, and more where a few keys hold most of the weight: 2.6e-3 lies between."""
+    dt = torch.bfloat16
+    kv = rand(B, Lk, 2, Hk, D, dt=dt, seed=1)
+    a = [t.requires_grad_(True) for t in (rand(B, Lq, H, D, dt=dt, scale=scale), kv[:, :, 0].clone(), kv[:, :, 1].clone())]
+    d = [t.detach().double().requires_grad_(True) for t in a]
+    y, z, g = F.cross_attention(*a), R.cross_attention(*d, None, None, D ** -0.5), rand(B, Lq, H, D, dt=dt, seed=3)
+    got, want = torch.autograd.grad(y, a, g), torch.autograd.grad(z, d, g.double())
+    errs = [R.rel(p, q) for p, q in zip((y, *got), (z, *want))]
+    print(" ".join(f"{e:.2e}" for e in errs), flush=True)
+    assert max(errs) <= 2.6e-3
