@@ -5,7 +5,7 @@
 // rows per (image, key head). Scores are held transposed, a lane per query (forward, dq) or per key (dk, dv), so that a
 // softmax row is one lane pair and the probabilities are the next product's operand as they leave the first. One pass
 // over the keys with a running maximum and sum; sums, statistics and accumulators are 32-bit floats, probabilities and
-// score gradients are rounded to the inputs' type for the matrix instructions only.
+// score gradients are rounded to the inputs' type for the matrix instructions only (or taken as two values of it).
 //
 // Keys that a length or a mask leaves out are replaced by zeros as they are loaded, so that nothing they hold (NaN
 // included) reaches a product; a row without valid keys gives zeros, and zero gradients.
@@ -23,6 +23,15 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kMaxSplits = 512;
+
+// Probabilities and score gradients are operands of the second products and rounded to bf16 for them, once: results of many
+// terms then are 2.35e-3 off where their own rounding is 1.66e-3. Few terms or few results do not average that (up to twice
+// a result's own rounding), and score gradients of short heads lose more against the keys' weighted mean, which their sum
+// of zero leaves out (dq of heads of 16 2.7e-3, of 40 2.5e-3, of 64 2.4e-3). Both are taken as sums of two bf16 values there
+// (1.66e-3): in the forward of at most 64 rows, where memory is waited for (a token of 92,160 keys 24.8 -> 25.9 us), in the
+// backward of at most kFineRows rows or keys (162 -> 163 us for 4 x 64 rows of 18,432 keys), and for dq of heads of at most
+// kFineHead (8,192 x 8,192, four heads, forward and backward: of 32 261 -> 288 us, of 48 354 -> 387).
+constexpr int kFineRows = 128, kFineHead = 48;
 
 struct Attn {
   splat_attention a;
@@ -90,18 +99,29 @@ __device__ __forceinline__ void scores(f32x16& acc, const T* t, const RowFrag<T,
   }
 }
 
-// acc[d][lane] += sum over the 32 LDS rows from t of row[d] * p[row][lane], p as the results of scores().
-template <typename T, int DP>
+// What rounding x to o leaves.
+template <typename O>
+__device__ __forceinline__ O left_of(float x, O o) { return (O)(x - (float)o); }
+
+// acc[d][lane] += sum over the 32 LDS rows from t of row[d] * p[row][lane], p as the results of scores(). Fine: p as the sum
+// of two bf16 values, its rounding and what that leaves.
+template <typename T, int DP, bool Fine>
 __device__ __forceinline__ void gather(RowAcc<T, DP>& acc, const T* t, const f32x16& p, int lane) {
   constexpr int V = kV<T>;
 #pragma unroll
   for (int c = 0; c < 16 / V; ++c) {
-    Chunk<T> b;
+    Chunk<T> b, r;
 #pragma unroll
-    for (int j = 0; j < V; ++j) b.v[j] = (T)p[c * V + j];
+    for (int j = 0; j < V; ++j) {
+      b.v[j] = (T)p[c * V + j];
+      if (Fine) r.v[j] = left_of(p[c * V + j], b.v[j]);
+    }
 #pragma unroll
-    for (int d = 0; d < Shape<T, DP>::nd; ++d)
-      mma(acc[d], col_frag<true>(t + 2 * V * c * Shape<T, DP>::ld + 32 * d, Shape<T, DP>::ld, lane), b);
+    for (int d = 0; d < Shape<T, DP>::nd; ++d) {
+      const Chunk<T> f = col_frag<true>(t + 2 * V * c * Shape<T, DP>::ld + 32 * d, Shape<T, DP>::ld, lane);
+      mma(acc[d], f, b);
+      if (Fine) mma(acc[d], f, r);
+    }
   }
 }
 
@@ -250,10 +270,6 @@ struct KeyTiles {
   }
 };
 
-// What rounding x to o leaves.
-template <typename O>
-__device__ __forceinline__ O left_of(float x, O o) { return (O)(x - (float)o); }
-
 // Writes the lane's row of DP values, scaled, from the accumulators; to `rest`, unless null, what rounding them leaves.
 template <typename T, typename O, int DP>
 __device__ __forceinline__ void store_row(O* row, const RowAcc<T, DP>& acc, float s, int D, bool in, int h,
@@ -289,6 +305,7 @@ __device__ __forceinline__ void store_row(O* row, const RowAcc<T, DP>& acc, floa
 template <typename T, int DP, int QW>
 struct FwdShape {
   static constexpr int KW = kWaves / QW;
+  static constexpr bool fine = sizeof(T) == 2 && QW < 4;
   static constexpr int KB = sizeof(T) == 2 && QW > 1 ? 2 : 1;   // 32-key blocks of a wave
   static constexpr int KT = 32 * KB * KW;
   static constexpr int tile = KT * Shape<T, DP>::ld;
@@ -385,7 +402,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restri
     for (int b = 0; b < F::KB; ++b) scores<T, DP, Part>(s[b], tk + (kw + 32 * b) * S::ld, fq, a.D, lane);
     softmax_step<T, DP, F::KB>(s, live, c, m, l, acc, h);
 #pragma unroll
-    for (int b = 0; b < F::KB; ++b) gather<T, DP>(acc, tv + (kw + 32 * b) * S::ld, s[b], lane);
+    for (int b = 0; b < F::KB; ++b) gather<T, DP, F::fine>(acc, tv + (kw + 32 * b) * S::ld, s[b], lane);
   }
   l += __shfl_xor(l, 32, 64);
   if (QW < kWaves) {   // the waves of the same rows: the first one adds the others' results in their order
@@ -582,7 +599,7 @@ template <typename T> constexpr int kBwdTile = sizeof(T) == 2 ? 64 : 32;
 // dk and dv: a wave holds 32 keys and values, the workgroup's four share tiles of query rows. With s = q k^T a lane is a
 // key: p and ds are the operands of dv = p^T do and dk = ds^T q as they are. 64 keys a wave would halve the LDS reads but
 // leave one wave a SIMD (1,014 us instead of 793).
-template <typename T, int DP, bool Part>
+template <typename T, int DP, bool Part, bool Fine>
 __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __restrict__ q, const T* __restrict__ k,
                                                           const T* __restrict__ v, const T* __restrict__ g,
                                                           const float* __restrict__ lse, const float* __restrict__ delta,
@@ -675,8 +692,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
           dp[i + e] *= s[i + e];
         }
       }
-      gather<T, DP>(av, tg + rb * S::ld, s, lane);
-      gather<T, DP>(ak, tq + rb * S::ld, dp, lane);
+      gather<T, DP, Fine>(av, tg + rb * S::ld, s, lane);
+      gather<T, DP, Fine>(ak, tq + rb * S::ld, dp, lane);
     }
   }
   if (!good) {   // the lane gathered what a key of zeros would get (infinite where the rows' scores are far below zero)
@@ -699,8 +716,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
 // dq: as the forward, a lane per query row; ds^T is the operand of dq^T = k^T ds^T as it is.
 // Three waves a SIMD for bf16 heads of 64 (with a few registers more there are two: 646 us instead of 578 at 36,864 rows
 // and 9,216 keys of 4 heads).
-template <typename T, int DP, bool Part>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 ? 3 : 1)
+template <typename T, int DP, bool Part, bool Fine>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 && !Fine ? 3 : 1)
 void k_attn_bwd_q(Attn n, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ g,
                   const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dq,
                   float* __restrict__ part) {
@@ -744,7 +761,7 @@ void k_attn_bwd_q(Attn n, const T* __restrict__ q, const T* __restrict__ k, cons
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] = (bits >> acc_row(i, 0)) & 1 ? dp[i] : 0.f;
       }
-      gather<T, DP>(acc, tk + k0 * S::ld, dp, lane);
+      gather<T, DP, Fine>(acc, tk + k0 * S::ld, dp, lane);
     }
   }
   if (part) {
@@ -987,16 +1004,18 @@ int splat_attention_bwd(const splat_attention* a, const void* q, const void* k, 
     if (a->Lk > 0) {
       const long long keys = (long long)a->B * a->Lk * a->Hk;
       float* pk = nk.splits > 1 ? part : nullptr;
-      k_attn_bwd_kv<T, DP, Part><<<nk.tiles * nk.splits * a->B * a->Hk, kThreads, 0, st>>>(nk, tq, tk, tv, tg, lse, delta,
-                                                                                           (T*)dk, (T*)dv, pk);
+      const bool fine = sizeof(T) == 2 && (nk.R <= kFineRows || a->Lk <= kFineRows);
+      (fine ? k_attn_bwd_kv<T, DP, Part && sizeof(T) == 4, sizeof(T) == 2> : k_attn_bwd_kv<T, DP, Part, false>)
+          <<<nk.tiles * nk.splits * a->B * a->Hk, kThreads, 0, st>>>(nk, tq, tk, tv, tg, lse, delta, (T*)dk, (T*)dv, pk);
       if (pk)
         k_attn_add<T><<<dim3(wgs(keys), 2), kThreads, 0, st>>>(nk, fast_div(quads), quads, pk, nk.splits, 2 * keys * a->D,
                                                                (int)keys, false, (T*)dk, (T*)dv);
     }
     if (a->Lq > 0) {
       float* pq = nq.splits > 1 ? part : nullptr;
-      k_attn_bwd_q<T, DP, Part><<<nq.tiles * nq.splits * a->B * a->Hk, kThreads, 0, st>>>(nq, tq, tk, tv, tg, lse, delta,
-                                                                                          (T*)dq, pq);
+      const bool fine = sizeof(T) == 2 && (a->D <= kFineHead || nq.R <= kFineRows || a->Lk <= kFineRows);
+      (fine ? k_attn_bwd_q<T, DP, Part && (sizeof(T) == 4 || DP <= 64), sizeof(T) == 2> : k_attn_bwd_q<T, DP, Part, false>)
+          <<<nq.tiles * nq.splits * a->B * a->Hk, kThreads, 0, st>>>(nq, tq, tk, tv, tg, lse, delta, (T*)dq, pq);
       if (pq)
         k_attn_add<T><<<wgs(rows), kThreads, 0, st>>>(nq, fast_div(quads), quads, pq, nq.splits, rows * a->D, (int)rows, true,
                                                       (T*)dq, (T*)nullptr);

@@ -183,7 +183,8 @@ def test_attention_of_part_heads_costs_no_more(dt, D, full):
     assert part < 1.5 * whole
 
 
-@pytest.mark.parametrize("B,Lq,Lk,H,Hk,D,scale", [(2, 300, 8, 4, 4, 32, 1.5), (3, 600, 71, 4, 2, 40, 1.5)])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hk,D,scale", [(2, 300, 8, 4, 4, 32, 1.5), (2, 300, 70, 4, 2, 32, 4.0),
+                                                  (3, 600, 71, 4, 2, 40, 1.5), (1, 1000, 2000, 4, 4, 16, 1.5)])
 def test_attention_gradients_round_twice(B, Lq, Lk, H, Hk, D, scale):
     """bfloat16 results carry two roundings: the probabilities' or score gradients' before the second product, and their
     own. A rounding is 1.66e-3 in the 2-norm of normal values, two are 2.35e-3, three (the output's, which the score
@@ -197,3 +198,18 @@ def test_attention_gradients_round_twice(B, Lq, Lk, H, Hk, D, scale):
     errs = [R.rel(p, q) for p, q in zip((y, *got), (z, *want))]
     print(" ".join(f"{e:.2e}" for e in errs), flush=True)
     assert max(errs) <= 2.6e-3
+
+
+@pytest.mark.parametrize("B,Lq,Lk,H,Hk,D", [(3, 1, 3000, 4, 4, 16), (2, 1, 102, 2, 2, 32), (4, 7, 613, 2, 2, 96),
+                                            (5, 1, 300, 8, 2, 64), (3, 2, 8, 16, 4, 64), (1, 64, 33, 1, 1, 40)])
+def test_attention_of_few_rows_rounds_once(B, Lq, Lk, H, Hk, D):
+    """Few rows' roundings do not average out: there bfloat16 results and gradients carry their own alone, to a tenth of it."""
+    dt = torch.bfloat16
+    kv = rand(B, Lk, 2, Hk, D, dt=dt, seed=1)
+    a = [t.requires_grad_(True) for t in (rand(B, Lq, H, D, dt=dt, scale=1.5), kv[:, :, 0].clone(), kv[:, :, 1].clone())]
+    d = [t.detach().double().requires_grad_(True) for t in a]
+    y, z, g = F.cross_attention(*a), R.cross_attention(*d, None, None, D ** -0.5), rand(B, Lq, H, D, dt=dt, seed=3)
+    got, want = torch.autograd.grad(y, a, g), torch.autograd.grad(z, d, g.double())
+    errs = [(R.rel(p, q), R.rel(q.to(dt), q)) for p, q in zip((y, *got), (z, *want))]
+    print(" ".join(f"{e:.2e}/{o:.2e}" for e, o in errs), flush=True)
+    assert all(e <= 1.1 * o for e, o in errs), errs
