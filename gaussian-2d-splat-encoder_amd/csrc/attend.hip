@@ -148,6 +148,21 @@ template <typename T>
 __device__ __forceinline__ T* rest_of(const splat_attention& a, long long at) {
   return sizeof(T) == 2 && a.rest ? (T*)a.rest + at : nullptr;
 }
+// The same of floats' inverse sums.
+template <typename T>
+__device__ __forceinline__ float* inverse_of(const splat_attention& a, long long at) {
+  return sizeof(T) == 4 && a.rest ? (float*)a.rest + at : nullptr;
+}
+
+// What the backward takes of a row: its maximum m in exponents of two and its sum l of 2^(score - m), as p = 2^(score - lse)
+// with lse = m + log2 l, or p = 2^(score - m) / l for floats: lse is a number of about 20, whose own last bit would move all
+// of a row's probabilities by 7e-7 (one token of 33,793 keys: dv 1.2e-6 off instead of 7.6e-7).
+template <typename T>
+__device__ __forceinline__ void keep_row(const splat_attention& a, float* lse, long long at, float m, float l) {
+  float* inv = inverse_of<T>(a, at);
+  lse[at] = l == 0.f ? INFINITY : inv ? m : m + hw_log2(l);
+  if (inv) *inv = l > 0.f ? 1.f / l : l;
+}
 
 // Address of row r's head vector in a tensor of strides (sb, sl, sh).
 template <typename T>
@@ -198,13 +213,26 @@ struct Rows {
     for (int i = 0; i < per; ++i)
       if (holds()) *(f32x4*)place(t, i) = *(const f32x4*)c[i].v;
   }
+  __device__ static void scale(Chunk<T>& x, float by) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) x.v[j] = (T)((float)x.v[j] * by);
+  }
+  __device__ void scale(const float (&by)[per]) {   // row i by by[i]
+#pragma unroll
+    for (int i = 0; i < per; ++i) scale(c[i], by[i]);
+  }
   template <typename F>
   __device__ static void copy(T* t, int D, F&& row) {
+    copy(t, D, row, [](int, Chunk<T>&) {});
+  }
+  template <typename F, typename G>
+  __device__ static void copy(T* t, int D, F&& row, G&& change) {   // change(i, chunk of row i)
 #pragma unroll 1
     for (int i = 0; i < per; ++i) {
       if (!holds()) continue;
       const T* p = row(row0() + i * RS);
-      const Chunk<T> x = load_chunk(p + col(), p ? D - col() : 0);
+      Chunk<T> x = load_chunk(p + col(), p ? D - col() : 0);
+      change(row0() + i * RS, x);
       *(f32x4*)place(t, i) = *(const f32x4*)x.v;
     }
   }
@@ -442,7 +470,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_fwd(Attn n, const T* __restri
     store_row<T, float, DP>(part + at * a.D, acc, 1.f, a.D, in, h);
   } else {
     const float inv = l > 0.f ? 1.f / l : l;   // 0 for a row without keys, NaN stays
-    if (lse && in && h == 0) lse[(long long)w.bh * n.R + r] = l == 0.f ? INFINITY : m + hw_log2(l);
+    if (lse && in && h == 0) keep_row<T>(a, lse, (long long)w.bh * n.R + r, m, l);
     const int qi = r / n.by_rep, j = r - qi * n.rep;
     const long long at = ((w.b * a.Lq + qi) * a.H + w.hk * n.rep + j) * a.D;
     store_row<T, T, DP>(o + at, acc, inv, a.D, in, h, rest_of<T>(a, at));
@@ -481,7 +509,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_attn_join(Attn n, const float*
     l = wave_add(l);
     if (lane == 0) {
       total = l > 0.f ? 1.f / l : l;
-      if (lse) lse[row] = l == 0.f ? INFINITY : m + hw_log2(l);
+      if (lse) keep_row<T>(a, lse, row, m, l);
     }
   }
   __syncthreads();
@@ -556,7 +584,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, FastDiv by_q
     for (int e = 0; e < 4; ++e) x[e] = s.v[e] - (float)(T)s.v[e];
     store_head(r, x, a.D - d);
   }
-  if (lse && d == 0) lse[row] = ml.y == 0.f ? INFINITY : ml.x + hw_log2(ml.y);
+  if (lse && d == 0) keep_row<T>(a, lse, row, ml.x, ml.y);
 }
 
 // ----------------------------------------------------------------------------------------------- backward
@@ -633,10 +661,13 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
   const T* gp = head_row<T>(g, n, w, 0, a.gb, a.gl, a.gh);
   const float* lp = lse + (long long)w.bh * n.R;
   const float* dp0 = delta + (long long)w.bh * n.R;
-  float sl = 0.f, sd = 0.f;
+  // Floats' probabilities lack the factor 1 / l, which the gradient's rows and delta carry instead: ds and dv take both.
+  const float* ip = inverse_of<T>(a, (long long)w.bh * n.R);
+  float sl = 0.f, sd = 0.f, inv[rg.per];
   int r0 = 0;
   auto qrow = [&](int i) { return r0 + i < n.R ? head_row<T>(q, n, w, r0 + i, a.qb, a.ql, a.qh) : nullptr; };
   auto grow = [&](int i) { return r0 + i < n.R ? head_row<T>(g, n, w, r0 + i, a.gb, a.gl, a.gh) : nullptr; };
+  auto inverse = [&](int i) { return ip[min(r0 + i, n.R - 1)]; };
   auto fetch = [&](int t) {
     r0 = t * QT;
     if (whole && r0 + QT <= n.R) {
@@ -647,10 +678,15 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
       rq.load(qrow);
       rg.load(grow);
     }
+    if (ip) {
+#pragma unroll
+      for (int i = 0; i < rg.per; ++i) inv[i] = inverse(rg.row0() + i * rg.RS);
+    }
     if (threadIdx.x < QT) {
       const int r = r0 + threadIdx.x;
       sl = r < n.R ? -lp[r] : -INFINITY;
       sd = r < n.R ? -dp0[r] : 0.f;
+      if (ip && r < n.R) sd *= ip[r];
     }
   };
   if (t0 < t1) fetch(t0);
@@ -661,10 +697,13 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
     float* td = tl + QT;
     if (n.chunked) {
       rq.put(tq);
+      if (ip) rg.scale(inv);
       rg.put(tg);
     } else {
       Rows<T, DP, QT>::copy(tq, a.D, qrow);
-      Rows<T, DP, QT>::copy(tg, a.D, grow);
+      Rows<T, DP, QT>::copy(tg, a.D, grow, [&](int i, Chunk<T>& x) {
+        if (ip) rg.scale(x, inverse(i));
+      });
     }
     if (threadIdx.x < QT) {
       tl[threadIdx.x] = sl;
@@ -764,12 +803,14 @@ void k_attn_bwd_q(Attn n, const T* __restrict__ q, const T* __restrict__ k, cons
       gather<T, DP, Fine>(acc, tk + k0 * S::ld, dp, lane);
     }
   }
+  const float* ip = inverse_of<T>(a, (long long)w.bh * n.R);
+  const float sc = ip && in ? a.scale * ip[r] : a.scale;
   if (part) {
     const long long rows = (long long)a.B * a.Hk * n.R;
-    store_row<T, float, DP>(part + (w.split * rows + (long long)w.bh * n.R + r) * a.D, acc, a.scale, a.D, in, h);
+    store_row<T, float, DP>(part + (w.split * rows + (long long)w.bh * n.R + r) * a.D, acc, sc, a.D, in, h);
   } else {
     const int qi = r / n.by_rep, j = r - qi * n.rep;
-    store_row<T, T, DP>(dq + ((w.b * a.Lq + qi) * a.H + w.hk * n.rep + j) * a.D, acc, a.scale, a.D, in, h);
+    store_row<T, T, DP>(dq + ((w.b * a.Lq + qi) * a.H + w.hk * n.rep + j) * a.D, acc, sc, a.D, in, h);
   }
 }
 

@@ -11,6 +11,7 @@ typedef struct splat_attention {
   long long mb, ml;                                // key_mask: bytes from image to image and from key to key
   const int* kv_lengths;                           // [B] keys of each image that count, the first ones; or NULL
   const unsigned char* key_mask;                   // [B, Lk], 0: the key is left out; or NULL
-  void* rest;                                      // bfloat16: what the outputs' rounding left, [B, Lq, H, D]; or NULL
+  void* rest;                                      // what the backward takes besides lse; or NULL: bfloat16: what the
+                                                   // outputs' rounding left, like them; float32: inverse sums, like lse
 } splat_attention;
 }

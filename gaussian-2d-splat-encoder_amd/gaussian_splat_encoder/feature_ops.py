@@ -275,11 +275,12 @@ def _describe(q, k, v, lengths, mask, scale, dt):
 
 
 def _attention_fwd(q, k, v, lengths, mask, scale, dt, save):
-    """(result, log sums, what the rounding to bfloat16 left of the result; the two None where no backward follows)"""
+    """(result, log sums, what rounding to bfloat16 left of the result or, for float32, inverse sums; the two None where no
+    backward follows)"""
     B, Lq, H, D = q.shape
     o = q.new_empty((B, Lq, H, D))
     lse = q.new_empty(B * Lq * H, dtype=torch.float32) if save else None
-    rest = torch.empty_like(o) if save and dt else None
+    rest = None if not save else torch.empty_like(o) if dt else torch.empty_like(lse)
     if o.numel():
         a = _describe(q, k, v, lengths, mask, scale, dt)
         a.rest = _ptr(rest)

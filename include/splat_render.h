@@ -337,8 +337,8 @@ int splat_linear_bwd(const void *x, long long ldx, const void *weight, const voi
 
 /* o[B, Lq, H, D] = softmax(scale q k^T) v over the keys that count, q[B, Lq, H, D], k and v[B, Lk, Hk, D]; H is a multiple
  * of Hk (query heads j H / Hk .. share key head j), D at most 128, head vectors dense. Rows without keys give zeros. lse
- * [B, Hk, Lq H / Hk] (or NULL) is what the backward takes, and for bfloat16 a->rest (the forward writes it, the backward adds it to the outputs); dq, dk and
- * dv are contiguous. */
+ * [B, Hk, Lq H / Hk] (or NULL) and a->rest, which the forward writes, are what the backward takes (both calls with rest, or
+ * both without, at a cost in digits); dq, dk and dv are contiguous. */
 typedef struct splat_attention {
   int dtype, B, H, Hk, D;                          /* element type; images; query heads; key heads; values per head */
   float scale;                                     /* of the scores, finite */
@@ -348,7 +348,8 @@ typedef struct splat_attention {
   long long mb, ml;                                /* key_mask: bytes from image to image and from key to key */
   const int *kv_lengths;                           /* [B] keys of each image that count, the first ones; or NULL */
   const unsigned char *key_mask;                   /* [B, Lk], 0: the key is left out; or NULL */
-  void *rest;                                      /* bfloat16: what the outputs' rounding left, [B, Lq, H, D]; or NULL */
+  void *rest;                                      /* what the backward takes besides lse; or NULL: bfloat16: what the
+                                                      outputs' rounding left, like them; float32: inverse sums, like lse */
 } splat_attention;
 size_t splat_attention_workspace_bytes(const splat_attention *a);
 int splat_attention_fwd(const splat_attention *a, const void *q, const void *k, const void *v, void *o, float *lse,

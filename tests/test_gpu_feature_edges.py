@@ -213,3 +213,19 @@ def test_attention_of_few_rows_rounds_once(B, Lq, Lk, H, Hk, D):
     errs = [(R.rel(p, q), R.rel(q.to(dt), q)) for p, q in zip((y, *got), (z, *want))]
     print(" ".join(f"{e:.2e}/{o:.2e}" for e, o in errs), flush=True)
     assert all(e <= 1.1 * o for e, o in errs), errs
+
+
+def test_attention_rows_keep_their_sums():
+    """One row's probabilities share its statistics: taken from the logarithm of their sum (about 20, whose last bit is 2e-6,
+    7e-7 of a probability after 2^x) each row's gradients would be off by that together. Over 24 rows of as many images the
+    mean of it stays below a third of it: a float32 gradient's other roundings go either way."""
+    B, Lk, D = 24, 30000, 40
+    q, k, v, g = (rand(*s, seed=i) for i, s in enumerate([(B, 1, 1, D), (B, Lk, 1, D), (B, Lk, 1, D), (B, 1, 1, D)]))
+    a = [t.requires_grad_(True) for t in (q, k, v)]
+    dv = torch.autograd.grad(F.cross_attention(*a), a, g)[2].double()
+    p = torch.softmax((q.double() * k.double()).sum(-1) * D ** -0.5, 1)
+    # dv = p g: the factor that a whole row is off by, in the least squares
+    want = p * g.double()[:, :, 0]
+    off = (dv[:, :, 0] * want).sum((1, 2)) / (want * want).sum((1, 2)) - 1
+    print(f"rows off by {off.abs().mean().item():.1e}, {off.abs().max().item():.1e} at most", flush=True)
+    assert off.abs().mean().item() <= 2.3e-7
