@@ -58,6 +58,7 @@ struct Gemm {
   long long lda, ldb;      // elements from row to row of the stored matrices
   int P, Q;
   long long K, kper;       // contraction; a slice's share of it
+  long long rest;          // where B is the sum of two matrices (Two): elements from the first to the second, otherwise 0
   int tp, tq;              // tiles along p and q
   // epilogues
   const void *bias, *res;
@@ -127,7 +128,7 @@ struct Stage {
 // A workgroup's WP x WQ waves take PB x QB blocks of 32 x 32 each. The epilogue passes the results through LDS, 32 WQ rows
 // of the output at a time, so that every load and store of it is a run of whole rows (stored straight from the matrix
 // instructions' layout, 32 bytes a row at a time, the writes were 1.5 times the output).
-template <typename T, int PB, int QB, int WP, int WQ, bool ACol, bool BCol, int Epi, int A>
+template <typename T, int PB, int QB, int WP, int WQ, bool ACol, bool BCol, int Epi, int A, bool Two>
 __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
   static_assert(WP * WQ * 64 == kThreads, "four waves");
   constexpr int V = kV<T>;
@@ -151,35 +152,38 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
 #pragma unroll
   for (int j = 0; j < V; ++j) one.v[j] = (T)1.f;
   const bool sums = Epi == kPartial && g.bpart && p0 == 0 && wp == 0;
-  SA sa;
-  SB sb;
-  sa.init((const T*)g.A, g.lda, p0, g.P, k0);
-  sb.init((const T*)g.B, g.ldb, q0, g.Q, k0);
-  sa.load(k1 - k0);
-  sb.load(k1 - k0);
-  for (long long k = k0; k < k1; k += SA::KE) {
-    __syncthreads();
-    sa.put(ta);
-    sb.put(tb);
-    __syncthreads();
-    if (k + SA::KE < k1) {
-      sa.load(k1 - k - SA::KE);
-      sb.load(k1 - k - SA::KE);
-    }
+  const T* B = (const T*)g.B;
+  for (int left = Two ? 2 : 1; left > 0; --left, B += g.rest) {
+    SA sa;
+    SB sb;
+    sa.init((const T*)g.A, g.lda, p0, g.P, k0);
+    sb.init(B, g.ldb, q0, g.Q, k0);
+    sa.load(k1 - k0);
+    sb.load(k1 - k0);
+    for (long long k = k0; k < k1; k += SA::KE) {
+      __syncthreads();
+      sa.put(ta);
+      sb.put(tb);
+      __syncthreads();
+      if (k + SA::KE < k1) {
+        sa.load(k1 - k - SA::KE);
+        sb.load(k1 - k - SA::KE);
+      }
 #pragma unroll
-    for (int s = 0; s < SA::KE; s += 2 * V) {
-      Chunk<T> a[PB], b[QB];
+      for (int s = 0; s < SA::KE; s += 2 * V) {
+        Chunk<T> a[PB], b[QB];
 #pragma unroll
-      for (int i = 0; i < PB; ++i) a[i] = SA::frag(ta, wp + 32 * i, s, lane);
+        for (int i = 0; i < PB; ++i) a[i] = SA::frag(ta, wp + 32 * i, s, lane);
 #pragma unroll
-      for (int i = 0; i < QB; ++i) b[i] = SB::frag(tb, 32 * WQ * i + wq, s, lane);
+        for (int i = 0; i < QB; ++i) b[i] = SB::frag(tb, 32 * WQ * i + wq, s, lane);
 #pragma unroll
-      for (int i = 0; i < PB; ++i)
+        for (int i = 0; i < PB; ++i)
 #pragma unroll
-        for (int j = 0; j < QB; ++j) mma(acc[i][j], a[i], b[j]);
-      if (sums) {
+          for (int j = 0; j < QB; ++j) mma(acc[i][j], a[i], b[j]);
+        if (sums) {
 #pragma unroll
-        for (int j = 0; j < QB; ++j) mma(bsum[j], one, b[j]);
+          for (int j = 0; j < QB; ++j) mma(bsum[j], one, b[j]);
+        }
       }
     }
   }
@@ -343,11 +347,12 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
   }
 }
 
-// g = dy act'(z) (z as it was kept) over `per` rows a workgroup, 64 chunks of columns wide, and the rows' sums of g before
-// its rounding. Bound by memory: 36,864 x 1,024 bf16 with gelu 43 us (5.2 TB/s).
-template <typename T, int A>
+// g = dy act'(z) (z as it was kept) over `per` rows a workgroup, 64 chunks of columns wide, the rows' sums of g before its
+// rounding, and (Two) `rest` elements behind g what the rounding leaves. Bound by memory: 36,864 x 1,024 bf16 with gelu 43 us (5.2 TB/s).
+template <typename T, int A, bool Two>
 __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ g,
-                                                  long long M, int N, int per, float* __restrict__ bpart) {
+                                                  long long rest, long long M, int N, int per,
+                                                  float* __restrict__ bpart) {
   constexpr int V = kV<T>;
   __shared__ float red[4][64 * V];
   const int col = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
@@ -358,14 +363,17 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
   RowStream<T, 4, true> in;
   in.begin(dy + r * N + col, 4LL * N, z + r * N + col, 4LL * N, rows, min(V, N - col));
   in.run([&](const Chunk<T>& d, const Chunk<T>& c, int i) {
-    Chunk<T> o;
+    Chunk<T> o, left;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float x = (float)d.v[j] * slope<A>(kept(c.v[j]));
       s[j] += x;
       o.v[j] = (T)x;
+      if (Two) left.v[j] = (T)(x - (float)o.v[j]);
     }
-    store_chunk(g + (r + 4LL * i) * N + col, o, N - col);
+    T* p = g + (r + 4LL * i) * N + col;
+    store_chunk(p, o, N - col);
+    if (Two) store_chunk(p + rest, left, N - col);
   });
   if (!bpart) return;
 #pragma unroll
@@ -377,25 +385,28 @@ __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, cons
   }
 }
 
-template <typename T, int PB, int QB, int WP, int WQ, bool ACol, bool BCol, int Epi, int A>
+template <typename T, int PB, int QB, int WP, int WQ, bool ACol, bool BCol, int Epi, int A, bool Two>
 int launch(Gemm g, int slices, hipStream_t st) {
   g.tp = div_up(g.P, PB * WP * 32);
   g.tq = div_up(g.Q, QB * WQ * 32);
   if ((long long)g.tp * g.tq >= kMaxThreads / kThreads)
     return set_error(kUnsupported, "product of %d x %d outputs", g.Q, g.P);
-  k_gemm<T, PB, QB, WP, WQ, ACol, BCol, Epi, A><<<dim3(g.tp * g.tq, slices), kThreads, 0, st>>>(g);
+  k_gemm<T, PB, QB, WP, WQ, ACol, BCol, Epi, A, Two><<<dim3(g.tp * g.tq, slices), kThreads, 0, st>>>(g);
   return kOk;
 }
 
 // Tiles of 128 x 128 where they fill the card, otherwise the smaller ones whose workgroups are more; 32 along an
 // output dimension that is no longer.
-template <typename T, bool ACol, bool BCol, int Epi, int A>
+template <typename T, bool ACol, bool BCol, int Epi, int A, bool Two = false>
 int gemm(const Gemm& g, int slices, hipStream_t st) {
+  if constexpr (sizeof(T) == 2 && Epi != kForward && !Two) {
+    if (g.rest) return gemm<T, ACol, BCol, Epi, A, true>(g, slices, st);
+  }
   const long long big = (long long)div_up(g.P, 128) * div_up(g.Q, 128) * slices;
-  if (g.P <= 32) return launch<T, 1, 1, 1, 4, ACol, BCol, Epi, A>(g, slices, st);
-  if (Epi != kForward && g.Q <= 32) return launch<T, 1, 1, 4, 1, ACol, BCol, Epi, A>(g, slices, st);
-  if (big >= 256) return launch<T, 2, 2, 2, 2, ACol, BCol, Epi, A>(g, slices, st);
-  return launch<T, 1, 1, 2, 2, ACol, BCol, Epi, A>(g, slices, st);
+  if (g.P <= 32) return launch<T, 1, 1, 1, 4, ACol, BCol, Epi, A, Two>(g, slices, st);
+  if (Epi != kForward && g.Q <= 32) return launch<T, 1, 1, 4, 1, ACol, BCol, Epi, A, Two>(g, slices, st);
+  if (big >= 256) return launch<T, 2, 2, 2, 2, ACol, BCol, Epi, A, Two>(g, slices, st);
+  return launch<T, 1, 1, 2, 2, ACol, BCol, Epi, A, Two>(g, slices, st);
 }
 
 // Slices of the contraction over M rows for a weight gradient [N, K]: about 512 workgroups, of at least 256 rows each.
@@ -413,6 +424,14 @@ int grad_rows(int dtype, long long M, int N) {
   const long long wide = div_up(N, 64 * (dtype == kF32 ? 4 : 8)), want = (1024 + wide - 1) / wide;
   const long long per = (M + want - 1) / want;
   return (int)(per < 16 ? 16 : per);
+}
+
+// Whether g goes into its products as the sum of two bf16 matrices. Rounded to one, results of many terms are 2.35e-3 off
+// where their own rounding is 1.66e-3; few terms or few results do not average that (76 x 17 -> 9 with a sigmoid: 2.7e-3).
+// Where g is small the second matrix does not show behind the call's launches, nor where the weight is (forward and backward
+// of 36,864 x 64 -> 64 131 and 132 us, of 128 x 1,024 -> 1,024 131 and 132).
+bool two_grads(int dtype, long long M, int N, int K, int act) {
+  return dtype == kBf16 && act != kActNone && (M * N <= 1 << 17 || (long long)N * K <= 1 << 12);
 }
 
 size_t grad_bytes(int dtype, long long M, int N) { return ((size_t)M * N * (dtype == kF32 ? 4 : 2) + 255) & ~(size_t)255; }
@@ -468,7 +487,7 @@ size_t splat_linear_bwd_workspace_bytes(int dtype, long long M, int N, int K, in
   if (check_linear("splat_linear_bwd_workspace_bytes", dtype, M, N, K, act) || M == 0) return 0;
   const size_t slices = weight_slices(M, N, K);
   if (act == kActNone) return sizeof(float) * slices * ((size_t)N * K + N);
-  return grad_bytes(dtype, M, N) + sizeof(float) * (slices * N * K + (size_t)div_up(M, grad_rows(dtype, M, N)) * N);
+  return grad_bytes(dtype, M, N) * (two_grads(dtype, M, N, K, act) ? 2 : 1) + sizeof(float) * (slices * N * K + (size_t)div_up(M, grad_rows(dtype, M, N)) * N);
 }
 
 int splat_linear_bwd(const void* x, long long ldx, const void* weight, const void* dy, const void* z, int dtype,
@@ -489,16 +508,20 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
     using T = decltype(t);
     const int s = weight_slices(M, N, K);
     const T* gr = (const T*)dy;
-    float* part = (float*)((char*)ws + (act == kActNone ? 0 : grad_bytes(dtype, M, N)));
+    const size_t gbytes = grad_bytes(dtype, M, N);
+    const long long rest = two_grads(dtype, M, N, K, act) ? gbytes / sizeof(T) : 0;
+    float* part = (float*)((char*)ws + (act == kActNone ? 0 : rest ? 2 * gbytes : gbytes));
     float* bpart = dbias ? part + (size_t)s * N * K : nullptr;
     int bslices = s;
     if (act != kActNone) {
       const int per = grad_rows(dtype, M, N);
       bslices = div_up(M, per);
       with_act(act, [&](auto a) {
-        if constexpr (decltype(a)::value != kActNone)
-          k_act_grad<T, decltype(a)::value><<<dim3(div_up(N, 64 * kV<T>), bslices), 256, 0, st>>>(
-              (const T*)dy, (const T*)z, (T*)ws, M, N, per, bpart);
+        if constexpr (decltype(a)::value != kActNone) {
+          constexpr int A = decltype(a)::value;
+          (rest ? k_act_grad<T, A, sizeof(T) == 2> : k_act_grad<T, A, false>)<<<dim3(div_up(N, 64 * kV<T>), bslices), 256, 0, st>>>(
+              (const T*)dy, (const T*)z, (T*)ws, rest, M, N, per, bpart);
+        }
         return kOk;
       });
       gr = (const T*)ws;
@@ -506,7 +529,7 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
     if (dx) {
       Gemm g{};
       g.A = weight; g.lda = K; g.P = K;
-      g.B = gr; g.ldb = N; g.Q = (int)M;
+      g.B = gr; g.ldb = N; g.Q = (int)M; g.rest = rest;
       g.K = g.kper = N;
       g.out = dx;
       if (const int rc = gemm<T, true, false, kOut, 0>(g, 1, st)) return rc;
@@ -516,7 +539,7 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
         Gemm g{};
         // dbias alone: one column of products, with the gradient itself for want of x
         g.A = dweight ? x : gr; g.lda = dweight ? ldx : N; g.P = dweight ? K : 1;
-        g.B = gr; g.ldb = N; g.Q = N;
+        g.B = gr; g.ldb = N; g.Q = N; g.rest = rest;
         g.K = M; g.kper = (M + s - 1) / s;
         g.part = part;
         g.bpart = act == kActNone ? bpart : nullptr;

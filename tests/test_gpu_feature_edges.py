@@ -229,3 +229,19 @@ def test_attention_rows_keep_their_sums():
     off = (dv[:, :, 0] * want).sum((1, 2)) / (want * want).sum((1, 2)) - 1
     print(f"rows off by {off.abs().mean().item():.1e}, {off.abs().max().item():.1e} at most", flush=True)
     assert off.abs().mean().item() <= 2.3e-7
+
+
+@pytest.mark.parametrize("M,K,N,name", [(76, 17, 9, "sigmoid"), (3, 212, 525, "silu"), (1304, 16, 16, "tanh"), (1, 64, 5, "gelu"),
+                                        (8, 797, 17, "tanh"), (300, 400, 400, "gelu"), (9000, 24, 130, "silu")])
+def test_linear_gradients_of_few_rows_or_weights_round_once(M, K, N, name):
+    """Where few terms or few results do not average roundings, bfloat16 gradients carry their own alone, to a tenth of it:
+    the kept input's (2^-11, in slopes that change by up to 2 z of it) is a quarter of a result's at most."""
+    dt = torch.bfloat16
+    a = [t.requires_grad_(True) for t in (rand(M, K, dt=dt), rand(N, K, dt=dt, seed=1, scale=K ** -0.5),
+                                          rand(N, dt=dt, seed=2, scale=0.2))]
+    d = [t.detach().double().requires_grad_(True) for t in a]
+    y, z, g = F.linear_act(*a, act=name), R.linear_act(*d, name, None), rand(M, N, dt=dt, seed=3)
+    got, want = torch.autograd.grad(y, a, g), torch.autograd.grad(z, d, g.double())
+    errs = [(R.rel(p, q), R.rel(q.to(dt), q)) for p, q in zip((y, *got), (z, *want))]
+    print(" ".join(f"{e:.2e}/{o:.2e}" for e, o in errs), flush=True)
+    assert all(e <= 1.1 * o for e, o in errs), errs
