@@ -40,7 +40,8 @@ struct Unit {
   int img, tile, split;
 };
 __device__ __forceinline__ Unit unit(const Norm& n) {
-  const int id = blockIdx.x, u = id / n.by_splits, img = u / n.by_tiles;
+  const int id = blockIdx.x, u = __builtin_amdgcn_readfirstlane(id / n.by_splits);
+  const int img = __builtin_amdgcn_readfirstlane(u / n.by_tiles);
   return {img, u - img * n.tiles, id - u * n.splits};
 }
 
@@ -444,11 +445,10 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
                                                              const float* __restrict__ gpart, T* __restrict__ dx,
                                                              float* __restrict__ dw, float* __restrict__ db) {
   __shared__ float ga[kTile], gb[kTile];
-  const Unit u = unit(n);
-  const int img = u.img, tile = u.tile, split = u.split;
-  if (img == n.B) {
+  const int maps = n.B * n.tiles * n.splits;   // workgroups of the maps
+  if ((int)blockIdx.x >= maps) {
     const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, nrow = kThreads / 32;
-    for (int c0 = (tile * n.splits + split) * 32; c0 < n.C; c0 += 32 * n.tiles * n.splits) {
+    for (int c0 = (blockIdx.x - maps) * 32; c0 < n.C; c0 += (gridDim.x - maps) * 32) {
       const int c = c0 + lane;
       float a = 0.f, q = 0.f;
       if (c < n.C) {
@@ -474,6 +474,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_apply(Norm n, const T* __
     }
     return;
   }
+  const Unit u = unit(n);
+  const int img = u.img, tile = u.tile, split = u.split;
   const Place p = place<T>(n, tile, split);
   RowStream<T, 2, true> xs;
   xs.begin(x + (long long)img * n.xsb + (p.lo + p.rt) * n.xsl + p.c, n.RT * n.xsl,
