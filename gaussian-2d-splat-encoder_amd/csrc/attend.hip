@@ -11,9 +11,9 @@
 // included) reaches a product; a row without valid keys gives zeros, and zero gradients.
 //
 // Measured on 36,864 rows and 9,216 keys of four heads of 64, bf16 (174 GFLOP a product; a large library
-// product reaches 1,394 TFLOP/s here): forward 460 us (755 TFLOP/s), dk and dv 780 us (890), dq 545 us (955). Matrix and
-// vector instructions take about the same time and overlap only in part: matrix units 36 to 47% busy, vector units 42 to
-// 63%, LDS 36 to 49%. One pass for all three gradients would do with five products instead of seven, but dq would need
+// product reaches 1,394 TFLOP/s here): forward 446 us (780 TFLOP/s), dk and dv 753 us (924), dq 543 us (962). Matrix and
+// vector instructions take about the same time and overlap only in part: matrix units 37 to 47% busy, vector units 41 to
+// 65%, LDS 54 to 60%. One pass for all three gradients would do with five products instead of seven, but dq would need
 // atomics (whose order changes results) or 2.7 GB of partial sums.
 #include "feat_common.h"
 #include "splat_attention.h"
@@ -329,7 +329,7 @@ __device__ __forceinline__ void store_row(O* row, const RowAcc<T, DP>& acc, floa
 // value tiles go through registers into two LDS buffers in turn: the next tile's loads are in flight during a step, and
 // one barrier a tile suffices (where only one buffer fits, two). Waves that shared keys join their results in LDS, splits
 // of the key axis in k_attn_join. Few rows are bound by reading keys and values: one token, 92,160 keys of four heads of 64
-// in bf16 (94 MB) 21 us, 4.5 TB/s, and 4 us to join.
+// in bf16 (94 MB) 22 us, 4.3 TB/s, and 4 us to join.
 template <typename T, int DP, int QW>
 struct FwdShape {
   static constexpr int KW = kWaves / QW;
@@ -550,7 +550,7 @@ __device__ __forceinline__ void store_head(T* p, const float (&s)[4], int left) 
 }
 
 // The same for few splits (rows are many then): a thread per four values of a row. Two splits of 147,456 rows of 64: 17 us
-// (5.5 TB/s).
+// (5.5 TB/s), 20 with what the outputs' rounding leaves.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, FastDiv by_quads, int quads, const float* __restrict__ part,
                                                             const float* __restrict__ stat, T* __restrict__ o,
@@ -590,8 +590,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_join_few(Attn n, FastDiv by_q
 // ----------------------------------------------------------------------------------------------- backward
 // delta[row] = sum over d of do * o, which the score gradients p (dp - delta) take, o with what its rounding left: where a few
 // keys hold most of a row's weight, dp - delta is far smaller than either, and a bf16 output's rounding four times the
-// gradients' own (8 keys, heads of 32: dq 5.9e-3 off instead of 2.3e-3). Bound by memory: 147,456 rows of 64 bf16
-// 12 us (3.2 TB/s).
+// gradients' own (8 keys, heads of 32: dq 5.9e-3 off instead of 2.3e-3). Bound by memory: 147,456 rows of 64 bf16 16.5 us
+// (3.4 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_attn_delta(Attn n, const T* __restrict__ o, const T* __restrict__ g,
                                                          float* __restrict__ delta) {
@@ -753,8 +753,8 @@ __global__ __launch_bounds__(kThreads) void k_attn_bwd_kv(Attn n, const T* __res
 }
 
 // dq: as the forward, a lane per query row; ds^T is the operand of dq^T = k^T ds^T as it is.
-// Three waves a SIMD for bf16 heads of 64 (with a few registers more there are two: 646 us instead of 578 at 36,864 rows
-// and 9,216 keys of 4 heads).
+// Three waves a SIMD for bf16 heads of 64, at the cost of 20 bytes of scratch a lane (with a few registers more there are two
+// waves: 646 us instead of 578 at 36,864 rows and 9,216 keys of 4 heads).
 template <typename T, int DP, bool Part, bool Fine>
 __global__ __launch_bounds__(kThreads, sizeof(T) == 2 && DP <= 64 && !Fine ? 3 : 1)
 void k_attn_bwd_q(Attn n, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ g,
@@ -890,8 +890,10 @@ int with_shape(const splat_attention& a, F&& f) {
 // split (64 rows and 18,432 masked bf16 keys: 16 us; 18 with four, 23 with eight).
 // A float tile takes sixteen times the matrix instructions' time: one workgroup a CU is a round there, and a split costs
 // about one tile. Where lengths or a mask, which only the device knows, may leave workgroups idle, more of them even out
-// what is left: two rounds are added to the estimate (dk and dv of 3 x 1,201 x 777, two heads of 40, one image empty, took
-// 97 us with half the splits and 67 with these; 59 since empty chunks are skipped).
+// what is left: two rounds are added to the estimate. Training calls' kernels with them and without, the last image empty,
+// lengths / mask: float, 3 x 1,201 x 777 (2 key heads of 40) 177 (205) / 206 (205) us, 2 x 4,000 x 3,000 (4 of 64) 612 (871)
+// / 826 (1,076), 4 x 300 x 5,000 (4 of 64) 335 (321) / 370 (389), 2 x 9,000 x 2,000 (2 of 32) 486 (654) / 641 (683). bf16
+// tiles are too short for it: the first two 75 (71) / 91 (83) and 175 (157) / 228 (202), the last 145 (159) / 196 (201).
 void split(Attn& n, long long groups, int tiles, int slots) {
   n.splits = 1;
   n.per = tiles < 1 ? 1 : tiles;
@@ -1055,7 +1057,8 @@ int splat_attention_bwd(const splat_attention* a, const void* q, const void* k, 
     if (a->Lq > 0) {
       float* pq = nq.splits > 1 ? part : nullptr;
       const bool fine = sizeof(T) == 2 && (a->D <= kFineHead || nq.R <= kFineRows || a->Lk <= kFineRows);
-      (fine ? k_attn_bwd_q<T, DP, Part && (sizeof(T) == 4 || DP <= 64), sizeof(T) == 2> : k_attn_bwd_q<T, DP, Part, false>)
+      (fine ? k_attn_bwd_q<T, DP, Part && (sizeof(T) == 4 || DP <= 64), sizeof(T) == 2>
+            : k_attn_bwd_q<T, DP, Part, false>)
           <<<nq.tiles * nq.splits * a->B * a->Hk, kThreads, 0, st>>>(nq, tq, tk, tv, tg, lse, delta, (T*)dq, pq);
       if (pq)
         k_attn_add<T><<<wgs(rows), kThreads, 0, st>>>(nq, fast_div(quads), quads, pq, nq.splits, rows * a->D, (int)rows, true,

@@ -6,10 +6,10 @@
 // floats. A long contraction with few outputs (dW) is cut into slices whose partial sums a second launch adds in order.
 //
 // Measured at 36,864 rows, bf16 (a large library product reaches 1,394 TFLOP/s here, a large copy 4.9 TB/s): 256 -> 1,024
-// 42 us (460 TFLOP/s, 2.2 TB/s), 50 us with gelu and its input kept; its dx 36 us (535), dW 39 us (490) and 10 us to join 32
-// slices. 1,024 -> 1,024: 105 us (735). float, 1,024 -> 1,024: 594 us (130 of 153). Operands reach the matrix units through
-// one LDS buffer and registers: three workgroups a CU hide the barriers better than two buffers with two workgroups (117 us
-// instead of 105) or smaller tiles (124 us).
+// 42 us (460 TFLOP/s, 2.2 TB/s), 57 us with gelu and its input kept; its dx 36 us (535), dW 40 us (480) and 10.5 us to join
+// 32 slices. 1,024 -> 1,024: 105 us (735). float, 1,024 -> 1,024: 594 us (130 of 153). Operands reach the matrix units
+// through one LDS buffer and registers: three workgroups a CU hide the barriers better than two buffers with two workgroups
+// (117 us instead of 105) or smaller tiles (124 us).
 #include "feat_common.h"
 
 namespace splat {
@@ -250,9 +250,11 @@ __global__ __launch_bounds__(kThreads) void k_gemm(Gemm g) {
 // The forward where outputs are few (tokens, small maps): bound by reading the weight, and for a small one by the chain of
 // its loads. A workgroup makes 32 outputs of 32 rows; its eight waves share the contraction and load their operands straight
 // from memory in the matrix instructions' layout, four steps in flight, and their sums meet in LDS once. Every 32 rows read
-// the weight and every 32 outputs the rows again, so it pays up to `few_tiles` workgroups. bf16, through k_gemm's staged
-// tiles after it: 1 x 256 -> 1,024 3.4 us (7.8), 256 x 1,024 -> 1,024 6.3 (9.2), 512 x 1,024 -> 1,024 9.9 (9.4); float:
-// 512 x 1,024 -> 1,024 19.5 (27.3), 1,024 x 1,024 -> 1,024 36 (28).
+// the weight and every 32 outputs the rows again, so it pays up to `few_tiles` workgroups, whatever the contraction. Kernel
+// times with k_gemm's staged tiles in brackets, K = 64 / 256 / 1,024 / 4,096: bf16, 256 workgroups (512 x 512 outputs) 3.3
+// (3.4) / 3.9 (4.5) / 6.7 (9.8) / 17 (38) us, 512 3.7 (3.5) / 5.0 (4.7) / 10.8 (12.2) / 31 (39), 1,024 5.1 (3.7) / 8.1 (4.9)
+// / 17 (12.5) / 59 (39); float, 512 4.8 (4.9) / 7.7 (9.2) / 20 (27) / 65 (98), 1,024 7.5 (5.3) / 14.8 (9.9) / 37 (28) / 123
+// (98). One row of 256 -> 1,024, bf16: 3.4 (7.8).
 constexpr int kFewThreads = 512;
 template <typename T> constexpr long long few_tiles = sizeof(T) == 4 ? 512 : 256;
 template <typename T, int A>
@@ -348,7 +350,8 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
 }
 
 // g = dy act'(z) (z as it was kept) over `per` rows a workgroup, 64 chunks of columns wide, the rows' sums of g before its
-// rounding, and (Two) `rest` elements behind g what the rounding leaves. Bound by memory: 36,864 x 1,024 bf16 with gelu 43 us (5.2 TB/s).
+// rounding, and (Two) `rest` elements behind g what the rounding leaves. Bound by memory: 36,864 x 1,024 bf16 with gelu 44 us
+// (5.1 TB/s).
 template <typename T, int A, bool Two>
 __global__ __launch_bounds__(256) void k_act_grad(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ g,
                                                   long long rest, long long M, int N, int per,
@@ -519,7 +522,8 @@ int splat_linear_bwd(const void* x, long long ldx, const void* weight, const voi
       with_act(act, [&](auto a) {
         if constexpr (decltype(a)::value != kActNone) {
           constexpr int A = decltype(a)::value;
-          (rest ? k_act_grad<T, A, sizeof(T) == 2> : k_act_grad<T, A, false>)<<<dim3(div_up(N, 64 * kV<T>), bslices), 256, 0, st>>>(
+          const dim3 grid(div_up(N, 64 * kV<T>), bslices);
+          (rest ? k_act_grad<T, A, sizeof(T) == 2> : k_act_grad<T, A, false>)<<<grid, 256, 0, st>>>(
               (const T*)dy, (const T*)z, (T*)ws, rest, M, N, per, bpart);
         }
         return kOk;
