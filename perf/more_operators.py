@@ -1,0 +1,476 @@
+"""Performance cases of the token operators: rotary positions of several axes, a paged cache of keys and values with the
+attention that reads it, and norms per token with a block's gate and residual; from a single token to the training step of a
+768 x 768 image's cells and to a stream of frames' splats.
+
+A case is a dict of plain values:
+  op        "rotary" (rotary), "append" (cache_append), "attend" (cached_attention) or "norm" (residual_norm, token_norm)
+  dtype     "float32" or "bfloat16" (norm parameters and shared gates are float32)
+  train     1: the outputs and the gradients of every input from given upstream gradients; 0: the outputs, no grad
+  dims      values of a head that each axis turns, as text ("" for no rotation), of heads of D; inter: pairs of neighbours
+  pos       "line" (a token's number), "grid" (row and column of a map, shared by the images), "frames" (time, row, column)
+            or "splats" (real-valued centres in [0, 1], with a gradient in training)
+  rotary    B images of L tokens, H heads of D values
+  append    B sequences, T new tokens each, Hk heads of D; pages of `page` tokens, up to n tokens a sequence; ragged: lengths
+            and new tokens differ, one sequence has none; masked: dead splats are marked
+  attend    the same cache; T new queries a sequence of H heads; causal or not; cap: tokens that a table has room for
+  norm      B images of L tokens of C channels; kind "rms" or "layer"; gate "none", "channel", "image" or "token" through
+            act; block 0 leaves the norm of tokens alone (token_norm)
+
+listed(), draw(rng), prepare(case, seed), run(state), work(case) and exact(case, seed) are what a measuring program needs.
+With `own` false, run() computes the operators from elementary torch operations in float32 (angles in float64); with it
+true, it calls the package.
+"""
+
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16}
+SCALE = {"line": 1.0, "grid": 1.0, "frames": 1.0, "splats": 96.0}   # splats: centres as cells of a 96 x 96 map
+AXES = {"line": 1, "grid": 2, "frames": 3, "splats": 2}
+EPS = 1e-6
+
+
+def listed():
+    # The sizes of an encoder of width 256 at an image of 768 x 768: 36,864 fine cells, 9,216 coarse ones, 92,160 splats;
+    # heads of 64 values, four of them; and generic ones for the models that read a stream of such images.
+    rot = dict(op="rotary", inter=0)
+    app = dict(op="append", train=0, inter=0)
+    att = dict(op="attend", train=0, inter=0)
+    norm = dict(op="norm", kind="rms", act="none", block=1)
+    return [
+        # one new token's queries: the smallest rotation, launches and latency
+        dict(rot, name="rotary_token", dtype="bfloat16", train=0, B=1, L=1, H=4, D=64, dims="64", pos="line"),
+        # the queries of every fine cell of four images in training, turned by row and column: the largest rotation
+        dict(rot, name="rotary_cells_train", dtype="bfloat16", train=1, B=4, L=36864, H=4, D=64, dims="32,32", pos="grid"),
+        # keys of predicted splats whose centres learn too: an odd number of them, heads of 40, neighbours paired
+        dict(rot, name="rotary_splats_train_f32", dtype="float32", train=1, B=2, L=18433, H=3, D=40, dims="20,16",
+             pos="splats", inter=1),
+        # one token of each of eight sequences: the smallest append, latency
+        dict(app, name="append_tokens", dtype="bfloat16", B=8, T=1, Hk=4, D=64, dims="16,24,24", pos="frames", page=64,
+             n=4096, ragged=0, masked=0),
+        # all splats of a new frame behind the three before it, dead ones marked
+        dict(app, name="append_frame", dtype="bfloat16", B=1, T=92160, Hk=4, D=64, dims="32,32", pos="splats", page=128,
+             n=368640, ragged=0, masked=1),
+        # one token over a short history in a table with room for a long one: the smallest attention, latency
+        dict(att, name="attend_short", dtype="bfloat16", B=1, T=1, H=4, Hk=4, D=64, dims="64", pos="line", page=64, n=900,
+             cap=32768, ragged=0, masked=0, causal=1),
+        # one token that reads the splats of the last four frames, dead ones marked
+        dict(att, name="attend_frames", dtype="bfloat16", B=1, T=1, H=4, Hk=4, D=64, dims="16,24,24", pos="frames",
+             page=128, n=368640, cap=368640, ragged=0, masked=1, causal=0),
+        # one new token in each of sixteen sequences of 0 to 32,768 tokens, heads sharing keys: the largest attention
+        dict(att, name="attend_ragged", dtype="bfloat16", B=16, T=1, H=32, Hk=8, D=128, dims="128", pos="line", page=64,
+             n=32768, cap=32768, ragged=1, masked=0, causal=1),
+        # several new tokens that see each other in order, odd heads and pages that end inside a tile
+        dict(att, name="attend_odd_f32", dtype="float32", B=3, T=5, H=6, Hk=2, D=40, dims="20,16", pos="splats", page=17,
+             n=7001, cap=8192, ragged=1, masked=1, causal=1),
+        # one token between a block and the next: the smallest norm, latency
+        dict(norm, name="norm_token", dtype="bfloat16", train=0, B=1, L=1, C=256, gate="channel"),
+        # every fine cell of two images in training, a gate of each image's own: the largest norm
+        dict(norm, name="norm_cells_train", dtype="bfloat16", train=1, B=2, L=36864, C=256, gate="image"),
+        # ragged tokens of an odd width in training, layer norms, a gate for every value
+        dict(norm, name="norm_odd_train_f32", dtype="float32", train=1, B=3, L=1667, C=517, gate="token", act="sigmoid",
+             kind="layer"),
+    ]
+
+
+def _logi(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def _axes(rng, D):
+    """pos and dims of heads of D values."""
+    pos = rng.choice(["line", "grid", "frames", "splats"])
+    A = AXES[pos]
+    if D < 2 * A:
+        return "line", str(D // 2 * 2)
+    if rng.random() < 0.6:       # the whole head, in equal shares of a multiple of two
+        d = [D // A // 2 * 2] * A
+    else:                        # a part of it
+        d = [2 * rng.randint(1, D // A // 2) for _ in range(A)]
+    return pos, ",".join(map(str, d))
+
+
+def draw(rng):
+    op = rng.choice(["rotary", "append", "attend", "attend", "norm"])
+    c = dict(op=op, dtype=rng.choice(["float32", "bfloat16", "bfloat16"]), train=0)
+    D = rng.choice([64, 64, 128, 32, 96, 40, 33, 80])
+    if op == "rotary":
+        pos, dims = _axes(rng, D)
+        c.update(train=int(rng.random() < 0.6), B=_logi(rng, 1, 16), L=rng.choice([1, _logi(rng, 2, 92160)]),
+                 H=_logi(rng, 1, 32), D=D, dims=dims, pos=pos, inter=int(rng.random() < 0.4))
+        while c["B"] * c["L"] * c["H"] * D > 4 * 36864 * 4 * 64:
+            c["L"] = c["L"] // 2 + 1
+            c["H"] = (c["H"] + 1) // 2
+    elif op in ("append", "attend"):
+        pos, dims = _axes(rng, D)
+        if pos == "grid":
+            pos = "splats"
+        if rng.random() < 0.15:
+            dims = ""
+        Hk = rng.choice([1, 2, 4, 8])
+        c.update(B=_logi(rng, 1, 64), Hk=Hk, D=D, dims=dims, pos=pos, inter=int(rng.random() < 0.3),
+                 page=rng.choice([16, 64, 64, 128, 256, 17, 48]), n=_logi(rng, 1, 131072), ragged=int(rng.random() < 0.6),
+                 masked=int(rng.random() < 0.3))
+        if op == "append":
+            c["T"] = rng.choice([1, _logi(rng, 2, 92160)])
+            c["n"] = max(c["n"], c["T"])
+            while c["B"] * c["T"] * Hk * D > 92160 * 4 * 64 or c["B"] * c["n"] * Hk * D > 368640 * 4 * 64:
+                c["T"] = c["T"] // 2 + 1 if c["T"] > 1 else 1
+                c["B"] = (c["B"] + 1) // 2
+                c["n"] = max(c["T"], c["n"] // 2)
+        else:
+            c.update(T=rng.choice([1, 1, 1, _logi(rng, 2, 32)]), H=Hk * rng.choice([1, 1, 2, 4, 8]),
+                     causal=int(rng.random() < 0.7))
+            while c["B"] * c["n"] * Hk * D > 16 * 16384 * 8 * 128 or c["B"] * c["n"] * c["T"] * c["H"] > 1 << 25:
+                c["B"] = (c["B"] + 1) // 2
+                c["T"] = (c["T"] + 1) // 2
+                c["n"] = c["n"] // 2 + 1
+            c["cap"] = c["n"] * rng.choice([1, 1, 2])
+    else:
+        c.update(train=int(rng.random() < 0.6), B=_logi(rng, 1, 16), L=rng.choice([1, _logi(rng, 2, 92160)]),
+                 C=_logi(rng, 32, 4096), kind=rng.choice(["rms", "rms", "layer"]),
+                 gate=rng.choice(["none", "channel", "channel", "image", "token"]),
+                 act=rng.choice(["none", "none", "sigmoid", "silu", "tanh"]), block=int(rng.random() < 0.8))
+        if rng.random() < 0.6:   # widths as networks have them
+            c["C"] = max(32, c["C"] // 32 * 32)
+        while c["B"] * c["L"] * c["C"] > 2 * 36864 * 256:
+            c["L"] = c["L"] // 2 + 1
+            c["B"] = (c["B"] + 1) // 2
+            c["C"] = max(32, c["C"] // 2)
+    return c
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def _dims(c):
+    return [int(d) for d in c["dims"].split(",")] if c["dims"] else []
+
+
+def _lengths(c):
+    """Tokens of each sequence, the new ones among them: all n, or from n down to none."""
+    B, n = c["B"], c["n"]
+    if not c["ragged"]:
+        return [n] * B
+    return [n if i == 0 else 0 if i == B - 1 else 1 + int((n - 1) * (i * 0.618034 % 1.0)) for i in range(B)]
+
+
+def _counts(c):
+    """New tokens of each sequence."""
+    return [min(n, c["T"] if i % 3 != 1 else (c["T"] + 1) // 2) for i, n in enumerate(_lengths(c))]
+
+
+def prepare(case, seed):
+    c = case
+    g = torch.Generator("cuda").manual_seed(int(seed))
+    dt = DTYPES[c["dtype"]]
+
+    def rand(*shape, dtype=dt, scale=1.0, shift=0.0):
+        return (torch.randn(*shape, generator=g, device="cuda") * scale + shift).to(dtype)
+
+    def positions(B, L):
+        """Of the last tokens of sequences that may be far from their start."""
+        first = torch.randint(0, 200000, (B, 1), generator=g, device="cuda")
+        at = torch.arange(L, device="cuda")
+        if c["pos"] == "line":
+            return (first + at).int()[..., None]
+        if c["pos"] == "grid":      # every image has the same cells
+            w = max(1, math.isqrt(L))
+            return torch.stack([at // w, at % w], -1).int()
+        if c["pos"] == "frames":    # a frame's cells row by row, frames numbered on
+            w = 96
+            return torch.stack([first + at // (w * w), (at // w % w).expand(B, L), (at % w).expand(B, L)], -1)
+        return torch.rand(B, L, 2, generator=g, device="cuda")
+
+    s = {"case": c, "leaves": []}
+    if c["op"] == "rotary":
+        B, L, H, D = c["B"], c["L"], c["H"], c["D"]
+        s["x"] = rand(B, L, H, D)
+        s["positions"] = positions(B, L)
+        leaves = ["x"] + (["positions"] if c["pos"] == "splats" else [])
+        s["up"] = [rand(B, L, H, D)] if c["train"] else None
+    elif c["op"] == "norm":
+        B, L, C = c["B"], c["L"], c["C"]
+        leaves = ["x"]
+        s["x"] = rand(B, L, C, scale=2.0)
+        names = ["next_weight", "next_bias"] + (["weight", "bias"] if c["block"] else [])
+        names = names if c["kind"] == "layer" else [n for n in names if "weight" in n]
+        for n in names:
+            s[n] = rand(C, dtype=torch.float32, scale=0.2, shift=1.0 if "weight" in n else 0.0)
+        leaves += names
+        if c["block"]:
+            s["h"] = rand(B, L, C, scale=0.7, shift=0.1)
+            leaves.append("h")
+            shape = {"none": None, "channel": (C,), "image": (B, 1, C), "token": (B, L, C)}[c["gate"]]
+            if shape:
+                s["gate"] = rand(*shape, dtype=dt if c["gate"] == "token" else torch.float32, scale=0.5, shift=0.3)
+                leaves.append("gate")
+        s["up"] = [rand(B, L, C) for _ in range(1 + c["block"])] if c["train"] else None
+    else:
+        B, T, Hk, D, P = c["B"], c["T"], c["Hk"], c["D"], c["page"]
+        lens = _lengths(c)
+        need = [-(-n // P) for n in lens]
+        width = -(-c.get("cap", c["n"]) // P)
+        pages = sum(need) + 1
+        ids = torch.randperm(pages, generator=g, device="cuda").int()
+        s["tables"] = torch.full((B, width), -1, dtype=torch.int32, device="cuda")
+        at = 0
+        for i, m in enumerate(need):
+            s["tables"][i, :m] = ids[at:at + m]
+            at += m
+        s["lengths"] = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        s["counts"] = torch.tensor(_counts(c), dtype=torch.int32, device="cuda") if c["ragged"] and T > 1 else None
+        for n in ("k_pages", "v_pages"):    # a page holds its tokens head by head
+            s[n] = rand(pages, Hk, P, D, scale=1.2 if n[0] == "k" else 1.0).transpose(1, 2)
+        s["live"] = torch.rand(pages, P, generator=g, device="cuda") < 0.6 if c["masked"] else None
+        s["positions"] = positions(B, T) if c["dims"] else None
+        if c["op"] == "append":
+            kv = rand(B, T, 2, Hk, D)       # one projection gives the keys and the values
+            s["k"], s["v"] = kv[:, :, 0], kv[:, :, 1]
+            s["key_mask"] = torch.rand(B, T, generator=g, device="cuda") < 0.6 if c["masked"] else None
+        else:
+            s["q"] = rand(B, T, c["H"], D, scale=1.2)
+        if own:
+            s["cache"] = _calls().PagedCache(s["k_pages"], s["v_pages"], s["live"])
+        leaves = []
+    if c.get("dims") and own:
+        s["axes"] = _calls().RotaryAxes(_dims(c), scale=SCALE[c["pos"]], interleaved=bool(c["inter"]))
+    if c["train"]:
+        for n in leaves:
+            s[n] = s[n].detach()
+            if s[n].is_floating_point():
+                s[n].requires_grad_(True)
+                s["leaves"].append(n)
+    return s
+
+
+# ------------------------------------------------------------------------------------------------ one pass
+def _calls():
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gaussian-2d-splat-encoder_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    from gaussian_splat_encoder import token_ops
+    return token_ops
+
+
+def run(s):
+    c = s["case"]
+    with torch.set_grad_enabled(bool(c["train"])):
+        y = (_own if own else _plain)(s, c)
+    y = y if isinstance(y, tuple) else (y,)
+    out = {f"y{i}": t.detach() for i, t in enumerate(y) if t is not None}
+    if c["train"]:
+        grads = torch.autograd.grad(y, [s[n] for n in s["leaves"]], s["up"])
+        out.update(("d" + n, t) for n, t in zip(s["leaves"], grads))
+    return out
+
+
+def _own(s, c):
+    F = _calls()
+    if c["op"] == "rotary":
+        return F.rotary(s["x"], s["positions"], s["axes"])
+    if c["op"] == "append":
+        F.cache_append(s["cache"], s["tables"], s["lengths"], s["k"], s["v"], counts=s["counts"],
+                       positions=s["positions"], axes=s.get("axes"), key_mask=s["key_mask"])
+        return s["k_pages"], s["v_pages"], s["live"]
+    if c["op"] == "attend":
+        return F.cached_attention(s["q"], s["cache"], s["tables"], s["lengths"], counts=s["counts"],
+                                  positions=s["positions"], axes=s.get("axes"), causal=bool(c["causal"]))
+    if not c["block"]:
+        return F.token_norm(s["x"], s["next_weight"], s.get("next_bias"), kind=c["kind"], eps=EPS)
+    return F.residual_norm(s["x"], s["h"], s["weight"], s.get("bias"), gate=s.get("gate"), gate_act=c["act"],
+                           next_weight=s["next_weight"], next_bias=s.get("next_bias"), kind=c["kind"], eps=EPS, scale=0.5)
+
+
+def _turned(x, positions, c):
+    """x [B, L, H, D] in float32 with its pairs turned."""
+    parts, at = [], 0
+    for a, d in enumerate(_dims(c)):
+        f = 10000.0 ** (-torch.arange(0, d, 2, device=x.device, dtype=torch.float64) / d) * SCALE[c["pos"]]
+        w = (positions[..., a, None].double() * f)[..., None, :]
+        cos, sin = torch.cos(w).float(), torch.sin(w).float()
+        v = x[..., at:at + d]
+        x0, x1 = (v[..., 0::2], v[..., 1::2]) if c["inter"] else (v[..., :d // 2], v[..., d // 2:])
+        y0, y1 = x0 * cos - x1 * sin, x0 * sin + x1 * cos
+        parts.append(torch.stack([y0, y1], -1).flatten(-2) if c["inter"] else torch.cat([y0, y1], -1))
+        at += d
+    return torch.cat(parts + [x[..., at:]], -1)
+
+
+def _normed(x, weight, bias, kind):
+    if kind == "layer":
+        x = x - x.mean(-1, keepdim=True)
+    x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS) * weight
+    return x if bias is None else x + bias
+
+
+def _plain(s, c):
+    dt = DTYPES[c["dtype"]]
+    if c["op"] == "rotary":
+        return _turned(s["x"].float(), s["positions"], c).to(dt)
+    if c["op"] == "norm":
+        y = s["x"].float()
+        if c["block"]:
+            z = _normed(s["h"].float(), s["weight"], s.get("bias"), c["kind"])
+            if "gate" in s:
+                g = s["gate"].float()
+                z = z * {"none": lambda t: t, "sigmoid": torch.sigmoid, "tanh": torch.tanh,
+                         "silu": lambda t: t * torch.sigmoid(t)}[c["act"]](g)
+            y = y + 0.5 * z
+        n = _normed(y, s["next_weight"], s.get("next_bias"), c["kind"]).to(dt)
+        return (y.to(dt), n) if c["block"] else n
+    B, T, Hk, D, P = c["B"], c["T"], c["Hk"], c["D"], c["page"]
+    lens = s["lengths"].long()
+    counts = torch.full_like(lens, T) if s["counts"] is None else s["counts"].long()
+    t = torch.arange(T, device=lens.device)
+    if c["op"] == "append":
+        k = s["k"].float()
+        k = _turned(k, s["positions"], c).to(dt) if c["dims"] else s["k"]
+        slot = (lens - counts)[:, None] + t
+        page = s["tables"].long().gather(1, slot.clamp_min(0) // P)
+        where, new = (page, slot.clamp_min(0) % P), (k, s["v"], s["key_mask"])
+        if c["ragged"]:
+            ok = (t < counts[:, None]) & (slot >= 0)
+            where, new = (page[ok], where[1][ok]), [None if x is None else x[ok] for x in new]
+        for pages, x in zip((s["k_pages"], s["v_pages"], s["live"]), new):
+            if pages is not None:
+                pages[where] = x
+        return s["k_pages"], s["v_pages"], s["live"]
+    H, n = c["H"], c["n"]
+    q = s["q"].float()
+    q = _turned(q, s["positions"], c) if c["dims"] else q
+    q = q.reshape(B, T, Hk, H // Hk, D).permute(0, 2, 3, 1, 4).reshape(B, Hk, H // Hk * T, D) * D ** -0.5
+    j = torch.arange(n, device=lens.device)
+    page = s["tables"].long().clamp_min(0)[:, j // P]
+    k = s["k_pages"][page, j % P].float().permute(0, 2, 3, 1).contiguous()
+    v = s["v_pages"][page, j % P].float().permute(0, 2, 1, 3).contiguous()
+    last = lens[:, None] - (counts[:, None] - 1 - t).clamp_min(0) if c["causal"] else lens[:, None].expand(B, T)
+    last = torch.where(t < counts[:, None], last, 0)
+    ok = j < last[..., None]                                     # [B, T, n]
+    if s["live"] is not None:
+        ok = ok & s["live"][page, j % P][:, None]
+    ok = ok[:, None, None].expand(B, 1, H // Hk, T, n).reshape(B, 1, H // Hk * T, n)
+    sc = (q @ k).masked_fill(~ok, -math.inf)
+    p = torch.exp(sc - sc.amax(-1, keepdim=True).clamp_min(-1e30))
+    o = (p @ v) / p.sum(-1, keepdim=True).clamp_min(1e-30)
+    return o.reshape(B, Hk, H // Hk, T, D).permute(0, 3, 1, 2, 4).reshape(B, T, H, D).to(dt)
+
+
+# ------------------------------------------------------------------------------------------------ what a pass needs
+def work(case):
+    c = case
+    e = 4 if c["dtype"] == "float32" else 2
+    if c["op"] == "rotary":
+        n = c["B"] * c["L"] * c["H"] * c["D"]
+        p = 4 * c["L"] * AXES[c["pos"]] * (1 if c["pos"] == "grid" else c["B"])
+        g = c["train"] and c["pos"] == "splats"
+        return {"bytes": n * e * (4 if c["train"] else 2) + p * (2 if g else 1),
+                "flops": n * (3 * (1 + c["train"]) + (3 if g else 0))}
+    if c["op"] == "norm":
+        n = c["B"] * c["L"] * c["C"]
+        t = (2 if not c["block"] else 4) + (c["block"] and c["gate"] == "token")
+        b = 3 + c["block"] * 3
+        g = {"image": 4 * c["B"] * c["C"]}.get(c["gate"], 4 * c["C"]) if c["block"] else 0
+        if c["train"]:      # the upstream gradients in, the inputs' gradients out
+            t += (2 if not c["block"] else 4) + (c["block"] and c["gate"] == "token")
+        return {"bytes": n * e * t + (g + 8 * c["C"]) * (1 + c["train"]), "flops": n * (b * 3 * (1 + 2 * c["train"]))}
+    lens, counts = _lengths(c), _counts(c) if c["ragged"] else [c["T"]] * c["B"]
+    if c["op"] == "append":
+        n = sum(counts) * c["Hk"] * c["D"]
+        return {"bytes": 4 * n * e + (2 * sum(counts) if c["masked"] else 0), "flops": 3 * n if c["dims"] else 0}
+    keys = sum(n for n, m in zip(lens, counts) if m) * (0.6 if c["masked"] else 1.0)
+    pairs = sum(n * m for n, m in zip(lens, counts)) * (0.6 if c["masked"] else 1.0)
+    rows = c["B"] * c["T"] * c["H"] * c["D"]
+    return {"bytes": e * (2 * rows + 2 * keys * c["Hk"] * c["D"]), "flops": 4 * pairs * c["H"] * c["D"]}
+
+
+# ------------------------------------------------------------------------------------------------ in 64 bits
+def _turn64(x, pos, c):
+    """The rotation as a product of complex numbers, x [B, L, H, D] and pos [B or nothing, L, axes] in float64."""
+    out, at = [], 0
+    for a, d in enumerate(_dims(c)):
+        i = torch.arange(d // 2, device=x.device, dtype=torch.float64)
+        w = pos[..., a].unsqueeze(-1).unsqueeze(-1) * (SCALE[c["pos"]] * torch.exp(-2 * i / d * math.log(10000.0)))
+        v = x[..., at:at + d].unflatten(-1, (d // 2, 2) if c["inter"] else (2, d // 2))
+        v = v if c["inter"] else v.transpose(-1, -2)
+        z = torch.complex(v[..., 0], v[..., 1]) * torch.complex(torch.cos(w), torch.sin(w))
+        r = torch.view_as_real(z)
+        out.append((r if c["inter"] else r.transpose(-1, -2)).flatten(-2))
+        at += d
+    return torch.cat(out + [x[..., at:]], -1) if out else x
+
+
+def exact(case, seed):
+    import torch.nn.functional as F
+    c = case
+    s = prepare(case, seed)
+    grad = bool(c["train"])
+    d = {n: s[n].detach().double().requires_grad_(grad and n in s["leaves"]) for n in s
+         if isinstance(s[n], torch.Tensor) and s[n].is_floating_point() and n not in ("k_pages", "v_pages")}
+    if c["op"] in ("rotary", "norm"):
+        with torch.set_grad_enabled(grad):
+            if c["op"] == "rotary":
+                ys = (_turn64(d["x"], d.get("positions", s["positions"].double()), c),)
+            else:
+                def norm(x, w, b):
+                    if c["kind"] == "layer":
+                        return F.layer_norm(x, (c["C"],), w, b, EPS)
+                    y = x * w / (x.square().mean(-1, keepdim=True) + EPS).sqrt()
+                    return y if b is None else y + b
+
+                y = d["x"]
+                if c["block"]:
+                    z = norm(d["h"], d["weight"], d.get("bias"))
+                    if "gate" in d:
+                        z = z * {"none": lambda t: t, "sigmoid": torch.sigmoid, "tanh": torch.tanh, "silu": F.silu}[c["act"]](
+                            d["gate"])
+                    y = y + z / 2
+                n = norm(y, d["next_weight"], d.get("next_bias"))
+                ys = (y, n) if c["block"] else (n,)
+        out = {f"y{i}": t.detach() for i, t in enumerate(ys)}
+        if grad:
+            up = [t.double() for t in s["up"]]
+            for n, t in zip(s["leaves"], torch.autograd.grad(ys, [d[n] for n in s["leaves"]], up)):
+                out["d" + n] = t
+        return out
+    B, T, Hk, D, P = c["B"], c["T"], c["Hk"], c["D"], c["page"]
+    lens, counts = _lengths(c), _counts(c) if s["counts"] is not None else [T] * B
+    pos = None if s["positions"] is None else s["positions"].double()
+    if c["op"] == "append":
+        if s["k_pages"].numel() > 1 << 27:
+            return None
+        out = {"y0": s["k_pages"].double(), "y1": s["v_pages"].double()}
+        if s["live"] is not None:
+            out["y2"] = s["live"]
+        k = _turn64(d["k"], pos, c) if c["dims"] else d["k"]
+        for b in range(B):
+            lo = max(0, counts[b] - lens[b])
+            slot = torch.arange(lens[b] - counts[b] + lo, lens[b], device=k.device)
+            page = s["tables"][b].long()[slot // P]
+            new = slice(lo, counts[b])
+            out["y0"][page, slot % P] = k[b, new]
+            out["y1"][page, slot % P] = d["v"][b, new]
+            if s["live"] is not None:
+                out["y2"][page, slot % P] = s["key_mask"][b, new]
+        return out
+    H = c["H"]
+    q = _turn64(d["q"], pos, c) if c["dims"] else d["q"]
+    o = torch.zeros_like(q)
+    for b in range(B):
+        j = torch.arange(lens[b], device=q.device)
+        page = s["tables"][b].long()[j // P]
+        keep = torch.ones_like(j, dtype=torch.bool) if s["live"] is None else s["live"][page, j % P]
+        for h in range(Hk):
+            k = s["k_pages"][page, j % P, h].double()
+            v = s["v_pages"][page, j % P, h].double()
+            for t in range(counts[b]):
+                see = keep & (j <= lens[b] - counts[b] + t) if c["causal"] else keep
+                if not lens[b]:
+                    continue
+                r = slice(h * (H // Hk), (h + 1) * (H // Hk))
+                sc = torch.where(see, torch.mm(q[b, t, r], k.t().contiguous()) / math.sqrt(D), -1e300)
+                o[b, t, r] = torch.mm(torch.softmax(sc, -1) * see, v)
+    return {"y0": o}
