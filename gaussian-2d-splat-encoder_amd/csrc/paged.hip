@@ -1,0 +1,612 @@
+// Attention of a few new tokens over a paged cache: o = softmax(scale q k^T) v for queries q[B, T, H, D] (turned by their
+// positions on the way in) over the tokens of each sequence's pages, all of them or (causal) those up to the query's own.
+//
+// The H / Hk heads that share keys are rows of one problem, r = token * rep + head within the group. Tokens are read once:
+// time is memory's, so the work is cut along the cache, each workgroup a piece of one sequence's tokens for one key head and up
+// to 32 rows. Pieces are as long for all sequences (each workgroup finds its own from the lengths on the device, so that ragged
+// batches fill the card and a captured graph follows its lengths); a second kernel joins them.
+//
+// A wave takes tiles of its own: 32 tokens (16 of floats), keys straight from memory into matrix-instruction operands, values
+// through LDS for a transposing read, the next tile in flight, places in the pages looked up three tiles ahead. Scores are held
+// transposed, a lane per row, so that probabilities are the second product's operand as they leave the first. Running maxima
+// and sums, accumulators and partial results are 32-bit floats. Probabilities, and queries that were turned, are taken as sums
+// of two bf16 values: matrix instructions wait for memory here, and a single rounding would show next to the result's own.
+//
+// Tokens past the length or marked dead are not read and count as zeros. Tokens after a causal query have probability zero; a
+// tile whose values there are not finite is multiplied query by query with those values as zeros.
+#include <algorithm>
+
+#include "token_common.h"
+
+namespace splat {
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kLeast = 128;      // tokens of a piece at least: one bf16 tile for each wave
+constexpr int kTarget = 768;     // workgroups aimed at
+
+struct Cached {
+  splat_cache c;
+  splat_rotation r;
+  splat_positions pos;
+  const void* q;
+  void* o;
+  long long qb, ql, qh;
+  float scale;                 // of the scores, times log2 e
+  int T, H, rep, R;            // new tokens; query heads; of a key head; rows = T rep
+  int tiles, pieces, causal;   // row tiles; pieces aimed at, over all sequences
+  int units;                   // of a head, single pairs
+  bool chunked, alike;         // heads are whole chunks; keys and values have the same strides
+  FastDiv by_rep, by_page, by_units;
+  float *part, *stat;          // rows of the pieces of split sequences; their maxima and sums
+};
+
+template <typename T> constexpr int kTile = sizeof(T) == 2 ? 32 : 16;   // tokens of a wave's tile
+
+__device__ __forceinline__ long long wave_sum(long long v) {
+#pragma unroll
+  for (int i = 32; i; i /= 2) v += __shfl_xor(v, i);
+  return v;
+}
+__device__ __forceinline__ int wave_scan(int v) {   // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) {
+    const int u = __shfl_up(v, i);
+    if (lane >= i) v += u;
+  }
+  return v;
+}
+
+// Tokens of a piece, the same for all sequences: what the aimed at number of pieces would have, at least kLeast.
+__device__ __forceinline__ int piece_length(const Cached& a) {
+  long long n = 0;
+  for (int b = threadIdx.x & 63; b < a.c.B; b += 64) n += cached_tokens(a.c, b);
+  n = wave_sum(n);
+  const long long per = ((n + a.pieces - 1) / a.pieces + kLeast - 1) / kLeast * kLeast;
+  return (int)max((long long)kLeast, min(per, 0x7fffff00LL));
+}
+
+// A sequence's pieces and the first one's slot among those of split sequences.
+struct Piece {
+  int b, i, n, len, slot;
+};
+// The sequence and piece of workgroup `s` (Of: of sequence `s` its first one); b < 0 where there is none.
+template <bool Of>
+__device__ __forceinline__ Piece find(const Cached& a, int s) {
+  const int per = piece_length(a), lane = threadIdx.x & 63;
+  int first = 0, slot = 0;
+  for (int b0 = 0; b0 < a.c.B; b0 += 64) {
+    const int b = b0 + lane, len = b < a.c.B ? cached_tokens(a.c, b) : 0;
+    const int n = b < a.c.B ? (len > 0 ? (len - 1) / per + 1 : 1) : 0, m = n > 1 ? n : 0;
+    const int upto = first + wave_scan(n), slots = slot + wave_scan(m);
+    const unsigned long long hit = __ballot(Of ? b == s : upto > s);
+    if (hit) {
+      const int f = __builtin_ctzll(hit);
+      const int nf = __shfl(n, f);
+      return {b0 + f, Of ? 0 : s - (__shfl(upto, f) - nf), nf, __shfl(len, f), __shfl(slots, f) - __shfl(m, f)};
+    }
+    first = __shfl(upto, 63);
+    slot = __shfl(slots, 63);
+  }
+  return {-1, 0, 0, 0, 0};
+}
+
+template <typename T, int DP>
+struct Form {
+  static constexpr int V = kV<T>, KT = kTile<T>, NT = KT / 16;
+  static constexpr int nc = DP / (4 * V);                  // chunks that a lane holds of a key
+  static constexpr int nd = DP / 16;                       // 16-wide blocks of a head
+  static constexpr int cp = DP == 96 ? 128 / V : DP / V;   // lanes along a row of values, a power of two
+  static constexpr int rs = 64 / cp, nv = KT / rs;         // rows of values a load; loads
+  static constexpr int ld = DP + V;                        // LDS row
+};
+
+// acc(16 x 16) += A(16 x 4V) B(4V x 16): lane l gives row (A) or column (B) l % 16 and the indices of its chunk, the same for
+// both; its four results are column l % 16 at the rows 4 (l / 16) + r.
+__device__ __forceinline__ void mma16(f32x4& acc, const Chunk<bf16>& a, const Chunk<bf16>& b) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)a.v, *(const bf16x8*)b.v, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma16(f32x4& acc, const Chunk<float>& a, const Chunk<float>& b) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], acc, 0, 0, 0);
+}
+
+// Largest and sum over the four lanes of a row (16 apart).
+__device__ __forceinline__ float row_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float row_add(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Values of the 16-wide block at t as an operand: the lane's column l % 16 of the tile's rows in the order of its probabilities.
+__device__ __forceinline__ Chunk<bf16> values16(const bf16* t, int ld, int lane) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const int g = lane >> 4, i = lane & 15;
+  const bf16* p = t + (g * 4 + (i >> 2)) * ld + (i & 3) * 4;
+  Chunk<bf16> c;
+  *(s16x4*)c.v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+  *(s16x4*)(c.v + 4) = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * ld));
+  return c;
+}
+__device__ __forceinline__ Chunk<float> values16(const float* t, int ld, int lane) {
+  const float* p = t + (lane >> 4) * 4 * ld + (lane & 15);
+  Chunk<float> c;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c.v[j] = p[j * ld];
+  return c;
+}
+
+// Keeps the wave's LDS writes and reads in the order of the source (the LDS itself takes a wave's accesses in order).
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// A lane's token of a tile: its page (-1: none) and place there.
+struct Place {
+  int page, off;
+};
+
+template <typename T, int DP, int NR>
+struct Lds {
+  using F = Form<T, DP>;
+  union alignas(16) {
+    T values[kWaves][F::KT * F::ld];
+    struct {
+      float o[kWaves][16 * NR][DP + 4];
+      float m[kWaves][16 * NR], l[kWaves][16 * NR];
+    } join;
+    T q[2][16 * NR * F::ld];   // the rows' queries, and what rounding them left
+  };
+};
+
+template <typename T, int DP, int NR>
+__global__ __launch_bounds__(kThreads) void k_cached(Cached a) {
+  using F = Form<T, DP>;
+  constexpr int V = F::V, KT = F::KT;
+  __shared__ Lds<T, DP, NR> lds;
+  const int rt = blockIdx.x % a.tiles, sh = blockIdx.x / a.tiles, hk = sh % a.c.Hk;
+  const Piece pc = find<false>(a, sh / a.c.Hk);
+  if (pc.b < 0) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, b = pc.b, len = pc.len;
+  const int per = ((len - 1) / pc.n + 32) / 32 * 32, k0 = pc.i * per, k1 = min(len, k0 + per);
+  const int tend = (k1 + KT - 1) / KT;
+  const int fresh = new_tokens(a.c, b, a.T), r0 = rt * 16 * NR;
+  const int* table = a.c.tables + b * a.c.tb;
+  const T *kb = (const T*)a.c.k + hk * a.c.kh, *vb = (const T*)a.c.v + hk * a.c.vh;
+
+  auto lookup = [&](int t) {
+    const int key = t * KT + (lane & (KT - 1));
+    Place p{-1, 0};
+    if (key < k1) {
+      const int i = key / a.by_page;
+      p.page = table[i];
+      p.off = key - i * a.c.page;
+    }
+    return p;
+  };
+  auto known = [&](const Place& p) { return p.page >= 0 && p.page < a.c.pages; };
+  auto alive = [&](const Place& p) {
+    return known(p) && a.c.live ? a.c.live[p.page * a.c.lp + p.off * a.c.lt] : (unsigned char)known(p);
+  };
+  Chunk<T> kf[F::NT][F::nc], vr[F::nv];
+  unsigned ok;   // the tile's tokens that count
+  auto fetch = [&](const Place& p, unsigned char m) {
+    ok = (unsigned)(__ballot(m != 0) & ((1ull << KT) - 1));
+    const long long ko = p.page * a.c.kp + p.off * a.c.kt, vo = a.alike ? ko : p.page * a.c.vp + p.off * a.c.vt;
+#pragma unroll
+    for (int t = 0; t < F::NT; ++t) {
+      const int row = 16 * t + (lane & 15);
+      const T* at = kb + __shfl(ko, row);
+      const bool in = (ok >> row) & 1;
+#pragma unroll
+      for (int c = 0; c < F::nc; ++c) {
+        const int d = (c * 4 + g) * V;
+        if (a.chunked) {
+          kf[t][c] = Chunk<T>{};
+          if (in && d < a.c.D) __builtin_memcpy(kf[t][c].v, at + d, 16);
+        } else {
+          kf[t][c] = load_chunk(at + d, in ? a.c.D - d : 0);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < F::nv; ++i) {
+      const int row = lane / F::cp + i * F::rs, d = lane % F::cp * V;
+      const T* at = vb + __shfl(vo, row);
+      const bool in = (ok >> row) & 1;
+      if (a.chunked) {
+        vr[i] = Chunk<T>{};
+        if (in && d < a.c.D) __builtin_memcpy(vr[i].v, at + d, 16);
+      } else {
+        vr[i] = load_chunk(at + d, in ? a.c.D - d : 0);
+      }
+    }
+  };
+
+  int t = k0 / KT + w;
+  Place p1 = lookup(t + kWaves), p2 = lookup(t + 2 * kWaves);
+  {
+    const Place p0 = lookup(t);
+    fetch(p0, alive(p0));
+  }
+  unsigned char m1 = alive(p1);
+
+  // the rows' queries
+  const int rows = min(16 * NR, a.R - r0);
+  for (int i = threadIdx.x; i < 16 * NR * a.units; i += kThreads) {
+    const int r = i / a.by_units;
+    const PairUnit u = pair_unit<1>(a.r, a.c.D, i - r * a.units);
+    float x[1] = {0.f}, y[1] = {0.f};
+    if (r < rows) {
+      const int qt = (r0 + r) / a.by_rep, h = hk * a.rep + (r0 + r - qt * a.rep);
+      const T* q = (const T*)a.q + b * a.qb + qt * a.ql + h * a.qh;
+      x[0] = (float)q[u.e0];
+      if (u.second) y[0] = (float)q[u.e1];
+      if (u.axis >= 0) {
+        float c[1], s[1];
+        turn(position(a.pos, b * a.pos.pb + qt * a.pos.pl + u.axis * a.pos.pa), a.r.quarters[u.pair], c[0], s[0]);
+        turn_runs<1, false>(x, y, c, s, false);
+      }
+    }
+    auto put = [&](int e, float f) {
+      const T hi = (T)f;
+      lds.q[0][r * F::ld + e] = hi;
+      if (sizeof(T) == 2) lds.q[1][r * F::ld + e] = fabsf((float)hi) < INFINITY ? (T)(f - (float)hi) : (T)0.f;
+    };
+    put(u.e0, x[0]);
+    if (u.second) put(u.e1, y[0]);
+  }
+  const int gap = DP - a.c.D;
+  for (int i = threadIdx.x; i < 16 * NR * gap; i += kThreads) {
+    const int r = i / gap, e = a.c.D + i - r * gap;
+    lds.q[0][r * F::ld + e] = (T)0.f;
+    if (sizeof(T) == 2) lds.q[1][r * F::ld + e] = (T)0.f;
+  }
+  __syncthreads();
+  const bool fine = sizeof(T) == 2 && a.r.axes > 0;
+  Chunk<T> qf[NR][F::nc], ql[NR][F::nc];
+  int lim[NR], own[NR], least = len;   // tokens that the lane's row sees; its query; the fewest of any row
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+#pragma unroll
+    for (int c = 0; c < F::nc; ++c) {
+      const int at = (16 * n + (lane & 15)) * F::ld + (c * 4 + g) * V;
+      *(f32x4*)qf[n][c].v = *(const f32x4*)&lds.q[0][at];
+      if (sizeof(T) == 2) *(f32x4*)ql[n][c].v = *(const f32x4*)&lds.q[1][at];
+    }
+    const int r = r0 + 16 * n + (lane & 15);
+    own[n] = r / a.by_rep;
+    lim[n] = r >= a.R ? len : own[n] >= fresh ? 0 : a.causal ? max(0, len - (fresh - 1 - own[n])) : len;
+    least = min(least, lim[n]);
+  }
+#pragma unroll
+  for (int i = 8; i; i /= 2) least = min(least, __shfl_xor(least, i));
+  least = __builtin_amdgcn_readfirstlane(least);
+  __syncthreads();
+
+  T* tv = lds.values[w];
+  float m[NR], l[NR];
+  f32x4 acc[NR][F::nd];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < F::nd; ++d) acc[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll 1
+  for (; t < tend; t += kWaves) {
+    const unsigned char m2 = alive(p2);
+    const Place p3 = lookup(t + 3 * kWaves);
+    // values to LDS; whether those that some row does not see are finite
+    bool odd = false;
+    const bool edge = (t + 1) * KT > least;
+    wave_order();
+#pragma unroll
+    for (int i = 0; i < F::nv; ++i) {
+      const int row = lane / F::cp + i * F::rs, d = lane % F::cp * V;
+      if (DP != 96 || d < DP) *(f32x4*)(tv + row * F::ld + d) = *(const f32x4*)vr[i].v;
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) odd |= !(fabsf((float)vr[i].v[j]) < INFINITY);
+      }
+    }
+    wave_order();
+    odd = __any(odd);
+    f32x4 s[NR][F::NT];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+#pragma unroll
+      for (int i = 0; i < F::NT; ++i) {
+        s[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < F::nc; ++c) mma16(s[n][i], kf[i][c], qf[n][c]);
+        if (fine) {
+#pragma unroll
+          for (int c = 0; c < F::nc; ++c) mma16(s[n][i], kf[i][c], ql[n][c]);
+        }
+      }
+    }
+    const unsigned here = ok;
+    fetch(p1, m1);
+    p1 = p2, m1 = m2, p2 = p3;
+
+    const bool all = !edge && here == (unsigned)((1ull << KT) - 1);
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < F::NT; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = 16 * i + 4 * g + r;
+          s[n][i][r] *= a.scale;
+          if (!all) s[n][i][r] = ((here >> key) & 1) && t * KT + key < lim[n] ? s[n][i][r] : -INFINITY;
+          top = fmaxf(top, s[n][i][r]);
+        }
+      }
+      top = fmaxf(m[n], row_max(top));
+      if (__any(top > m[n])) {
+        const float by = m[n] == -INFINITY ? 0.f : hw_exp2(m[n] - top);
+        m[n] = top;
+        l[n] *= by;
+#pragma unroll
+        for (int d = 0; d < F::nd; ++d) acc[n][d] *= by;
+      }
+      const float base = m[n] == -INFINITY ? 0.f : m[n];
+#pragma unroll
+      for (int i = 0; i < F::NT; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[n][i][r] = hw_exp2(s[n][i][r] - base);
+          l[n] += s[n][i][r];
+        }
+      }
+    }
+    // acc += values p. Part: for the rows of one query, whose values from `seen` on count as zeros.
+    auto add = [&](bool part, int query, int seen) {
+      Chunk<T> hi[NR], lo[NR];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float p = s[n][j / 4][j % 4];
+          hi[n].v[j] = (T)p;
+          if (sizeof(T) == 2) lo[n].v[j] = (T)(p - (float)hi[n].v[j]);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < F::nd; ++d) {
+        Chunk<T> f = values16(tv + 16 * d, F::ld, lane);
+        if (part) {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (t * KT + 16 * (j / 4) + 4 * g + j % 4 >= seen) f.v[j] = (T)0.f;
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          f32x4 o = acc[n][d];
+          mma16(o, f, hi[n]);
+          if (sizeof(T) == 2) mma16(o, f, lo[n]);
+          if (!part || own[n] == query) acc[n][d] = o;   // a lane's results are its own row's
+        }
+      }
+    };
+    if (!odd) {
+      add(false, 0, 0);
+    } else {
+      const int last = (min(a.R, r0 + 16 * NR) - 1) / a.by_rep;
+      for (int q = r0 / a.by_rep; q <= last; ++q)
+        add(true, q, q >= fresh ? 0 : a.causal ? max(0, len - (fresh - 1 - q)) : len);
+    }
+  }
+
+  // the waves' rows
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int r = 16 * n + (lane & 15);
+    const float sum = row_add(l[n]);
+    if (g == 0) {
+      lds.join.m[w][r] = m[n];
+      lds.join.l[w][r] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < F::nd; ++d) *(f32x4*)&lds.join.o[w][r][16 * d + 4 * g] = acc[n][d];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * NR * (DP / 4); i += kThreads) {
+    const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+    if (r >= rows || d >= a.c.D) continue;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) top = fmaxf(top, lds.join.m[k][r]);
+    const float base = top == -INFINITY ? 0.f : top;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+      const float by = hw_exp2(lds.join.m[k][r] - base);
+      sum = fmaf(lds.join.l[k][r], by, sum);
+      o += *(const f32x4*)&lds.join.o[k][r][d] * by;
+    }
+    if (pc.n == 1) {
+      const int qt = (r0 + r) / a.by_rep, h = hk * a.rep + (r0 + r - qt * a.rep);
+      T* to = (T*)a.o + (((long long)b * a.T + qt) * a.H + h) * a.c.D + d;
+      const float by = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (d + j < a.c.D) to[j] = (T)(sum == 0.f ? 0.f : o[j] * by);
+    } else {
+      const long long at = ((long long)(pc.slot + pc.i) * a.c.Hk + hk) * a.R + r0 + r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (d + j < a.c.D) a.part[at * a.c.D + d + j] = o[j];
+      if (d == 0) {
+        a.stat[2 * at] = top;
+        a.stat[2 * at + 1] = sum;
+      }
+    }
+  }
+}
+
+// Joins the pieces of a split sequence's row, one workgroup a row: a thread has four values of a head in every 256 / (D / 4)-th
+// piece, partial sums are added in order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_cached_join(Cached a) {
+  __shared__ float tops[kThreads], weight[kThreads];
+  __shared__ f32x4 part[kThreads];
+  __shared__ float sums[kThreads];
+  const int row = blockIdx.x, b = row / (a.c.Hk * a.R), hr = row - b * (a.c.Hk * a.R), hk = hr / a.R, r = hr - hk * a.R;
+  const Piece pc = find<true>(a, b);
+  if (pc.n <= 1) return;
+  const int quads = (a.c.D + 3) / 4, groups = kThreads / quads, q = threadIdx.x % quads, gr = threadIdx.x / quads;
+  auto at = [&](int i) { return ((long long)(pc.slot + i) * a.c.Hk + hk) * a.R + r; };
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < pc.n; i += kThreads) top = fmaxf(top, a.stat[2 * at(i)]);
+  tops[threadIdx.x] = top;
+  __syncthreads();
+  for (int i = kThreads / 2; i; i /= 2) {
+    if ((int)threadIdx.x < i) tops[threadIdx.x] = fmaxf(tops[threadIdx.x], tops[threadIdx.x + i]);
+    __syncthreads();
+  }
+  top = tops[0];
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+  for (int i0 = 0; i0 < pc.n; i0 += kThreads) {
+    __syncthreads();
+    const int n = min(kThreads, pc.n - i0);
+    if ((int)threadIdx.x < n) {
+      weight[threadIdx.x] = hw_exp2(a.stat[2 * at(i0 + threadIdx.x)] - base);
+      sum += a.stat[2 * at(i0 + threadIdx.x) + 1] * weight[threadIdx.x];
+    }
+    __syncthreads();
+    if (gr < groups) {
+#pragma unroll 4
+      for (int i = gr; i < n; i += groups) {
+        const float* p = a.part + at(i0 + i) * a.c.D + 4 * q;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (4 * q + 4 <= a.c.D) {
+          __builtin_memcpy(&v, p, 16);
+        } else {
+          for (int j = 0; j < a.c.D - 4 * q; ++j) v[j] = p[j];
+        }
+        o += v * weight[i];
+      }
+    }
+  }
+  part[threadIdx.x] = o;
+  sums[threadIdx.x] = sum;
+  __syncthreads();
+  for (int i = kThreads / 2; i; i /= 2) {
+    if ((int)threadIdx.x < i) sums[threadIdx.x] += sums[threadIdx.x + i];
+    __syncthreads();
+  }
+  if (gr != 0) return;
+  for (int i = 1; i < groups; ++i) o += part[i * quads + q];
+  sum = sums[0];
+  const int qt = r / a.by_rep, h = hk * a.rep + (r - qt * a.rep);
+  T* to = (T*)a.o + (((long long)b * a.T + qt) * a.H + h) * a.c.D + 4 * q;
+  const float by = sum == 0.f ? 0.f : 1.f / sum;
+  for (int j = 0; j < min(4, a.c.D - 4 * q); ++j) to[j] = (T)(sum == 0.f ? 0.f : o[j] * by);
+}
+
+int check_call(const char* who, const splat_cache* c, const splat_rotation* r, const splat_positions* p, int H, long long T,
+               float scale) {
+  if (const int rc = check_cache(who, c)) return rc;
+  if (H < 1 || H % c->Hk || T < 0) return set_error(kInvalid, "%s: %d heads over %d, %lld tokens", who, H, c->Hk, T);
+  if (!(fabsf(scale) <= 3.402823466e38f)) return set_error(kInvalid, "%s: scale %g", who, scale);
+  if (T > 0x7fffffffLL || T * H > 0x7fffffffLL || c->B * T * H > 0x7fffffffLL)
+    return set_error(kUnsupported, "%s: %d x %lld tokens of %d heads", who, c->B, T, H);
+  return check_rotation(who, r, p, c->D);
+}
+
+Cached plan(const splat_cache& c, int H, int T) {
+  Cached n{};
+  n.c = c;
+  n.H = H;
+  n.T = T;
+  n.rep = H / c.Hk;
+  n.R = T * n.rep;
+  n.tiles = div_up(n.R, n.R > 16 ? 32 : 16);
+  n.pieces = std::max(1, div_up(kTarget, (long long)c.Hk * n.tiles));
+  n.by_rep = fast_div(n.rep);
+  n.by_page = fast_div(c.page);
+  return n;
+}
+
+// Slots of the pieces of split sequences: those have more than one piece, each more than half as long as the others.
+bool may_split(const Cached& n) { return (long long)n.c.page * n.c.width > kLeast && n.pieces > 1; }
+size_t slots(const Cached& n) { return may_split(n) ? (size_t)2 * n.pieces : 0; }
+
+template <typename F>
+int with_form(int dtype, int D, int R, F&& f) {
+  auto rows = [&](auto t, auto dp) {
+    return R > 16 ? f(t, dp, std::integral_constant<int, 2>{}) : f(t, dp, std::integral_constant<int, 1>{});
+  };
+  auto head = [&](auto t) {
+    if (D <= 32) return rows(t, std::integral_constant<int, 32>{});
+    if (D <= 64) return rows(t, std::integral_constant<int, 64>{});
+    if (D <= 96) return rows(t, std::integral_constant<int, 96>{});
+    return rows(t, std::integral_constant<int, 128>{});
+  };
+  return dtype == kF32 ? head(float{}) : head(bf16{});
+}
+
+}  // namespace
+}  // namespace splat
+
+using namespace splat;
+
+extern "C" {
+
+size_t splat_cached_attention_workspace_bytes(const splat_cache* c, int H, long long T) {
+  if (check_call("splat_cached_attention_workspace_bytes", c, nullptr, nullptr, H, T, 0.f) || c->B == 0 || T == 0) return 0;
+  const Cached n = plan(*c, H, (int)T);
+  return sizeof(float) * slots(n) * c->Hk * n.R * (c->D + 2);
+}
+
+int splat_cached_attention(const splat_cache* c, const splat_rotation* r, const splat_positions* p, const void* q, long long qb,
+                           long long ql, long long qh, int H, long long T, float scale, int causal, void* o, void* ws,
+                           size_t ws_bytes, void* stream) {
+  if (const int rc = check_call("splat_cached_attention", c, r, p, H, T, scale)) return rc;
+  if (c->B == 0 || T == 0) return kOk;
+  if (!q || !o) return set_error(kInvalid, "splat_cached_attention: null pointer");
+  Cached n = plan(*c, H, (int)T);
+  const size_t need = splat_cached_attention_workspace_bytes(c, H, T);
+  if (need && (!ws || ws_bytes < need))
+    return set_error(kWorkspace, "splat_cached_attention: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  const long long grid = ((long long)n.pieces + c->B) * c->Hk * n.tiles;
+  if (grid > 0x7fffffffLL) return set_error(kUnsupported, "splat_cached_attention: %d sequences of %d heads", c->B, H);
+  if (r) n.r = *r;
+  if (p) n.pos = *p;
+  n.q = q, n.o = o, n.qb = qb, n.ql = ql, n.qh = qh, n.causal = causal;
+  n.scale = scale * kLog2e;
+  n.units = pair_units(n.r, c->D, 1).n;
+  n.by_units = fast_div(n.units);
+  n.chunked = c->D % (c->dtype == kF32 ? 4 : 8) == 0;
+  n.alike = c->kp == c->vp && c->kt == c->vt;
+  if (need) {
+    n.stat = (float*)ws;
+    n.part = n.stat + 2 * slots(n) * c->Hk * n.R;
+  }
+  const hipStream_t st = (hipStream_t)stream;
+  return with_form(c->dtype, c->D, n.R, [&](auto t, auto dp, auto nr) {
+    using E = decltype(t);
+    k_cached<E, decltype(dp)::value, decltype(nr)::value><<<(unsigned)grid, kThreads, 0, st>>>(n);
+    if (need) k_cached_join<E><<<(unsigned)(c->B * c->Hk * n.R), kThreads, 0, st>>>(n);
+    return check_launch("splat_cached_attention");
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,563 @@
+// Norms per token with a block's gate and residual, forward and backward, on rows of C channels:
+//
+//   u = (h - m1) r1, z = w1 u + b1, y = x + scale act(gate) z, v = (y - m2) r2, n = w2 v + b2
+//
+// layer norms: m the row's mean, r = 1 / sqrt(mean((h - m)^2) + eps); root-mean-square norms: m = 0. Either norm may be left
+// out, and with h the whole block: then y = x, and n is a plain norm per token. The gate has a row for all tokens, for each
+// image's, or for every token. Backward, with dv = dn w2:
+//
+//   dy' = dy + r2 (dv - mean(dv) - v mean(dv v)), dx = dy', dz = scale act(gate) dy', dgate = scale act'(gate) dy' z,
+//   du = dz w1, dh = r1 (du - mean(du) - u mean(du u)); the means of dv and du of layer norms only
+//   dw2 = sum dn v, db2 = sum dn, dw1 = sum dz u, db1 = sum dz over the tokens
+//
+// A row is held by TPR threads, K 16-byte chunks each, in registers; it is read once, and its sums are exchanged within a wave
+// (TPR <= 64) or through LDS. A workgroup takes a range of rows with the parameters' columns in registers. The backward reads x
+// and h again (y's rounding would show in the parameters' float32 gradients) with the rows' statistics kept by the forward, and
+// sums columns in registers over its rows, whose partial sums a second kernel adds in order.
+#include <algorithm>
+
+#include "feat_common.h"
+#include "splat_tokens.h"
+
+namespace splat {
+namespace {
+
+constexpr int kMaxChannels = 8192;   // a row's values and column sums in the registers of 1,024 threads
+enum Gate : int { kNoGate = 0, kRowGate = 1, kTokenGate = 2 };   // none; a row for each segment of tokens; a row for each token
+
+struct TokenNorm {
+  splat_token_norm a;
+  const void *x, *h, *gate, *dy, *dn;
+  const float *w1, *b1, *w2, *b2;
+  void *y, *n, *dx, *dh, *dgate;  // dgate: of a gate for every token
+  float4* stat;                   // m1, r1, m2, r2 of each row
+  float *cols, *gates;            // partial sums [workgroups][4][C] of dw1, db1, dw2, db2; [segments][splits][C] of the gate
+  long long seg;                  // rows of a segment
+  int segs, splits, whole;        // segments; workgroups of one, or whole segments of a workgroup (the other is 1)
+  long long per;                  // rows of a split
+};
+
+// Sum over groups of TPR lanes, the same in each lane.
+template <int TPR>
+__device__ __forceinline__ float lanes_add(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  if constexpr (TPR >= 2) v += dpp(v, std::integral_constant<int, 0xb1>{});
+  if constexpr (TPR >= 4) v += dpp(v, std::integral_constant<int, 0x4e>{});
+  if constexpr (TPR >= 8) v += dpp(v, std::integral_constant<int, 0x141>{});
+  if constexpr (TPR >= 16) v += dpp(v, std::integral_constant<int, 0x140>{});
+  if constexpr (TPR >= 32) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  }
+  if constexpr (TPR >= 64) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  }
+  return v;
+}
+
+// Sums of N values over a row's threads. Rows of more than a wave exchange through LDS: two buffers in turn, so that one
+// barrier a sum does.
+template <int TPR, int N>
+struct RowSum {
+  float (*red)[2][N][16];
+  int flip = 0;
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lanes_add<TPR < 64 ? TPR : 64>(v[i]);
+    if constexpr (TPR > 64) {
+      const int w = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) (*red)[flip][i][w] = v[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < TPR / 64; ++k) s += (*red)[flip][i][k];
+        v[i] = s;
+      }
+      flip ^= 1;
+    }
+  }
+};
+
+template <typename T, int TPR, int K>
+struct Cols {
+  static constexpr int V = kV<T>;
+  int C, c[K], nv[K];   // channels; the thread's first one of each chunk, and its channels there
+  __device__ __forceinline__ Cols(int n) : C(n) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      c[k] = (k * TPR + (threadIdx.x & (TPR - 1))) * V;
+      nv[k] = max(0, min(V, C - c[k]));
+    }
+  }
+};
+
+template <typename T, int K>
+using Vals = float[K][kV<T>];
+
+template <typename T, int TPR, int K>
+__device__ __forceinline__ void load_row(const T* p, const Cols<T, TPR, K>& at, Vals<T, K>& f) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const Chunk<T> c = load_chunk(p + at.c[k], at.nv[k]);
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j) f[k][j] = (float)c.v[j];
+  }
+}
+template <typename T, int TPR, int K>
+__device__ __forceinline__ void store_row(T* p, const Cols<T, TPR, K>& at, const Vals<T, K>& f) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    Chunk<T> c;
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j) c.v[j] = (T)f[k][j];
+    store_chunk(p + at.c[k], c, at.nv[k]);
+  }
+}
+// A row of float parameters, `none` where there are none.
+template <typename T, int TPR, int K>
+__device__ __forceinline__ void load_params(const float* p, const Cols<T, TPR, K>& at, float none, Vals<T, K>& f) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j) f[k][j] = none;
+    if (p && at.nv[k] == kV<T>) {
+      __builtin_memcpy(f[k], p + at.c[k], sizeof(f[k]));
+    } else if (p) {
+#pragma unroll
+      for (int j = 0; j < kV<T>; ++j)
+        if (j < at.nv[k]) f[k][j] = p[at.c[k] + j];
+    }
+  }
+}
+
+__device__ __forceinline__ float gate_of(int act, float g) {
+  return act == kActNone ? g : act == kActSigmoid ? sigmoidf(g) : act == kActSilu ? act_fwd<kActSilu>(g) : tanh_of(g);
+}
+__device__ __forceinline__ float gate_grad(int act, float g) {
+  return act == kActNone      ? 1.f
+         : act == kActSigmoid ? act_grad<kActSigmoid>(g)
+         : act == kActSilu    ? act_grad<kActSilu>(g)
+                              : act_grad<kActTanh>(g);
+}
+
+// Mean and inverse deviation of a row whose channels past C are zeros.
+template <int TPR, int K, typename T, typename Sum>
+__device__ __forceinline__ float2 row_stats(const TokenNorm& a, const Cols<T, TPR, K>& at, const Vals<T, K>& f, Sum& sum) {
+  const float inv = 1.f / (float)a.a.C;
+  float m = 0.f, q[1] = {0.f};
+  if (a.a.layer) {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < kV<T>; ++j) s[0] += f[k][j];
+    sum(s);
+    m = s[0] * inv;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j) {
+      const float d = j < at.nv[k] ? f[k][j] - m : 0.f;
+      q[0] = fmaf(d, d, q[0]);
+    }
+  sum(q);
+  return make_float2(m, 1.f / sqrtf(fmaf(q[0], inv, a.a.eps)));
+}
+
+template <int TPR>
+constexpr int kBlock = TPR > 256 ? TPR : 256;
+
+// f(first row, rows, segment) for the workgroup's ranges, each within one segment.
+template <typename F>
+__device__ __forceinline__ void ranges(const TokenNorm& a, F&& f) {
+  const int s0 = blockIdx.x / a.splits * a.whole, split = blockIdx.x % a.splits;
+  for (int s = s0; s < min(a.segs, s0 + a.whole); ++s) {
+    const long long lo = split * a.per, n = min(a.per, a.seg - lo);
+    f(s * a.seg + lo, n < 0 ? 0 : n, s, split);
+  }
+}
+
+template <typename T, int TPR, int K>
+__global__ __launch_bounds__(kBlock<TPR>) void k_token_norm(TokenNorm a) {
+  constexpr int RB = kBlock<TPR> / TPR;
+  __shared__ float red[2][1][16];
+  const Cols<T, TPR, K> at(a.a.C);
+  RowSum<TPR, 1> sum{&red};
+  Vals<T, K> w1, b1, w2, b2, gs;
+  if (a.a.post) {
+    load_params(a.w1, at, 1.f, w1);
+    load_params(a.b1, at, 0.f, b1);
+  }
+  if (a.a.next) {
+    load_params(a.w2, at, 1.f, w2);
+    load_params(a.b2, at, 0.f, b2);
+  }
+  ranges(a, [&](long long row0, long long rows, int seg, int) {
+    if (a.a.gate != kTokenGate && a.h) {
+      load_params(a.a.gate ? (const float*)a.gate + (long long)seg * a.a.C : nullptr, at, 1.f, gs);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * (a.a.gate ? gate_of(a.a.act, gs[k][j]) : 1.f);
+    }
+    const int r = threadIdx.x / TPR;
+    for (long long i = r; i < rows; i += RB) {
+      const long long row = row0 + i;
+      Vals<T, K> x, h;
+      load_row((const T*)a.x + row * a.a.xl, at, x);
+      float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (a.h) {
+        load_row((const T*)a.h + row * a.a.hl, at, h);
+        if (a.a.gate == kTokenGate) {
+          load_row((const T*)a.gate + row * a.a.gl, at, gs);
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * gate_of(a.a.act, gs[k][j]);
+        }
+        if (a.a.post) {
+          const float2 s = row_stats(a, at, h, sum);
+          st.x = s.x, st.y = s.y;
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int j = 0; j < kV<T>; ++j) h[k][j] = fmaf((h[k][j] - s.x) * s.y, w1[k][j], b1[k][j]);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < kV<T>; ++j) x[k][j] = j < at.nv[k] ? fmaf(gs[k][j], h[k][j], x[k][j]) : 0.f;
+        store_row((T*)a.y + row * a.a.C, at, x);
+      }
+      if (a.a.next) {
+        const float2 s = row_stats(a, at, x, sum);
+        st.z = s.x, st.w = s.y;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < kV<T>; ++j) x[k][j] = fmaf((x[k][j] - s.x) * s.y, w2[k][j], b2[k][j]);
+        store_row((T*)a.n + row * a.a.C, at, x);
+      }
+      if (a.stat && (threadIdx.x & (TPR - 1)) == 0) a.stat[row] = st;
+    }
+  });
+}
+
+// Column sums over the workgroup's row groups, in their order: out[c] for the chunks of the first group.
+template <typename T, int TPR, int K>
+__device__ __forceinline__ void fold_rows(Vals<T, K>& f, const Cols<T, TPR, K>& at, float* lds, float* out) {
+  constexpr int RB = kBlock<TPR> / TPR, V = kV<T>;
+  const int r = threadIdx.x / TPR, l = threadIdx.x & (TPR - 1);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if constexpr (RB > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < V; ++j) lds[(r * TPR + l) * V + j] = f[k][j];
+      __syncthreads();
+      // columns of the chunk round k, spread over all threads
+      for (int c = threadIdx.x; c < TPR * V; c += kBlock<TPR>) {
+        float s = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < RB; ++i) s += lds[i * TPR * V + c];
+        const int col = k * TPR * V + c;
+        if (col < at.C) out[col] = s;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < at.nv[k]) out[at.c[k] + j] = f[k][j];
+    }
+  }
+}
+
+template <typename T, int TPR, int K>
+__global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
+  constexpr int RB = kBlock<TPR> / TPR;
+  __shared__ float red[2][2][16];
+  __shared__ float lds[RB > 1 ? kBlock<TPR> * kV<T> : 1];
+  const Cols<T, TPR, K> at(a.a.C);
+  RowSum<TPR, 2> sum{&red};
+  const float inv = 1.f / (float)a.a.C, mean = a.a.layer ? inv : 0.f;
+  Vals<T, K> w1, b1, w2, gs, aw1 = {}, ab1 = {}, aw2 = {}, ab2 = {}, ag = {};
+  load_params(a.a.post ? a.w1 : nullptr, at, 1.f, w1);
+  load_params(a.a.post ? a.b1 : nullptr, at, 0.f, b1);
+  load_params(a.a.next ? a.w2 : nullptr, at, 1.f, w2);
+  ranges(a, [&](long long row0, long long rows, int seg, int split) {
+    if (a.a.gate != kTokenGate && a.h) {
+      load_params(a.a.gate ? (const float*)a.gate + (long long)seg * a.a.C : nullptr, at, 1.f, gs);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * (a.a.gate ? gate_of(a.a.act, gs[k][j]) : 1.f);
+    }
+    const int r = threadIdx.x / TPR;
+    for (long long i = r; i < rows; i += RB) {
+      const long long row = row0 + i;
+      Vals<T, K> x, h, g, d;   // y, then v; u, then dh; the gate, then its slope; dn, then dy'
+      load_row((const T*)a.x + row * a.a.xl, at, x);
+      if (a.h) load_row((const T*)a.h + row * a.a.hl, at, h);
+      if (a.a.gate == kTokenGate) load_row((const T*)a.gate + row * a.a.gl, at, g);
+      Vals<T, K> up;
+      if (a.dy) load_row((const T*)a.dy + row * a.a.dyl, at, up);
+      if (a.dn) load_row((const T*)a.dn + row * a.a.dnl, at, d);
+      const float4 st = a.stat[row];
+      if (a.a.gate == kTokenGate) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < kV<T>; ++j) {
+            gs[k][j] = a.a.scale * gate_of(a.a.act, g[k][j]);
+            g[k][j] = a.a.scale * gate_grad(a.a.act, g[k][j]);
+          }
+      }
+      if (a.h) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < kV<T>; ++j) {
+            if (a.a.post) h[k][j] = (h[k][j] - st.x) * st.y;
+            x[k][j] = fmaf(gs[k][j], fmaf(h[k][j], w1[k][j], b1[k][j]), x[k][j]);
+          }
+      }
+      if (a.dn) {
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < kV<T>; ++j) {
+            x[k][j] = (x[k][j] - st.z) * st.w;
+            ab2[k][j] += d[k][j];
+            aw2[k][j] = fmaf(d[k][j], x[k][j], aw2[k][j]);
+            d[k][j] *= w2[k][j];
+            s[0] += d[k][j];
+            s[1] = fmaf(d[k][j], x[k][j], s[1]);
+          }
+        sum(s);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < kV<T>; ++j) {
+            const float t = st.w * fmaf(-x[k][j], s[1] * inv, d[k][j] - s[0] * mean);
+            d[k][j] = j < at.nv[k] ? (a.dy ? up[k][j] + t : t) : 0.f;
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < kV<T>; ++j) d[k][j] = up[k][j];
+      }
+      if (a.dx) store_row((T*)a.dx + row * a.a.C, at, d);
+      if (!a.h) continue;
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < kV<T>; ++j) {
+          const float dz = gs[k][j] * d[k][j], z = fmaf(h[k][j], w1[k][j], b1[k][j]);
+          ag[k][j] = fmaf(d[k][j], z, ag[k][j]);
+          g[k][j] *= d[k][j] * z;
+          ab1[k][j] += dz;
+          aw1[k][j] = fmaf(dz, h[k][j], aw1[k][j]);
+          d[k][j] = dz * w1[k][j];
+          s[0] += d[k][j];
+          s[1] = fmaf(d[k][j], h[k][j], s[1]);
+        }
+      if (a.dgate) store_row((T*)a.dgate + row * a.a.C, at, g);
+      if (a.a.post) {
+        sum(s);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < kV<T>; ++j) d[k][j] = st.y * fmaf(-h[k][j], s[1] * inv, d[k][j] - s[0] * mean);
+      }
+      if (a.dh) store_row((T*)a.dh + row * a.a.C, at, d);
+    }
+    if (a.gates) {
+      fold_rows(ag, at, lds, a.gates + ((long long)seg * a.splits + split) * a.a.C);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < kV<T>; ++j) ag[k][j] = 0.f;
+    }
+  });
+  if (a.cols) {
+    float* out = a.cols + (long long)blockIdx.x * 4 * a.a.C;
+    if (a.a.post) {
+      fold_rows(aw1, at, lds, out);
+      fold_rows(ab1, at, lds, out + a.a.C);
+    }
+    if (a.dn) {
+      fold_rows(aw2, at, lds, out + 2 * a.a.C);
+      fold_rows(ab2, at, lds, out + 3 * a.a.C);
+    }
+  }
+}
+
+// Adds the workgroups' column sums in a fixed order: 64 columns a workgroup, its waves each a part of the sums. Entries 0 to 3
+// are the parameters' gradients, the others the gate's rows.
+constexpr int kJoin = 1024;
+__global__ __launch_bounds__(kJoin) void k_token_norm_join(TokenNorm a, int wgs, int tiles, float* dw1, float* db1, float* dw2,
+                                                           float* db2, float* dgate) {
+  __shared__ float part[kJoin / 64][64];
+  const int e = blockIdx.x / tiles, c = (blockIdx.x - e * tiles) * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const long long seg = e - 4;
+  float* out = e == 0 ? dw1 : e == 1 ? db1 : e == 2 ? dw2 : e == 3 ? db2 : dgate + seg * a.a.C;
+  if (e < 4 && !out) return;
+  const long long step = e < 4 ? 4LL * a.a.C : a.a.C;
+  const float* p = e < 4 ? a.cols + (long long)e * a.a.C : a.gates + seg * a.splits * a.a.C;
+  const int n = e < 4 ? wgs : a.splits;
+  float s = 0.f;
+  if (c < a.a.C) {
+#pragma unroll 4
+    for (int i = w; i < n; i += kJoin / 64) s += p[i * step + c];
+  }
+  part[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && c < a.a.C) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoin / 64; ++i) t += part[i][threadIdx.x & 63];
+    if (e >= 4) t *= a.a.scale * gate_grad(a.a.act, ((const float*)a.gate)[seg * a.a.C + c]);
+    out[c] = t;
+  }
+}
+
+struct Shape {
+  int tpr, k, rows;   // threads of a row; chunks of a thread; rows of a workgroup at a time
+};
+Shape shape_of(int dtype, int C) {
+  const int chunks = div_up(C, dtype == kF32 ? 4 : 8);
+  int tpr = 4;
+  while (tpr < 64 && tpr < chunks) tpr *= 2;
+  if (chunks > 128) tpr = chunks > 512 ? 1024 : 256;
+  return {tpr, chunks > tpr ? 2 : 1, std::max(1, 256 / tpr)};
+}
+
+template <typename F>
+int with_shape(int dtype, const Shape& s, F&& f) {
+  auto type = [&](auto t) {
+    auto k = [&](auto tpr) {
+      return s.k == 2 ? f(t, tpr, std::integral_constant<int, 2>{}) : f(t, tpr, std::integral_constant<int, 1>{});
+    };
+    auto one = [&](auto tpr) { return f(t, tpr, std::integral_constant<int, 1>{}); };
+    switch (s.tpr) {
+      case 4: return one(std::integral_constant<int, 4>{});
+      case 8: return one(std::integral_constant<int, 8>{});
+      case 16: return one(std::integral_constant<int, 16>{});
+      case 32: return one(std::integral_constant<int, 32>{});
+      case 64: return k(std::integral_constant<int, 64>{});
+      case 256: return k(std::integral_constant<int, 256>{});
+    }
+    if constexpr (sizeof(t) == 4) return k(std::integral_constant<int, 1024>{});
+    else return one(std::integral_constant<int, 1024>{});
+  };
+  return dtype == kF32 ? type(float{}) : type(bf16{});
+}
+
+int check_norm(const char* who, const splat_token_norm* a) {
+  if (!a) return set_error(kInvalid, "%s: no description", who);
+  if (a->dtype != kF32 && a->dtype != kBf16) return set_error(kInvalid, "%s: unknown element type %d", who, a->dtype);
+  if (a->C < 1 || a->M < 0 || a->gate < 0 || a->gate > 2 || !(a->eps >= 0.f))
+    return set_error(kInvalid, "%s: C %d, M %lld, gate %d, eps %g", who, a->C, a->M, a->gate, a->eps);
+  if (a->act != kActNone && a->act != kActSigmoid && a->act != kActSilu && a->act != kActTanh)
+    return set_error(kInvalid, "%s: activation %d of a gate", who, a->act);
+  if (a->C > kMaxChannels) return set_error(kUnsupported, "%s: %d channels, %d at most", who, a->C, kMaxChannels);
+  if (a->gate == kRowGate && (a->segs < 1 || a->M % a->segs))
+    return set_error(kInvalid, "%s: %lld tokens do not divide over %lld gates", who, a->M, a->segs);
+  if (a->M > 0x7fffffffLL || (a->gate == kRowGate && a->segs > 0x1000000LL))
+    return set_error(kUnsupported, "%s: %lld tokens, %lld gates", who, a->M, a->segs);
+  return kOk;
+}
+
+// Ranges of rows for about `target` workgroups. Returns their number.
+unsigned plan(TokenNorm& n, const Shape& s, long long target) {
+  n.segs = n.a.gate == kRowGate ? (int)n.a.segs : 1;
+  n.seg = n.a.M / n.segs;
+  n.whole = (int)((n.segs + target - 1) / target);
+  const long long most = std::max<long long>(1, (n.seg + s.rows - 1) / s.rows);
+  const long long splits = std::min(most, n.segs >= target ? 1 : (target + n.segs - 1) / n.segs);
+  n.per = std::max<long long>(1, (n.seg + splits - 1) / splits);
+  n.per = (n.per + s.rows - 1) / s.rows * s.rows;
+  n.splits = (int)std::max<long long>(1, (n.seg + n.per - 1) / n.per);
+  return (unsigned)((n.segs + n.whole - 1) / n.whole * n.splits);
+}
+
+constexpr long long kForward = 1024, kBackward = 768;   // workgroups aimed at
+
+}  // namespace
+}  // namespace splat
+
+using namespace splat;
+
+extern "C" {
+
+int splat_token_norm_fwd(const splat_token_norm* a, const void* x, const void* h, const void* gate, const float* w1,
+                         const float* b1, const float* w2, const float* b2, void* y, void* n, float* stat, void* stream) {
+  if (const int rc = check_norm("splat_token_norm_fwd", a)) return rc;
+  if (a->M == 0) return kOk;
+  if (!x || (h && !y) || (a->next && !n) || (!h && (a->post || a->gate || !a->next)) || (a->gate && !gate))
+    return set_error(kInvalid, "splat_token_norm_fwd: null pointer");
+  TokenNorm p{};
+  p.a = *a;
+  p.x = x, p.h = h, p.gate = gate, p.w1 = w1, p.b1 = b1, p.w2 = w2, p.b2 = b2, p.y = y, p.n = n, p.stat = (float4*)stat;
+  const Shape s = shape_of(a->dtype, a->C);
+  const unsigned grid = plan(p, s, kForward);
+  return with_shape(a->dtype, s, [&](auto t, auto tpr, auto k) {
+    constexpr int TPR = decltype(tpr)::value;
+    k_token_norm<decltype(t), TPR, decltype(k)::value><<<grid, kBlock<TPR>, 0, (hipStream_t)stream>>>(p);
+    return check_launch("splat_token_norm_fwd");
+  });
+}
+
+size_t splat_token_norm_bwd_workspace_bytes(const splat_token_norm* a) {
+  if (check_norm("splat_token_norm_bwd_workspace_bytes", a) || a->M == 0) return 0;
+  TokenNorm p{};
+  p.a = *a;
+  const size_t grid = plan(p, shape_of(a->dtype, a->C), kBackward);
+  return sizeof(float) * a->C * (4 * grid + (a->gate == kRowGate ? (size_t)p.segs * p.splits : 0));
+}
+
+int splat_token_norm_bwd(const splat_token_norm* a, const void* x, const void* h, const void* gate, const float* w1,
+                         const float* b1, const float* w2, const void* dy, const void* dn, const float* stat, void* dx, void* dh,
+                         void* dgate, float* dw1, float* db1, float* dw2, float* db2, void* ws, size_t ws_bytes, void* stream) {
+  if (const int rc = check_norm("splat_token_norm_bwd", a)) return rc;
+  if (a->M == 0) return kOk;
+  if (!x || !stat || (!dy && !dn) || (dn && !a->next) || (!h && (a->post || a->gate || !dn)) || (a->gate && !gate) ||
+      ((dw1 || db1) && !a->post) || ((dw2 || db2) && !dn) || (dh && !h) || (dgate && !a->gate))
+    return set_error(kInvalid, "splat_token_norm_bwd: null pointer");
+  TokenNorm p{};
+  p.a = *a;
+  p.x = x, p.h = h, p.gate = gate, p.w1 = w1, p.b1 = b1, p.w2 = w2, p.dy = dy, p.dn = dn, p.stat = (float4*)stat;
+  p.dx = dx, p.dh = dh, p.dgate = a->gate == kTokenGate ? dgate : nullptr;
+  const Shape s = shape_of(a->dtype, a->C);
+  const unsigned grid = plan(p, s, kBackward);
+  const bool cols = dw1 || db1 || dw2 || db2, gates = dgate && a->gate == kRowGate;
+  const size_t need = cols || gates ? splat_token_norm_bwd_workspace_bytes(a) : 0;
+  if (need && (!ws || ws_bytes < need))
+    return set_error(kWorkspace, "splat_token_norm_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  if (cols) p.cols = (float*)ws;
+  if (gates) p.gates = (float*)ws + (size_t)4 * grid * a->C;
+  const hipStream_t st = (hipStream_t)stream;
+  return with_shape(a->dtype, s, [&](auto t, auto tpr, auto k) {
+    constexpr int TPR = decltype(tpr)::value;
+    k_token_norm_bwd<decltype(t), TPR, decltype(k)::value><<<grid, kBlock<TPR>, 0, st>>>(p);
+    if (need) {
+      const int tiles = div_up(a->C, 64);
+      k_token_norm_join<<<tiles * (4 + (gates ? p.segs : 0)), kJoin, 0, st>>>(p, (int)grid, tiles, dw1, db1, dw2, db2,
+                                                                              gates ? (float*)dgate : nullptr);
+    }
+    return check_launch("splat_token_norm_bwd");
+  });
+}
+
+}  // extern "C"

@@ -35,6 +35,9 @@ SOURCES = {
     "norm.hip": [],
     "linear.hip": _VGPR_ACC,
     "attend.hip": _VGPR_ACC,
+    "rotary.hip": [],
+    "token_norm.hip": [],
+    "paged.hip": _VGPR_ACC,
 }
 
 

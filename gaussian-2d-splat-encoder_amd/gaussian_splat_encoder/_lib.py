@@ -37,8 +37,35 @@ class SplatAttention(ctypes.Structure):
                 ("mb", _LL), ("ml", _LL), ("kv_lengths", _VP), ("key_mask", _VP), ("rest", _VP)]
 
 
+class SplatRotation(ctypes.Structure):
+    """struct splat_rotation: quarter turns of each pair of a head's values per unit of its axis' position."""
+    _fields_ = [("axes", _I), ("interleaved", _I), ("dims", _I * 4), ("quarters", ctypes.c_double * 64)]
+
+
+class SplatPositions(ctypes.Structure):
+    """struct splat_positions: positions of tokens on several axes."""
+    _fields_ = [("p", _VP), ("type", _I), ("pb", _LL), ("pl", _LL), ("pa", _LL)]
+
+
+class SplatCache(ctypes.Structure):
+    """struct splat_cache: a paged cache of keys and values and the tables of its sequences."""
+    _fields_ = [("dtype", _I), ("B", _I), ("Hk", _I), ("D", _I), ("page", _I), ("width", _I), ("pages", _LL), ("k", _VP),
+                ("v", _VP), ("live", _VP), ("kp", _LL), ("kt", _LL), ("kh", _LL), ("vp", _LL), ("vt", _LL), ("vh", _LL),
+                ("lp", _LL), ("lt", _LL), ("tables", _VP), ("tb", _LL), ("lengths", _VP), ("counts", _VP)]
+
+
+class SplatTokenNorm(ctypes.Structure):
+    """struct splat_token_norm: norms per token around a block's gate and residual."""
+    _fields_ = [("dtype", _I), ("C", _I), ("M", _LL), ("layer", _I), ("post", _I), ("next", _I), ("gate", _I), ("act", _I),
+                ("segs", _LL), ("eps", _F), ("scale", _F), ("xl", _LL), ("hl", _LL), ("gl", _LL), ("dyl", _LL), ("dnl", _LL)]
+
+
 _LV = ctypes.POINTER(SplatLevels)
 _AT = ctypes.POINTER(SplatAttention)
+_RO = ctypes.POINTER(SplatRotation)
+_PO = ctypes.POINTER(SplatPositions)
+_CA = ctypes.POINTER(SplatCache)
+_TN = ctypes.POINTER(SplatTokenNorm)
 _U = ctypes.c_uint
 
 # name -> (restype, argtypes)
@@ -102,6 +129,16 @@ _SIGS = {
     "splat_attention_fwd": (_I, [_AT, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "splat_attention_bwd_workspace_bytes": (_SZ, [_AT]),
     "splat_attention_bwd": (_I, [_AT, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "splat_rotary": (_I, [_RO, _PO, _VP, _LL, _LL, _LL, _I, _I, _LL, _I, _I, _I, _VP, _VP]),
+    "splat_rotary_bwd_workspace_bytes": (_SZ, [_I, _LL, _I, _I]),
+    "splat_rotary_bwd": (_I, [_RO, _PO, _VP, _LL, _LL, _LL, _VP, _LL, _LL, _LL, _I, _I, _LL, _I, _I, _VP, _VP, _I, _VP, _SZ,
+                              _VP]),
+    "splat_cache_append": (_I, [_CA, _RO, _PO, _VP, _LL, _LL, _LL, _VP, _LL, _LL, _LL, _VP, _LL, _LL, _LL, _VP]),
+    "splat_cached_attention_workspace_bytes": (_SZ, [_CA, _I, _LL]),
+    "splat_cached_attention": (_I, [_CA, _RO, _PO, _VP, _LL, _LL, _LL, _I, _LL, _F, _I, _VP, _VP, _SZ, _VP]),
+    "splat_token_norm_fwd": (_I, [_TN] + [_VP] * 11),
+    "splat_token_norm_bwd_workspace_bytes": (_SZ, [_TN]),
+    "splat_token_norm_bwd": (_I, [_TN] + [_VP] * 17 + [_SZ, _VP]),
 }
 
 EXPORTED = tuple(_SIGS)

@@ -1,0 +1,411 @@
+"""Operators of tokens that read splats frame by frame, on hand-written HIP kernels (gfx950): rotary positions of several axes,
+a paged cache of keys and values with the attention that reads it, norms per token with a block's gate and residual.
+
+They stand beside feature_ops and follow it: float32 or bfloat16 on a HIP device, the last dimension dense (anything else is
+copied first), sums and softmax statistics in float32, fixed orders of summation, the current stream, no waits. rotary,
+residual_norm and token_norm have gradients (reverse-mode, of first order); the cache is for inference and refuses inputs that
+require one. The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._lib import SplatCache, SplatPositions, SplatRotation, SplatTokenNorm
+from .feature_ops import _MAX_FLOAT, MAX_HEAD, _args, _dense, _launch, _norm_param, _ptr, _rows, _scratch, _wants_grad
+
+MAX_CHANNELS = 8192   # of a norm per token
+MAX_AXES = 4
+_POSITIONS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
+_KINDS = {"rms": 0, "layer": 1}
+_GATE_CODES = {"none": 0, "sigmoid": 5, "silu": 2, "tanh": 4}
+
+
+# ------------------------------------------------------------------------------------------------ rotary positions
+class RotaryAxes:
+    """Rates of a rotation by positions of several axes (time, row, column; a splat's centre).
+
+    dims: values of a head that each axis turns, even, one axis after another; values past them pass. Pair i of axis a turns by
+    position[a] * scale[a] * base[a] ** (-2 i / dims[a]) radians. base and scale: one number, or one for each axis.
+    interleaved: an axis' pairs are neighbours (2 i, 2 i + 1), not (i, i + dims[a] / 2)."""
+
+    def __init__(self, dims, base=10000.0, scale=1.0, interleaved=False):
+        self.dims = tuple(int(d) for d in dims)
+        if not 1 <= len(self.dims) <= MAX_AXES:
+            raise ValueError(f"1 to {MAX_AXES} axes are needed, got {len(self.dims)}")
+        if any(d < 2 or d % 2 for d in self.dims) or sum(self.dims) > MAX_HEAD:
+            raise ValueError(f"dims must be even, at least 2 and {MAX_HEAD} at most together, got {list(self.dims)}")
+        self.base, self.scale = self._each("base", base), self._each("scale", scale)
+        if not all(0 < b < math.inf for b in self.base) or not all(abs(s) < math.inf for s in self.scale):
+            raise ValueError(f"base must be positive and both finite, got {self.base} and {self.scale}")
+        self.interleaved = bool(interleaved)
+        rates = [s * b ** (-2 * i / d) * 2 / math.pi for d, b, s in zip(self.dims, self.base, self.scale)
+                 for i in range(d // 2)]
+        self._c = SplatRotation(len(self.dims), int(self.interleaved), (ctypes.c_int * 4)(*self.dims),
+                                (ctypes.c_double * 64)(*rates))
+        self._ref = ctypes.byref(self._c)
+
+    def _each(self, name, v):
+        v = tuple(float(x) for x in v) if isinstance(v, (tuple, list)) else (float(v),) * len(self.dims)
+        if len(v) != len(self.dims):
+            raise ValueError(f"{name} needs one number or {len(self.dims)}, got {len(v)}")
+        return v
+
+    def __repr__(self):
+        return f"RotaryAxes({self.dims}, base={self.base}, scale={self.scale}, interleaved={self.interleaved})"
+
+
+def _positions(positions, axes, B, L, D, x):
+    """C description of positions [B, L, axes] or [L, axes] of x's tokens."""
+    if not isinstance(axes, RotaryAxes):
+        raise ValueError(f"axes must be RotaryAxes, got {type(axes).__name__}")
+    if sum(axes.dims) > D:
+        raise ValueError(f"axes of {list(axes.dims)} values do not fit heads of {D}")
+    if positions is None:
+        raise ValueError("axes need positions")
+    A = len(axes.dims)
+    shape, kind = positions.shape, _POSITIONS.get(positions.dtype)
+    if len(shape) not in (2, 3) or shape[-2:] != (L, A) or (len(shape) == 3 and shape[0] not in (1, B)):
+        raise ValueError(f"positions must be [{B}, {L}, {A}] or [{L}, {A}], got {list(shape)}")
+    if kind is None:
+        raise ValueError(f"positions must be float32, int32 or int64, got {positions.dtype}")
+    if positions.get_device() != x.get_device():
+        raise ValueError(f"positions are on {positions.device}, the tokens on {x.device}")
+    st = positions.stride()
+    return SplatPositions(positions.data_ptr(), kind, st[0] if len(shape) == 3 and shape[0] == B else 0, st[-2], st[-1])
+
+
+def _turn(x, positions, axes, dt, back):
+    B, L, H, D = x.shape
+    y = torch.empty((B, L, H, D), dtype=x.dtype, device=x.device)
+    if y.numel():
+        p = _positions(positions, axes, B, L, D, x)
+        _launch(x, "splat_rotary", axes._ref, ctypes.byref(p), x.data_ptr(), *x.stride()[:3], dt, B, L, H, D, back,
+                y.data_ptr())
+    return y
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, positions, axes, dt):
+        x = _dense(x)
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, positions)
+        ctx.args = (axes, dt)
+        return _turn(x, positions, axes, dt, 0)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, positions = ctx.saved_tensors
+        axes, dt = ctx.args
+        g = _dense(g)
+        if not ctx.needs_input_grad[1]:
+            return _turn(g, positions, axes, dt, 1), None, None, None
+        x = _dense(x)
+        B, L, H, D = x.shape
+        dx = torch.empty((B, L, H, D), dtype=x.dtype, device=x.device)
+        shared = positions.dim() == 2 or positions.shape[0] != B
+        new = torch.empty if dx.numel() else torch.zeros
+        dp = new(positions.shape, dtype=torch.float32, device=x.device)
+        if dx.numel():
+            p = _positions(positions, axes, B, L, D, x)
+            n = _lib.load().splat_rotary_bwd_workspace_bytes(B, L, len(axes.dims), shared)
+            keep, ws = _scratch(n, x)
+            _launch(x, "splat_rotary_bwd", axes._ref, ctypes.byref(p), x.data_ptr(), *x.stride()[:3], g.data_ptr(),
+                    *g.stride()[:3], dt, B, L, H, D, dx.data_ptr(), dp.data_ptr(), shared, ws, n)
+        return dx if ctx.needs_input_grad[0] else None, dp, None, None
+
+
+def rotary(x, positions, axes):
+    """Turns the pairs of x's heads by their tokens' positions: x [B, L, H, D] (heads may be views) -> the same shape and type.
+
+    positions [B, L, axes], or [L, axes] and [1, L, axes] for all images: float32 (splat centres; they have a gradient, summed
+    over the images that share them), int32 or int64. axes: RotaryAxes. Angles are taken in 64 bits: positions up to 2^31
+    keep theirs to 1e-6 of a turn."""
+    dt, _ = _args("none", x)
+    if x.dim() != 4 or not 1 <= x.shape[3] <= MAX_HEAD or x.shape[2] < 1:
+        raise ValueError(f"x must be [B, L, H, D] with heads of 1 to {MAX_HEAD} values, got {list(x.shape)}")
+    _positions(positions, axes, x.shape[0], x.shape[1], x.shape[3], x)
+    if _wants_grad(x, positions):
+        return _Rotary.apply(x, positions, axes, dt)
+    return _turn(_dense(x), positions, axes, dt, 0)
+
+
+# ------------------------------------------------------------------------------------------------ the paged cache
+class PagedCache:
+    """Pages of keys and values: k and v [pages, page, Hk, D] (any strides with dense heads), and live [pages, page] (bool) or
+    None: tokens that are False do not count. Which pages a sequence's tokens lie on is in its table (cache_append)."""
+
+    def __init__(self, k, v, live=None):
+        self.dt, _ = _args("none", k, v)
+        if k.dim() != 4 or v.shape != k.shape or k.shape[1] < 1 or k.shape[2] < 1 or not 1 <= k.shape[3] <= MAX_HEAD:
+            raise ValueError(f"k and v must be [pages, page, Hk, D] with heads of 1 to {MAX_HEAD} values, got "
+                             f"{list(k.shape)} and {list(v.shape)}")
+        if any(t.shape[3] != 1 and t.stride(3) != 1 for t in (k, v)):
+            raise ValueError("a cache's heads must be dense")
+        if live is not None and (live.shape != k.shape[:2] or live.dtype is not torch.bool
+                                 or live.get_device() != k.get_device()):
+            raise ValueError(f"live must be {list(k.shape[:2])} bool on {k.device}, got {list(live.shape)} {live.dtype} on "
+                             f"{live.device}")
+        if k.requires_grad or v.requires_grad:
+            raise ValueError("a cache's pages must not require a gradient")
+        self.k, self.v, self.live = k, v, live
+        self.pages, self.page, self.heads, self.head_dim = k.shape
+
+    @classmethod
+    def empty(cls, pages, page, heads, head_dim, dtype=torch.bfloat16, device="cuda", masked=False):
+        """A cache of zeros whose pages hold their tokens head by head (what the attention reads lies together)."""
+        k, v = (torch.zeros(pages, heads, page, head_dim, dtype=dtype, device=device).transpose(1, 2) for _ in range(2))
+        return cls(k, v, torch.zeros(pages, page, dtype=torch.bool, device=device) if masked else None)
+
+    def tables(self, sequences, first=0):
+        """Tables [sequences, pages / sequences] (int32) that share the pages from `first` on out evenly, in order."""
+        width = (self.pages - first) // max(1, sequences)
+        t = torch.arange(first, first + sequences * width, dtype=torch.int32, device=self.k.device)
+        return t.view(sequences, width)
+
+    def _describe(self, tables, lengths, counts, B, T):
+        dev = self.k.get_device()
+        if tables.dim() != 2 or tables.shape[0] != B or tables.dtype is not torch.int32 or tables.get_device() != dev:
+            raise ValueError(f"tables must be [{B}, pages of a sequence] int32 on {self.k.device}, got {list(tables.shape)} "
+                             f"{tables.dtype} on {tables.device}")
+        if tables.shape[1] > 1 and tables.stride(1) != 1:
+            tables = tables.contiguous()
+        lengths = self._numbers("lengths", lengths, B, 2 ** 31 - 1)
+        counts = None if counts is None else self._numbers("counts", counts, B, T)
+        k, v, live = self.k, self.v, self.live
+        c = SplatCache(self.dt, B, self.heads, self.head_dim, self.page, tables.shape[1], self.pages, k.data_ptr(),
+                       v.data_ptr(), _ptr(live), *k.stride()[:3], *v.stride()[:3], *((0, 0) if live is None else live.stride()),
+                       tables.data_ptr(), tables.stride(0), lengths.data_ptr(), _ptr(counts))
+        return c, (tables, lengths, counts)
+
+    def _numbers(self, name, t, B, most):
+        if t.shape != (B,) or t.dtype not in (torch.int32, torch.int64) or t.get_device() != self.k.get_device():
+            raise ValueError(f"{name} must be [{B}] int32 or int64 on {self.k.device}, got {list(t.shape)} {t.dtype} on "
+                             f"{t.device}")
+        if t.dtype is torch.int64:
+            t = t.clamp(0, most).to(torch.int32)
+        return t if t.is_contiguous() else t.contiguous()
+
+
+def _of_cache(cache, *ts):
+    """The checks that both operators of a cache share."""
+    if not isinstance(cache, PagedCache):
+        raise ValueError(f"cache must be a PagedCache, got {type(cache).__name__}")
+    _args("none", cache.k, *ts)
+    if _wants_grad(*ts):
+        raise NotImplementedError("the paged cache is for inference: its operators have no gradients")
+
+
+def cache_append(cache, tables, lengths, k, v, counts=None, positions=None, axes=None, key_mask=None):
+    """Writes new tokens' keys and values k, v [B, T, Hk, D] into the cache's pages, the keys turned by positions and axes as by
+    rotary where axes is given.
+
+    tables [B, pages of a sequence] (int32): token j of sequence b lies on page tables[b, j // page], place j % page.
+    lengths [B] (int32 or int64) counts each sequence's tokens with the new ones; counts [B]: new tokens of each sequence, the
+    first ones of its T (all by default): token t goes to place lengths[b] - counts[b] + t. Tokens past their count, before
+    the sequence's start, behind its table or on an entry that is no page of the cache are left out, and all other places stay
+    as they were. Two tokens of a call must not go to one place. key_mask [B, T] (bool, for a cache with `live`): tokens
+    that are False do not count (all do by default). Every tensor is on the device: a captured call follows them."""
+    _of_cache(cache, k, v)
+    B, T = k.shape[:2] if k.dim() == 4 else (0, 0)
+    if k.dim() != 4 or k.shape != v.shape or k.shape[2:] != cache.k.shape[2:]:
+        raise ValueError(f"k and v must be [B, T, {cache.heads}, {cache.head_dim}], got {list(k.shape)} and {list(v.shape)}")
+    if key_mask is not None:
+        if cache.live is None:
+            raise ValueError("key_mask needs a cache with `live`")
+        if key_mask.shape != (B, T) or key_mask.dtype is not torch.bool or key_mask.get_device() != k.get_device():
+            raise ValueError(f"key_mask must be [{B}, {T}] bool on {k.device}, got {list(key_mask.shape)} {key_mask.dtype} on "
+                             f"{key_mask.device}")
+    c, keep = cache._describe(tables, lengths, counts, B, T)
+    p = r = None
+    if axes is not None:
+        p, r = ctypes.byref(_positions(positions, axes, B, T, cache.head_dim, k)), axes._ref
+    if B and T and cache.pages and c.width:
+        k, v = _dense(k), _dense(v)
+        _launch(k, "splat_cache_append", ctypes.byref(c), r, p, k.data_ptr(), *k.stride()[:3], v.data_ptr(),
+                *v.stride()[:3], _ptr(key_mask), *((0, 0) if key_mask is None else key_mask.stride()), T)
+
+
+def cached_attention(q, cache, tables, lengths, counts=None, positions=None, axes=None, causal=True, scale=None):
+    """Attention of new tokens' queries q [B, T, H, D] over their sequences' cached tokens -> [B, T, H, D]. H is a multiple of the
+    cache's heads (each serves H / Hk neighbouring query heads); meant for one to some tens of new tokens.
+
+    tables, lengths, counts as in cache_append: the queries are the last counts[b] tokens that lengths[b] counts. causal: query t
+    sees the tokens up to its own place, lengths[b] - counts[b] + t; otherwise all. Tokens that the cache's `live` marks
+    False, or whose table entry is no page, do not count, whatever they hold. A query without any token, and those past their
+    sequence's count, give zeros. positions, axes: turns q as by rotary. scale defaults to D ** -0.5."""
+    _of_cache(cache, q)
+    if q.dim() != 4 or q.shape[3] != cache.head_dim or q.shape[2] < 1 or q.shape[2] % cache.heads:
+        raise ValueError(f"q must be [B, T, a multiple of {cache.heads}, {cache.head_dim}], got {list(q.shape)}")
+    B, T, H, D = q.shape
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not abs(scale) <= _MAX_FLOAT:
+        raise ValueError(f"scale must be a finite float32, got {scale}")
+    c, keep = cache._describe(tables, lengths, counts, B, T)
+    p = r = None
+    if axes is not None:
+        p, r = ctypes.byref(_positions(positions, axes, B, T, D, q)), axes._ref
+    o = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+    if o.numel():
+        q = _dense(q)
+        ref = ctypes.byref(c)
+        n = _lib.load().splat_cached_attention_workspace_bytes(ref, H, T)
+        held, ws = _scratch(n, q)
+        _launch(q, "splat_cached_attention", ref, r, p, q.data_ptr(), *q.stride()[:3], H, T, scale, int(bool(causal)),
+                o.data_ptr(), ws, n)
+    return o
+
+
+# ------------------------------------------------------------------------------------------------ norms per token
+def _norm_args(x, h, gate, kind, eps, scale, act, post, nxt, dt):
+    """C description, x and h as rows, the gate as rows of its kind."""
+    C, M = x.shape[-1], math.prod(x.shape[:-1])
+    a = SplatTokenNorm(dt, C, M, _KINDS[kind], post, nxt, 0, _GATE_CODES[act], 0, eps, scale)
+    x2 = _rows(x)
+    a.xl = x2.stride(0)
+    h2 = None
+    if h is not None:
+        h2 = _rows(h)
+        a.hl = h2.stride(0)
+    if gate is not None:
+        if gate.shape == x.shape and gate.dtype is x.dtype and gate.numel() != C:
+            gate = _rows(gate)
+            a.gate, a.gl = 2, gate.stride(0)
+        else:
+            gate = gate.reshape(-1, C).contiguous()
+            a.gate, a.segs = 1, gate.shape[0]
+    return a, x2, h2, gate
+
+
+def _norm_fwd(x, h, w1, b1, gate, w2, b2, cfg, save):
+    """(y or None, n or None, statistics or None)"""
+    a, x2, h2, g2 = _norm_args(x, h, gate, *cfg)
+    new = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)   # noqa: E731
+    y = new() if h is not None else None
+    n = new() if a.next else None
+    stat = torch.empty((a.M, 4), dtype=torch.float32, device=x.device) if save else None
+    if a.M:
+        _launch(x, "splat_token_norm_fwd", ctypes.byref(a), x2.data_ptr(), _ptr(h2), _ptr(g2), _ptr(w1), _ptr(b1), _ptr(w2),
+                _ptr(b2), _ptr(y), _ptr(n), _ptr(stat))
+    return y, n, stat
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, h, w1, b1, gate, w2, b2, cfg):
+        y, n, stat = _norm_fwd(x, h, w1, b1, gate, w2, b2, cfg, True)
+        ctx.save_for_backward(x, h, w1, b1, gate, w2, stat)
+        ctx.cfg = cfg
+        ctx.set_materialize_grads(False)
+        return (y, n) if y is not None and n is not None else n if y is None else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *up):
+        x, h, w1, b1, gate, w2, stat = ctx.saved_tensors
+        a, x2, h2, g2 = _norm_args(x, h, gate, *ctx.cfg)
+        dy, dn = up if len(up) == 2 else (None, up[0]) if a.next else (up[0], None)
+        need = ctx.needs_input_grad
+        if dy is None and dn is None:
+            return (None,) * 8
+        dev = x.device
+        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)   # noqa: E731
+        dx = new(x) if need[0] else None
+        dh = new(h) if need[1] else None
+        small = torch.empty if a.M else torch.zeros
+        par = [small(a.C, dtype=torch.float32, device=dev) if f else None for f in (need[2], need[3], need[5], need[6])]
+        if dn is None:      # nothing reached the second norm's parameters
+            par[2:] = [None if t is None else t.zero_() for t in par[2:]]
+        dgate = None
+        if need[4]:
+            dgate = new(gate) if a.M else torch.zeros_like(gate)
+        if a.M:
+            dy, dn = (None if t is None else _rows(t) for t in (dy, dn))
+            a.dyl, a.dnl = (0 if t is None else t.stride(0) for t in (dy, dn))
+            n = _lib.load().splat_token_norm_bwd_workspace_bytes(ctypes.byref(a))
+            keep, ws = _scratch(n, x)
+            w2p = par[2:] if dn is not None else [None, None]
+            _launch(x, "splat_token_norm_bwd", ctypes.byref(a), x2.data_ptr(), _ptr(h2), _ptr(g2), _ptr(w1), _ptr(b1),
+                    _ptr(w2), _ptr(dy), _ptr(dn), stat.data_ptr(), _ptr(dx), _ptr(dh), _ptr(dgate), _ptr(par[0]),
+                    _ptr(par[1]), _ptr(w2p[0]), _ptr(w2p[1]), ws, n)
+        return dx, dh, par[0], par[1], dgate, par[2], par[3], None
+
+
+def _check_norm(x, kind, eps):
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_CHANNELS:
+        raise ValueError(f"x must be [..., C] of 1 to {MAX_CHANNELS} channels, got {list(x.shape)}")
+    if kind not in _KINDS:
+        raise ValueError(f"unknown norm {kind!r}: one of {sorted(_KINDS)}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+
+
+def token_norm(x, weight=None, bias=None, kind="rms", eps=1e-6):
+    """A norm of each token's channels: x [..., C] -> weight * norm(x) + bias, of x's shape and type. kind "rms":
+    x / sqrt(mean(x^2) + eps); "layer": of x less its mean. weight and bias [C] may be None; they are used, and their gradients
+    returned, in float32. C at most 8,192. (group_norm_act normalises over an image's positions.)"""
+    dt, _ = _args("none", x)
+    _check_norm(x, kind, eps)
+    C = x.shape[-1]
+    weight, bias = _norm_param("weight", weight, C, x), _norm_param("bias", bias, C, x)
+    cfg = (kind, float(eps), 1.0, "none", 0, 1, dt)
+    if _wants_grad(x, weight, bias):
+        return _ResidualNorm.apply(x, None, None, None, None, weight, bias, cfg)
+    return _norm_fwd(x, None, None, None, None, weight, bias, cfg, False)[1]
+
+
+def residual_norm(x, h, weight=None, bias=None, gate=None, gate_act="none", next_weight=None, next_bias=None, kind="rms",
+                  eps=1e-6, scale=1.0, norm_block=True, norm_next=True):
+    """What lies between one block of a model and the next, in one kernel: x [..., C] the residual stream, h (like x) the block's
+    output ->
+
+        y = x + scale * gate_act(gate) * (weight * norm(h) + bias)        the new residual stream
+        n = next_weight * norm(y) + next_bias                             the next block's input, of y before its rounding
+
+    as (y, n). norm_block=False takes h as it is, norm_next=False returns y alone. kind, parameters and their gradients as in
+    token_norm. gate: None; [C] (a learned one), or [B, C] or [B, 1, .., C] (a row for each image of x [B, ..., C]), used in
+    float32; or x's shape and type (a row for each token). gate_act: "none", "sigmoid", "silu" or "tanh"."""
+    dt, _ = _args("none", x, h)
+    _check_norm(x, kind, eps)
+    if h.shape != x.shape:
+        raise ValueError(f"h must be {list(x.shape)}, got {list(h.shape)}")
+    if gate_act not in _GATE_CODES:
+        raise ValueError(f"unknown activation {gate_act!r} of a gate: one of {sorted(_GATE_CODES)}")
+    scale = float(scale)
+    if not abs(scale) <= _MAX_FLOAT:
+        raise ValueError(f"scale must be a finite float32, got {scale}")
+    C = x.shape[-1]
+    if not norm_block and (weight is not None or bias is not None):
+        raise ValueError("weight and bias belong to the block's norm, which norm_block=False leaves out")
+    if not norm_next and (next_weight is not None or next_bias is not None):
+        raise ValueError("next_weight and next_bias belong to the next norm, which norm_next=False leaves out")
+    weight, bias = _norm_param("weight", weight, C, x), _norm_param("bias", bias, C, x)
+    next_weight, next_bias = _norm_param("next_weight", next_weight, C, x), _norm_param("next_bias", next_bias, C, x)
+    if gate is not None:
+        gate = _gate(gate, x)
+    cfg = (kind, float(eps), scale, gate_act, int(bool(norm_block)), int(bool(norm_next)), dt)
+    if _wants_grad(x, h, weight, bias, gate, next_weight, next_bias):
+        return _ResidualNorm.apply(x, h, weight, bias, gate, next_weight, next_bias, cfg)
+    y, n, _ = _norm_fwd(x, h, weight, bias, gate, next_weight, next_bias, cfg, False)
+    return (y, n) if norm_next else y
+
+
+def _gate(gate, x):
+    """The gate as it is (a row for each token), or in float32 (one row, or one for each image)."""
+    shape, B, C = gate.shape, x.shape[0] if x.dim() > 1 else 1, x.shape[-1]
+    if gate.get_device() != x.get_device():
+        raise ValueError(f"gate is on {gate.device}, x on {x.device}")
+    if shape == x.shape and gate.dtype is x.dtype and gate.numel() != C:
+        return gate
+    one = (1,) * (x.dim() - 1) + (C,)
+    image = (B,) + (1,) * (x.dim() - 2) + (C,)
+    if shape != (C,) and shape != one and (x.dim() < 3 or shape not in (image, (B, C))):
+        if shape == x.shape:
+            raise ValueError(f"a gate for each token must be {x.dtype}, got {gate.dtype}")
+        raise ValueError(f"gate must be [{C}], {list(image)} or {list(x.shape)}, got {list(shape)}")
+    return gate if gate.dtype is torch.float32 else gate.float()

@@ -359,6 +359,85 @@ int splat_attention_bwd(const splat_attention *a, const void *q, const void *k, 
                         const float *lse, const void *g, void *dq, void *dk, void *dv, void *ws, size_t ws_bytes,
                         void *stream);
 
+/* ---------------------------------------------------------------------------------------------- token operators
+ * Positions, a paged cache with the attention that reads it, and norms per token, for models that read splats frame by frame
+ * (no counterpart in the reference). dtype, act, strides and zero sizes as above. */
+
+/* A rotation by positions of several axes: axis a has dims[a] of a head's D values, one axis after another; its pair i (values
+ * i and i + dims[a] / 2 of the axis, or 2 i and 2 i + 1 where interleaved) turns by position[a] * quarters[pair] quarter turns,
+ * quarters listed over all axes' pairs. Values past the axes pass. Angles are taken in 64 bits and reduced to a turn. */
+typedef struct splat_rotation {
+  int axes, interleaved;         /* axes (0: nothing turns, 4 at most); pairs of neighbours instead of halves */
+  int dims[4];                   /* values of a head that each axis turns, even, at most 128 together */
+  double quarters[64];           /* quarter turns of each pair per unit of its axis' position */
+} splat_rotation;
+typedef struct splat_positions {
+  const void *p;                 /* NULL: none */
+  int type;                      /* 0 float32, 1 int32, 2 int64 */
+  long long pb, pl, pa;          /* elements from image to image (0: shared), token to token, axis to axis */
+} splat_positions;
+
+/* y[B, L, H, D] (contiguous) = x turned by its tokens' positions, or back (back = 1: the input's gradient); D at most 128.
+ * splat_rotary_bwd gives the gradients of x and of float32 positions, dpos[B, L, axes], or [L, axes] where the images share
+ * them (shared = 1: summed in the images' order). */
+int splat_rotary(const splat_rotation *r, const splat_positions *p, const void *x, long long xb, long long xl, long long xh,
+                 int dtype, int B, long long L, int H, int D, int back, void *y, void *stream);
+size_t splat_rotary_bwd_workspace_bytes(int B, long long L, int axes, int shared);
+int splat_rotary_bwd(const splat_rotation *r, const splat_positions *p, const void *x, long long xb, long long xl,
+                     long long xh, const void *g, long long gb, long long gl, long long gh, int dtype, int B, long long L,
+                     int H, int D, void *dx, float *dpos, int shared, void *ws, size_t ws_bytes, void *stream);
+
+/* A paged cache: token j of sequence b lies on page tables[b][j / page] at place j % page. What `lengths` counts includes the
+ * new tokens of a call, the last counts[b] (all T where counts is NULL) of each sequence. */
+typedef struct splat_cache {
+  int dtype, B, Hk, D;           /* element type; sequences; key heads; values per head, at most 128 */
+  int page, width;               /* tokens of a page; pages of a sequence's table */
+  long long pages;               /* pages of the cache; a table's entry outside [0, pages) is no page */
+  void *k, *v;                   /* [pages, page, Hk, D] */
+  unsigned char *live;           /* [pages, page], 0: the token is left out; or NULL */
+  long long kp, kt, kh, vp, vt, vh, lp, lt;   /* elements from page to page, token to token, head to head */
+  const int *tables;             /* [B, width] */
+  long long tb;                  /* elements from table to table */
+  const int *lengths, *counts;   /* [B]; counts may be NULL */
+} splat_cache;
+
+/* Writes new keys k[B, T, Hk, D] (turned by r and p where r has axes; r may be NULL) and values v to their places, with mask
+ * [B, T] (bytes, or NULL: all 1) to `live` where the cache has that. Tokens past their sequence's count, before its first place,
+ * behind its table or without a page are left out; two tokens of a call must not share a place. */
+int splat_cache_append(const splat_cache *c, const splat_rotation *r, const splat_positions *p, const void *k, long long kb,
+                       long long kl, long long kh, const void *v, long long vb, long long vl, long long vh,
+                       const unsigned char *mask, long long mb, long long ml, long long T, void *stream);
+
+/* o[B, T, H, D] (contiguous) = softmax(scale q k^T) v over the cached tokens of each sequence: all that lengths counts, or
+ * (causal) those up to the query's own place. q is turned first where r has axes. Rows without tokens, and rows past counts,
+ * give zeros. */
+size_t splat_cached_attention_workspace_bytes(const splat_cache *c, int H, long long T);
+int splat_cached_attention(const splat_cache *c, const splat_rotation *r, const splat_positions *p, const void *q,
+                           long long qb, long long ql, long long qh, int H, long long T, float scale, int causal, void *o,
+                           void *ws, size_t ws_bytes, void *stream);
+
+/* y = x + scale act(gate) (w1 norm(h) + b1) and n = w2 norm(y) + b2 over rows of C channels (at most 8,192): root-mean-square
+ * norms x / sqrt(mean(x^2) + eps), or layer norms. post = 0 leaves the first norm out, next = 0 the second; h = NULL the block:
+ * then y = x is not written and n is a norm per token. Outputs and gradients are contiguous; parameters (NULL: ones, zeros), gates
+ * of kind 1 and their gradients are float32, gates of kind 2 (a row for each token) have the rows' type. stat[M, 4] is what
+ * the backward takes. Backward: dy or dn may be NULL (zeros); NULL gradients are skipped. act: none, silu, tanh, sigmoid. */
+typedef struct splat_token_norm {
+  int dtype, C;                  /* element type; channels */
+  long long M;                   /* tokens */
+  int layer, post, next;         /* layer norms; which norms there are */
+  int gate, act;                 /* 0 none, 1 a row for each of `segs` equal runs of tokens, 2 a row for each token */
+  long long segs;
+  float eps, scale;
+  long long xl, hl, gl, dyl, dnl;   /* elements from token to token of x, h, the gate (kind 2), the gradients of y and n */
+} splat_token_norm;
+int splat_token_norm_fwd(const splat_token_norm *a, const void *x, const void *h, const void *gate, const float *w1,
+                         const float *b1, const float *w2, const float *b2, void *y, void *n, float *stat, void *stream);
+size_t splat_token_norm_bwd_workspace_bytes(const splat_token_norm *a);
+int splat_token_norm_bwd(const splat_token_norm *a, const void *x, const void *h, const void *gate, const float *w1,
+                         const float *b1, const float *w2, const void *dy, const void *dn, const float *stat, void *dx,
+                         void *dh, void *dgate, float *dw1, float *db1, float *dw2, float *db2, void *ws, size_t ws_bytes,
+                         void *stream);
+
 #ifdef __cplusplus
 }
 #endif
