@@ -36,7 +36,7 @@ struct Cached {
   int T, H, rep, R;            // new tokens; query heads; of a key head; rows = T rep
   int tiles, pieces, causal;   // row tiles; pieces aimed at, over all sequences
   int units;                   // of a head, single pairs
-  bool chunked, alike;         // heads are whole chunks; keys and values have the same strides
+  bool alike;                  // keys and values have the same strides
   FastDiv by_rep, by_page, by_units;
   float *part, *stat;          // rows of the pieces of split sequences; their maxima and sums
 };
@@ -151,9 +151,10 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// A lane's token of a tile: its page (-1: none) and place there.
+// A lane's token of a tile: its page and place there, and whether the piece holds it.
 struct Place {
   int page, off;
+  bool in;
 };
 
 template <typename T, int DP, int NR>
@@ -169,7 +170,10 @@ struct Lds {
   };
 };
 
-template <typename T, int DP, int NR>
+// What a head's width asks of its loads: nothing (D = DP), zeros behind its chunks, or its last chunk value by value.
+enum Fill : int { kFull = 0, kChunks = 1, kValues = 2 };
+
+template <typename T, int DP, int NR, int Fit>
 __global__ __launch_bounds__(kThreads) void k_cached(Cached a) {
   using F = Form<T, DP>;
   constexpr int V = F::V, KT = F::KT;
@@ -184,62 +188,55 @@ __global__ __launch_bounds__(kThreads) void k_cached(Cached a) {
   const int* table = a.c.tables + b * a.c.tb;
   const T *kb = (const T*)a.c.k + hk * a.c.kh, *vb = (const T*)a.c.v + hk * a.c.vh;
 
+  // Loads below have no conditions of their own, so that they are all under way before the first is waited for: places past
+  // the piece are those of its last token, rows that do not count those of the tile's first one that does.
   auto lookup = [&](int t) {
-    const int key = t * KT + (lane & (KT - 1));
-    Place p{-1, 0};
-    if (key < k1) {
-      const int i = key / a.by_page;
-      p.page = table[i];
-      p.off = key - i * a.c.page;
-    }
-    return p;
+    const int key = t * KT + (lane & (KT - 1)), at = min(key, k1 - 1), i = at / a.by_page;
+    return Place{table[i], at - i * a.c.page, key < k1};
   };
-  auto known = [&](const Place& p) { return p.page >= 0 && p.page < a.c.pages; };
   auto alive = [&](const Place& p) {
-    return known(p) && a.c.live ? a.c.live[p.page * a.c.lp + p.off * a.c.lt] : (unsigned char)known(p);
+    const bool known = p.page >= 0 && p.page < a.c.pages;
+    return (unsigned char)(a.c.live ? a.c.live[(known ? p.page : 0) * a.c.lp + p.off * a.c.lt] : 1);
   };
   Chunk<T> kf[F::NT][F::nc], vr[F::nv];
   unsigned ok;   // the tile's tokens that count
   auto fetch = [&](const Place& p, unsigned char m) {
-    ok = (unsigned)(__ballot(m != 0) & ((1ull << KT) - 1));
+    ok = (unsigned)(__ballot(p.in && p.page >= 0 && p.page < a.c.pages && m != 0) & ((1ull << KT) - 1));
+    if (!ok) return;
+    const int first = __builtin_ctz(ok);
     const long long ko = p.page * a.c.kp + p.off * a.c.kt, vo = a.alike ? ko : p.page * a.c.vp + p.off * a.c.vt;
+    auto chunk = [&](const T* at, int d) {
+      Chunk<T> c;
+      if (Fit == kValues) return load_chunk(at + d, a.c.D - d);
+      __builtin_memcpy(c.v, at + ((Fit == kFull && DP != 96) || d < a.c.D ? d : 0), 16);
+      return c;
+    };
 #pragma unroll
     for (int t = 0; t < F::NT; ++t) {
       const int row = 16 * t + (lane & 15);
-      const T* at = kb + __shfl(ko, row);
-      const bool in = (ok >> row) & 1;
+      const T* at = kb + __shfl(ko, (ok >> row) & 1 ? row : first);
 #pragma unroll
-      for (int c = 0; c < F::nc; ++c) {
-        const int d = (c * 4 + g) * V;
-        if (a.chunked) {
-          kf[t][c] = Chunk<T>{};
-          if (in && d < a.c.D) __builtin_memcpy(kf[t][c].v, at + d, 16);
-        } else {
-          kf[t][c] = load_chunk(at + d, in ? a.c.D - d : 0);
-        }
-      }
+      for (int c = 0; c < F::nc; ++c) kf[t][c] = chunk(at, (c * 4 + g) * V);
     }
 #pragma unroll
     for (int i = 0; i < F::nv; ++i) {
-      const int row = lane / F::cp + i * F::rs, d = lane % F::cp * V;
-      const T* at = vb + __shfl(vo, row);
-      const bool in = (ok >> row) & 1;
-      if (a.chunked) {
-        vr[i] = Chunk<T>{};
-        if (in && d < a.c.D) __builtin_memcpy(vr[i].v, at + d, 16);
-      } else {
-        vr[i] = load_chunk(at + d, in ? a.c.D - d : 0);
-      }
+      const int row = lane / F::cp + i * F::rs;
+      vr[i] = chunk(vb + __shfl(vo, (ok >> row) & 1 ? row : first), lane % F::cp * V);
     }
   };
 
   int t = k0 / KT + w;
-  Place p1 = lookup(t + kWaves), p2 = lookup(t + 2 * kWaves);
-  {
+  Place p1{}, p2{};
+  unsigned char m1 = 0;
+  ok = 0;
+  if (k1 > k0) {
     const Place p0 = lookup(t);
-    fetch(p0, alive(p0));
+    p1 = lookup(t + kWaves);
+    p2 = lookup(t + 2 * kWaves);
+    const unsigned char m0 = alive(p0);
+    m1 = alive(p1);
+    fetch(p0, m0);
   }
-  unsigned char m1 = alive(p1);
 
   // the rows' queries
   const int rows = min(16 * NR, a.R - r0);
@@ -308,38 +305,43 @@ __global__ __launch_bounds__(kThreads) void k_cached(Cached a) {
   for (; t < tend; t += kWaves) {
     const unsigned char m2 = alive(p2);
     const Place p3 = lookup(t + 3 * kWaves);
-    // values to LDS; whether those that some row does not see are finite
-    bool odd = false;
+    const unsigned here = ok;
     const bool edge = (t + 1) * KT > least;
-    wave_order();
-#pragma unroll
-    for (int i = 0; i < F::nv; ++i) {
-      const int row = lane / F::cp + i * F::rs, d = lane % F::cp * V;
-      if (DP != 96 || d < DP) *(f32x4*)(tv + row * F::ld + d) = *(const f32x4*)vr[i].v;
-      if (edge) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) odd |= !(fabsf((float)vr[i].v[j]) < INFINITY);
-      }
-    }
-    wave_order();
-    odd = __any(odd);
+    bool odd = false;   // values that some row does not see are not finite
     f32x4 s[NR][F::NT];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
+    if (here) {
 #pragma unroll
       for (int i = 0; i < F::NT; ++i) {
-        s[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < F::nc; ++c) mma16(s[n][i], kf[i][c], qf[n][c]);
-        if (fine) {
+        for (int c = 0; c < F::nc; ++c)
+          if (Fit == kChunks && (c * 4 + g) * V >= a.c.D) kf[i][c] = Chunk<T>{};
 #pragma unroll
-          for (int c = 0; c < F::nc; ++c) mma16(s[n][i], kf[i][c], ql[n][c]);
+        for (int n = 0; n < NR; ++n) {
+          s[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < F::nc; ++c) mma16(s[n][i], kf[i][c], qf[n][c]);
+          if (fine) {
+#pragma unroll
+            for (int c = 0; c < F::nc; ++c) mma16(s[n][i], kf[i][c], ql[n][c]);
+          }
         }
       }
+      wave_order();
+#pragma unroll
+      for (int i = 0; i < F::nv; ++i) {
+        const int row = lane / F::cp + i * F::rs, d = lane % F::cp * V;
+        if (DP != 96 || d < DP) *(f32x4*)(tv + row * F::ld + d) = *(const f32x4*)vr[i].v;
+        if (edge) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) odd |= !(fabsf((float)vr[i].v[j]) < INFINITY);
+        }
+      }
+      wave_order();
+      odd = __any(odd);
     }
-    const unsigned here = ok;
     fetch(p1, m1);
     p1 = p2, m1 = m2, p2 = p3;
+    if (!here) continue;
 
     const bool all = !edge && here == (unsigned)((1ull << KT) - 1);
 #pragma unroll
@@ -391,7 +393,10 @@ __global__ __launch_bounds__(kThreads) void k_cached(Cached a) {
         if (part) {
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            if (t * KT + 16 * (j / 4) + 4 * g + j % 4 >= seen) f.v[j] = (T)0.f;
+            {
+              const int key = 16 * (j / 4) + 4 * g + j % 4;
+              if (t * KT + key >= seen || !((here >> key) & 1)) f.v[j] = (T)0.f;
+            }
         }
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
@@ -551,8 +556,13 @@ size_t slots(const Cached& n) { return may_split(n) ? (size_t)2 * n.pieces : 0; 
 
 template <typename F>
 int with_form(int dtype, int D, int R, F&& f) {
+  auto fit = [&](auto t, auto dp, auto nr) {
+    if (D == decltype(dp)::value) return f(t, dp, nr, std::integral_constant<int, kFull>{});
+    if (D % kV<decltype(t)> == 0) return f(t, dp, nr, std::integral_constant<int, kChunks>{});
+    return f(t, dp, nr, std::integral_constant<int, kValues>{});
+  };
   auto rows = [&](auto t, auto dp) {
-    return R > 16 ? f(t, dp, std::integral_constant<int, 2>{}) : f(t, dp, std::integral_constant<int, 1>{});
+    return R > 16 ? fit(t, dp, std::integral_constant<int, 2>{}) : fit(t, dp, std::integral_constant<int, 1>{});
   };
   auto head = [&](auto t) {
     if (D <= 32) return rows(t, std::integral_constant<int, 32>{});
@@ -583,6 +593,7 @@ int splat_cached_attention(const splat_cache* c, const splat_rotation* r, const 
   if (c->B == 0 || T == 0) return kOk;
   if (!q || !o) return set_error(kInvalid, "splat_cached_attention: null pointer");
   Cached n = plan(*c, H, (int)T);
+  if (c->pages == 0) n.c.width = 0;   // nothing can be read: no sequence has tokens
   const size_t need = splat_cached_attention_workspace_bytes(c, H, T);
   if (need && (!ws || ws_bytes < need))
     return set_error(kWorkspace, "splat_cached_attention: workspace of %zu bytes, %zu needed", ws_bytes, need);
@@ -594,16 +605,15 @@ int splat_cached_attention(const splat_cache* c, const splat_rotation* r, const 
   n.scale = scale * kLog2e;
   n.units = pair_units(n.r, c->D, 1).n;
   n.by_units = fast_div(n.units);
-  n.chunked = c->D % (c->dtype == kF32 ? 4 : 8) == 0;
   n.alike = c->kp == c->vp && c->kt == c->vt;
   if (need) {
     n.stat = (float*)ws;
     n.part = n.stat + 2 * slots(n) * c->Hk * n.R;
   }
   const hipStream_t st = (hipStream_t)stream;
-  return with_form(c->dtype, c->D, n.R, [&](auto t, auto dp, auto nr) {
+  return with_form(c->dtype, c->D, n.R, [&](auto t, auto dp, auto nr, auto fit) {
     using E = decltype(t);
-    k_cached<E, decltype(dp)::value, decltype(nr)::value><<<(unsigned)grid, kThreads, 0, st>>>(n);
+    k_cached<E, decltype(dp)::value, decltype(nr)::value, decltype(fit)::value><<<(unsigned)grid, kThreads, 0, st>>>(n);
     if (need) k_cached_join<E><<<(unsigned)(c->B * c->Hk * n.R), kThreads, 0, st>>>(n);
     return check_launch("splat_cached_attention");
   });
