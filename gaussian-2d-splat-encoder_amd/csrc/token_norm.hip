@@ -34,7 +34,7 @@ struct TokenNorm {
   float *cols, *gates;            // partial sums [workgroups][4][C] of dw1, db1, dw2, db2; [segments][splits][C] of the gate
   long long seg;                  // rows of a segment
   int segs, splits, whole;        // segments; workgroups of one, or whole segments of a workgroup (the other is 1)
-  long long per;                  // rows of a split
+  long long step;                 // rows that a segment's workgroups take at a time
 };
 
 // Sum over groups of TPR lanes, the same in each lane.
@@ -102,14 +102,26 @@ struct Cols {
 template <typename T, int K>
 using Vals = float[K][kV<T>];
 
-template <typename T, int TPR, int K>
-__device__ __forceinline__ void load_row(const T* p, const Cols<T, TPR, K>& at, Vals<T, K>& f) {
+// A row's chunks as they lie in memory. Whole: C is whole chunks, and the lanes past it load the first one, so that no load has
+// a condition of its own and the next row's are under way while this one is worked on.
+template <typename T, int K>
+using Raw = Chunk<T>[K];
+
+template <bool Whole, typename T, int TPR, int K>
+__device__ __forceinline__ void load_raw(const T* p, const Cols<T, TPR, K>& at, Raw<T, K>& f) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const Chunk<T> c = load_chunk(p + at.c[k], at.nv[k]);
-#pragma unroll
-    for (int j = 0; j < kV<T>; ++j) f[k][j] = (float)c.v[j];
+    if (Whole) __builtin_memcpy(f[k].v, p + (at.nv[k] ? at.c[k] : 0), 16);
+    else f[k] = load_chunk(p + at.c[k], at.nv[k]);
   }
+}
+// Their values, zeros past C.
+template <bool Whole, typename T, int TPR, int K>
+__device__ __forceinline__ void values(const Raw<T, K>& c, const Cols<T, TPR, K>& at, Vals<T, K>& f) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < kV<T>; ++j) f[k][j] = !Whole || at.nv[k] ? (float)c[k].v[j] : 0.f;
 }
 template <typename T, int TPR, int K>
 __device__ __forceinline__ void store_row(T* p, const Cols<T, TPR, K>& at, const Vals<T, K>& f) {
@@ -149,11 +161,11 @@ __device__ __forceinline__ float gate_grad(int act, float g) {
 }
 
 // Mean and inverse deviation of a row whose channels past C are zeros.
-template <int TPR, int K, typename T, typename Sum>
+template <bool Lean, int TPR, int K, typename T, typename Sum>
 __device__ __forceinline__ float2 row_stats(const TokenNorm& a, const Cols<T, TPR, K>& at, const Vals<T, K>& f, Sum& sum) {
   const float inv = 1.f / (float)a.a.C;
   float m = 0.f, q[1] = {0.f};
-  if (a.a.layer) {
+  if (!Lean && a.a.layer) {
     float s[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -176,61 +188,72 @@ __device__ __forceinline__ float2 row_stats(const TokenNorm& a, const Cols<T, TP
 template <int TPR>
 constexpr int kBlock = TPR > 256 ? TPR : 256;
 
-// f(first row, rows, segment) for the workgroup's ranges, each within one segment.
+// f(segment's first row, segment, split) for the workgroup's segments. Its rows of each are split * RB + r, a.step apart: those
+// that workgroups work on at a time lie together.
 template <typename F>
-__device__ __forceinline__ void ranges(const TokenNorm& a, F&& f) {
+__device__ __forceinline__ void segments(const TokenNorm& a, F&& f) {
   const int s0 = blockIdx.x / a.splits * a.whole, split = blockIdx.x % a.splits;
-  for (int s = s0; s < min(a.segs, s0 + a.whole); ++s) {
-    const long long lo = split * a.per, n = min(a.per, a.seg - lo);
-    f(s * a.seg + lo, n < 0 ? 0 : n, s, split);
-  }
+  for (int s = s0; s < min(a.segs, s0 + a.whole); ++s) f(s * a.seg, s, split);
 }
 
-template <typename T, int TPR, int K>
+// Lean: root-mean-square norms without biases, whose registers and sums it saves.
+template <typename T, int TPR, int K, bool Whole, bool Lean>
 __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm(TokenNorm a) {
   constexpr int RB = kBlock<TPR> / TPR;
   __shared__ float red[2][1][16];
   const Cols<T, TPR, K> at(a.a.C);
   RowSum<TPR, 1> sum{&red};
+  const bool block = a.h, token = a.a.gate == kTokenGate;
   Vals<T, K> w1, b1, w2, b2, gs;
-  if (a.a.post) {
-    load_params(a.w1, at, 1.f, w1);
-    load_params(a.b1, at, 0.f, b1);
+  load_params(a.a.post ? a.w1 : nullptr, at, 1.f, w1);
+  load_params(a.a.next ? a.w2 : nullptr, at, 1.f, w2);
+  if (!Lean) {
+    load_params(a.a.post ? a.b1 : nullptr, at, 0.f, b1);
+    load_params(a.a.next ? a.b2 : nullptr, at, 0.f, b2);
   }
-  if (a.a.next) {
-    load_params(a.w2, at, 1.f, w2);
-    load_params(a.b2, at, 0.f, b2);
-  }
-  ranges(a, [&](long long row0, long long rows, int seg, int) {
-    if (a.a.gate != kTokenGate && a.h) {
+  segments(a, [&](long long row0, int seg, int split) {
+    const long long rows = a.seg, r = split * RB + threadIdx.x / TPR;
+    if (r >= rows) return;
+    Raw<T, K> rx, rh, rg;
+    auto fetch = [&](long long i) {
+      const long long row = row0 + min(i, rows - 1);
+      load_raw<Whole>((const T*)a.x + row * a.a.xl, at, rx);
+      if (block) load_raw<Whole>((const T*)a.h + row * a.a.hl, at, rh);
+      if (token) load_raw<Whole>((const T*)a.gate + row * a.a.gl, at, rg);
+    };
+    fetch(r);
+    if (!token && block) {
       load_params(a.a.gate ? (const float*)a.gate + (long long)seg * a.a.C : nullptr, at, 1.f, gs);
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * (a.a.gate ? gate_of(a.a.act, gs[k][j]) : 1.f);
     }
-    const int r = threadIdx.x / TPR;
-    for (long long i = r; i < rows; i += RB) {
+    for (long long i = r; i < rows; i += a.step) {
       const long long row = row0 + i;
       Vals<T, K> x, h;
-      load_row((const T*)a.x + row * a.a.xl, at, x);
+      values<Whole>(rx, at, x);
+      if (block) values<Whole>(rh, at, h);
+      if (token) {
+        values<Whole>(rg, at, gs);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * gate_of(a.a.act, gs[k][j]);
+      }
+      fetch(i + a.step);
       float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (a.h) {
-        load_row((const T*)a.h + row * a.a.hl, at, h);
-        if (a.a.gate == kTokenGate) {
-          load_row((const T*)a.gate + row * a.a.gl, at, gs);
-#pragma unroll
-          for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * gate_of(a.a.act, gs[k][j]);
-        }
+      if (block) {
         if (a.a.post) {
-          const float2 s = row_stats(a, at, h, sum);
+          const float2 s = row_stats<Lean>(a, at, h, sum);
           st.x = s.x, st.y = s.y;
 #pragma unroll
           for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int j = 0; j < kV<T>; ++j) h[k][j] = fmaf((h[k][j] - s.x) * s.y, w1[k][j], b1[k][j]);
+            for (int j = 0; j < kV<T>; ++j) {
+              const float u = (Lean ? h[k][j] : h[k][j] - s.x) * s.y;
+              h[k][j] = Lean ? u * w1[k][j] : fmaf(u, w1[k][j], b1[k][j]);
+            }
         }
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -239,12 +262,15 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm(TokenNorm a) {
         store_row((T*)a.y + row * a.a.C, at, x);
       }
       if (a.a.next) {
-        const float2 s = row_stats(a, at, x, sum);
+        const float2 s = row_stats<Lean>(a, at, x, sum);
         st.z = s.x, st.w = s.y;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int j = 0; j < kV<T>; ++j) x[k][j] = fmaf((x[k][j] - s.x) * s.y, w2[k][j], b2[k][j]);
+          for (int j = 0; j < kV<T>; ++j) {
+            const float v = (Lean ? x[k][j] : x[k][j] - s.x) * s.y;
+            x[k][j] = Lean ? v * w2[k][j] : fmaf(v, w2[k][j], b2[k][j]);
+          }
         store_row((T*)a.n + row * a.a.C, at, x);
       }
       if (a.stat && (threadIdx.x & (TPR - 1)) == 0) a.stat[row] = st;
@@ -280,38 +306,70 @@ __device__ __forceinline__ void fold_rows(Vals<T, K>& f, const Cols<T, TPR, K>& 
   }
 }
 
-template <typename T, int TPR, int K>
+template <typename T, int TPR, int K, bool Whole, bool Lean>
 __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
   constexpr int RB = kBlock<TPR> / TPR;
   __shared__ float red[2][2][16];
   __shared__ float lds[RB > 1 ? kBlock<TPR> * kV<T> : 1];
   const Cols<T, TPR, K> at(a.a.C);
   RowSum<TPR, 2> sum{&red};
-  const float inv = 1.f / (float)a.a.C, mean = a.a.layer ? inv : 0.f;
+  RowSum<TPR, 1> sum1{(float(*)[2][1][16])&red};
+  const bool block = a.h, token = a.a.gate == kTokenGate;
+  const float inv = 1.f / (float)a.a.C, mean = !Lean && a.a.layer ? inv : 0.f;
   Vals<T, K> w1, b1, w2, gs, aw1 = {}, ab1 = {}, aw2 = {}, ab2 = {}, ag = {};
   load_params(a.a.post ? a.w1 : nullptr, at, 1.f, w1);
-  load_params(a.a.post ? a.b1 : nullptr, at, 0.f, b1);
   load_params(a.a.next ? a.w2 : nullptr, at, 1.f, w2);
-  ranges(a, [&](long long row0, long long rows, int seg, int split) {
-    if (a.a.gate != kTokenGate && a.h) {
+  if (!Lean) load_params(a.a.post ? a.b1 : nullptr, at, 0.f, b1);
+  // the row's sums of f and of f v
+  auto both = [&](const Vals<T, K>& f, const Vals<T, K>& v, float& m, float& q) {
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < kV<T>; ++j) {
+        if (!Lean) s[0] += f[k][j];
+        s[1] = fmaf(f[k][j], v[k][j], s[1]);
+      }
+    if (Lean) {
+      float t[1] = {s[1]};
+      sum1(t);
+      m = 0.f, q = t[0] * inv;
+    } else {
+      sum(s);
+      m = s[0] * mean, q = s[1] * inv;
+    }
+  };
+  segments(a, [&](long long row0, int seg, int split) {
+    const long long rows = a.seg, r = split * RB + threadIdx.x / TPR;
+    Raw<T, K> rx, rh, rg, ry, rn;
+    float4 rs;
+    auto fetch = [&](long long i) {
+      const long long row = row0 + min(i, rows - 1);
+      load_raw<Whole>((const T*)a.x + row * a.a.xl, at, rx);
+      if (block) load_raw<Whole>((const T*)a.h + row * a.a.hl, at, rh);
+      if (token) load_raw<Whole>((const T*)a.gate + row * a.a.gl, at, rg);
+      if (a.dy) load_raw<Whole>((const T*)a.dy + row * a.a.dyl, at, ry);
+      if (a.dn) load_raw<Whole>((const T*)a.dn + row * a.a.dnl, at, rn);
+      rs = a.stat[row];
+    };
+    if (r < rows) fetch(r);
+    if (!token && block) {
       load_params(a.a.gate ? (const float*)a.gate + (long long)seg * a.a.C : nullptr, at, 1.f, gs);
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * (a.a.gate ? gate_of(a.a.act, gs[k][j]) : 1.f);
     }
-    const int r = threadIdx.x / TPR;
-    for (long long i = r; i < rows; i += RB) {
+    for (long long i = r; i < rows; i += a.step) {
       const long long row = row0 + i;
-      Vals<T, K> x, h, g, d;   // y, then v; u, then dh; the gate, then its slope; dn, then dy'
-      load_row((const T*)a.x + row * a.a.xl, at, x);
-      if (a.h) load_row((const T*)a.h + row * a.a.hl, at, h);
-      if (a.a.gate == kTokenGate) load_row((const T*)a.gate + row * a.a.gl, at, g);
-      Vals<T, K> up;
-      if (a.dy) load_row((const T*)a.dy + row * a.a.dyl, at, up);
-      if (a.dn) load_row((const T*)a.dn + row * a.a.dnl, at, d);
-      const float4 st = a.stat[row];
-      if (a.a.gate == kTokenGate) {
+      Vals<T, K> x, h, g, d, up;   // y, then v; u; the gate's slope; dn, then dy', then dh
+      values<Whole>(rx, at, x);
+      if (block) values<Whole>(rh, at, h);
+      if (a.dy) values<Whole>(ry, at, up);
+      if (a.dn) values<Whole>(rn, at, d);
+      const float4 st = rs;
+      if (token) {
+        values<Whole>(rg, at, g);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -320,34 +378,34 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
             g[k][j] = a.a.scale * gate_grad(a.a.act, g[k][j]);
           }
       }
-      if (a.h) {
+      fetch(i + a.step);
+      if (block) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int j = 0; j < kV<T>; ++j) {
-            if (a.a.post) h[k][j] = (h[k][j] - st.x) * st.y;
-            x[k][j] = fmaf(gs[k][j], fmaf(h[k][j], w1[k][j], b1[k][j]), x[k][j]);
+            if (a.a.post) h[k][j] = (Lean ? h[k][j] : h[k][j] - st.x) * st.y;
+            const float z = Lean ? h[k][j] * w1[k][j] : fmaf(h[k][j], w1[k][j], b1[k][j]);
+            x[k][j] = fmaf(gs[k][j], z, x[k][j]);
           }
       }
       if (a.dn) {
-        float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int j = 0; j < kV<T>; ++j) {
-            x[k][j] = (x[k][j] - st.z) * st.w;
-            ab2[k][j] += d[k][j];
+            x[k][j] = (Lean ? x[k][j] : x[k][j] - st.z) * st.w;
+            if (!Lean) ab2[k][j] += d[k][j];
             aw2[k][j] = fmaf(d[k][j], x[k][j], aw2[k][j]);
             d[k][j] *= w2[k][j];
-            s[0] += d[k][j];
-            s[1] = fmaf(d[k][j], x[k][j], s[1]);
           }
-        sum(s);
+        float m, q;
+        both(d, x, m, q);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int j = 0; j < kV<T>; ++j) {
-            const float t = st.w * fmaf(-x[k][j], s[1] * inv, d[k][j] - s[0] * mean);
+            const float t = st.w * fmaf(-x[k][j], q, Lean ? d[k][j] : d[k][j] - m);
             d[k][j] = j < at.nv[k] ? (a.dy ? up[k][j] + t : t) : 0.f;
           }
       } else {
@@ -357,28 +415,26 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
           for (int j = 0; j < kV<T>; ++j) d[k][j] = up[k][j];
       }
       if (a.dx) store_row((T*)a.dx + row * a.a.C, at, d);
-      if (!a.h) continue;
-      float s[2] = {0.f, 0.f};
+      if (!block) continue;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int j = 0; j < kV<T>; ++j) {
-          const float dz = gs[k][j] * d[k][j], z = fmaf(h[k][j], w1[k][j], b1[k][j]);
-          ag[k][j] = fmaf(d[k][j], z, ag[k][j]);
-          g[k][j] *= d[k][j] * z;
-          ab1[k][j] += dz;
+          const float dz = gs[k][j] * d[k][j], z = Lean ? h[k][j] * w1[k][j] : fmaf(h[k][j], w1[k][j], b1[k][j]);
+          if (token) g[k][j] *= d[k][j] * z;
+          else ag[k][j] = fmaf(d[k][j], z, ag[k][j]);
+          if (!Lean) ab1[k][j] += dz;
           aw1[k][j] = fmaf(dz, h[k][j], aw1[k][j]);
           d[k][j] = dz * w1[k][j];
-          s[0] += d[k][j];
-          s[1] = fmaf(d[k][j], h[k][j], s[1]);
         }
-      if (a.dgate) store_row((T*)a.dgate + row * a.a.C, at, g);
+      if (token && a.dgate) store_row((T*)a.dgate + row * a.a.C, at, g);
       if (a.a.post) {
-        sum(s);
+        float m, q;
+        both(d, h, m, q);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int j = 0; j < kV<T>; ++j) d[k][j] = st.y * fmaf(-h[k][j], s[1] * inv, d[k][j] - s[0] * mean);
+          for (int j = 0; j < kV<T>; ++j) d[k][j] = st.y * fmaf(-h[k][j], q, Lean ? d[k][j] : d[k][j] - m);
       }
       if (a.dh) store_row((T*)a.dh + row * a.a.C, at, d);
     }
@@ -392,13 +448,11 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
   });
   if (a.cols) {
     float* out = a.cols + (long long)blockIdx.x * 4 * a.a.C;
-    if (a.a.post) {
-      fold_rows(aw1, at, lds, out);
-      fold_rows(ab1, at, lds, out + a.a.C);
-    }
-    if (a.dn) {
-      fold_rows(aw2, at, lds, out + 2 * a.a.C);
-      fold_rows(ab2, at, lds, out + 3 * a.a.C);
+    if (a.a.post) fold_rows(aw1, at, lds, out);
+    if (a.dn) fold_rows(aw2, at, lds, out + 2 * a.a.C);
+    if (!Lean) {
+      if (a.a.post) fold_rows(ab1, at, lds, out + a.a.C);
+      if (a.dn) fold_rows(ab2, at, lds, out + 3 * a.a.C);
     }
   }
 }
@@ -434,32 +488,40 @@ __global__ __launch_bounds__(kJoin) void k_token_norm_join(TokenNorm a, int wgs,
 
 struct Shape {
   int tpr, k, rows;   // threads of a row; chunks of a thread; rows of a workgroup at a time
+  bool whole, lean;
 };
-Shape shape_of(int dtype, int C) {
-  const int chunks = div_up(C, dtype == kF32 ? 4 : 8);
+Shape shape_of(const splat_token_norm& a, bool biases) {
+  const int V = a.dtype == kF32 ? 4 : 8, chunks = div_up(a.C, V);
   int tpr = 4;
   while (tpr < 64 && tpr < chunks) tpr *= 2;
   if (chunks > 128) tpr = chunks > 512 ? 1024 : 256;
-  return {tpr, chunks > tpr ? 2 : 1, std::max(1, 256 / tpr)};
+  const bool whole = a.C % V == 0;
+  return {tpr, chunks > tpr ? 2 : 1, std::max(1, 256 / tpr), whole, whole && !a.layer && !biases};
 }
 
 template <typename F>
 int with_shape(int dtype, const Shape& s, F&& f) {
+  using std::integral_constant;
+  auto kind = [&](auto t, auto tpr, auto k) {
+    if (s.lean) return f(t, tpr, k, std::true_type{}, std::true_type{});
+    if (s.whole) return f(t, tpr, k, std::true_type{}, std::false_type{});
+    return f(t, tpr, k, std::false_type{}, std::false_type{});
+  };
   auto type = [&](auto t) {
     auto k = [&](auto tpr) {
-      return s.k == 2 ? f(t, tpr, std::integral_constant<int, 2>{}) : f(t, tpr, std::integral_constant<int, 1>{});
+      return s.k == 2 ? kind(t, tpr, integral_constant<int, 2>{}) : kind(t, tpr, integral_constant<int, 1>{});
     };
-    auto one = [&](auto tpr) { return f(t, tpr, std::integral_constant<int, 1>{}); };
+    auto one = [&](auto tpr) { return kind(t, tpr, integral_constant<int, 1>{}); };
     switch (s.tpr) {
-      case 4: return one(std::integral_constant<int, 4>{});
-      case 8: return one(std::integral_constant<int, 8>{});
-      case 16: return one(std::integral_constant<int, 16>{});
-      case 32: return one(std::integral_constant<int, 32>{});
-      case 64: return k(std::integral_constant<int, 64>{});
-      case 256: return k(std::integral_constant<int, 256>{});
+      case 4: return one(integral_constant<int, 4>{});
+      case 8: return one(integral_constant<int, 8>{});
+      case 16: return one(integral_constant<int, 16>{});
+      case 32: return one(integral_constant<int, 32>{});
+      case 64: return k(integral_constant<int, 64>{});
+      case 256: return k(integral_constant<int, 256>{});
     }
-    if constexpr (sizeof(t) == 4) return k(std::integral_constant<int, 1024>{});
-    else return one(std::integral_constant<int, 1024>{});
+    if constexpr (sizeof(t) == 4) return k(integral_constant<int, 1024>{});
+    else return one(integral_constant<int, 1024>{});
   };
   return dtype == kF32 ? type(float{}) : type(bf16{});
 }
@@ -479,20 +541,24 @@ int check_norm(const char* who, const splat_token_norm* a) {
   return kOk;
 }
 
-// Ranges of rows for about `target` workgroups. Returns their number.
+// Segments and splits for about `target` workgroups. Returns their number.
 unsigned plan(TokenNorm& n, const Shape& s, long long target) {
   n.segs = n.a.gate == kRowGate ? (int)n.a.segs : 1;
   n.seg = n.a.M / n.segs;
   n.whole = (int)((n.segs + target - 1) / target);
   const long long most = std::max<long long>(1, (n.seg + s.rows - 1) / s.rows);
-  const long long splits = std::min(most, n.segs >= target ? 1 : (target + n.segs - 1) / n.segs);
-  n.per = std::max<long long>(1, (n.seg + splits - 1) / splits);
-  n.per = (n.per + s.rows - 1) / s.rows * s.rows;
-  n.splits = (int)std::max<long long>(1, (n.seg + n.per - 1) / n.per);
+  n.splits = (int)std::min(most, n.segs >= target ? 1 : (target + n.segs - 1) / n.segs);
+  n.step = (long long)n.splits * s.rows;
   return (unsigned)((n.segs + n.whole - 1) / n.whole * n.splits);
 }
 
-constexpr long long kForward = 1024, kBackward = 768;   // workgroups aimed at
+// Workgroups aimed at: what the card holds at once, by the registers of a lane (four, and in the backward three, two or one
+// waves a SIMD for 4, 8 or 16 values a lane). Backward of 73,728 x 256 bf16, with its join: 512 workgroups 55 us, 768 69, 1,024
+// 60; of 5,001 x 517 floats 768 39 us, 512 45, 1,024 50.
+long long resident(const Shape& s, int dtype, bool back) {
+  const int values = s.k * (dtype == kF32 ? 4 : 8), waves = !back ? 4 : values == 4 ? 3 : values == 8 ? 2 : 1;
+  return 256LL * waves * 4 * 64 / std::max(256, s.tpr);
+}
 
 }  // namespace
 }  // namespace splat
@@ -510,11 +576,11 @@ int splat_token_norm_fwd(const splat_token_norm* a, const void* x, const void* h
   TokenNorm p{};
   p.a = *a;
   p.x = x, p.h = h, p.gate = gate, p.w1 = w1, p.b1 = b1, p.w2 = w2, p.b2 = b2, p.y = y, p.n = n, p.stat = (float4*)stat;
-  const Shape s = shape_of(a->dtype, a->C);
-  const unsigned grid = plan(p, s, kForward);
-  return with_shape(a->dtype, s, [&](auto t, auto tpr, auto k) {
+  const Shape s = shape_of(*a, b1 || b2);
+  const unsigned grid = plan(p, s, resident(s, a->dtype, false));
+  return with_shape(a->dtype, s, [&](auto t, auto tpr, auto k, auto whole, auto lean) {
     constexpr int TPR = decltype(tpr)::value;
-    k_token_norm<decltype(t), TPR, decltype(k)::value><<<grid, kBlock<TPR>, 0, (hipStream_t)stream>>>(p);
+    k_token_norm<decltype(t), TPR, decltype(k)::value, decltype(whole)::value, decltype(lean)::value><<<grid, kBlock<TPR>, 0, (hipStream_t)stream>>>(p);
     return check_launch("splat_token_norm_fwd");
   });
 }
@@ -523,7 +589,8 @@ size_t splat_token_norm_bwd_workspace_bytes(const splat_token_norm* a) {
   if (check_norm("splat_token_norm_bwd_workspace_bytes", a) || a->M == 0) return 0;
   TokenNorm p{};
   p.a = *a;
-  const size_t grid = plan(p, shape_of(a->dtype, a->C), kBackward);
+  const Shape s = shape_of(*a, false);
+  const size_t grid = plan(p, s, resident(s, a->dtype, true));
   return sizeof(float) * a->C * (4 * grid + (a->gate == kRowGate ? (size_t)p.segs * p.splits : 0));
 }
 
@@ -539,8 +606,8 @@ int splat_token_norm_bwd(const splat_token_norm* a, const void* x, const void* h
   p.a = *a;
   p.x = x, p.h = h, p.gate = gate, p.w1 = w1, p.b1 = b1, p.w2 = w2, p.dy = dy, p.dn = dn, p.stat = (float4*)stat;
   p.dx = dx, p.dh = dh, p.dgate = a->gate == kTokenGate ? dgate : nullptr;
-  const Shape s = shape_of(a->dtype, a->C);
-  const unsigned grid = plan(p, s, kBackward);
+  const Shape s = shape_of(*a, b1 || db1 || db2);
+  const unsigned grid = plan(p, s, resident(s, a->dtype, true));
   const bool cols = dw1 || db1 || dw2 || db2, gates = dgate && a->gate == kRowGate;
   const size_t need = cols || gates ? splat_token_norm_bwd_workspace_bytes(a) : 0;
   if (need && (!ws || ws_bytes < need))
@@ -548,9 +615,9 @@ int splat_token_norm_bwd(const splat_token_norm* a, const void* x, const void* h
   if (cols) p.cols = (float*)ws;
   if (gates) p.gates = (float*)ws + (size_t)4 * grid * a->C;
   const hipStream_t st = (hipStream_t)stream;
-  return with_shape(a->dtype, s, [&](auto t, auto tpr, auto k) {
+  return with_shape(a->dtype, s, [&](auto t, auto tpr, auto k, auto whole, auto lean) {
     constexpr int TPR = decltype(tpr)::value;
-    k_token_norm_bwd<decltype(t), TPR, decltype(k)::value><<<grid, kBlock<TPR>, 0, st>>>(p);
+    k_token_norm_bwd<decltype(t), TPR, decltype(k)::value, decltype(whole)::value, decltype(lean)::value><<<grid, kBlock<TPR>, 0, st>>>(p);
     if (need) {
       const int tiles = div_up(a->C, 64);
       k_token_norm_join<<<tiles * (4 + (gates ? p.segs : 0)), kJoin, 0, st>>>(p, (int)grid, tiles, dw1, db1, dw2, db2,

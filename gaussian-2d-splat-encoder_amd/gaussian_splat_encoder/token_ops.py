@@ -79,23 +79,28 @@ def _positions(positions, axes, B, L, D, x):
     return SplatPositions(positions.data_ptr(), kind, st[0] if len(shape) == 3 and shape[0] == B else 0, st[-2], st[-1])
 
 
-def _turn(x, positions, axes, dt, back):
-    B, L, H, D = x.shape
-    y = torch.empty((B, L, H, D), dtype=x.dtype, device=x.device)
+def _like(t):
+    """A new contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _turn(x, p, axes, dt, back):
+    """x (dense heads) turned by the positions that p describes, or back."""
+    y = _like(x)
     if y.numel():
-        p = _positions(positions, axes, B, L, D, x)
-        _launch(x, "splat_rotary", axes._ref, ctypes.byref(p), x.data_ptr(), *x.stride()[:3], dt, B, L, H, D, back,
-                y.data_ptr())
+        B, L, H, D = x.shape
+        sb, sl, sh, _ = x.stride()
+        _launch(x, "splat_rotary", axes._ref, p, x.data_ptr(), sb, sl, sh, dt, B, L, H, D, back, y.data_ptr())
     return y
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, positions, axes, dt):
+    def forward(ctx, x, positions, axes, p, dt):
         x = _dense(x)
         ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, positions)
         ctx.args = (axes, dt)
-        return _turn(x, positions, axes, dt, 0)
+        return _turn(x, p, axes, dt, 0)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -103,21 +108,21 @@ class _Rotary(torch.autograd.Function):
         x, positions = ctx.saved_tensors
         axes, dt = ctx.args
         g = _dense(g)
+        B, L, H, D = g.shape
+        p = _positions(positions, axes, B, L, D, g)
         if not ctx.needs_input_grad[1]:
-            return _turn(g, positions, axes, dt, 1), None, None, None
+            return _turn(g, p, axes, dt, 1), None, None, None, None
         x = _dense(x)
-        B, L, H, D = x.shape
-        dx = torch.empty((B, L, H, D), dtype=x.dtype, device=x.device)
+        dx = _like(x)
         shared = positions.dim() == 2 or positions.shape[0] != B
         new = torch.empty if dx.numel() else torch.zeros
         dp = new(positions.shape, dtype=torch.float32, device=x.device)
         if dx.numel():
-            p = _positions(positions, axes, B, L, D, x)
             n = _lib.load().splat_rotary_bwd_workspace_bytes(B, L, len(axes.dims), shared)
             keep, ws = _scratch(n, x)
-            _launch(x, "splat_rotary_bwd", axes._ref, ctypes.byref(p), x.data_ptr(), *x.stride()[:3], g.data_ptr(),
-                    *g.stride()[:3], dt, B, L, H, D, dx.data_ptr(), dp.data_ptr(), shared, ws, n)
-        return dx if ctx.needs_input_grad[0] else None, dp, None, None
+            _launch(x, "splat_rotary_bwd", axes._ref, p, x.data_ptr(), *x.stride()[:3], g.data_ptr(), *g.stride()[:3], dt, B,
+                    L, H, D, dx.data_ptr(), dp.data_ptr(), shared, ws, n)
+        return dx if ctx.needs_input_grad[0] else None, dp, None, None, None
 
 
 def rotary(x, positions, axes):
@@ -127,12 +132,13 @@ def rotary(x, positions, axes):
     over the images that share them), int32 or int64. axes: RotaryAxes. Angles are taken in 64 bits: positions up to 2^31
     keep theirs to 1e-6 of a turn."""
     dt, _ = _args("none", x)
-    if x.dim() != 4 or not 1 <= x.shape[3] <= MAX_HEAD or x.shape[2] < 1:
-        raise ValueError(f"x must be [B, L, H, D] with heads of 1 to {MAX_HEAD} values, got {list(x.shape)}")
-    _positions(positions, axes, x.shape[0], x.shape[1], x.shape[3], x)
+    shape = x.shape
+    if len(shape) != 4 or not 1 <= shape[3] <= MAX_HEAD or shape[2] < 1:
+        raise ValueError(f"x must be [B, L, H, D] with heads of 1 to {MAX_HEAD} values, got {list(shape)}")
+    p = _positions(positions, axes, shape[0], shape[1], shape[3], x)
     if _wants_grad(x, positions):
-        return _Rotary.apply(x, positions, axes, dt)
-    return _turn(_dense(x), positions, axes, dt, 0)
+        return _Rotary.apply(x, positions, axes, p, dt)
+    return _turn(_dense(x), p, axes, dt, 0)
 
 
 # ------------------------------------------------------------------------------------------------ the paged cache
@@ -224,10 +230,10 @@ def cache_append(cache, tables, lengths, k, v, counts=None, positions=None, axes
     c, keep = cache._describe(tables, lengths, counts, B, T)
     p = r = None
     if axes is not None:
-        p, r = ctypes.byref(_positions(positions, axes, B, T, cache.head_dim, k)), axes._ref
+        p, r = _positions(positions, axes, B, T, cache.head_dim, k), axes._ref
     if B and T and cache.pages and c.width:
         k, v = _dense(k), _dense(v)
-        _launch(k, "splat_cache_append", ctypes.byref(c), r, p, k.data_ptr(), *k.stride()[:3], v.data_ptr(),
+        _launch(k, "splat_cache_append", c, r, p, k.data_ptr(), *k.stride()[:3], v.data_ptr(),
                 *v.stride()[:3], _ptr(key_mask), *((0, 0) if key_mask is None else key_mask.stride()), T)
 
 
@@ -249,49 +255,53 @@ def cached_attention(q, cache, tables, lengths, counts=None, positions=None, axe
     c, keep = cache._describe(tables, lengths, counts, B, T)
     p = r = None
     if axes is not None:
-        p, r = ctypes.byref(_positions(positions, axes, B, T, D, q)), axes._ref
-    o = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+        p, r = _positions(positions, axes, B, T, D, q), axes._ref
+    o = _like(q)
     if o.numel():
         q = _dense(q)
-        ref = ctypes.byref(c)
-        n = _lib.load().splat_cached_attention_workspace_bytes(ref, H, T)
+        n = _lib.load().splat_cached_attention_workspace_bytes(c, H, T)
         held, ws = _scratch(n, q)
-        _launch(q, "splat_cached_attention", ref, r, p, q.data_ptr(), *q.stride()[:3], H, T, scale, int(bool(causal)),
+        _launch(q, "splat_cached_attention", c, r, p, q.data_ptr(), *q.stride()[:3], H, T, scale, int(bool(causal)),
                 o.data_ptr(), ws, n)
     return o
 
 
 # ------------------------------------------------------------------------------------------------ norms per token
+def _lay(t, C):
+    """t [..., C] as rows (itself where it is contiguous, whatever its shape) and the elements from row to row."""
+    if t.is_contiguous():
+        return t, C
+    t = _rows(t)
+    return t, t.stride(0)
+
+
 def _norm_args(x, h, gate, kind, eps, scale, act, post, nxt, dt):
-    """C description, x and h as rows, the gate as rows of its kind."""
-    C, M = x.shape[-1], math.prod(x.shape[:-1])
-    a = SplatTokenNorm(dt, C, M, _KINDS[kind], post, nxt, 0, _GATE_CODES[act], 0, eps, scale)
-    x2 = _rows(x)
-    a.xl = x2.stride(0)
-    h2 = None
+    """C description; x, h and the gate as rows."""
+    C = x.shape[-1]
+    x, xl = _lay(x, C)
+    hl = gl = segs = code = 0
     if h is not None:
-        h2 = _rows(h)
-        a.hl = h2.stride(0)
+        h, hl = _lay(h, C)
     if gate is not None:
-        if gate.shape == x.shape and gate.dtype is x.dtype and gate.numel() != C:
-            gate = _rows(gate)
-            a.gate, a.gl = 2, gate.stride(0)
+        n = gate.numel()
+        if n == C or n != x.numel() or gate.dtype is not x.dtype:
+            gate, code, segs = gate.contiguous(), 1, n // C
         else:
-            gate = gate.reshape(-1, C).contiguous()
-            a.gate, a.segs = 1, gate.shape[0]
-    return a, x2, h2, gate
+            code = 2
+            gate, gl = _lay(gate, C)
+    a = SplatTokenNorm(dt, C, x.numel() // C, kind, post, nxt, code, act, segs, eps, scale, xl, hl, gl)
+    return a, x, h, gate
 
 
 def _norm_fwd(x, h, w1, b1, gate, w2, b2, cfg, save):
     """(y or None, n or None, statistics or None)"""
     a, x2, h2, g2 = _norm_args(x, h, gate, *cfg)
-    new = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)   # noqa: E731
-    y = new() if h is not None else None
-    n = new() if a.next else None
-    stat = torch.empty((a.M, 4), dtype=torch.float32, device=x.device) if save else None
+    y = None if h is None else _like(x)
+    n = _like(x) if a.next else None
+    stat = x.new_empty((a.M, 4), dtype=torch.float32) if save else None
     if a.M:
-        _launch(x, "splat_token_norm_fwd", ctypes.byref(a), x2.data_ptr(), _ptr(h2), _ptr(g2), _ptr(w1), _ptr(b1), _ptr(w2),
-                _ptr(b2), _ptr(y), _ptr(n), _ptr(stat))
+        _launch(x, "splat_token_norm_fwd", a, x2.data_ptr(), _ptr(h2), _ptr(g2), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2),
+                _ptr(y), _ptr(n), _ptr(stat))
     return y, n, stat
 
 
@@ -313,31 +323,37 @@ class _ResidualNorm(torch.autograd.Function):
         need = ctx.needs_input_grad
         if dy is None and dn is None:
             return (None,) * 8
-        dev = x.device
-        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)   # noqa: E731
-        dx = new(x) if need[0] else None
-        dh = new(h) if need[1] else None
-        small = torch.empty if a.M else torch.zeros
-        par = [small(a.C, dtype=torch.float32, device=dev) if f else None for f in (need[2], need[3], need[5], need[6])]
-        if dn is None:      # nothing reached the second norm's parameters
-            par[2:] = [None if t is None else t.zero_() for t in par[2:]]
+        dx = _like(x) if need[0] else None
+        dh = _like(h) if need[1] else None
         dgate = None
         if need[4]:
-            dgate = new(gate) if a.M else torch.zeros_like(gate)
+            dgate = _like(gate) if a.M else torch.zeros_like(gate)
+        # the parameters' gradients are rows of one tensor; nothing reaches those of the second norm without dn
+        rows = (2, 3, 5, 6) if a.M and dn is not None else (2, 3) if a.M else ()
+        rows = [i for i in rows if need[i]]
+        grads, ptrs, C = {}, [None] * 7, a.C
+        if rows:
+            par = x.new_empty((len(rows), C), dtype=torch.float32)
+            at = par.data_ptr()
+            for k, (i, t) in enumerate(zip(rows, par.unbind())):
+                grads[i], ptrs[i] = t, at + 4 * C * k
+        for i in (2, 3, 5, 6):
+            if need[i] and i not in grads:
+                grads[i] = x.new_zeros(C, dtype=torch.float32)
         if a.M:
-            dy, dn = (None if t is None else _rows(t) for t in (dy, dn))
-            a.dyl, a.dnl = (0 if t is None else t.stride(0) for t in (dy, dn))
-            n = _lib.load().splat_token_norm_bwd_workspace_bytes(ctypes.byref(a))
+            if dy is not None:
+                dy, a.dyl = _lay(dy, C)
+            if dn is not None:
+                dn, a.dnl = _lay(dn, C)
+            n = _lib.load().splat_token_norm_bwd_workspace_bytes(a) if rows or a.gate == 1 else 0
             keep, ws = _scratch(n, x)
-            w2p = par[2:] if dn is not None else [None, None]
-            _launch(x, "splat_token_norm_bwd", ctypes.byref(a), x2.data_ptr(), _ptr(h2), _ptr(g2), _ptr(w1), _ptr(b1),
-                    _ptr(w2), _ptr(dy), _ptr(dn), stat.data_ptr(), _ptr(dx), _ptr(dh), _ptr(dgate), _ptr(par[0]),
-                    _ptr(par[1]), _ptr(w2p[0]), _ptr(w2p[1]), ws, n)
-        return dx, dh, par[0], par[1], dgate, par[2], par[3], None
+            _launch(x, "splat_token_norm_bwd", a, x2.data_ptr(), _ptr(h2), _ptr(g2), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(dy),
+                    _ptr(dn), stat.data_ptr(), _ptr(dx), _ptr(dh), _ptr(dgate), ptrs[2], ptrs[3], ptrs[5], ptrs[6], ws, n)
+        return dx, dh, grads.get(2), grads.get(3), dgate, grads.get(5), grads.get(6), None
 
 
 def _check_norm(x, kind, eps):
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_CHANNELS:
+    if not x.dim() or not 1 <= x.shape[-1] <= MAX_CHANNELS:
         raise ValueError(f"x must be [..., C] of 1 to {MAX_CHANNELS} channels, got {list(x.shape)}")
     if kind not in _KINDS:
         raise ValueError(f"unknown norm {kind!r}: one of {sorted(_KINDS)}")
@@ -353,7 +369,7 @@ def token_norm(x, weight=None, bias=None, kind="rms", eps=1e-6):
     _check_norm(x, kind, eps)
     C = x.shape[-1]
     weight, bias = _norm_param("weight", weight, C, x), _norm_param("bias", bias, C, x)
-    cfg = (kind, float(eps), 1.0, "none", 0, 1, dt)
+    cfg = (_KINDS[kind], float(eps), 1.0, 0, 0, 1, dt)
     if _wants_grad(x, weight, bias):
         return _ResidualNorm.apply(x, None, None, None, None, weight, bias, cfg)
     return _norm_fwd(x, None, None, None, None, weight, bias, cfg, False)[1]
@@ -388,7 +404,7 @@ def residual_norm(x, h, weight=None, bias=None, gate=None, gate_act="none", next
     next_weight, next_bias = _norm_param("next_weight", next_weight, C, x), _norm_param("next_bias", next_bias, C, x)
     if gate is not None:
         gate = _gate(gate, x)
-    cfg = (kind, float(eps), scale, gate_act, int(bool(norm_block)), int(bool(norm_next)), dt)
+    cfg = (_KINDS[kind], float(eps), scale, _GATE_CODES[gate_act], int(bool(norm_block)), int(bool(norm_next)), dt)
     if _wants_grad(x, h, weight, bias, gate, next_weight, next_bias):
         return _ResidualNorm.apply(x, h, weight, bias, gate, next_weight, next_bias, cfg)
     y, n, _ = _norm_fwd(x, h, weight, bias, gate, next_weight, next_bias, cfg, False)
