@@ -7,4 +7,7 @@ Public entry points (the reference's render API):
 Operators of channels-last feature maps and of models that read them:
   feature_ops.group_norm_act, linear_act, cross_attention
   cell_reader.CellReader
+Operators of tokens that read splats frame by frame:
+  token_ops.rotary, RotaryAxes, PagedCache, cache_append, cached_attention, residual_norm, token_norm
+  token_reader.TokenReader
 """
