@@ -6,7 +6,8 @@
 //
 // All of it is bound by memory. A thread has a unit of W pairs (16 bytes a run where the axes allow it) of a token, computes
 // their angles once in 64 bits and turns the unit in several heads; a token's threads lie side by side, so that a wave's loads
-// cover whole heads. Workgroups walk over tokens with the unit's rates in registers.
+// cover whole heads. Measured (a large copy moves 4.9 TB/s here): 147,456 tokens of 4 heads of 64 bf16 33.7 us each way (4.5 TB/s);
+// 92,160 tokens of 4 heads of 64 bf16 appended 48 us (3.9 TB/s), whose writes go to a page and head of their own each.
 #include <algorithm>
 
 #include "token_common.h"
@@ -15,7 +16,7 @@ namespace splat {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGrid = 2048;   // workgroups at most
+constexpr int kGrid = 1 << 16;   // workgroups at most
 
 struct Turn {
   splat_rotation r;
@@ -36,39 +37,66 @@ __device__ __forceinline__ Seat seat(int units, int hs, int rows, FastDiv by_uni
   return {row, k - h * units, h, row < rows};
 }
 
+// Cosines and sines of a unit's pairs at the position of token l of image b.
 template <int W>
-__device__ __forceinline__ void rates(const splat_rotation& r, const PairUnit& u, double (&f)[W]) {
+__device__ __forceinline__ void angles(const splat_rotation& r, const splat_positions& pos, const PairUnit& u, int b, int l,
+                                       float (&c)[W], float (&s)[W]) {
+  const double p = position(pos, b * pos.pb + l * pos.pl + u.axis * pos.pa);
 #pragma unroll
-  for (int j = 0; j < W; ++j) f[j] = u.axis >= 0 ? r.quarters[u.pair + j] : 0.0;
+  for (int j = 0; j < W; ++j) turn(p, r.quarters[u.pair + j], c[j], s[j]);
 }
 
-template <int W>
-__device__ __forceinline__ void angles(double p, const double (&f)[W], float (&c)[W], float (&s)[W]) {
+// A unit of HB heads of a tensor, `step` heads apart from h on, as it lies in memory. Loads have no conditions, so that all are
+// under way at once: heads past the last are the last one, a run that is none the first.
+template <typename T, int W, int HB>
+struct Runs {
+  T a[HB][W], b[HB][W];
+  __device__ __forceinline__ void load(const T* p, long long sh, const PairUnit& u, int h, int step, int H) {
 #pragma unroll
-  for (int j = 0; j < W; ++j) turn(p, f[j], c[j], s[j]);
-}
+    for (int i = 0; i < HB; ++i) {
+      const T* at = p + min(h + i * step, H - 1) * sh;
+      __builtin_memcpy(a[i], at + u.e0, sizeof(a[i]));
+      __builtin_memcpy(b[i], at + (u.second ? u.e1 : u.e0), sizeof(b[i]));
+    }
+  }
+  __device__ __forceinline__ void get(int i, float (&p)[W], float (&q)[W]) const {
+#pragma unroll
+    for (int j = 0; j < W; ++j) p[j] = (float)a[i][j], q[j] = (float)b[i][j];
+  }
+  __device__ __forceinline__ void put(int i, T* p, T* q, bool second) const {
+    T x[W], y[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) x[j] = a[i][j], y[j] = b[i][j];
+    __builtin_memcpy(p, x, sizeof(x));
+    if (second) __builtin_memcpy(q, y, sizeof(y));
+  }
+};
 
-// y = x turned (Back: turned back).
-template <typename T, int W, bool Back>
+// y = x turned (Back: turned back), HB heads at a time.
+template <typename T, int W, int HB, bool Back>
 __global__ __launch_bounds__(kThreads) void k_rotary(Turn n, const T* __restrict__ x, T* __restrict__ y) {
   const Seat at = seat(n.units, n.hs, n.rows, n.by_units, n.by_row);
   if (!at.in) return;
   const PairUnit u = pair_unit<W>(n.r, n.D, at.u);
-  double f[W];
-  rates<W>(n.r, u, f);
   for (long long m = (long long)blockIdx.x * n.rows + at.row; m < n.M; m += (long long)gridDim.x * n.rows) {
     const int b = (int)m / n.by_L, l = (int)m - b * n.L;
-    float c[W], s[W];
-    if (u.axis >= 0) angles<W>(position(n.pos, b * n.pos.pb + l * n.pos.pl + u.axis * n.pos.pa), f, c, s);
     const T* xp = x + b * n.xb + l * n.xl;
     T* yp = y + m * n.H * n.D;
-    for (int h = at.h; h < n.H; h += n.hs) {
-      float p[W], q[W] = {};
-      load_run<T, W>(xp + h * n.xh + u.e0, p);
-      if (u.second) load_run<T, W>(xp + h * n.xh + u.e1, q);
-      if (u.axis >= 0) turn_runs<W, Back>(p, q, c, s, n.r.interleaved);
-      store_run<T, W>(yp + (long long)h * n.D + u.e0, p);
-      if (u.second) store_run<T, W>(yp + (long long)h * n.D + u.e1, q);
+    float c[W], s[W];
+    for (int h0 = at.h; h0 < n.H; h0 += HB * n.hs) {
+      Runs<T, W, HB> r;
+      r.load(xp, n.xh, u, h0, n.hs, n.H);
+      if (u.axis >= 0 && h0 == at.h) angles<W>(n.r, n.pos, u, b, l, c, s);
+#pragma unroll
+      for (int i = 0; i < HB; ++i) {
+        const int h = h0 + i * n.hs;
+        if (HB > 1 && h >= n.H) continue;
+        float p[W], q[W];
+        r.get(i, p, q);
+        if (u.axis >= 0) turn_runs<W, Back>(p, q, c, s, n.r.interleaved);
+        store_run<T, W>(yp + (long long)h * n.D + u.e0, p);
+        if (u.second) store_run<T, W>(yp + (long long)h * n.D + u.e1, q);
+      }
     }
   }
 }
@@ -93,41 +121,44 @@ __device__ __forceinline__ void add_pairs(float (&sum)[W], const float (&p)[W], 
 
 // The gradients of x and of the positions ([B, L, axes], every image's own): a token's threads are its units, each over all
 // heads; an axis' units are added in order by one thread.
-template <typename T, int W>
+template <typename T, int W, int HB>
 __global__ __launch_bounds__(kThreads) void k_rotary_bwd(Turn n, const T* __restrict__ x, const T* __restrict__ g,
                                                          T* __restrict__ dx, float* __restrict__ dpos) {
   __shared__ float part[2][kThreads];
   const Seat at = seat(n.units, 1, n.rows, n.by_units, n.by_row);
   const PairUnit u = pair_unit<W>(n.r, n.D, at.u);
-  double f[W];
-  rates<W>(n.r, u, f);
   int flip = 0;
   for (long long m0 = (long long)blockIdx.x * n.rows; m0 < n.M; m0 += (long long)gridDim.x * n.rows, flip ^= 1) {
     const long long m = m0 + at.row;
     if (at.in && m < n.M) {
       const int b = (int)m / n.by_L, l = (int)m - b * n.L;
       float c[W], s[W], sum[W] = {};
-      if (u.axis >= 0) angles<W>(position(n.pos, b * n.pos.pb + l * n.pos.pl + u.axis * n.pos.pa), f, c, s);
+      if (u.axis >= 0) angles<W>(n.r, n.pos, u, b, l, c, s);
       const T *xp = x + b * n.xb + l * n.xl, *gp = g + b * n.gb + l * n.gl;
       T* yp = dx + m * n.H * n.D;
-      for (int h = 0; h < n.H; ++h) {
-        float p[W], q[W] = {};
-        load_run<T, W>(gp + h * n.gh + u.e0, p);
-        if (u.second) load_run<T, W>(gp + h * n.gh + u.e1, q);
-        if (u.axis >= 0) {
-          float a[W], e[W];
-          load_run<T, W>(xp + h * n.xh + u.e0, a);
-          load_run<T, W>(xp + h * n.xh + u.e1, e);
-          turn_runs<W, true>(p, q, c, s, n.r.interleaved);
-          add_pairs<W>(sum, p, q, a, e, n.r.interleaved);
+      for (int h0 = 0; h0 < n.H; h0 += HB) {
+        Runs<T, W, HB> gr, xr;
+        gr.load(gp, n.gh, u, h0, 1, n.H);
+        if (u.axis >= 0) xr.load(xp, n.xh, u, h0, 1, n.H);
+#pragma unroll
+        for (int i = 0; i < HB; ++i) {
+          const int h = h0 + i;
+          if (HB > 1 && h >= n.H) continue;
+          float p[W], q[W], a[W], e[W];
+          gr.get(i, p, q);
+          if (u.axis >= 0) {
+            xr.get(i, a, e);
+            turn_runs<W, true>(p, q, c, s, n.r.interleaved);
+            add_pairs<W>(sum, p, q, a, e, n.r.interleaved);
+          }
+          store_run<T, W>(yp + (long long)h * n.D + u.e0, p);
+          if (u.second) store_run<T, W>(yp + (long long)h * n.D + u.e1, q);
         }
-        store_run<T, W>(yp + (long long)h * n.D + u.e0, p);
-        if (u.second) store_run<T, W>(yp + (long long)h * n.D + u.e1, q);
       }
       constexpr float kHalfPi = 1.57079632679489662f;   // a quarter turn
       float t = 0.f;
 #pragma unroll
-      for (int j = 0; j < W; ++j) t = fmaf(sum[j], (float)f[j], t);
+      for (int j = 0; j < W; ++j) t = fmaf(sum[j], u.axis >= 0 ? (float)n.r.quarters[u.pair + j] : 0.f, t);
       part[flip][threadIdx.x] = t * kHalfPi;
     }
     __syncthreads();   // the other half is read before the next one, so one barrier a round does
@@ -166,72 +197,84 @@ struct Append {
 
 // New token t of sequence b goes to place lengths[b] - counts[b] + t of its pages; tokens past the count, before the
 // sequence's first place, behind its table or on a page that is none are left out.
-template <typename T, int W>
+template <typename T, int W, int HB>
 __global__ __launch_bounds__(kThreads) void k_append(Append n, const T* __restrict__ k, const T* __restrict__ v) {
   const Seat at = seat(n.units, n.hs, n.rows, n.by_units, n.by_row);
   if (!at.in) return;
   const PairUnit u = pair_unit<W>(n.r, n.c.D, at.u);
-  double f[W];
-  rates<W>(n.r, u, f);
   const long long room = (long long)n.c.page * n.c.width;
   for (long long m = (long long)blockIdx.x * n.rows + at.row; m < n.M; m += (long long)gridDim.x * n.rows) {
-    const int b = (int)m / n.by_T, t = (int)m - b * n.T, fresh = new_tokens(n.c, b, n.T);
+    const int b = (int)m / n.by_T, t = (int)m - b * n.T;
+    const T *kp = k + b * n.kb + t * n.kl, *vp = v + b * n.vb + t * n.vl;
+    Runs<T, W, HB> kr, vr;
+    kr.load(kp, n.kh, u, at.h, n.hs, n.c.Hk);
+    vr.load(vp, n.vh, u, at.h, n.hs, n.c.Hk);
+    const int fresh = new_tokens(n.c, b, n.T);
     const long long slot = (long long)n.c.lengths[b] - fresh + t;
     if (t >= fresh || slot < 0 || slot >= room) continue;
     const int index = (int)slot / n.by_page, page = n.c.tables[b * n.c.tb + index], off = (int)slot - index * n.c.page;
-    if (page < 0 || page >= n.c.pages) continue;
     float c[W], s[W];
-    if (u.axis >= 0) angles<W>(position(n.pos, b * n.pos.pb + t * n.pos.pl + u.axis * n.pos.pa), f, c, s);
-    const T *kp = k + b * n.kb + t * n.kl, *vp = v + b * n.vb + t * n.vl;
+    if (u.axis >= 0) angles<W>(n.r, n.pos, u, b, t, c, s);
+    if (page < 0 || page >= n.c.pages) continue;
     T* ko = (T*)n.c.k + page * n.c.kp + off * n.c.kt;
     T* vo = (T*)n.c.v + page * n.c.vp + off * n.c.vt;
-    for (int h = at.h; h < n.c.Hk; h += n.hs) {
-      float p[W], q[W] = {};
-      T v0[W], v1[W];
-      load_run<T, W>(kp + h * n.kh + u.e0, p);
-      __builtin_memcpy(v0, vp + h * n.vh + u.e0, sizeof(v0));
-      if (u.second) {
-        load_run<T, W>(kp + h * n.kh + u.e1, q);
-        __builtin_memcpy(v1, vp + h * n.vh + u.e1, sizeof(v1));
+    for (int h0 = at.h;;) {
+#pragma unroll
+      for (int i = 0; i < HB; ++i) {
+        const int h = h0 + i * n.hs;
+        if (HB > 1 && h >= n.c.Hk) continue;
+        float p[W], q[W];
+        kr.get(i, p, q);
+        if (u.axis >= 0) turn_runs<W, false>(p, q, c, s, n.r.interleaved);
+        store_run<T, W>(ko + h * n.c.kh + u.e0, p);
+        vr.put(i, vo + h * n.c.vh + u.e0, vo + h * n.c.vh + u.e1, u.second);
+        if (u.second) store_run<T, W>(ko + h * n.c.kh + u.e1, q);
       }
-      if (u.axis >= 0) turn_runs<W, false>(p, q, c, s, n.r.interleaved);
-      store_run<T, W>(ko + h * n.c.kh + u.e0, p);
-      __builtin_memcpy(vo + h * n.c.vh + u.e0, v0, sizeof(v0));
-      if (u.second) {
-        store_run<T, W>(ko + h * n.c.kh + u.e1, q);
-        __builtin_memcpy(vo + h * n.c.vh + u.e1, v1, sizeof(v1));
-      }
+      h0 += HB * n.hs;
+      if (h0 >= n.c.Hk) break;
+      kr.load(kp, n.kh, u, h0, n.hs, n.c.Hk);
+      vr.load(vp, n.vh, u, h0, n.hs, n.c.Hk);
     }
     if (n.c.live && at.u == 0 && at.h == 0)
       n.c.live[page * n.c.lp + off * n.c.lt] = !n.mask || n.mask[b * n.mb + t * n.ml] != 0;
   }
 }
 
-// Threads of a token and tokens of a workgroup: as many heads side by side as fit.
+// Threads of a token and tokens of a workgroup. A thread turns several heads by the angles it computes once, two at a time, as
+// long as `lanes` threads are left. 36,864 tokens, 8 heads of 64 floats: 2^18 29.7 us, 2^19 28.0; appending 8,192 tokens of 8 heads
+// of 128: 2^18 15.0, 2^19 18.2; 92,160 of 4 heads of 64: 48.0 and 49.8. (Four heads at a time: 30.7 us for the first of these; the next
+// token's loads under way while one is turned: 31.0, as the registers cost waves.)
+constexpr long long kTurnLanes = 1 << 19, kAppendLanes = 1 << 18;
 template <typename N>
-void seats(N& n, const Units& u, int H, bool one) {
+int seats(N& n, const Units& u, int H, long long lanes) {
   n.units = u.n;
-  n.hs = one ? 1 : std::min(H, std::max(1, kThreads / u.n));
+  n.hs = 1;
+  while (n.hs < H && (n.hs + 1) * u.n <= kThreads && (long long)n.M * u.n * n.hs < lanes) ++n.hs;
   n.rows = kThreads / (n.units * n.hs);
   n.by_units = fast_div(n.units);
   n.by_row = fast_div(n.units * n.hs);
+  return H > n.hs ? 2 : 1;
 }
 
 template <typename F>
-int with_run(int dtype, int W, F&& f) {
+int with_run(int dtype, int W, int HB, F&& f) {
+  using std::integral_constant;
+  auto heads = [&](auto t, auto w) {
+    return HB == 2 ? f(t, w, integral_constant<int, 2>{}) : f(t, w, integral_constant<int, 1>{});
+  };
   auto width = [&](auto t) {
     switch (W) {
-      case 8: return sizeof(t) == 2 ? f(t, std::integral_constant<int, sizeof(t) == 2 ? 8 : 4>{}) : -1;
-      case 4: return f(t, std::integral_constant<int, 4>{});
-      case 2: return f(t, std::integral_constant<int, 2>{});
+      case 8: return heads(t, integral_constant<int, sizeof(t) == 2 ? 8 : 4>{});   // floats: 4 at most
+      case 4: return heads(t, integral_constant<int, 4>{});
+      case 2: return heads(t, integral_constant<int, 2>{});
     }
-    return f(t, std::integral_constant<int, 1>{});
+    return heads(t, integral_constant<int, 1>{});
   };
   return dtype == kF32 ? width(float{}) : width(bf16{});
 }
 
 int plan_turn(const char* who, const splat_rotation* r, const splat_positions* p, int dtype, int B, long long L, int H, int D,
-              bool one, Turn* n, Units* u) {
+              bool one, Turn* n, Units* u, int* heads) {
   if (dtype != kF32 && dtype != kBf16) return set_error(kInvalid, "%s: unknown element type %d", who, dtype);
   if (B < 0 || L < 0 || H < 1 || D < 1) return set_error(kInvalid, "%s: B %d, L %lld, H %d, D %d", who, B, L, H, D);
   if (D > kMaxHead) return set_error(kUnsupported, "%s: heads of %d values, %d at most", who, D, kMaxHead);
@@ -246,14 +289,14 @@ int plan_turn(const char* who, const splat_rotation* r, const splat_positions* p
   n->D = D;
   n->M = (int)(B * L);
   *u = pair_units(*r, D, dtype == kF32 ? 4 : 8);
-  seats(*n, *u, H, one);
+  *heads = seats(*n, *u, H, one ? 0 : kTurnLanes);
   n->by_L = fast_div(std::max(1, n->L));
   n->by_axes = fast_div(std::max(1, r->axes));
   return kOk;
 }
 
 template <typename N>
-unsigned grid_of(const N& n) { return (unsigned)std::min<long long>(kGrid, div_up(n.M, n.rows)); }
+unsigned grid_of(const N& n) { return (unsigned)std::min(kGrid, div_up(n.M, n.rows)); }
 
 }  // namespace
 }  // namespace splat
@@ -266,14 +309,15 @@ int splat_rotary(const splat_rotation* r, const splat_positions* p, const void* 
                  int dtype, int B, long long L, int H, int D, int back, void* y, void* stream) {
   Turn n{};
   Units u;
-  if (const int rc = plan_turn("splat_rotary", r, p, dtype, B, L, H, D, false, &n, &u)) return rc;
+  int heads;
+  if (const int rc = plan_turn("splat_rotary", r, p, dtype, B, L, H, D, false, &n, &u, &heads)) return rc;
   if (n.M == 0) return kOk;
   if (!x || !y) return set_error(kInvalid, "splat_rotary: null pointer");
   n.xb = xb, n.xl = xl, n.xh = xh;
-  return with_run(dtype, u.W, [&](auto t, auto w) {
+  return with_run(dtype, u.W, heads, [&](auto t, auto w, auto hb) {
     using T = decltype(t);
-    constexpr int W = decltype(w)::value;
-    (back ? k_rotary<T, W, true> : k_rotary<T, W, false>)<<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const T*)x,
+    constexpr int W = decltype(w)::value, HB = decltype(hb)::value;
+    (back ? k_rotary<T, W, HB, true> : k_rotary<T, W, HB, false>)<<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const T*)x,
                                                                                                            (T*)y);
     return check_launch("splat_rotary");
   });
@@ -288,7 +332,8 @@ int splat_rotary_bwd(const splat_rotation* r, const splat_positions* p, const vo
                      void* dx, float* dpos, int shared, void* ws, size_t ws_bytes, void* stream) {
   Turn n{};
   Units u;
-  if (const int rc = plan_turn("splat_rotary_bwd", r, p, dtype, B, L, H, D, true, &n, &u)) return rc;
+  int heads;
+  if (const int rc = plan_turn("splat_rotary_bwd", r, p, dtype, B, L, H, D, true, &n, &u, &heads)) return rc;
   if (!r->axes) return set_error(kInvalid, "splat_rotary_bwd: no axes");
   if (n.M == 0) return kOk;
   if (!x || !g || !dx || !dpos) return set_error(kInvalid, "splat_rotary_bwd: null pointer");
@@ -297,10 +342,10 @@ int splat_rotary_bwd(const splat_rotation* r, const splat_positions* p, const vo
     return set_error(kWorkspace, "splat_rotary_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
   n.xb = xb, n.xl = xl, n.xh = xh, n.gb = gb, n.gl = gl, n.gh = gh;
   float* each = need ? (float*)ws : dpos;
-  return with_run(dtype, u.W, [&](auto t, auto w) {
+  return with_run(dtype, u.W, heads, [&](auto t, auto w, auto hb) {
     using T = decltype(t);
-    constexpr int W = decltype(w)::value;
-    k_rotary_bwd<T, W><<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const T*)x, (const T*)g, (T*)dx, each);
+    constexpr int W = decltype(w)::value, HB = decltype(hb)::value;
+    k_rotary_bwd<T, W, HB><<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const T*)x, (const T*)g, (T*)dx, each);
     if (need) {
       const long long m = L * r->axes;
       k_rotary_join<<<(unsigned)div_up(m, kThreads), kThreads, 0, (hipStream_t)stream>>>(each, dpos, B, m);
@@ -327,12 +372,12 @@ int splat_cache_append(const splat_cache* c, const splat_rotation* r, const spla
   n.T = (int)T;
   n.M = (int)(c->B * T);
   const Units u = pair_units(n.r, c->D, c->dtype == kF32 ? 4 : 8);
-  seats(n, u, c->Hk, false);
+  const int heads = seats(n, u, c->Hk, kAppendLanes);
   n.by_T = fast_div(n.T);
   n.by_page = fast_div(c->page);
-  return with_run(c->dtype, u.W, [&](auto t, auto w) {
+  return with_run(c->dtype, u.W, heads, [&](auto t, auto w, auto hb) {
     using E = decltype(t);
-    k_append<E, decltype(w)::value><<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const E*)k, (const E*)v);
+    k_append<E, decltype(w)::value, decltype(hb)::value><<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const E*)k, (const E*)v);
     return check_launch("splat_cache_append");
   });
 }
