@@ -23,7 +23,9 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kLeast = 128;      // tokens of a piece at least: one bf16 tile for each wave
-constexpr int kTarget = 768;     // workgroups aimed at
+constexpr int kRounds = 4;       // of workgroups, where sequences are many
+// Workgroups that a CU holds, by the registers of their kernels (16 NR rows, heads of DP).
+constexpr int held(int DP, int NR) { return NR == 1 ? DP == 32 ? 4 : DP == 64 ? 3 : 2 : DP == 32 ? 3 : DP == 64 ? 2 : 1; }
 
 struct Cached {
   splat_cache c;
@@ -36,60 +38,63 @@ struct Cached {
   int T, H, rep, R;            // new tokens; query heads; of a key head; rows = T rep
   int tiles, pieces, causal;   // row tiles; pieces aimed at, over all sequences
   int units;                   // of a head, single pairs
-  bool alike;                  // keys and values have the same strides
+  bool alike, fit;             // keys and values have the same strides; all pieces shall be on the card at once
   FastDiv by_rep, by_page, by_units;
-  float *part, *stat;          // rows of the pieces of split sequences; their maxima and sums
+  float* part;                 // rows of the pieces of split sequences
+  float2* stat;                // their maxima and sums
+  int2* split;                 // pieces of each sequence and the first one's slot
 };
 
 template <typename T> constexpr int kTile = sizeof(T) == 2 ? 32 : 16;   // tokens of a wave's tile
 
-__device__ __forceinline__ long long wave_sum(long long v) {
-#pragma unroll
-  for (int i = 32; i; i /= 2) v += __shfl_xor(v, i);
+// Inclusive sums over a wave's lanes, without LDS: within rows of 16, then rows' last ones added to the rows behind them.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);    // one lane up within 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);    // lane 15 of rows 0 and 2 to rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);    // lane 31 to rows 2 and 3
   return v;
 }
-__device__ __forceinline__ int wave_scan(int v) {   // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int i = 1; i < 64; i *= 2) {
-    const int u = __shfl_up(v, i);
-    if (lane >= i) v += u;
-  }
-  return v;
-}
+__device__ __forceinline__ int last_of(int v) { return __builtin_amdgcn_readlane(v, 63); }
 
-// Tokens of a piece, the same for all sequences: what the aimed at number of pieces would have, at least kLeast.
-__device__ __forceinline__ int piece_length(const Cached& a) {
-  long long n = 0;
-  for (int b = threadIdx.x & 63; b < a.c.B; b += 64) n += cached_tokens(a.c, b);
-  n = wave_sum(n);
-  const long long per = ((n + a.pieces - 1) / a.pieces + kLeast - 1) / kLeast * kLeast;
-  return (int)max((long long)kLeast, min(per, 0x7fffff00LL));
-}
-
-// A sequence's pieces and the first one's slot among those of split sequences.
+// The piece of a workgroup: `i` of the n of sequence b (n < 1: none), which has len tokens; `slot` is the sequence's first one
+// among those of split sequences. Pieces are as long for all sequences, in units of kLeast tokens: what the aimed at number of
+// them would have, and where all shall be on the card at once (`fit`) longer until their number is no more than that; a
+// sequence without tokens has one.
 struct Piece {
   int b, i, n, len, slot;
 };
-// The sequence and piece of workgroup `s` (Of: of sequence `s` its first one); b < 0 where there is none.
-template <bool Of>
 __device__ __forceinline__ Piece find(const Cached& a, int s) {
-  const int per = piece_length(a), lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63;
+  long long units = 0;
+  int len = 0;   // of the lane's sequence
+  for (int b0 = 0; b0 < a.c.B; b0 += 64) {
+    len = b0 + lane < a.c.B ? cached_tokens(a.c, b0 + lane) : 0;
+    units += last_of(wave_scan((len + kLeast - 1) / kLeast));   // 2^24 a sequence at most
+  }
+  int per = max(1, (int)min((units + a.pieces - 1) / a.pieces, 0xffffffLL));   // units of a piece
+  for (int i = 0; a.fit && i < 3; ++i) {   // at most 64 sequences
+    const int n = last_of(wave_scan(len > 0 ? (len - 1) / kLeast / per + 1 : 0));
+    if (n <= a.pieces) break;
+    per = (int)(((long long)per * n + a.pieces - 1) / a.pieces);
+  }
   int first = 0, slot = 0;
   for (int b0 = 0; b0 < a.c.B; b0 += 64) {
-    const int b = b0 + lane, len = b < a.c.B ? cached_tokens(a.c, b) : 0;
-    const int n = b < a.c.B ? (len > 0 ? (len - 1) / per + 1 : 1) : 0, m = n > 1 ? n : 0;
-    const int upto = first + wave_scan(n), slots = slot + wave_scan(m);
-    const unsigned long long hit = __ballot(Of ? b == s : upto > s);
+    if (a.c.B > 64) len = b0 + lane < a.c.B ? cached_tokens(a.c, b0 + lane) : 0;
+    const int n = b0 + lane < a.c.B ? len > 0 ? (len - 1) / kLeast / per + 1 : 1 : 0, m = n > 1 ? n : 0;
+    const int upto = wave_scan(n), slots = wave_scan(m);
+    const unsigned long long hit = __ballot(first + upto > s);
     if (hit) {
-      const int f = __builtin_ctzll(hit);
-      const int nf = __shfl(n, f);
-      return {b0 + f, Of ? 0 : s - (__shfl(upto, f) - nf), nf, __shfl(len, f), __shfl(slots, f) - __shfl(m, f)};
+      const int f = __builtin_ctzll(hit), nf = __builtin_amdgcn_readlane(n, f);
+      return {b0 + f, s - (first + __builtin_amdgcn_readlane(upto, f) - nf), nf, __builtin_amdgcn_readlane(len, f),
+              slot + __builtin_amdgcn_readlane(slots, f) - __builtin_amdgcn_readlane(m, f)};
     }
-    first = __shfl(upto, 63);
-    slot = __shfl(slots, 63);
+    first += last_of(upto);
+    slot += last_of(slots);
   }
-  return {-1, 0, 0, 0, 0};
+  return {0, 0, 0, 0, 0};
 }
 
 template <typename T, int DP>
@@ -174,13 +179,14 @@ struct Lds {
 enum Fill : int { kFull = 0, kChunks = 1, kValues = 2 };
 
 template <typename T, int DP, int NR, int Fit>
-__global__ __launch_bounds__(kThreads) void k_cached(Cached a) {
+__global__ __launch_bounds__(kThreads, held(DP, NR)) void k_cached(Cached a) {
   using F = Form<T, DP>;
   constexpr int V = F::V, KT = F::KT;
   __shared__ Lds<T, DP, NR> lds;
   const int rt = blockIdx.x % a.tiles, sh = blockIdx.x / a.tiles, hk = sh % a.c.Hk;
-  const Piece pc = find<false>(a, sh / a.c.Hk);
-  if (pc.b < 0) return;
+  const Piece pc = find(a, sh / a.c.Hk);
+  if (pc.n < 1) return;
+  if (a.split && pc.i == 0 && hk == 0 && rt == 0 && threadIdx.x == 0) a.split[pc.b] = make_int2(pc.n, pc.slot);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, b = pc.b, len = pc.len;
   const int per = ((len - 1) / pc.n + 32) / 32 * 32, k0 = pc.i * per, k1 = min(len, k0 + per);
   const int tend = (k1 + KT - 1) / KT;
@@ -456,74 +462,63 @@ __global__ __launch_bounds__(kThreads) void k_cached(Cached a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (d + j < a.c.D) a.part[at * a.c.D + d + j] = o[j];
-      if (d == 0) {
-        a.stat[2 * at] = top;
-        a.stat[2 * at + 1] = sum;
-      }
+      if (d == 0) a.stat[at] = make_float2(top, sum);
     }
   }
 }
 
-// Joins the pieces of a split sequence's row, one workgroup a row: a thread has four values of a head in every 256 / (D / 4)-th
-// piece, partial sums are added in order.
+// Joins the pieces of a split sequence's row, one workgroup a row: a thread has four values of the head in every 256 / (D / 4)-th
+// piece, with a running maximum and sum of its own; those are joined in order. One pass: 4 us, the launch and two loads in a
+// row, for 8 to 190 pieces.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_cached_join(Cached a) {
-  __shared__ float tops[kThreads], weight[kThreads];
   __shared__ f32x4 part[kThreads];
-  __shared__ float sums[kThreads];
+  __shared__ float tops[kThreads], sums[kThreads];
   const int row = blockIdx.x, b = row / (a.c.Hk * a.R), hr = row - b * (a.c.Hk * a.R), hk = hr / a.R, r = hr - hk * a.R;
-  const Piece pc = find<true>(a, b);
-  if (pc.n <= 1) return;
-  const int quads = (a.c.D + 3) / 4, groups = kThreads / quads, q = threadIdx.x % quads, gr = threadIdx.x / quads;
-  auto at = [&](int i) { return ((long long)(pc.slot + i) * a.c.Hk + hk) * a.R + r; };
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < pc.n; i += kThreads) top = fmaxf(top, a.stat[2 * at(i)]);
-  tops[threadIdx.x] = top;
-  __syncthreads();
-  for (int i = kThreads / 2; i; i /= 2) {
-    if ((int)threadIdx.x < i) tops[threadIdx.x] = fmaxf(tops[threadIdx.x], tops[threadIdx.x + i]);
-    __syncthreads();
-  }
-  top = tops[0];
-  const float base = top == -INFINITY ? 0.f : top;
+  const int2 sp = a.split[b];
+  if (sp.x <= 1) return;
+  const int D = a.c.D, quads = (D + 3) / 4, groups = kThreads / quads, q = threadIdx.x % quads, gr = threadIdx.x / quads;
+  float top = -INFINITY, sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-  for (int i0 = 0; i0 < pc.n; i0 += kThreads) {
-    __syncthreads();
-    const int n = min(kThreads, pc.n - i0);
-    if ((int)threadIdx.x < n) {
-      weight[threadIdx.x] = hw_exp2(a.stat[2 * at(i0 + threadIdx.x)] - base);
-      sum += a.stat[2 * at(i0 + threadIdx.x) + 1] * weight[threadIdx.x];
-    }
-    __syncthreads();
-    if (gr < groups) {
+  if (gr < groups) {
 #pragma unroll 4
-      for (int i = gr; i < n; i += groups) {
-        const float* p = a.part + at(i0 + i) * a.c.D + 4 * q;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (4 * q + 4 <= a.c.D) {
-          __builtin_memcpy(&v, p, 16);
-        } else {
-          for (int j = 0; j < a.c.D - 4 * q; ++j) v[j] = p[j];
-        }
-        o += v * weight[i];
+    for (int i = gr; i < sp.x; i += groups) {
+      const long long at = ((long long)(sp.y + i) * a.c.Hk + hk) * a.R + r;
+      const float2 st = a.stat[at];
+      const float* p = a.part + at * D + 4 * q;
+      f32x4 v;
+      if (D % 4 == 0) {
+        __builtin_memcpy(&v, p, 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = p[min(j, D - 1 - 4 * q)];
       }
+      const float now = fmaxf(top, st.x), base = now == -INFINITY ? 0.f : now;
+      const float by = hw_exp2(top - base), w = hw_exp2(st.x - base);
+      top = now;
+      sum = fmaf(sum, by, st.y * w);
+      o = o * by + v * w;
     }
   }
   part[threadIdx.x] = o;
+  tops[threadIdx.x] = top;
   sums[threadIdx.x] = sum;
   __syncthreads();
-  for (int i = kThreads / 2; i; i /= 2) {
-    if ((int)threadIdx.x < i) sums[threadIdx.x] += sums[threadIdx.x + i];
-    __syncthreads();
-  }
   if (gr != 0) return;
-  for (int i = 1; i < groups; ++i) o += part[i * quads + q];
-  sum = sums[0];
+  for (int i = 1; i < groups; ++i) top = fmaxf(top, tops[i * quads + q]);
+  const float base = top == -INFINITY ? 0.f : top;
+  o = f32x4{0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  for (int i = 0; i < groups; ++i) {
+    const float w = hw_exp2(tops[i * quads + q] - base);
+    sum = fmaf(sums[i * quads + q], w, sum);
+    o += part[i * quads + q] * w;
+  }
   const int qt = r / a.by_rep, h = hk * a.rep + (r - qt * a.rep);
-  T* to = (T*)a.o + (((long long)b * a.T + qt) * a.H + h) * a.c.D + 4 * q;
+  T* to = (T*)a.o + (((long long)b * a.T + qt) * a.H + h) * D + 4 * q;
   const float by = sum == 0.f ? 0.f : 1.f / sum;
-  for (int j = 0; j < min(4, a.c.D - 4 * q); ++j) to[j] = (T)(sum == 0.f ? 0.f : o[j] * by);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (4 * q + j < D) to[j] = (T)(sum == 0.f ? 0.f : o[j] * by);
 }
 
 int check_call(const char* who, const splat_cache* c, const splat_rotation* r, const splat_positions* p, int H, long long T,
@@ -544,7 +539,12 @@ Cached plan(const splat_cache& c, int H, int T) {
   n.rep = H / c.Hk;
   n.R = T * n.rep;
   n.tiles = div_up(n.R, n.R > 16 ? 32 : 16);
-  n.pieces = std::max(1, div_up(kTarget, (long long)c.Hk * n.tiles));
+  // One round of workgroups, as many as the card holds, while there are sequences to cut; rounds of smaller pieces, which make
+  // up for different lengths, where there are many.
+  const int all = 256 * held(c.D <= 32 ? 32 : c.D <= 64 ? 64 : c.D <= 96 ? 96 : 128, n.R > 16 ? 2 : 1);
+  const long long each = (long long)c.Hk * n.tiles, once = std::max(1LL, all / each);
+  n.fit = c.B <= 64 && 2 * c.B <= once;
+  n.pieces = (int)(n.fit ? once : (kRounds * all + each - 1) / each);
   n.by_rep = fast_div(n.rep);
   n.by_page = fast_div(c.page);
   return n;
@@ -583,7 +583,8 @@ extern "C" {
 size_t splat_cached_attention_workspace_bytes(const splat_cache* c, int H, long long T) {
   if (check_call("splat_cached_attention_workspace_bytes", c, nullptr, nullptr, H, T, 0.f) || c->B == 0 || T == 0) return 0;
   const Cached n = plan(*c, H, (int)T);
-  return sizeof(float) * slots(n) * c->Hk * n.R * (c->D + 2);
+  const size_t rows = slots(n) * c->Hk * n.R;
+  return rows ? sizeof(float) * rows * (c->D + 2) + sizeof(int2) * c->B : 0;
 }
 
 int splat_cached_attention(const splat_cache* c, const splat_rotation* r, const splat_positions* p, const void* q, long long qb,
@@ -607,8 +608,10 @@ int splat_cached_attention(const splat_cache* c, const splat_rotation* r, const 
   n.by_units = fast_div(n.units);
   n.alike = c->kp == c->vp && c->kt == c->vt;
   if (need) {
-    n.stat = (float*)ws;
-    n.part = n.stat + 2 * slots(n) * c->Hk * n.R;
+    const size_t rows = slots(n) * c->Hk * n.R;
+    n.split = (int2*)ws;
+    n.stat = (float2*)(n.split + c->B);
+    n.part = (float*)(n.stat + rows);
   }
   const hipStream_t st = (hipStream_t)stream;
   return with_form(c->dtype, c->D, n.R, [&](auto t, auto dp, auto nr, auto fit) {
