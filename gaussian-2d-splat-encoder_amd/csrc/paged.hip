@@ -278,7 +278,8 @@ __global__ __launch_bounds__(kThreads, held(DP, NR)) void k_cached(Cached a) {
   __syncthreads();
   const bool fine = sizeof(T) == 2 && a.r.axes > 0;
   Chunk<T> qf[NR][F::nc], ql[NR][F::nc];
-  int lim[NR], own[NR], least = len;   // tokens that the lane's row sees; its query; the fewest of any row
+  int lim[NR], own[NR];   // tokens that the lane's row sees; its query
+  auto seen_by = [&](int q) { return q >= fresh ? 0 : a.causal ? max(0, len - (fresh - 1 - q)) : len; };
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
 #pragma unroll
@@ -289,12 +290,10 @@ __global__ __launch_bounds__(kThreads, held(DP, NR)) void k_cached(Cached a) {
     }
     const int r = r0 + 16 * n + (lane & 15);
     own[n] = r / a.by_rep;
-    lim[n] = r >= a.R ? len : own[n] >= fresh ? 0 : a.causal ? max(0, len - (fresh - 1 - own[n])) : len;
-    least = min(least, lim[n]);
+    lim[n] = r >= a.R ? len : seen_by(own[n]);
   }
-#pragma unroll
-  for (int i = 8; i; i /= 2) least = min(least, __shfl_xor(least, i));
-  least = __builtin_amdgcn_readfirstlane(least);
+  // the fewest tokens that a row sees: its first query's, or none where the last one is past the new tokens
+  const int q0 = r0 / a.by_rep, q1 = (r0 + rows - 1) / a.by_rep, least = q1 >= fresh ? 0 : seen_by(q0);
   __syncthreads();
 
   T* tv = lds.values[w];
@@ -416,9 +415,7 @@ __global__ __launch_bounds__(kThreads, held(DP, NR)) void k_cached(Cached a) {
     if (!odd) {
       add(false, 0, 0);
     } else {
-      const int last = (min(a.R, r0 + 16 * NR) - 1) / a.by_rep;
-      for (int q = r0 / a.by_rep; q <= last; ++q)
-        add(true, q, q >= fresh ? 0 : a.causal ? max(0, len - (fresh - 1 - q)) : len);
+      for (int q = q0; q <= q1; ++q) add(true, q, seen_by(q));
     }
   }
 
