@@ -27,6 +27,9 @@ constexpr int kRounds = 4;       // of workgroups, where sequences are many
 // Workgroups that a CU holds, by the registers of their kernels (16 NR rows, heads of DP).
 constexpr int held(int DP, int NR) { return NR == 1 ? DP == 32 ? 4 : DP == 64 ? 3 : 2 : DP == 32 ? 3 : DP == 64 ? 2 : 1; }
 
+// Sequences are whole, cut by a scan in each workgroup (up to 64 of them), or as a list has it.
+enum Cut : int { kWhole = 0, kScanned = 1, kMapped = 2 };
+
 struct Cached {
   splat_cache c;
   splat_rotation r;
@@ -39,6 +42,8 @@ struct Cached {
   int tiles, pieces, causal;   // row tiles; pieces aimed at, over all sequences
   int units;                   // of a head, single pairs
   bool alike, fit;             // keys and values have the same strides; all pieces shall be on the card at once
+  int cut;                     // how a workgroup finds its piece
+  int4* map;                   // the pieces, where many sequences are cut
   FastDiv by_rep, by_page, by_units;
   float* part;                 // rows of the pieces of split sequences
   float2* stat;                // their maxima and sums
@@ -59,6 +64,11 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 __device__ __forceinline__ int last_of(int v) { return __builtin_amdgcn_readlane(v, 63); }
 
+// Pieces of a sequence of len tokens (!in: of none).
+__device__ __forceinline__ int pieces_of(int len, int per, bool in) {
+  return in ? len > 0 ? (len - 1) / kLeast / per + 1 : 1 : 0;
+}
+
 // The piece of a workgroup: `i` of the n of sequence b (n < 1: none), which has len tokens; `slot` is the sequence's first one
 // among those of split sequences. Pieces are as long for all sequences, in units of kLeast tokens: what the aimed at number of
 // them would have, and where all shall be on the card at once (`fit`) longer until their number is no more than that; a
@@ -67,34 +77,65 @@ struct Piece {
   int b, i, n, len, slot;
 };
 __device__ __forceinline__ Piece find(const Cached& a, int s) {
-  const int lane = threadIdx.x & 63;
-  long long units = 0;
-  int len = 0;   // of the lane's sequence
-  for (int b0 = 0; b0 < a.c.B; b0 += 64) {
-    len = b0 + lane < a.c.B ? cached_tokens(a.c, b0 + lane) : 0;
-    units += last_of(wave_scan((len + kLeast - 1) / kLeast));   // 2^24 a sequence at most
+  if (a.cut == kWhole) return s < a.c.B ? Piece{s, 0, 1, cached_tokens(a.c, s), 0} : Piece{};
+  if (a.cut == kMapped) {
+    const int4 m = a.map[s];
+    return m.z ? Piece{m.x, m.y, m.z, cached_tokens(a.c, m.x), m.w} : Piece{};
   }
-  int per = max(1, (int)min((units + a.pieces - 1) / a.pieces, 0xffffffLL));   // units of a piece
-  for (int i = 0; a.fit && i < 3; ++i) {   // at most 64 sequences
+  const int lane = threadIdx.x & 63;
+  int len = 0;   // of the lane's sequence
+  if (lane < a.c.B) len = cached_tokens(a.c, lane);
+  const int units = last_of(wave_scan((len + kLeast - 1) / kLeast));   // 2^24 a sequence at most
+  int per = max(1, (units + a.pieces - 1) / a.pieces);                 // units of a piece
+  for (int i = 0; a.fit && i < 3; ++i) {
     const int n = last_of(wave_scan(len > 0 ? (len - 1) / kLeast / per + 1 : 0));
     if (n <= a.pieces) break;
     per = (int)(((long long)per * n + a.pieces - 1) / a.pieces);
   }
-  int first = 0, slot = 0;
-  for (int b0 = 0; b0 < a.c.B; b0 += 64) {
-    if (a.c.B > 64) len = b0 + lane < a.c.B ? cached_tokens(a.c, b0 + lane) : 0;
-    const int n = b0 + lane < a.c.B ? len > 0 ? (len - 1) / kLeast / per + 1 : 1 : 0, m = n > 1 ? n : 0;
-    const int upto = wave_scan(n), slots = wave_scan(m);
-    const unsigned long long hit = __ballot(first + upto > s);
-    if (hit) {
-      const int f = __builtin_ctzll(hit), nf = __builtin_amdgcn_readlane(n, f);
-      return {b0 + f, s - (first + __builtin_amdgcn_readlane(upto, f) - nf), nf, __builtin_amdgcn_readlane(len, f),
-              slot + __builtin_amdgcn_readlane(slots, f) - __builtin_amdgcn_readlane(m, f)};
-    }
-    first += last_of(upto);
-    slot += last_of(slots);
+  const int n = pieces_of(len, per, lane < a.c.B), m = n > 1 ? n : 0, upto = wave_scan(n), slots = wave_scan(m);
+  const unsigned long long hit = __ballot(upto > s);
+  if (!hit) return Piece{};
+  const int f = __builtin_ctzll(hit), nf = __builtin_amdgcn_readlane(n, f);
+  return {f, s - (__builtin_amdgcn_readlane(upto, f) - nf), nf, __builtin_amdgcn_readlane(len, f),
+          __builtin_amdgcn_readlane(slots, f) - __builtin_amdgcn_readlane(m, f)};
+}
+
+// The same for more than 64 sequences, whose scan each workgroup would repeat: one workgroup writes all pieces into a.map
+// (sequence, piece, pieces of the sequence, its first slot), and zeros behind them.
+constexpr int kPlan = 1024;
+__global__ __launch_bounds__(kPlan) void k_cached_plan(Cached a) {
+  __shared__ long long part[kPlan / 64];
+  __shared__ int sums[2][kPlan / 64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  long long units = 0;
+  for (int b0 = 0; b0 < a.c.B; b0 += kPlan) {
+    const int b = b0 + threadIdx.x, len = b < a.c.B ? cached_tokens(a.c, b) : 0;
+    units += last_of(wave_scan((len + kLeast - 1) / kLeast));   // of the wave's 64
   }
-  return {0, 0, 0, 0, 0};
+  if (lane == 0) part[w] = units;
+  __syncthreads();
+  units = 0;
+#pragma unroll
+  for (int i = 0; i < kPlan / 64; ++i) units += part[i];
+  const int per = max(1, (int)min((units + a.pieces - 1) / a.pieces, 0xffffffLL));
+  int first = 0, slot = 0;
+  for (int b0 = 0; b0 < a.c.B; b0 += kPlan) {
+    const int b = b0 + threadIdx.x, len = b < a.c.B ? cached_tokens(a.c, b) : 0;
+    const int n = pieces_of(len, per, b < a.c.B), m = n > 1 ? n : 0, upto = wave_scan(n), slots = wave_scan(m);
+    if (lane == 63) sums[0][w] = upto, sums[1][w] = slots;
+    __syncthreads();
+    int at = first + upto - n, sl = slot + slots - m;
+#pragma unroll
+    for (int i = 0; i < kPlan / 64; ++i) {
+      at += i < w ? sums[0][i] : 0;
+      sl += i < w ? sums[1][i] : 0;
+      first += sums[0][i];
+      slot += sums[1][i];
+    }
+    for (int i = 0; i < n; ++i) a.map[at + i] = make_int4(b, i, n, sl);
+    __syncthreads();
+  }
+  for (int i = first + threadIdx.x; i < a.pieces + a.c.B; i += kPlan) a.map[i] = make_int4(0, 0, 0, 0);
 }
 
 template <typename T, int DP>
@@ -464,58 +505,63 @@ __global__ __launch_bounds__(kThreads, held(DP, NR)) void k_cached(Cached a) {
   }
 }
 
-// Joins the pieces of a split sequence's row, one workgroup a row: a thread has four values of the head in every 256 / (D / 4)-th
+// Joins the pieces of a split sequence's rows, `share` workgroups a sequence: a thread has four values of the head in every 256 / (D / 4)-th
 // piece, with a running maximum and sum of its own; those are joined in order. One pass: 4 us, the launch and two loads in a
 // row, for 8 to 190 pieces.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_cached_join(Cached a) {
+__global__ __launch_bounds__(kThreads) void k_cached_join(Cached a, int share) {
   __shared__ f32x4 part[kThreads];
   __shared__ float tops[kThreads], sums[kThreads];
-  const int row = blockIdx.x, b = row / (a.c.Hk * a.R), hr = row - b * (a.c.Hk * a.R), hk = hr / a.R, r = hr - hk * a.R;
+  const int b = blockIdx.x / share, first = blockIdx.x - b * share;
   const int2 sp = a.split[b];
   if (sp.x <= 1) return;
   const int D = a.c.D, quads = (D + 3) / 4, groups = kThreads / quads, q = threadIdx.x % quads, gr = threadIdx.x / quads;
-  float top = -INFINITY, sum = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  if (gr < groups) {
+  for (int row = first; row < a.c.Hk * a.R; row += share) {
+    const int hk = row / a.R, r = row - hk * a.R;
+    float top = -INFINITY, sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (gr < groups) {
 #pragma unroll 4
-    for (int i = gr; i < sp.x; i += groups) {
-      const long long at = ((long long)(sp.y + i) * a.c.Hk + hk) * a.R + r;
-      const float2 st = a.stat[at];
-      const float* p = a.part + at * D + 4 * q;
-      f32x4 v;
-      if (D % 4 == 0) {
-        __builtin_memcpy(&v, p, 16);
-      } else {
+      for (int i = gr; i < sp.x; i += groups) {
+        const long long at = ((long long)(sp.y + i) * a.c.Hk + hk) * a.R + r;
+        const float2 st = a.stat[at];
+        const float* p = a.part + at * D + 4 * q;
+        f32x4 v;
+        if (D % 4 == 0) {
+          __builtin_memcpy(&v, p, 16);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = p[min(j, D - 1 - 4 * q)];
+          for (int j = 0; j < 4; ++j) v[j] = p[min(j, D - 1 - 4 * q)];
+        }
+        const float now = fmaxf(top, st.x), base = now == -INFINITY ? 0.f : now;
+        const float by = hw_exp2(top - base), w = hw_exp2(st.x - base);
+        top = now;
+        sum = fmaf(sum, by, st.y * w);
+        o = o * by + v * w;
       }
-      const float now = fmaxf(top, st.x), base = now == -INFINITY ? 0.f : now;
-      const float by = hw_exp2(top - base), w = hw_exp2(st.x - base);
-      top = now;
-      sum = fmaf(sum, by, st.y * w);
-      o = o * by + v * w;
     }
-  }
-  part[threadIdx.x] = o;
-  tops[threadIdx.x] = top;
-  sums[threadIdx.x] = sum;
-  __syncthreads();
-  if (gr != 0) return;
-  for (int i = 1; i < groups; ++i) top = fmaxf(top, tops[i * quads + q]);
-  const float base = top == -INFINITY ? 0.f : top;
-  o = f32x4{0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  for (int i = 0; i < groups; ++i) {
-    const float w = hw_exp2(tops[i * quads + q] - base);
-    sum = fmaf(sums[i * quads + q], w, sum);
-    o += part[i * quads + q] * w;
-  }
-  const int qt = r / a.by_rep, h = hk * a.rep + (r - qt * a.rep);
-  T* to = (T*)a.o + (((long long)b * a.T + qt) * a.H + h) * D + 4 * q;
-  const float by = sum == 0.f ? 0.f : 1.f / sum;
+    part[threadIdx.x] = o;
+    tops[threadIdx.x] = top;
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+    if (gr == 0) {
+      for (int i = 1; i < groups; ++i) top = fmaxf(top, tops[i * quads + q]);
+      const float base = top == -INFINITY ? 0.f : top;
+      o = f32x4{0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+      for (int i = 0; i < groups; ++i) {
+        const float w = hw_exp2(tops[i * quads + q] - base);
+        sum = fmaf(sums[i * quads + q], w, sum);
+        o += part[i * quads + q] * w;
+      }
+      const int qt = r / a.by_rep, h = hk * a.rep + (r - qt * a.rep);
+      T* to = (T*)a.o + (((long long)b * a.T + qt) * a.H + h) * D + 4 * q;
+      const float by = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (4 * q + j < D) to[j] = (T)(sum == 0.f ? 0.f : o[j] * by);
+      for (int j = 0; j < 4; ++j)
+        if (4 * q + j < D) to[j] = (T)(sum == 0.f ? 0.f : o[j] * by);
+    }
+    __syncthreads();
+  }
 }
 
 int check_call(const char* who, const splat_cache* c, const splat_rotation* r, const splat_positions* p, int H, long long T,
@@ -542,14 +588,23 @@ Cached plan(const splat_cache& c, int H, int T) {
   const long long each = (long long)c.Hk * n.tiles, once = std::max(1LL, all / each);
   n.fit = c.B <= 64 && 2 * c.B <= once;
   n.pieces = (int)(n.fit ? once : (kRounds * all + each - 1) / each);
+  n.cut = (long long)c.page * c.width <= kLeast || n.pieces <= 1 ? kWhole : c.B <= 64 ? kScanned : kMapped;
   n.by_rep = fast_div(n.rep);
   n.by_page = fast_div(c.page);
   return n;
 }
 
-// Slots of the pieces of split sequences: those have more than one piece, each more than half as long as the others.
-bool may_split(const Cached& n) { return (long long)n.c.page * n.c.width > kLeast && n.pieces > 1; }
-size_t slots(const Cached& n) { return may_split(n) ? (size_t)2 * n.pieces : 0; }
+// Parts of the workspace: the list of pieces, the sequences' pieces, statistics and rows of the pieces of split sequences, of
+// which there are at most twice as many as aimed at (each sequence has fewer than one more than its tokens would fill).
+struct Bytes {
+  size_t map, split, rows, all;
+};
+Bytes bytes_of(const Cached& n) {
+  if (n.cut == kWhole) return {0, 0, 0, 0};
+  const size_t map = n.cut == kMapped ? sizeof(int4) * ((size_t)n.pieces + n.c.B) : 0, split = sizeof(int2) * n.c.B;
+  const size_t rows = (size_t)2 * n.pieces * n.c.Hk * n.R;
+  return {map, split, rows, map + split + sizeof(float) * rows * (n.c.D + 2)};
+}
 
 template <typename F>
 int with_form(int dtype, int D, int R, F&& f) {
@@ -580,8 +635,7 @@ extern "C" {
 size_t splat_cached_attention_workspace_bytes(const splat_cache* c, int H, long long T) {
   if (check_call("splat_cached_attention_workspace_bytes", c, nullptr, nullptr, H, T, 0.f) || c->B == 0 || T == 0) return 0;
   const Cached n = plan(*c, H, (int)T);
-  const size_t rows = slots(n) * c->Hk * n.R;
-  return rows ? sizeof(float) * rows * (c->D + 2) + sizeof(int2) * c->B : 0;
+  return bytes_of(n).all;
 }
 
 int splat_cached_attention(const splat_cache* c, const splat_rotation* r, const splat_positions* p, const void* q, long long qb,
@@ -595,8 +649,8 @@ int splat_cached_attention(const splat_cache* c, const splat_rotation* r, const 
   const size_t need = splat_cached_attention_workspace_bytes(c, H, T);
   if (need && (!ws || ws_bytes < need))
     return set_error(kWorkspace, "splat_cached_attention: workspace of %zu bytes, %zu needed", ws_bytes, need);
-  const long long grid = ((long long)n.pieces + c->B) * c->Hk * n.tiles;
-  if (grid > 0x7fffffffLL) return set_error(kUnsupported, "splat_cached_attention: %d sequences of %d heads", c->B, H);
+  const long long grid = ((long long)(n.cut == kWhole ? 0 : n.pieces) + c->B) * c->Hk * n.tiles;
+  if (grid > 0xffffffLL) return set_error(kUnsupported, "splat_cached_attention: %d sequences of %d heads", c->B, H);
   if (r) n.r = *r;
   if (p) n.pos = *p;
   n.q = q, n.o = o, n.qb = qb, n.ql = ql, n.qh = qh, n.causal = causal;
@@ -605,16 +659,21 @@ int splat_cached_attention(const splat_cache* c, const splat_rotation* r, const 
   n.by_units = fast_div(n.units);
   n.alike = c->kp == c->vp && c->kt == c->vt;
   if (need) {
-    const size_t rows = slots(n) * c->Hk * n.R;
-    n.split = (int2*)ws;
-    n.stat = (float2*)(n.split + c->B);
-    n.part = (float*)(n.stat + rows);
+    const Bytes at = bytes_of(n);
+    n.map = (int4*)ws;
+    n.split = (int2*)((char*)ws + at.map);
+    n.stat = (float2*)((char*)n.split + at.split);
+    n.part = (float*)(n.stat + at.rows);
   }
   const hipStream_t st = (hipStream_t)stream;
   return with_form(c->dtype, c->D, n.R, [&](auto t, auto dp, auto nr, auto fit) {
     using E = decltype(t);
+    if (n.cut == kMapped) k_cached_plan<<<1, kPlan, 0, st>>>(n);
     k_cached<E, decltype(dp)::value, decltype(nr)::value, decltype(fit)::value><<<(unsigned)grid, kThreads, 0, st>>>(n);
-    if (need) k_cached_join<E><<<(unsigned)(c->B * c->Hk * n.R), kThreads, 0, st>>>(n);
+    if (need) {   // a workgroup a row for few sequences; of many, the most are not split
+      const int share = std::max(1, std::min(c->Hk * n.R, 16384 / c->B));
+      k_cached_join<E><<<(unsigned)(c->B * share), kThreads, 0, st>>>(n, share);
+    }
     return check_launch("splat_cached_attention");
   });
 }

@@ -177,11 +177,11 @@ __global__ __launch_bounds__(kThreads) void k_rotary_bwd(Turn n, const T* __rest
 // dpos[l, a] = sum over the images of part[b, l, a], in their order.
 __global__ __launch_bounds__(kThreads) void k_rotary_join(const float* __restrict__ part, float* __restrict__ dpos, int B,
                                                           long long n) {
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= n) return;
-  float t = 0.f;
-  for (int b = 0; b < B; ++b) t += part[b * n + i];
-  dpos[i] = t;
+  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kThreads) {
+    float t = 0.f;
+    for (int b = 0; b < B; ++b) t += part[b * n + i];
+    dpos[i] = t;
+  }
 }
 
 struct Append {
@@ -348,7 +348,7 @@ int splat_rotary_bwd(const splat_rotation* r, const splat_positions* p, const vo
     k_rotary_bwd<T, W, HB><<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const T*)x, (const T*)g, (T*)dx, each);
     if (need) {
       const long long m = L * r->axes;
-      k_rotary_join<<<(unsigned)div_up(m, kThreads), kThreads, 0, (hipStream_t)stream>>>(each, dpos, B, m);
+      k_rotary_join<<<(unsigned)std::min(kGrid, div_up(m, kThreads)), kThreads, 0, (hipStream_t)stream>>>(each, dpos, B, m);
     }
     return check_launch("splat_rotary_bwd");
   });

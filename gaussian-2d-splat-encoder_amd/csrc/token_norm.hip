@@ -460,29 +460,33 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
 // Adds the workgroups' column sums in a fixed order: 64 columns a workgroup, its waves each a part of the sums. Entries 0 to 3
 // are the parameters' gradients, the others the gate's rows.
 constexpr int kJoin = 1024;
-__global__ __launch_bounds__(kJoin) void k_token_norm_join(TokenNorm a, int wgs, int tiles, float* dw1, float* db1, float* dw2,
+__global__ __launch_bounds__(kJoin) void k_token_norm_join(TokenNorm a, int wgs, int tiles, long long units, float* dw1, float* db1, float* dw2,
                                                            float* db2, float* dgate) {
   __shared__ float part[kJoin / 64][64];
-  const int e = blockIdx.x / tiles, c = (blockIdx.x - e * tiles) * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  const long long seg = e - 4;
-  float* out = e == 0 ? dw1 : e == 1 ? db1 : e == 2 ? dw2 : e == 3 ? db2 : dgate + seg * a.a.C;
-  if (e < 4 && !out) return;
-  const long long step = e < 4 ? 4LL * a.a.C : a.a.C;
-  const float* p = e < 4 ? a.cols + (long long)e * a.a.C : a.gates + seg * a.splits * a.a.C;
-  const int n = e < 4 ? wgs : a.splits;
-  float s = 0.f;
-  if (c < a.a.C) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const long long e = unit / tiles, seg = e - 4;
+    const int c = (int)(unit - e * tiles) * 64 + lane;
+    float* out = e == 0 ? dw1 : e == 1 ? db1 : e == 2 ? dw2 : e == 3 ? db2 : dgate + seg * a.a.C;
+    if (e < 4 && !out) continue;
+    const long long step = e < 4 ? 4LL * a.a.C : a.a.C;
+    const float* p = e < 4 ? a.cols + e * a.a.C : a.gates + seg * a.splits * a.a.C;
+    const int n = e < 4 ? wgs : a.splits;
+    float s = 0.f;
+    if (c < a.a.C) {
 #pragma unroll 4
-    for (int i = w; i < n; i += kJoin / 64) s += p[i * step + c];
-  }
-  part[w][threadIdx.x & 63] = s;
-  __syncthreads();
-  if (w == 0 && c < a.a.C) {
-    float t = 0.f;
+      for (int i = w; i < n; i += kJoin / 64) s += p[i * step + c];
+    }
+    part[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && c < a.a.C) {
+      float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < kJoin / 64; ++i) t += part[i][threadIdx.x & 63];
-    if (e >= 4) t *= a.a.scale * gate_grad(a.a.act, ((const float*)a.gate)[seg * a.a.C + c]);
-    out[c] = t;
+      for (int i = 0; i < kJoin / 64; ++i) t += part[i][lane];
+      if (e >= 4) t *= a.a.scale * gate_grad(a.a.act, ((const float*)a.gate)[seg * a.a.C + c]);
+      out[c] = t;
+    }
+    __syncthreads();
   }
 }
 
@@ -620,8 +624,9 @@ int splat_token_norm_bwd(const splat_token_norm* a, const void* x, const void* h
     k_token_norm_bwd<decltype(t), TPR, decltype(k)::value, decltype(whole)::value, decltype(lean)::value><<<grid, kBlock<TPR>, 0, st>>>(p);
     if (need) {
       const int tiles = div_up(a->C, 64);
-      k_token_norm_join<<<tiles * (4 + (gates ? p.segs : 0)), kJoin, 0, st>>>(p, (int)grid, tiles, dw1, db1, dw2, db2,
-                                                                              gates ? (float*)dgate : nullptr);
+      const long long units = (long long)tiles * (4 + (gates ? p.segs : 0));
+      k_token_norm_join<<<(unsigned)std::min(units, 1LL << 20), kJoin, 0, st>>>(p, (int)grid, tiles, units, dw1, db1, dw2, db2,
+                                                                                gates ? (float*)dgate : nullptr);
     }
     return check_launch("splat_token_norm_bwd");
   });

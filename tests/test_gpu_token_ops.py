@@ -278,7 +278,8 @@ def test_attention_of_long_and_many_sequences(dt, B, n, T, H, Hk):
     width = -(-n // page)
     c = make_cache(max(8, B * width // 16), page, Hk, D, dt)
     tables = randint(0, c.pages, (B, width), 3)              # pages may be shared where they are only read
-    lengths = torch.tensor([n if i % 7 == 0 else (i * 37) % (n // 3) for i in range(B)], device="cuda")
+    lengths = torch.tensor([n if i % (7 if B < 1000 else 301) == 0 else (i * 37) % (n // 3) if B < 1000 else i % 140
+                            for i in range(B)], device="cuda")
     check_attention(rand(B, T, H, D, dt=dt, seed=1, scale=1.5), c, tables, lengths)
 
 
@@ -618,6 +619,27 @@ def test_norm_gradients_against_differences():
     ana = sum((p.double() * d.double()).sum().item() for p, d in zip(torch.autograd.grad(run(a), a, g), dirs))
     third = abs(f(3 * t) - 3 * f(t) + 3 * f(-t) - f(-3 * t)) / (8 * t ** 3) * t * t / 6
     assert abs(num - ana) <= 3e-4 * math.sqrt(2 * 6 * C) + 2 * third
+
+
+def test_rows_past_2_31_values():
+    """Tensors of more than 2^31 values whose last rows are compared: their own values, and gradients."""
+    n, C = 8_600_000, 256
+    x = torch.empty(n, C, dtype=torch.bfloat16, device="cuda")
+    x.view(-1, 1000 * C).copy_(rand(1000 * C, dt=torch.bfloat16))
+    x[-3:] = rand(3, C, dt=torch.bfloat16, seed=1)
+    w, gate = rand(C, seed=2, shift=1.0), rand(C, seed=3)
+    y, m = F.residual_norm(x, x, w, gate=gate, next_weight=w)
+    a, b = F.residual_norm(x[-3:], x[-3:], w, gate=gate, next_weight=w)
+    assert torch.equal(y[-3:], a) and torch.equal(m[-3:], b)
+    xs, = torch.autograd.grad(F.token_norm(x.requires_grad_(True), w), x, x.detach())
+    part = x[-3:].detach().requires_grad_(True)
+    assert torch.equal(xs[-3:], torch.autograd.grad(F.token_norm(part, w), part, part.detach())[0])
+    del xs, y, m
+    x = x.detach()
+    pos = torch.arange(n, device="cuda", dtype=torch.int32)[:, None]
+    ax = F.RotaryAxes((64,))
+    r = F.rotary(x.view(1, n, 4, 64), pos, ax)
+    assert torch.equal(r[0, -3:], F.rotary(x[-3:].view(1, 3, 4, 64), pos[-3:], ax)[0])
 
 
 def test_a_captured_training_step():

@@ -197,6 +197,8 @@ def test_attention_workspaces_are_bounded():
     assert ask() == 0            # 128 tokens at most: no split
     c.width = 512
     # two slots a piece, of four rows a key head with their two statistics; at most four rounds of 512 workgroups
-    assert 0 < ask() <= 2 * (4 * 512 // 8 + 1) * 8 * 4 * (128 + 2) * 4 + 8
-    c.B = 4096                            # two numbers a sequence besides
-    assert 0 < ask() <= 2 * (4 * 512 // 8 + 1) * 8 * 4 * (128 + 2) * 4 + 8 * 4096
+    pieces = 4 * 512 // 8
+    rows = 2 * pieces * 8 * 4 * (128 + 2) * 4
+    assert 0 < ask() <= rows + 8
+    c.B = 4096                            # two numbers a sequence and a list of pieces besides
+    assert 0 < ask() <= rows + 8 * 4096 + 16 * (pieces + 4096)
