@@ -58,8 +58,8 @@ __device__ __forceinline__ float lanes_add(float v) {
   return v;
 }
 
-// Sums of N values over a row's threads. Rows of more than a wave exchange through LDS: two buffers in turn, so that one
-// barrier a sum does.
+// Sums of N values over a row's threads. Rows of more than a wave exchange through LDS (all threads of the workgroup take part):
+// two buffers in turn, so that one barrier a sum does.
 template <int TPR, int N>
 struct RowSum {
   float (*red)[2][N][16];
@@ -78,7 +78,7 @@ struct RowSum {
       for (int i = 0; i < N; ++i) {
         float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < TPR / 64; ++k) s += (*red)[flip][i][k];
+        for (int k = 0; k < TPR / 64; ++k) s += (*red)[flip][i][w / (TPR / 64) * (TPR / 64) + k];
         v[i] = s;
       }
       flip ^= 1;
@@ -117,11 +117,11 @@ __device__ __forceinline__ void load_raw(const T* p, const Cols<T, TPR, K>& at, 
 }
 // Their values, zeros past C.
 template <bool Whole, typename T, int TPR, int K>
-__device__ __forceinline__ void values(const Raw<T, K>& c, const Cols<T, TPR, K>& at, Vals<T, K>& f) {
+__device__ __forceinline__ void values(const Raw<T, K>& c, const Cols<T, TPR, K>& at, Vals<T, K>& f, bool in = true) {
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int j = 0; j < kV<T>; ++j) f[k][j] = !Whole || at.nv[k] ? (float)c[k].v[j] : 0.f;
+    for (int j = 0; j < kV<T>; ++j) f[k][j] = in && (!Whole || at.nv[k]) ? (float)c[k].v[j] : 0.f;
 }
 template <typename T, int TPR, int K>
 __device__ __forceinline__ void store_row(T* p, const Cols<T, TPR, K>& at, const Vals<T, K>& f) {
@@ -212,8 +212,9 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm(TokenNorm a) {
     load_params(a.a.next ? a.b2 : nullptr, at, 0.f, b2);
   }
   segments(a, [&](long long row0, int seg, int split) {
-    const long long rows = a.seg, r = split * RB + threadIdx.x / TPR;
-    if (r >= rows) return;
+    const long long rows = a.seg, r0 = split * RB;
+    const int r = threadIdx.x / TPR;
+    if (r0 >= rows) return;
     Raw<T, K> rx, rh, rg;
     auto fetch = [&](long long i) {
       const long long row = row0 + min(i, rows - 1);
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm(TokenNorm a) {
       if (block) load_raw<Whole>((const T*)a.h + row * a.a.hl, at, rh);
       if (token) load_raw<Whole>((const T*)a.gate + row * a.a.gl, at, rg);
     };
-    fetch(r);
+    fetch(r0 + r);
     if (!token && block) {
       load_params(a.a.gate ? (const float*)a.gate + (long long)seg * a.a.C : nullptr, at, 1.f, gs);
 #pragma unroll
@@ -229,8 +230,9 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm(TokenNorm a) {
 #pragma unroll
         for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * (a.a.gate ? gate_of(a.a.act, gs[k][j]) : 1.f);
     }
-    for (long long i = r; i < rows; i += a.step) {
-      const long long row = row0 + i;
+    for (long long i = r0; i < rows; i += a.step) {
+      const bool in = RB == 1 || i + r < rows;
+      const long long row = row0 + i + r;
       Vals<T, K> x, h;
       values<Whole>(rx, at, x);
       if (block) values<Whole>(rh, at, h);
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm(TokenNorm a) {
 #pragma unroll
           for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * gate_of(a.a.act, gs[k][j]);
       }
-      fetch(i + a.step);
+      fetch(i + r + a.step);
       float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
       if (block) {
         if (a.a.post) {
@@ -259,7 +261,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm(TokenNorm a) {
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int j = 0; j < kV<T>; ++j) x[k][j] = j < at.nv[k] ? fmaf(gs[k][j], h[k][j], x[k][j]) : 0.f;
-        store_row((T*)a.y + row * a.a.C, at, x);
+        if (in) store_row((T*)a.y + row * a.a.C, at, x);
       }
       if (a.a.next) {
         const float2 s = row_stats<Lean>(a, at, x, sum);
@@ -271,9 +273,9 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm(TokenNorm a) {
             const float v = (Lean ? x[k][j] : x[k][j] - s.x) * s.y;
             x[k][j] = Lean ? v * w2[k][j] : fmaf(v, w2[k][j], b2[k][j]);
           }
-        store_row((T*)a.n + row * a.a.C, at, x);
+        if (in) store_row((T*)a.n + row * a.a.C, at, x);
       }
-      if (a.stat && (threadIdx.x & (TPR - 1)) == 0) a.stat[row] = st;
+      if (a.stat && in && (threadIdx.x & (TPR - 1)) == 0) a.stat[row] = st;
     }
   });
 }
@@ -340,7 +342,8 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
     }
   };
   segments(a, [&](long long row0, int seg, int split) {
-    const long long rows = a.seg, r = split * RB + threadIdx.x / TPR;
+    const long long rows = a.seg, r0 = split * RB;
+    const int r = threadIdx.x / TPR;
     Raw<T, K> rx, rh, rg, ry, rn;
     float4 rs;
     auto fetch = [&](long long i) {
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
       if (a.dn) load_raw<Whole>((const T*)a.dn + row * a.a.dnl, at, rn);
       rs = a.stat[row];
     };
-    if (r < rows) fetch(r);
+    if (r0 < rows) fetch(r0 + r);
     if (!token && block) {
       load_params(a.a.gate ? (const float*)a.gate + (long long)seg * a.a.C : nullptr, at, 1.f, gs);
 #pragma unroll
@@ -360,13 +363,14 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
 #pragma unroll
         for (int j = 0; j < kV<T>; ++j) gs[k][j] = a.a.scale * (a.a.gate ? gate_of(a.a.act, gs[k][j]) : 1.f);
     }
-    for (long long i = r; i < rows; i += a.step) {
-      const long long row = row0 + i;
+    for (long long i = r0; i < rows; i += a.step) {
+      const bool in = RB == 1 || i + r < rows;   // rows past the last one count as the last one without gradients
+      const long long row = row0 + i + r;
       Vals<T, K> x, h, g, d, up;   // y, then v; u; the gate's slope; dn, then dy', then dh
       values<Whole>(rx, at, x);
       if (block) values<Whole>(rh, at, h);
-      if (a.dy) values<Whole>(ry, at, up);
-      if (a.dn) values<Whole>(rn, at, d);
+      if (a.dy) values<Whole>(ry, at, up, in);
+      if (a.dn) values<Whole>(rn, at, d, in);
       const float4 st = rs;
       if (token) {
         values<Whole>(rg, at, g);
@@ -378,7 +382,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
             g[k][j] = a.a.scale * gate_grad(a.a.act, g[k][j]);
           }
       }
-      fetch(i + a.step);
+      fetch(i + r + a.step);
       if (block) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -414,7 +418,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
 #pragma unroll
           for (int j = 0; j < kV<T>; ++j) d[k][j] = up[k][j];
       }
-      if (a.dx) store_row((T*)a.dx + row * a.a.C, at, d);
+      if (a.dx && in) store_row((T*)a.dx + row * a.a.C, at, d);
       if (!block) continue;
 #pragma unroll
       for (int k = 0; k < K; ++k)
@@ -427,7 +431,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
           aw1[k][j] = fmaf(dz, h[k][j], aw1[k][j]);
           d[k][j] = dz * w1[k][j];
         }
-      if (token && a.dgate) store_row((T*)a.dgate + row * a.a.C, at, g);
+      if (token && a.dgate && in) store_row((T*)a.dgate + row * a.a.C, at, g);
       if (a.a.post) {
         float m, q;
         both(d, h, m, q);
@@ -436,7 +440,7 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
 #pragma unroll
           for (int j = 0; j < kV<T>; ++j) d[k][j] = st.y * fmaf(-h[k][j], q, Lean ? d[k][j] : d[k][j] - m);
       }
-      if (a.dh) store_row((T*)a.dh + row * a.a.C, at, d);
+      if (a.dh && in) store_row((T*)a.dh + row * a.a.C, at, d);
     }
     if (a.gates) {
       fold_rows(ag, at, lds, a.gates + ((long long)seg * a.splits + split) * a.a.C);
@@ -490,17 +494,21 @@ __global__ __launch_bounds__(kJoin) void k_token_norm_join(TokenNorm a, int wgs,
   }
 }
 
+// At most 8 values a lane. Rows of 65 to 128 chunks: of floats two chunks in each lane of a wave (73,728 x 300 in training 106 us,
+// one in each of two waves 118), of bf16 one in each of two waves (18,432 x 1,024 94 us, two a lane 112); 4,096 bf16 values one
+// in each of eight waves (102 us, two in each of four 117); 517 floats one in each of four waves (57 us, three a lane 65).
 struct Shape {
   int tpr, k, rows;   // threads of a row; chunks of a thread; rows of a workgroup at a time
   bool whole, lean;
 };
 Shape shape_of(const splat_token_norm& a, bool biases) {
-  const int V = a.dtype == kF32 ? 4 : 8, chunks = div_up(a.C, V);
+  const bool f32 = a.dtype == kF32, whole = a.C % (f32 ? 4 : 8) == 0;
+  const int chunks = div_up(a.C, f32 ? 4 : 8);
   int tpr = 4;
-  while (tpr < 64 && tpr < chunks) tpr *= 2;
-  if (chunks > 128) tpr = chunks > 512 ? 1024 : 256;
-  const bool whole = a.C % V == 0;
-  return {tpr, chunks > tpr ? 2 : 1, std::max(1, 256 / tpr), whole, whole && !a.layer && !biases};
+  while (tpr < (f32 ? 64 : 512) && tpr < chunks) tpr *= 2;
+  if (f32 && chunks > 128) tpr = 256;
+  if (chunks > 512) tpr = 1024;
+  return {tpr, div_up(chunks, tpr), std::max(1, 256 / tpr), whole, whole && !a.layer && !biases};
 }
 
 template <typename F>
@@ -512,20 +520,26 @@ int with_shape(int dtype, const Shape& s, F&& f) {
     return f(t, tpr, k, std::false_type{}, std::false_type{});
   };
   auto type = [&](auto t) {
-    auto k = [&](auto tpr) {
-      return s.k == 2 ? kind(t, tpr, integral_constant<int, 2>{}) : kind(t, tpr, integral_constant<int, 1>{});
-    };
+    constexpr bool f32 = sizeof(t) == 4;
     auto one = [&](auto tpr) { return kind(t, tpr, integral_constant<int, 1>{}); };
+    auto two = [&](auto tpr) {   // chunks of floats
+      if constexpr (f32)
+        if (s.k == 2) return kind(t, tpr, integral_constant<int, 2>{});
+      return one(tpr);
+    };
     switch (s.tpr) {
       case 4: return one(integral_constant<int, 4>{});
       case 8: return one(integral_constant<int, 8>{});
       case 16: return one(integral_constant<int, 16>{});
       case 32: return one(integral_constant<int, 32>{});
-      case 64: return k(integral_constant<int, 64>{});
-      case 256: return k(integral_constant<int, 256>{});
+      case 64: return two(integral_constant<int, 64>{});
+      case 256: return two(integral_constant<int, 256>{});
     }
-    if constexpr (sizeof(t) == 4) return k(integral_constant<int, 1024>{});
-    else return one(integral_constant<int, 1024>{});
+    if constexpr (!f32) {
+      if (s.tpr == 128) return one(integral_constant<int, 128>{});
+      if (s.tpr == 512) return one(integral_constant<int, 512>{});
+    }
+    return two(integral_constant<int, 1024>{});
   };
   return dtype == kF32 ? type(float{}) : type(bf16{});
 }
@@ -556,11 +570,11 @@ unsigned plan(TokenNorm& n, const Shape& s, long long target) {
   return (unsigned)((n.segs + n.whole - 1) / n.whole * n.splits);
 }
 
-// Workgroups aimed at: what the card holds at once, by the registers of a lane (four, and in the backward three, two or one
-// waves a SIMD for 4, 8 or 16 values a lane). Backward of 73,728 x 256 bf16, with its join: 512 workgroups 55 us, 768 69, 1,024
+// Workgroups aimed at: what the card holds at once, by the registers of a lane (four waves a SIMD; in the backward three or two for
+// 4 or 8 values a lane, four of 1,024 threads, whose registers spill). Backward of 73,728 x 256 bf16, with its join: 512 workgroups 55 us, 768 69, 1,024
 // 60; of 5,001 x 517 floats 768 39 us, 512 45, 1,024 50.
 long long resident(const Shape& s, int dtype, bool back) {
-  const int values = s.k * (dtype == kF32 ? 4 : 8), waves = !back ? 4 : values == 4 ? 3 : values == 8 ? 2 : 1;
+  const int values = s.k * (dtype == kF32 ? 4 : 8), waves = !back || s.tpr == 1024 ? 4 : values == 4 ? 3 : 2;
   return 256LL * waves * 4 * 64 / std::max(256, s.tpr);
 }
 
