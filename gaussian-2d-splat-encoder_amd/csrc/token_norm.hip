@@ -11,9 +11,13 @@
 //   dw2 = sum dn v, db2 = sum dn, dw1 = sum dz u, db1 = sum dz over the tokens
 //
 // A row is held by TPR threads, K 16-byte chunks each, in registers; it is read once, and its sums are exchanged within a wave
-// (TPR <= 64) or through LDS. A workgroup takes a range of rows with the parameters' columns in registers. The backward reads x
+// (TPR <= 64) or through LDS. A workgroup takes rows a step apart with the parameters' columns in registers. The backward reads x
 // and h again (y's rounding would show in the parameters' float32 gradients) with the rows' statistics kept by the forward, and
 // sums columns in registers over its rows, whose partial sums a second kernel adds in order.
+//
+// Bound by memory: 73,728 x 256 bf16 with a gate of each image's (a large copy moves 4.9 TB/s here) forward 38 us (151 MB, 4.0
+// TB/s), backward 52 (227 MB, 4.4 TB/s), the join of 512 partial sums 5, the launch and two rounds of loads. (Stores that pass the
+// caches by take 4 us off the forward alone, and cost the product that reads its result 7.)
 #include <algorithm>
 
 #include "feat_common.h"
@@ -102,26 +106,47 @@ struct Cols {
 template <typename T, int K>
 using Vals = float[K][kV<T>];
 
-// A row's chunks as they lie in memory. Whole: C is whole chunks, and the lanes past it load the first one, so that no load has
-// a condition of its own and the next row's are under way while this one is worked on.
+// A row's chunks as they lie in memory. Lanes past C load the first chunk, and where C is not whole chunks (!Whole) the lane of
+// the last ones loads the row's last 16 bytes, so that no load has a condition of its own and the next row's are under way
+// while this one is worked on (60,033 x 333 bf16 in training: 203 us with conditions, 169 without).
 template <typename T, int K>
 using Raw = Chunk<T>[K];
 
 template <bool Whole, typename T, int TPR, int K>
 __device__ __forceinline__ void load_raw(const T* p, const Cols<T, TPR, K>& at, Raw<T, K>& f) {
+  constexpr int V = kV<T>;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    if (Whole) __builtin_memcpy(f[k].v, p + (at.nv[k] ? at.c[k] : 0), 16);
-    else f[k] = load_chunk(p + at.c[k], at.nv[k]);
+    if (!Whole && TPR == 4 && at.C < V) f[k] = load_chunk(p, at.nv[k]);
+    else __builtin_memcpy(f[k].v, p + (at.nv[k] == V ? at.c[k] : Whole || at.nv[k] == 0 ? 0 : at.C - V), 16);
   }
 }
-// Their values, zeros past C.
+// Their values, zeros past C (and everywhere unless `in`).
 template <bool Whole, typename T, int TPR, int K>
 __device__ __forceinline__ void values(const Raw<T, K>& c, const Cols<T, TPR, K>& at, Vals<T, K>& f, bool in = true) {
+  constexpr int V = kV<T>;
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int k = 0; k < K; ++k) {
 #pragma unroll
-    for (int j = 0; j < kV<T>; ++j) f[k][j] = in && (!Whole || at.nv[k]) ? (float)c[k].v[j] : 0.f;
+    for (int j = 0; j < V; ++j) f[k][j] = (float)c[k].v[j];
+    if (!Whole) {   // the lane of the last values: they end its chunk
+      float t[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) t[j] = f[k][j];
+      const int up = TPR == 4 && at.C < V ? 0 : (V - at.C % V) % V;
+#pragma unroll
+      for (int s = 1; s < V; s *= 2) {
+        if (up & s) {
+#pragma unroll
+          for (int j = 0; j + s < V; ++j) t[j] = t[j + s];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[k][j] = at.nv[k] == V ? f[k][j] : j < at.nv[k] ? t[j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[k][j] = in && (!Whole || at.nv[k]) ? f[k][j] : 0.f;
+  }
 }
 template <typename T, int TPR, int K>
 __device__ __forceinline__ void store_row(T* p, const Cols<T, TPR, K>& at, const Vals<T, K>& f) {

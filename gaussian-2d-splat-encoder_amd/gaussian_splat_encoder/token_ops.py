@@ -4,7 +4,8 @@ a paged cache of keys and values with the attention that reads it, norms per tok
 They stand beside feature_ops and follow it: float32 or bfloat16 on a HIP device, the last dimension dense (anything else is
 copied first), sums and softmax statistics in float32, fixed orders of summation, the current stream, no waits. rotary,
 residual_norm and token_norm have gradients (reverse-mode, of first order); the cache is for inference and refuses inputs that
-require one. The reference has no counterpart.
+require one. All may be captured into a graph (a backward pass only while no eager graph of the same leaves is alive: torch's
+engine would wait for the eager one's stream). The reference has no counterpart.
 """
 
 from __future__ import annotations
@@ -239,7 +240,8 @@ def cache_append(cache, tables, lengths, k, v, counts=None, positions=None, axes
 
 def cached_attention(q, cache, tables, lengths, counts=None, positions=None, axes=None, causal=True, scale=None):
     """Attention of new tokens' queries q [B, T, H, D] over their sequences' cached tokens -> [B, T, H, D]. H is a multiple of the
-    cache's heads (each serves H / Hk neighbouring query heads); meant for one to some tens of new tokens.
+    cache's heads (each serves H / Hk neighbouring query heads). Meant for one to some tens of new tokens: any number is right, but
+    hundreds run at a fraction of cross_attention's rate.
 
     tables, lengths, counts as in cache_append: the queries are the last counts[b] tokens that lengths[b] counts. causal: query t
     sees the tokens up to its own place, lengths[b] - counts[b] + t; otherwise all. Tokens that the cache's `live` marks
