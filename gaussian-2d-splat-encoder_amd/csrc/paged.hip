@@ -325,7 +325,8 @@ __global__ __launch_bounds__(kThreads, held(DP, NR)) void k_cached(Cached a) {
   const bool fine = sizeof(T) == 2 && a.r.axes > 0;
   Chunk<T> qf[NR][F::nc], ql[NR][F::nc];
   int lim[NR], own[NR];   // tokens that the lane's row sees; its query
-  auto seen_by = [&](int q) { return q >= fresh ? 0 : a.causal ? max(0, len - (fresh - 1 - q)) : len; };
+  const int all = max(0, a.c.lengths[b]);   // with those that the table has no room for: a query's place goes by them
+  auto seen_by = [&](int q) { return q >= fresh ? 0 : a.causal ? min(len, max(0, all - (fresh - 1 - q))) : len; };
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
 #pragma unroll

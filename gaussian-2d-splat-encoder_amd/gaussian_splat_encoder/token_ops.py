@@ -48,7 +48,9 @@ class RotaryAxes:
                  for i in range(d // 2)]
         self._c = SplatRotation(len(self.dims), int(self.interleaved), (ctypes.c_int * 4)(*self.dims),
                                 (ctypes.c_double * 64)(*rates))
-        self._ref = ctypes.byref(self._c)
+
+    def __reduce__(self):
+        return type(self), (self.dims, self.base, self.scale, self.interleaved)
 
     def _each(self, name, v):
         v = tuple(float(x) for x in v) if isinstance(v, (tuple, list)) else (float(v),) * len(self.dims)
@@ -91,7 +93,7 @@ def _turn(x, p, axes, dt, back):
     if y.numel():
         B, L, H, D = x.shape
         sb, sl, sh, _ = x.stride()
-        _launch(x, "splat_rotary", axes._ref, p, x.data_ptr(), sb, sl, sh, dt, B, L, H, D, back, y.data_ptr())
+        _launch(x, "splat_rotary", axes._c, p, x.data_ptr(), sb, sl, sh, dt, B, L, H, D, back, y.data_ptr())
     return y
 
 
@@ -121,7 +123,7 @@ class _Rotary(torch.autograd.Function):
         if dx.numel():
             n = _lib.load().splat_rotary_bwd_workspace_bytes(B, L, len(axes.dims), shared)
             keep, ws = _scratch(n, x)
-            _launch(x, "splat_rotary_bwd", axes._ref, p, x.data_ptr(), *x.stride()[:3], g.data_ptr(), *g.stride()[:3], dt, B,
+            _launch(x, "splat_rotary_bwd", axes._c, p, x.data_ptr(), *x.stride()[:3], g.data_ptr(), *g.stride()[:3], dt, B,
                     L, H, D, dx.data_ptr(), dp.data_ptr(), shared, ws, n)
         return dx if ctx.needs_input_grad[0] else None, dp, None, None, None
 
@@ -130,8 +132,8 @@ def rotary(x, positions, axes):
     """Turns the pairs of x's heads by their tokens' positions: x [B, L, H, D] (heads may be views) -> the same shape and type.
 
     positions [B, L, axes], or [L, axes] and [1, L, axes] for all images: float32 (splat centres; they have a gradient, summed
-    over the images that share them), int32 or int64. axes: RotaryAxes. Angles are taken in 64 bits: positions up to 2^31
-    keep theirs to 1e-6 of a turn."""
+    over the images that share them), int32 or int64. axes: RotaryAxes. Angles are taken in 64 bits: up to 2^31
+    radians they are right to 1e-6."""
     dt, _ = _args("none", x)
     shape = x.shape
     if len(shape) != 4 or not 1 <= shape[3] <= MAX_HEAD or shape[2] < 1:
@@ -231,7 +233,7 @@ def cache_append(cache, tables, lengths, k, v, counts=None, positions=None, axes
     c, keep = cache._describe(tables, lengths, counts, B, T)
     p = r = None
     if axes is not None:
-        p, r = _positions(positions, axes, B, T, cache.head_dim, k), axes._ref
+        p, r = _positions(positions, axes, B, T, cache.head_dim, k), axes._c
     if B and T and cache.pages and c.width:
         k, v = _dense(k), _dense(v)
         _launch(k, "splat_cache_append", c, r, p, k.data_ptr(), *k.stride()[:3], v.data_ptr(),
@@ -257,7 +259,7 @@ def cached_attention(q, cache, tables, lengths, counts=None, positions=None, axe
     c, keep = cache._describe(tables, lengths, counts, B, T)
     p = r = None
     if axes is not None:
-        p, r = _positions(positions, axes, B, T, D, q), axes._ref
+        p, r = _positions(positions, axes, B, T, D, q), axes._c
     o = _like(q)
     if o.numel():
         q = _dense(q)

@@ -65,7 +65,7 @@ def attention(q, kc, vc, live, tables, lengths, counts, causal, scale):
         j, p, at = j[ok], p[ok], at[ok]
         k, v = kc[p, at].double(), vc[p, at].double()            # [keys, Hk, D]
         for t in range(c):
-            see = j < n - (c - 1 - t) if causal else j >= 0
+            see = j < max(0, int(lengths[b])) - (c - 1 - t) if causal else j >= 0
             if not bool(see.any()):
                 continue
             kt, vt = k[see].repeat_interleave(rep, 1), v[see].repeat_interleave(rep, 1)

@@ -316,6 +316,16 @@ def test_what_is_left_out_has_no_effect(dt):
         c.k.copy_(k), c.v.copy_(v)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+def test_lengths_past_the_table(dt):
+    """A query's place goes by its sequence's length, also where the table has no room for all of it."""
+    c = make_cache(20, 16, 2, 64, dt)
+    tables = make_tables(4, 5, 20)
+    lengths = torch.tensor([80, 83, 90, 2 ** 31 - 1], device="cuda", dtype=torch.int32)
+    check_attention(rand(4, 9, 4, 64, dt=dt, seed=1), c, tables, lengths)
+    check_attention(rand(4, 9, 4, 64, dt=dt, seed=1), c, tables, lengths, counts=torch.tensor([9, 5, 9, 2], device="cuda"))
+
+
 def test_attention_of_nothing():
     c = F.PagedCache.empty(4, 8, 2, 16)
     q = rand(3, 2, 4, 16, dt=torch.bfloat16)

@@ -123,6 +123,16 @@ def test_rates():
     assert got[:3] == pytest.approx([2 / math.pi, 2 / math.pi / 10, 6 / math.pi], rel=1e-15) and not any(got[3:])
 
 
+def test_axes_are_copied_and_stored_with_their_module():
+    import copy
+    import pickle
+
+    from gaussian_splat_encoder.token_reader import TokenReader
+    a = F.RotaryAxes((8, 4), base=(100.0, 7.0), scale=(1.0, 3.0), interleaved=True)
+    for b in (copy.deepcopy(a), pickle.loads(pickle.dumps(a)), copy.deepcopy(TokenReader(48, 8, a)).axes):
+        assert bytes(b._c) == bytes(a._c) and repr(b) == repr(a)
+
+
 def test_c_entry_points_refuse_before_any_launch():
     lib = _lib.load()
     ref = ctypes.byref
