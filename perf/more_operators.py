@@ -330,8 +330,9 @@ def _plain(s, c):
         k = s["k"].float()
         k = _turned(k, s["positions"], c).to(dt) if c["dims"] else s["k"]
         slot = (lens - counts)[:, None] + t
-        page = s["tables"].long().gather(1, slot.clamp_min(0) // P)
-        where, new = (page, slot.clamp_min(0) % P), (k, s["v"], s["key_mask"])
+        at = slot.clamp(0, s["tables"].shape[1] * P - 1)     # tokens past their count may lie behind the table
+        page = s["tables"].long().gather(1, at // P)
+        where, new = (page, at % P), (k, s["v"], s["key_mask"])
         if c["ragged"]:
             ok = (t < counts[:, None]) & (slot >= 0)
             where, new = (page[ok], where[1][ok]), [None if x is None else x[ok] for x in new]
