@@ -15,10 +15,10 @@
 // Tokens past the length or marked dead are not read and count as zeros. Tokens after a causal query have probability zero; a
 // tile whose values there are not finite is multiplied query by query with those values as zeros.
 //
-// Measured: one token in each of sixteen sequences of 0 to 32,768 tokens, 32 heads over 8 of 128 bf16 (1.06 GB) 187 us, 5.7 TB/s;
-// one token over 368,640, of which 60% count, 4 heads of 64 bf16 (226 MB) 49 us, 4.6 TB/s, with a join of 190 pieces 5; one over 900
-// tokens 7.7 us, six loads behind each other, and a join of 4. Many rows are not what this is for: 1,024 tokens of 32 heads over
-// 8,192 take 683 us (190 TFLOP/s), rows of 32 a workgroup and two products for one.
+// Measured: one token in each of sixteen sequences of 0 to 32,768 tokens, 32 heads over 8 of 128 bf16 (1.06 GB) 187 us, 5.7
+// TB/s; one token over 368,640, of which 60% count, 4 heads of 64 bf16 (226 MB) 49 us, 4.6 TB/s, with a join of 190 pieces 5;
+// one over 900 tokens 7.7 us, six loads behind each other, and a join of 4. Many rows are not what this is for: 1,024 tokens of
+// 32 heads over 8,192 take 683 us (190 TFLOP/s), rows of 32 a workgroup and two products for one.
 #include <algorithm>
 
 #include "token_common.h"
@@ -511,9 +511,9 @@ __global__ __launch_bounds__(kThreads, held(DP, NR)) void k_cached(Cached a) {
   }
 }
 
-// Joins the pieces of a split sequence's rows, `share` workgroups a sequence: a thread has four values of the head in every 256 / (D / 4)-th
-// piece, with a running maximum and sum of its own; those are joined in order. 4 us for 8 pieces, 5 for 190: the launch and two
-// loads behind each other.
+// Joins the pieces of a split sequence's rows, `share` workgroups a sequence: a thread has four values of the head in every
+// 256 / (D / 4)-th piece, with a running maximum and sum of its own; those are joined in order. 4 us for 8 pieces, 5 for 190: the
+// launch and two loads behind each other.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_cached_join(Cached a, int share) {
   __shared__ f32x4 part[kThreads];

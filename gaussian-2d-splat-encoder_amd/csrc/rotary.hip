@@ -6,8 +6,8 @@
 //
 // All of it is bound by memory. A thread has a unit of W pairs (16 bytes a run where the axes allow it) of a token, computes
 // their angles once in 64 bits and turns the unit in several heads; a token's threads lie side by side, so that a wave's loads
-// cover whole heads. Measured (a large copy moves 4.9 TB/s here): 147,456 tokens of 4 heads of 64 bf16 33.7 us each way (4.5 TB/s);
-// 92,160 tokens of 4 heads of 64 bf16 appended 48 us (3.9 TB/s), whose writes go to a page and head of their own each.
+// cover whole heads. Measured (a large copy moves 4.9 TB/s here): 147,456 tokens of 4 heads of 64 bf16 33.7 us each way (4.5
+// TB/s); 92,160 tokens of 4 heads of 64 bf16 appended 48 us (3.9 TB/s), whose writes go to a page and head of their own each.
 #include <algorithm>
 
 #include "token_common.h"
@@ -241,9 +241,9 @@ __global__ __launch_bounds__(kThreads) void k_append(Append n, const T* __restri
 }
 
 // Threads of a token and tokens of a workgroup. A thread turns several heads by the angles it computes once, two at a time, as
-// long as `lanes` threads are left. 36,864 tokens, 8 heads of 64 floats: 2^18 29.7 us, 2^19 28.0; appending 8,192 tokens of 8 heads
-// of 128: 2^18 15.0, 2^19 18.2; 92,160 of 4 heads of 64: 48.0 and 49.8. (Four heads at a time: 30.7 us for the first of these; the next
-// token's loads under way while one is turned: 31.0, as the registers cost waves.)
+// long as `lanes` threads are left. 36,864 tokens, 8 heads of 64 floats: 2^18 29.7 us, 2^19 28.0; appending 8,192 tokens of 8
+// heads of 128: 2^18 15.0, 2^19 18.2; 92,160 of 4 heads of 64: 48.0 and 49.8. (Four heads at a time: 30.7 us for the first of
+// these; the next token's loads under way while one is turned: 31.0, as the registers cost waves.)
 constexpr long long kTurnLanes = 1 << 19, kAppendLanes = 1 << 18;
 template <typename N>
 int seats(N& n, const Units& u, int H, long long lanes) {
@@ -317,8 +317,8 @@ int splat_rotary(const splat_rotation* r, const splat_positions* p, const void* 
   return with_run(dtype, u.W, heads, [&](auto t, auto w, auto hb) {
     using T = decltype(t);
     constexpr int W = decltype(w)::value, HB = decltype(hb)::value;
-    (back ? k_rotary<T, W, HB, true> : k_rotary<T, W, HB, false>)<<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const T*)x,
-                                                                                                           (T*)y);
+    (back ? k_rotary<T, W, HB, true> : k_rotary<T, W, HB, false>)<<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(
+        n, (const T*)x, (T*)y);
     return check_launch("splat_rotary");
   });
 }
@@ -359,7 +359,8 @@ int splat_cache_append(const splat_cache* c, const splat_rotation* r, const spla
                        const unsigned char* mask, long long mb, long long ml, long long T, void* stream) {
   if (const int rc = check_cache("splat_cache_append", c)) return rc;
   if (T < 0) return set_error(kInvalid, "splat_cache_append: %lld tokens", T);
-  if (T > 0x7fffffffLL || c->B * T > 0x7fffffffLL) return set_error(kUnsupported, "splat_cache_append: %d x %lld tokens", c->B, T);
+  if (T > 0x7fffffffLL || c->B * T > 0x7fffffffLL)
+    return set_error(kUnsupported, "splat_cache_append: %d x %lld tokens", c->B, T);
   if (const int rc = check_rotation("splat_cache_append", r, p, c->D)) return rc;
   if (mask && !c->live) return set_error(kInvalid, "splat_cache_append: a key mask for a cache without one");
   if (c->B == 0 || T == 0 || c->pages == 0 || c->width == 0) return kOk;
@@ -377,7 +378,8 @@ int splat_cache_append(const splat_cache* c, const splat_rotation* r, const spla
   n.by_page = fast_div(c->page);
   return with_run(c->dtype, u.W, heads, [&](auto t, auto w, auto hb) {
     using E = decltype(t);
-    k_append<E, decltype(w)::value, decltype(hb)::value><<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const E*)k, (const E*)v);
+    k_append<E, decltype(w)::value, decltype(hb)::value><<<grid_of(n), kThreads, 0, (hipStream_t)stream>>>(n, (const E*)k,
+                                                                                                           (const E*)v);
     return check_launch("splat_cache_append");
   });
 }

@@ -35,7 +35,7 @@ __device__ __forceinline__ double position(const splat_positions& p, long long a
 }
 
 // A unit of a head: two runs of W values at e0 and e1 that turn as pairs (halves: run 0's value i with run 1's; neighbours:
-// the 2 W values from e0 on, two by two), or that pass (axis < 0). `pair` is its first pair, n1 whether there is a second run.
+// the 2 W values from e0 on, two by two), or that pass (axis < 0). `pair` is its first pair, `second` whether there is a second run.
 struct PairUnit {
   int axis, pair, e0, e1;
   bool second;

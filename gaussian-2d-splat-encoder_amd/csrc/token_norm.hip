@@ -489,8 +489,8 @@ __global__ __launch_bounds__(kBlock<TPR>) void k_token_norm_bwd(TokenNorm a) {
 // Adds the workgroups' column sums in a fixed order: 64 columns a workgroup, its waves each a part of the sums. Entries 0 to 3
 // are the parameters' gradients, the others the gate's rows.
 constexpr int kJoin = 1024;
-__global__ __launch_bounds__(kJoin) void k_token_norm_join(TokenNorm a, int wgs, int tiles, long long units, float* dw1, float* db1, float* dw2,
-                                                           float* db2, float* dgate) {
+__global__ __launch_bounds__(kJoin) void k_token_norm_join(TokenNorm a, int wgs, int tiles, long long units, float* dw1,
+                                                           float* db1, float* dw2, float* db2, float* dgate) {
   __shared__ float part[kJoin / 64][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
@@ -595,9 +595,9 @@ unsigned plan(TokenNorm& n, const Shape& s, long long target) {
   return (unsigned)((n.segs + n.whole - 1) / n.whole * n.splits);
 }
 
-// Workgroups aimed at: what the card holds at once, by the registers of a lane (four waves a SIMD; in the backward three or two for
-// 4 or 8 values a lane, four of 1,024 threads, whose registers spill). Backward of 73,728 x 256 bf16, with its join: 512 workgroups 55 us, 768 69, 1,024
-// 60; of 5,001 x 517 floats 768 39 us, 512 45, 1,024 50.
+// Workgroups aimed at: what the card holds at once, by the registers of a lane (four waves a SIMD; in the backward three or two
+// for 4 or 8 values a lane, four of 1,024 threads, whose registers spill). Backward of 73,728 x 256 bf16, with its join: 512
+// workgroups 55 us, 768 69, 1,024 60; of 5,001 x 517 floats 768 39 us, 512 45, 1,024 50.
 long long resident(const Shape& s, int dtype, bool back) {
   const int values = s.k * (dtype == kF32 ? 4 : 8), waves = !back || s.tpr == 1024 ? 4 : values == 4 ? 3 : 2;
   return 256LL * waves * 4 * 64 / std::max(256, s.tpr);
@@ -623,7 +623,8 @@ int splat_token_norm_fwd(const splat_token_norm* a, const void* x, const void* h
   const unsigned grid = plan(p, s, resident(s, a->dtype, false));
   return with_shape(a->dtype, s, [&](auto t, auto tpr, auto k, auto whole, auto lean) {
     constexpr int TPR = decltype(tpr)::value;
-    k_token_norm<decltype(t), TPR, decltype(k)::value, decltype(whole)::value, decltype(lean)::value><<<grid, kBlock<TPR>, 0, (hipStream_t)stream>>>(p);
+    k_token_norm<decltype(t), TPR, decltype(k)::value, decltype(whole)::value, decltype(lean)::value>
+        <<<grid, kBlock<TPR>, 0, (hipStream_t)stream>>>(p);
     return check_launch("splat_token_norm_fwd");
   });
 }
@@ -660,7 +661,8 @@ int splat_token_norm_bwd(const splat_token_norm* a, const void* x, const void* h
   const hipStream_t st = (hipStream_t)stream;
   return with_shape(a->dtype, s, [&](auto t, auto tpr, auto k, auto whole, auto lean) {
     constexpr int TPR = decltype(tpr)::value;
-    k_token_norm_bwd<decltype(t), TPR, decltype(k)::value, decltype(whole)::value, decltype(lean)::value><<<grid, kBlock<TPR>, 0, st>>>(p);
+    k_token_norm_bwd<decltype(t), TPR, decltype(k)::value, decltype(whole)::value, decltype(lean)::value>
+        <<<grid, kBlock<TPR>, 0, st>>>(p);
     if (need) {
       const int tiles = div_up(a->C, 64);
       const long long units = (long long)tiles * (4 + (gates ? p.segs : 0));

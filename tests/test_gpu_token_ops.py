@@ -631,6 +631,43 @@ def test_norm_gradients_against_differences():
     assert abs(num - ana) <= 3e-4 * math.sqrt(2 * 6 * C) + 2 * third
 
 
+def test_saved_tensors_may_come_back_dense():
+    """A hook that stores what the backward needs elsewhere gives dense copies back for strided views."""
+    big = rand(2, 30, 3, 4, 32)
+    x, h, g = big[:, :, 0].flatten(2), big[:, :, 1].flatten(2), big[:, :, 2].flatten(2)
+    v, pos = big.transpose(1, 3)[:, :, 0].transpose(1, 2), rand(2, 30, 5, seed=1)[..., 1:3]
+    ax, up = F.RotaryAxes((16, 8)), rand(2, 30, 128, seed=2)
+
+    def grads():
+        a = [t.detach().requires_grad_(True) for t in (x, h, g, v, pos)]
+        y, n = F.residual_norm(a[0], a[1], gate=a[2], gate_act="silu")
+        r = F.rotary(a[3], a[4], ax)
+        return torch.autograd.grad([y, n, r], a, [up, 2 * up, rand(*r.shape, seed=3)])
+
+    want = grads()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda().contiguous()):
+        got = grads()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_broadcast_inputs():
+    """Expanded inputs: their gradients are summed over what they were expanded to."""
+    one, row, up = rand(1, 1, 2, 16), rand(1, 1, 48, seed=1), rand(3, 7, 48, seed=2)
+    pos, h = rand(3, 7, 1, seed=3), rand(3, 7, 48, seed=4)
+    ax = F.RotaryAxes((16,))
+    a, b, p = one.requires_grad_(True), row.requires_grad_(True), pos[:1, :1].detach().requires_grad_(True)
+    r = F.rotary(a.expand(3, 7, 2, 16), p.expand(3, 7, 1), ax)
+    y, n = F.residual_norm(b.expand(3, 7, 48), h)
+    got = torch.autograd.grad([r, y, n], [a, b, p], [rand(3, 7, 2, 16, seed=5), up, up])
+    d = [t.detach().double().requires_grad_(True) for t in (a, b, p)]
+    rd = R.rotary(d[0].expand(3, 7, 2, 16), d[2].expand(3, 7, 1), ax)
+    yd, nd = R.residual_norm(d[1].expand(3, 7, 48), h.double(), None, None, None, "none", None, None, "rms", 1e-6, 1.0, True,
+                             True)
+    want = torch.autograd.grad([rd, yd, nd], d, [rand(3, 7, 2, 16, seed=5).double(), up.double(), up.double()])
+    for g, w in zip(got, want):
+        close(g, w)
+
+
 def test_rows_past_2_31_values():
     """Tensors of more than 2^31 values whose last rows are compared: their own values, and gradients."""
     n, C = 8_600_000, 256
