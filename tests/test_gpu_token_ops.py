@@ -240,7 +240,9 @@ LENGTHS = [0, 1, 15, 16, 17, 31, 33, 127, 128, 129, 255, 257, 700]
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("page,H,Hk,D,T", [(16, 4, 4, 64, 1), (1, 2, 1, 16, 3), (7, 6, 2, 40, 5), (64, 8, 1, 128, 2),
                                            (100, 3, 3, 33, 1), (17, 5, 1, 96, 7), (32, 2, 2, 80, 20), (24, 40, 1, 1, 1),
-                                           (48, 4, 2, 127, 33)])
+                                           (48, 4, 2, 127, 33), (16, 8, 1, 128, 5), (16, 8, 1, 96, 5), (16, 8, 1, 64, 5),
+                                           (16, 8, 1, 32, 5), (16, 8, 1, 24, 5), (16, 8, 1, 56, 3), (16, 8, 1, 112, 3),
+                                           (32, 2, 1, 24, 1), (32, 2, 1, 112, 1), (32, 2, 1, 32, 1), (32, 2, 1, 3, 9)])
 def test_attention(dt, causal, page, H, Hk, D, T):
     B, width = len(LENGTHS), -(-700 // page)
     for layout, masked in (("heads", False), ("tokens", True)):
@@ -496,6 +498,8 @@ WIDTHS = [4, 8, 31, 64, 100, 200, 256, 333, 512, 517, 1000, 1024, 1500, 2048, 30
 def test_residual_norm_widths(dt, kind, C):
     check_norm((2, 37, C), dt, kind, gate=(C,))
     check_norm((3, 5, C), dt, kind, gate=(3, 5, C), act="sigmoid")
+    check_norm((2, 37, C), dt, kind, gate=(2, C), act="silu", params="weights")
+    check_norm((1, 9, C), dt, kind, gate=(1, 9, C), act="tanh", params="none")
 
 
 @pytest.mark.parametrize("dt", TYPES)
