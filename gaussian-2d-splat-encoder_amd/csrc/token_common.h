@@ -10,11 +10,13 @@ constexpr int kMaxAxes = 4, kMaxHead = 128;
 
 // cos and sin of w quarter turns: w is reduced to the nearest quarter in 64 bits (adding 1.5 * 2^52 leaves the whole number in
 // the last bits), what is left by polynomials fitted for the least error on half a quarter either side (3e-9 and 5e-11, 9e-8
-// evaluated in float32). A position of 2^31 still has 22 bits behind the quarter's point.
+// evaluated in float32). A position of 2^31 still has 22 bits behind the quarter's point. Past 2^51 quarters none are left and
+// the steps of the 64-bit sum leave more than half a quarter, which counts as half of one: any angle, but always a rotation.
 __device__ __forceinline__ void turn(double p, double quarters, float& c, float& s) {
   constexpr double kRound = 6755399441055744.0;
   const double t = fma(p, quarters, kRound), q = t - kRound;
-  const float x = (float)fma(p, quarters, -q);
+  float x = (float)fma(p, quarters, -q);
+  x = fabsf(x) > 0.5f ? 0.5f : x;   // no number stays none
   const unsigned n = (unsigned)__double2loint(t);
   const float z = x * x;
   float a = fmaf(-0.00460165785625577f, z, 0.07968003302812576f);

@@ -133,7 +133,7 @@ def rotary(x, positions, axes):
 
     positions [B, L, axes], or [L, axes] and [1, L, axes] for all images: float32 (splat centres; they have a gradient, summed
     over the images that share them), int32 or int64. axes: RotaryAxes. Angles are taken in 64 bits: up to 2^31
-    radians they are right to 1e-6."""
+    radians they are right to 1e-6; far past that they mean nothing, but pairs still keep their length."""
     dt, _ = _args("none", x)
     shape = x.shape
     if len(shape) != 4 or not 1 <= shape[3] <= MAX_HEAD or shape[2] < 1:

@@ -1,0 +1,80 @@
+"""The token operators on the GPU where sizes, positions and values are at the ends of what they accept."""
+
+import math
+
+import pytest
+import torch
+
+import _token_ref as R
+from _feature_ref import rel
+from gaussian_splat_encoder import token_ops as F
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16]
+
+
+def rand(*shape, dt=torch.float32, seed=0, scale=1.0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dt)
+
+
+# ------------------------------------------------------------------------------------------------ positions
+# nanoseconds of a clock, the ends of the types, both sides of where a 64-bit product has no quarter turns left (2^51 of them)
+FAR = {torch.int64: [1765000000000000001, 2 ** 62 - 12345, -2 ** 62 + 7, 2 ** 63 - 1, -2 ** 63, 2 ** 52 + 3, -2 ** 52 - 3,
+                     2 ** 50 + 11, 2 ** 53 + 2, 2 ** 31],
+       torch.float32: [1e20, -1e20, 3.4e38, -3.4e38, 2.0 ** 51, -2.0 ** 53, 1e15, 6e15, -7e25, 1.5]}
+
+
+def pair_norms(x, dims, interleaved):
+    out, at = [], 0
+    for d in dims:
+        v = x[..., at:at + d].double()
+        v = v.unflatten(-1, (d // 2, 2)) if interleaved else v.unflatten(-1, (2, d // 2)).transpose(-1, -2)
+        out.append(v.norm(dim=-1))
+        at += d
+    return torch.cat(out, -1)
+
+
+@pytest.mark.parametrize("kind", list(FAR))
+@pytest.mark.parametrize("inter", [False, True])
+def test_far_positions_still_turn(kind, inter):
+    """Past 2^31 radians the angle loses its accuracy, but what comes out is a rotation: pairs keep their length. Cosines and
+    sines are 1.5e-7 off at most, so that their squares' sum is 4.3e-7 off one and a length 2.2e-7; two products and a sum of
+    pairs add 2 sqrt(2) 2^-24 of it."""
+    p = torch.tensor(FAR[kind], dtype=kind, device="cuda")[:, None]
+    n, dims = p.shape[0], (8, 6)
+    p = torch.cat([p, p.flip(0)], 1).contiguous()
+    ax = F.RotaryAxes(dims, base=100.0, scale=(1.0, 40.0), interleaved=inter)
+    bound = 2.2e-7 + 2 * math.sqrt(2) * 2.0 ** -24
+    x, g = rand(1, n, 3, 16), rand(1, n, 3, 16, seed=1)
+
+    def same(a, b):
+        return bool(((pair_norms(a, dims, inter) / pair_norms(b, dims, inter) - 1).abs() <= bound).all())
+
+    a = x.clone().requires_grad_(True)
+    y = F.rotary(a, p, ax)
+    assert same(y, x) and torch.equal(y[..., 14:], x[..., 14:])
+    assert same(torch.autograd.grad(y, a, g)[0], g)
+    if kind is torch.float32:       # |dp| is at most the sum over pairs of rate |g| |x|
+        q = p.clone().requires_grad_(True)
+        dx, dp = torch.autograd.grad(F.rotary(a, q, ax), [a, q], g)
+        assert same(dx, g)
+        top = (pair_norms(x, dims, inter) * pair_norms(g, dims, inter)).sum((0, 2, 3))
+        assert bool((dp.abs().double() <= 1.0001 * 40.0 * top.sum()).all())
+    c = F.PagedCache.empty(1, n, 3, 16, dtype=torch.float32)
+    tables, lengths = c.tables(1), torch.tensor([n], device="cuda")
+    F.cache_append(c, tables, lengths, x, x, positions=p, axes=ax)
+    assert torch.equal(c.k[0], y.detach()[0])
+    o = F.cached_attention(x, c, tables, lengths, positions=p, axes=ax)
+    assert rel(o, R.attention(y.detach().double(), c.k, c.v, None, tables, lengths, None, True, 0.25)) <= R.bound_of(torch.float32)
+
+
+def test_positions_that_are_no_number_stay_in_their_token():
+    p = torch.tensor([[1.0], [math.inf], [2.0], [math.nan], [-math.inf], [3.0]], device="cuda")
+    x = rand(1, 6, 2, 8)
+    y = F.rotary(x, p, F.RotaryAxes((4,)))
+    bad = torch.tensor([1, 3, 4], device="cuda")
+    assert bool(torch.isnan(y[:, bad, :, :4]).all()) and torch.equal(y[..., 4:], x[..., 4:])
+    good = torch.tensor([0, 2, 5], device="cuda")
+    assert torch.equal(y[:, good], F.rotary(x[:, good], p[good], F.RotaryAxes((4,))))
