@@ -234,7 +234,8 @@ __global__ __launch_bounds__(kThreads, held(DP, NR)) void k_cached(Cached a) {
   if (pc.n < 1) return;
   if (a.split && pc.i == 0 && hk == 0 && rt == 0 && threadIdx.x == 0) a.split[pc.b] = make_int2(pc.n, pc.slot);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, b = pc.b, len = pc.len;
-  const int per = ((len - 1) / pc.n + 32) / 32 * 32, k0 = pc.i * per, k1 = min(len, k0 + per);
+  const int per = ((len - 1) / pc.n + 32) / 32 * 32, k0 = pc.i * per;
+  const int k1 = len - k0 < per ? len : k0 + per;   // the last piece's k0 + per may be past 2^31
   const int tend = (k1 + KT - 1) / KT;
   const int fresh = new_tokens(a.c, b, a.T), r0 = rt * 16 * NR;
   const int* table = a.c.tables + b * a.c.tb;

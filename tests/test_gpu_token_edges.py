@@ -78,3 +78,28 @@ def test_positions_that_are_no_number_stay_in_their_token():
     assert bool(torch.isnan(y[:, bad, :, :4]).all()) and torch.equal(y[..., 4:], x[..., 4:])
     good = torch.tensor([0, 2, 5], device="cuda")
     assert torch.equal(y[:, good], F.rotary(x[:, good], p[good], F.RotaryAxes((4,))))
+
+
+# ------------------------------------------------------------------------------------------------ pieces
+def test_one_sequence_of_nearly_2_31_tokens_among_many():
+    """The most tokens that a table may have room for, cut into 4,096 pieces of 2^19, of which the last one ends past 2^31. All
+    pages but the last seven of the table are one page of small values; the last seven, of other values, have most of the
+    weight. Scores are sums of 8 products, exact to 2^-24 of themselves."""
+    page, width, B, D, last = 65536, 32767, 65, 8, 7
+    k = torch.zeros(2, page, 1, D, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    k[1, :, :, 0] = 10.0                     # scores: 10 in the last pages, 0 elsewhere
+    v[0], v[1] = 0.25, rand(page, 1, D, dt=torch.bfloat16)
+    tables = torch.zeros(B, width, dtype=torch.int32, device="cuda")
+    tables[0, -last:] = 1
+    lengths = torch.zeros(B, dtype=torch.int32, device="cuda")
+    lengths[0], lengths[B - 1] = page * width, 5
+    q = torch.zeros(B, 1, 1, D, dtype=torch.bfloat16, device="cuda")
+    q[:, :, :, 0] = 1.0
+    c = F.PagedCache(k, v)
+    for causal in (True, False):
+        o = F.cached_attention(q, c, tables, lengths, causal=causal, scale=1.0)
+        far, near = last * page * math.exp(10.0), (width - last) * page * 1.0
+        want = (v[1, :, 0].double().mean(0) * far + 0.25 * near) / (far + near)
+        assert rel(o[0, 0, 0], want) <= R.bound_of(torch.bfloat16)
+        assert torch.equal(o[B - 1, 0, 0], torch.full_like(o[0, 0, 0], 0.25)) and not bool(o[1:B - 1].any())
