@@ -201,12 +201,12 @@ class PagedCache:
         return t if t.is_contiguous() else t.contiguous()
 
 
-def _of_cache(cache, *ts):
+def _of_cache(cache, positions, axes, *ts):
     """The checks that both operators of a cache share."""
     if not isinstance(cache, PagedCache):
         raise ValueError(f"cache must be a PagedCache, got {type(cache).__name__}")
     _args("none", cache.k, *ts)
-    if _wants_grad(*ts):
+    if _wants_grad(cache.k, cache.v, None if axes is None else positions, *ts):
         raise NotImplementedError("the paged cache is for inference: its operators have no gradients")
 
 
@@ -220,7 +220,7 @@ def cache_append(cache, tables, lengths, k, v, counts=None, positions=None, axes
     the sequence's start, behind its table or on an entry that is no page of the cache are left out, and all other places stay
     as they were. Two tokens of a call must not go to one place. key_mask [B, T] (bool, for a cache with `live`): tokens
     that are False do not count (all do by default). Every tensor is on the device: a captured call follows them."""
-    _of_cache(cache, k, v)
+    _of_cache(cache, positions, axes, k, v)
     B, T = k.shape[:2] if k.dim() == 4 else (0, 0)
     if k.dim() != 4 or k.shape != v.shape or k.shape[2:] != cache.k.shape[2:]:
         raise ValueError(f"k and v must be [B, T, {cache.heads}, {cache.head_dim}], got {list(k.shape)} and {list(v.shape)}")
@@ -250,7 +250,7 @@ def cached_attention(q, cache, tables, lengths, counts=None, positions=None, axe
     False, or whose table entry is no page, do not count, whatever they hold. A query without any token, and those past their
     sequence's count, give zeros; an infinite value that counts may give NaN for bfloat16. positions, axes: turns q as by
     rotary. scale defaults to D ** -0.5."""
-    _of_cache(cache, q)
+    _of_cache(cache, positions, axes, q)
     if q.dim() != 4 or q.shape[3] != cache.head_dim or q.shape[2] < 1 or q.shape[2] % cache.heads:
         raise ValueError(f"q must be [B, T, a multiple of {cache.heads}, {cache.head_dim}], got {list(q.shape)}")
     B, T, H, D = q.shape

@@ -1,0 +1,49 @@
+"""Refusals and bookkeeping of the token operators on the host (CPU; no kernel runs)."""
+
+import pytest
+import torch
+
+from gaussian_splat_encoder import token_ops as F
+from test_token_args import cache, ints, t
+
+AX = F.RotaryAxes((8, 4))
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    """The names of what would be launched."""
+    names = []
+    monkeypatch.setattr(F, "_launch", lambda x, name, *args: names.append(name))
+    return names
+
+
+def calls(positions, c=None):
+    c = cache() if c is None else c
+    return (lambda: F.cache_append(c, ints(1, 2), ints(1), t(1, 1, 2, 16), t(1, 1, 2, 16), positions=positions, axes=AX),
+            lambda: F.cached_attention(t(1, 1, 2, 16), c, ints(1, 2), ints(1), positions=positions, axes=AX))
+
+
+def test_the_cache_has_no_gradients_of_positions(no_launch):
+    """Splat centres that learn: their gradient would be dropped without a word."""
+    learnt = t(1, 1, 2).requires_grad_(True)
+    for call in calls(learnt):
+        with pytest.raises(NotImplementedError, match="inference"):
+            call()
+        with torch.no_grad():
+            call()
+    for call in calls(learnt.detach()):
+        call()
+    assert len(no_launch) == 4
+    with torch.autograd.forward_ad.dual_level():
+        for call in calls(torch.autograd.forward_ad.make_dual(t(1, 1, 2), t(1, 1, 2))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+
+
+def test_pages_that_came_to_require_a_gradient_are_refused(no_launch):
+    c = cache()
+    c.v.requires_grad_(True)
+    for call in calls(t(1, 1, 2), c):
+        with pytest.raises(NotImplementedError, match="inference"):
+            call()
+    assert not no_launch
