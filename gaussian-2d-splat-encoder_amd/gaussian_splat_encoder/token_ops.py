@@ -14,6 +14,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import SplatCache, SplatPositions, SplatRotation, SplatTokenNorm
@@ -219,7 +220,8 @@ def cache_append(cache, tables, lengths, k, v, counts=None, positions=None, axes
     first ones of its T (all by default): token t goes to place lengths[b] - counts[b] + t. Tokens past their count, before
     the sequence's start, behind its table or on an entry that is no page of the cache are left out, and all other places stay
     as they were. Two tokens of a call must not go to one place. key_mask [B, T] (bool, for a cache with `live`): tokens
-    that are False do not count (all do by default). Every tensor is on the device: a captured call follows them."""
+    that are False do not count (all do by default). Every tensor is on the device: a captured call follows them. For autograd
+    a call is a write in place of the cache's tensors."""
     _of_cache(cache, positions, axes, k, v)
     B, T = k.shape[:2] if k.dim() == 4 else (0, 0)
     if k.dim() != 4 or k.shape != v.shape or k.shape[2:] != cache.k.shape[2:]:
@@ -238,6 +240,8 @@ def cache_append(cache, tables, lengths, k, v, counts=None, positions=None, axes
         k, v = _dense(k), _dense(v)
         _launch(k, "splat_cache_append", c, r, p, k.data_ptr(), *k.stride()[:3], v.data_ptr(),
                 *v.stride()[:3], _ptr(key_mask), *((0, 0) if key_mask is None else key_mask.stride()), T)
+        # the kernel wrote through pointers: what saved a page for its backward has to notice
+        increment_version((cache.k, cache.v) if cache.live is None else (cache.k, cache.v, cache.live))
 
 
 def cached_attention(q, cache, tables, lengths, counts=None, positions=None, axes=None, causal=True, scale=None):

@@ -103,3 +103,18 @@ def test_one_sequence_of_nearly_2_31_tokens_among_many():
         want = (v[1, :, 0].double().mean(0) * far + 0.25 * near) / (far + near)
         assert rel(o[0, 0, 0], want) <= R.bound_of(torch.bfloat16)
         assert torch.equal(o[B - 1, 0, 0], torch.full_like(o[0, 0, 0], 0.25)) and not bool(o[1:B - 1].any())
+
+
+# ------------------------------------------------------------------------------------------------ the cache and autograd
+def test_an_append_under_a_saved_page_is_noticed():
+    """A dense attention over a page saves it for its backward, which must not run on what an append wrote over it."""
+    from gaussian_splat_encoder import feature_ops
+    c = F.PagedCache.empty(1, 32, 2, 16, dtype=torch.float32)
+    c.k.copy_(rand(*c.k.shape)), c.v.copy_(rand(*c.v.shape, seed=1))
+    q = rand(1, 3, 2, 16, seed=2).requires_grad_(True)
+    o = feature_ops.cross_attention(q, c.k, c.v)
+    F.cached_attention(q.detach(), c, c.tables(1), torch.tensor([9], device="cuda"))      # only reads
+    torch.autograd.grad(o.sum(), q, retain_graph=True)
+    F.cache_append(c, c.tables(1), torch.tensor([9], device="cuda"), rand(1, 1, 2, 16), rand(1, 1, 2, 16))
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(o.sum(), q)

@@ -47,3 +47,24 @@ def test_pages_that_came_to_require_a_gradient_are_refused(no_launch):
         with pytest.raises(NotImplementedError, match="inference"):
             call()
     assert not no_launch
+
+
+def test_an_append_counts_as_a_write(no_launch):
+    """Autograd knows of writes by its tensors' version counters; views of a page share them."""
+    for c in (cache(), cache(masked=True)):
+        page = c.k[0]
+        before = [x._version for x in (c.k, c.v, page)] + ([] if c.live is None else [c.live._version])
+        read = calls(t(1, 1, 2), c)
+        read[1]()
+        now = lambda: [x._version for x in (c.k, c.v, page)] + ([] if c.live is None else [c.live._version])  # noqa: E731
+        assert now() == before
+        read[0]()
+        assert all(a > b for a, b in zip(now(), before))
+        after = now()
+        F.cache_append(c, ints(1, 2), ints(1), t(1, 0, 2, 16), t(1, 0, 2, 16))      # writes nothing
+        assert now() == after and no_launch.count("splat_cache_append") == 1
+        no_launch.clear()
+    with torch.inference_mode():        # tensors without counters
+        c = cache()
+        calls(t(1, 1, 2), c)[0]()
+    assert no_launch == ["splat_cache_append"]
