@@ -252,8 +252,8 @@ def cached_attention(q, cache, tables, lengths, counts=None, positions=None, axe
     tables, lengths, counts as in cache_append: the queries are the last counts[b] tokens that lengths[b] counts. causal: query t
     sees the tokens up to its own place, lengths[b] - counts[b] + t; otherwise all. Tokens that the cache's `live` marks
     False, or whose table entry is no page, do not count, whatever they hold. A query without any token, and those past their
-    sequence's count, give zeros; an infinite value that counts may give NaN for bfloat16. positions, axes: turns q as by
-    rotary. scale defaults to D ** -0.5."""
+    sequence's count, give zeros; an infinite value that counts may give NaN for bfloat16, and for float32 where its probability
+    is less than 2^-126. positions, axes: turns q as by rotary. scale defaults to D ** -0.5."""
     _of_cache(cache, positions, axes, q)
     if q.dim() != 4 or q.shape[3] != cache.head_dim or q.shape[2] < 1 or q.shape[2] % cache.heads:
         raise ValueError(f"q must be [B, T, a multiple of {cache.heads}, {cache.head_dim}], got {list(q.shape)}")

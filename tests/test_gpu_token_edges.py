@@ -118,3 +118,33 @@ def test_an_append_under_a_saved_page_is_noticed():
     F.cache_append(c, c.tables(1), torch.tensor([9], device="cuda"), rand(1, 1, 2, 16), rand(1, 1, 2, 16))
     with pytest.raises(RuntimeError, match="inplace"):
         torch.autograd.grad(o.sum(), q)
+
+
+# ------------------------------------------------------------------------------------------------ values
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("T", [1, 6])
+def test_infinite_values_that_count(T, causal):
+    """Float32: an infinite value makes its column infinite in every row that sees it, also where dead tokens lie beside it, and
+    leaves the other columns as they are. Scores differ by 20 at most, so that no probability vanishes."""
+    H, Hk, D, page, width = 4, 2, 40, 16, 20
+    g = torch.Generator("cuda").manual_seed(3)
+    k, v = rand(width, page, Hk, D, seed=1), rand(width, page, Hk, D, seed=2)
+    live = torch.rand(width, page, generator=g, device="cuda") < 0.5
+    c = F.PagedCache(k, v, live)
+    tables, lengths = c.tables(1), torch.tensor([303], device="cuda")
+    q = rand(1, T, H, D, seed=4)
+    clean = F.cached_attention(q, c, tables, lengths, causal=causal)
+    for i, (j, d, bad) in enumerate([(0, 3, math.inf), (37, 0, -math.inf), (100, 39, math.inf), (211, 17, -math.inf),
+                                     (290, 20, math.inf)]):
+        p, at = j // page, j % page
+        live[p, at] = True
+        want = F.cached_attention(q, c, tables, lengths, causal=causal).clone()
+        old = v[p, at, 0, d].clone()
+        v[p, at, 0, d] = bad
+        o = F.cached_attention(q, c, tables, lengths, causal=causal)
+        want[:, :, :H // Hk, d] = bad
+        hit = torch.isinf(want)
+        assert torch.equal(o[hit], want[hit]), (j, d)
+        assert rel(o[~hit], want[~hit]) <= R.bound_of(torch.float32), (j, d)
+        v[p, at, 0, d] = old
+    assert bool(torch.isfinite(clean).all())
