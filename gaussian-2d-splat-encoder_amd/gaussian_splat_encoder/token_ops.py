@@ -45,10 +45,14 @@ class RotaryAxes:
         if not all(0 < b < math.inf for b in self.base) or not all(abs(s) < math.inf for s in self.scale):
             raise ValueError(f"base must be positive and both finite, got {self.base} and {self.scale}")
         self.interleaved = bool(interleaved)
-        rates = [s * b ** (-2 * i / d) * 2 / math.pi for d, b, s in zip(self.dims, self.base, self.scale)
-                 for i in range(d // 2)]
+        try:
+            rates = [s * b ** (-2 * i / d) for d, b, s in zip(self.dims, self.base, self.scale) for i in range(d // 2)]
+        except OverflowError:
+            rates = [math.inf]
+        if not all(abs(r) <= _MAX_FLOAT for r in rates):
+            raise ValueError(f"rates scale * base ** (-2 i / dims) must be finite float32, got base {self.base}, scale {self.scale}")
         self._c = SplatRotation(len(self.dims), int(self.interleaved), (ctypes.c_int * 4)(*self.dims),
-                                (ctypes.c_double * 64)(*rates))
+                                (ctypes.c_double * 64)(*(r * 2 / math.pi for r in rates)))
 
     def __reduce__(self):
         return type(self), (self.dims, self.base, self.scale, self.interleaved)

@@ -68,3 +68,12 @@ def test_an_append_counts_as_a_write(no_launch):
         c = cache()
         calls(t(1, 1, 2), c)[0]()
     assert no_launch == ["splat_cache_append"]
+
+
+@pytest.mark.parametrize("kw", [dict(dims=(64,), base=1e-320), dict(dims=(64,), base=1e-300, scale=1e300),
+                                dict(dims=(4,), scale=1e300), dict(dims=(4, 4), scale=(1.0, -3.5e38))])
+def test_rates_past_float32_are_refused(kw):
+    """A position's product with them would pass 64 bits, its gradient float32."""
+    with pytest.raises(ValueError, match="rates"):
+        F.RotaryAxes(**kw)
+    F.RotaryAxes((4,), scale=-3.4e38, base=1.0)
