@@ -148,3 +148,99 @@ def test_infinite_values_that_count(T, causal):
         assert rel(o[~hit], want[~hit]) <= R.bound_of(torch.float32), (j, d)
         v[p, at, 0, d] = old
     assert bool(torch.isfinite(clean).all())
+
+
+# ------------------------------------------------------------------------------------------------ plans
+def plan(B, H, Hk, D, T, lengths, page, width):
+    """How cached_attention cuts its sequences: the way, the pieces aimed at, the units (128 tokens) and those of a piece."""
+    R_ = T * H // Hk
+    two = R_ > 16
+    held = {32: (4, 3), 64: (3, 2), 96: (2, 1), 128: (2, 1)}[-(-D // 32) * 32][two]
+    each = Hk * -(-R_ // (32 if two else 16))
+    once = max(1, 256 * held // each)
+    fit = B <= 64 and 2 * B <= once
+    pieces = once if fit else -(-4 * 256 * held // each)
+    cut = "whole" if page * width <= 128 or pieces <= 1 else "scanned" if B <= 64 else "mapped"
+    units = sum(-(-n // 128) for n in lengths)
+    return cut, fit, pieces, units, max(1, -(-units // pieces))
+
+
+def workspace(cut, pieces, B, H, Hk, D, T):
+    if cut == "whole":
+        return 0
+    return (16 * (pieces + B) if cut == "mapped" else 0) + 8 * B + 4 * 2 * pieces * T * H * (D + 2)
+
+
+def attention(q, c, tables, lengths):
+    """One token of each sequence over all its tokens in float64, sequences of a length near each other at a time."""
+    B, _, H, D = q.shape
+    o = torch.zeros(B, 1, H, D, dtype=torch.float64, device="cuda")
+    order = sorted((n, b) for b, n in enumerate(lengths.tolist()) if n > 0)
+    rep = H // c.heads
+    while order:
+        m = order[-1][0]
+        some = [b for n, b in order if 2 * n > m][-max(1, (1 << 22) // (m * H * D)):]
+        gone = set(some)
+        order = [x for x in order if x[1] not in gone]
+        b = torch.tensor(some, device="cuda")
+        j = torch.arange(m, device="cuda")
+        at = tables[b].long()[:, j.clamp(max=tables.shape[1] * c.page - 1) // c.page]
+        k, v = (t[at, j % c.page].double().repeat_interleave(rep, 2) for t in (c.k, c.v))        # [n, m, H, D]
+        s = (q[b].double() * k).sum(-1) * D ** -0.5
+        s = s.masked_fill((j >= lengths[b][:, None])[..., None], -math.inf)
+        w = torch.exp(s - s.amax(1, keepdim=True))
+        o[b, 0] = (w[..., None] * v).sum(1) / w.sum(1)[..., None]
+    return o
+
+
+def spread(B, most, long, n):
+    """B lengths of 0 to `most` tokens, every `long`-th one of n."""
+    return [n - i % 77 if i % long == long // 2 else (i * 7919) % (most + 1) for i in range(B)]
+
+
+# (sequences, heads, key heads, D, lengths), and the plan: how they are cut, whether all pieces fit the card at once, pieces of one unit of
+# 128 tokens or of more
+PLANS = [
+    (2500, 2, 1, 64, spread(2500, 130, 400, 9000), "mapped", False, False),       # three rounds of 1,024 sequences
+    (2500, 2, 1, 64, spread(2500, 300, 300, 60000), "mapped", False, True),
+    (1025, 1, 1, 32, [0] * 1024 + [40000], "mapped", False, False),               # all in the second round's only one
+    (3000, 4, 4, 128, spread(3000, 40, 1500, 20000), "mapped", False, True),
+    (17000, 1, 1, 16, spread(17000, 60, 8000, 3000), "mapped", False, True),      # more than workgroups join
+    (100, 8, 8, 128, spread(100, 700, 9, 3000), "mapped", False, True),
+    (200, 16, 8, 64, spread(200, 300, 50, 5000), "mapped", False, True),
+    (65, 8, 8, 128, spread(65, 200, 30, 500), "mapped", False, False),
+    (40, 8, 8, 128, spread(40, 900, 11, 1500), "scanned", False, False),
+    (40, 8, 8, 128, spread(40, 900, 11, 12000), "scanned", False, True),
+    (64, 4, 4, 64, spread(64, 500, 60, 30000), "scanned", True, True),
+    (64, 32, 8, 96, spread(64, 2000, 20, 9000), "scanned", False, True),
+    (30, 8, 8, 128, spread(30, 900, 11, 3000), "scanned", True, True),
+    (3, 2, 1, 64, [300000, 0, 5000], "scanned", True, True),
+]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("B,H,Hk,D,lengths,cut,fit,longer", PLANS)
+def test_every_way_of_cutting(dt, B, H, Hk, D, lengths, cut, fit, longer):
+    import ctypes
+
+    from gaussian_splat_encoder import _lib
+    page = 64
+    width = -(-max(lengths) // page)
+    got = plan(B, H, Hk, D, 1, lengths, page, width)
+    assert got[:2] == (cut, fit) and (got[4] > 1) == longer
+    pages = 97
+    g = torch.Generator("cuda").manual_seed(B)
+    k, v = (torch.randn(pages, Hk, page, D, generator=g, device="cuda").to(dt).transpose(1, 2) for _ in range(2))
+    c = F.PagedCache(k, v)
+    tables = torch.randint(0, pages, (B, width), generator=g, device="cuda", dtype=torch.int32)   # pages are only read
+    n = torch.tensor(lengths, device="cuda", dtype=torch.int32)
+    q = rand(B, 1, H, D, dt=dt, seed=1, scale=1.3)
+    d, keep = c._describe(tables, n, None, B, 1)
+    assert _lib.load().splat_cached_attention_workspace_bytes(ctypes.byref(d), H, 1) == workspace(cut, got[2], B, H, Hk, D, 1)
+    o = F.cached_attention(q, c, tables, n)
+    want = attention(q, c, tables, n)
+    assert rel(o, want) <= R.bound_of(dt)
+    bad = (o.double() - want).flatten(1).norm(dim=1) / want.flatten(1).norm(dim=1).clamp_min(1e-30)
+    full = n > 0                             # each sequence by itself: a lost piece of one does not show among thousands
+    assert bool((bad[full] <= R.bound_of(dt)).all()) and not bool(o[~full].any())
+    assert torch.equal(F.cached_attention(q, c, tables, n), o)
