@@ -244,3 +244,21 @@ def test_every_way_of_cutting(dt, B, H, Hk, D, lengths, cut, fit, longer):
     full = n > 0                             # each sequence by itself: a lost piece of one does not show among thousands
     assert bool((bad[full] <= R.bound_of(dt)).all()) and not bool(o[~full].any())
     assert torch.equal(F.cached_attention(q, c, tables, n), o)
+
+
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("H,Hk,D,n", [(4, 4, 64, 300), (8, 2, 128, 129), (32, 1, 96, 61)])
+def test_bfloat16_attention_rounds_its_result_alone(H, Hk, D, n, turned):
+    """Probabilities and turned queries are sums of two bfloat16 values, 2^-17 of them off: the result is as far from float64 as
+    the exact one rounded, within 5%. (One value for the two: 15% to 82% more, test_token_edges.)"""
+    B, page = 12, 32
+    width = -(-n // page)
+    k, v = rand(B * width, page, Hk, D, dt=torch.bfloat16, seed=1, scale=1.3), rand(B * width, page, Hk, D, dt=torch.bfloat16, seed=2)
+    c = F.PagedCache(k, v)
+    tables, lengths = c.tables(B), torch.full((B,), n, device="cuda")
+    q = rand(B, 1, H, D, dt=torch.bfloat16, seed=3, scale=1.3)
+    ax, pos = (F.RotaryAxes((D,)), torch.full((B, 1, 1), 12345, device="cuda")) if turned else (None, None)
+    o = F.cached_attention(q, c, tables, lengths, positions=pos, axes=ax)
+    qd = R.rotary(q.double(), pos.double(), ax) if turned else q.double()
+    want = R.attention(qd, c.k, c.v, None, tables, lengths, None, True, D ** -0.5)
+    assert rel(o, want) <= 1.05 * rel(want.to(torch.bfloat16), want)

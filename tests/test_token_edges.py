@@ -77,3 +77,26 @@ def test_rates_past_float32_are_refused(kw):
     with pytest.raises(ValueError, match="rates"):
         F.RotaryAxes(**kw)
     F.RotaryAxes((4,), scale=-3.4e38, base=1.0)
+
+
+@pytest.mark.parametrize("H,Hk,D,n", [(4, 4, 64, 300), (8, 2, 128, 129), (32, 1, 96, 61)])
+def test_one_bfloat16_value_for_two_would_show(H, Hk, D, n):
+    """What test_gpu_token_edges allows a bfloat16 attention (1.05 of the exact result's own rounding) is passed where a
+    probability or a turned query loses its second value: planted in the float64 attention."""
+    import _token_ref as R
+    from _feature_ref import rel
+    b = torch.bfloat16
+    g = torch.Generator().manual_seed(1)
+    q, k, v = ((torch.randn(12, *s, D, generator=g) * f).to(b).double() for s, f in (((H,), 1.3), ((n, Hk), 1.3), ((n, Hk), 1.0)))
+    k, v = k.repeat_interleave(H // Hk, 2), v.repeat_interleave(H // Hk, 2)
+    q = R.rotary(q[:, None], torch.full((12, 1, 1), 12345.0, dtype=torch.float64), F.RotaryAxes((D,)))[:, 0]
+
+    def attend(q, lose):
+        s = (q[:, None] * k).sum(-1) * D ** -0.5
+        w = torch.exp(s - s.amax(1, keepdim=True))
+        return ((w.to(b).double() if lose else w)[..., None] * v).sum(1) / w.sum(1)[..., None]
+
+    want = attend(q, False)
+    own = rel(want.to(b), want)
+    assert rel(attend(q, True).to(b), want) > 1.1 * own
+    assert rel(attend(q.to(b).double(), False).to(b), want) > 1.5 * own
