@@ -262,3 +262,26 @@ def test_bfloat16_attention_rounds_its_result_alone(H, Hk, D, n, turned):
     qd = R.rotary(q.double(), pos.double(), ax) if turned else q.double()
     want = R.attention(qd, c.k, c.v, None, tables, lengths, None, True, D ** -0.5)
     assert rel(o, want) <= 1.05 * rel(want.to(torch.bfloat16), want)
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_reader_gradients_of_key_and_value_biases(kind):
+    """The values' half of to_kv's bias has the bound of the reader's other parameters. The keys' half is a sum over all states
+    that mostly cancels (a bias moves all scores nearly alike): the same bound, of the terms' magnitudes."""
+    from test_gpu_token_reader import make, plain, where
+    r = make(kind=kind)
+    B, L, N = 2, 9, 150
+    x, s, pos, spos = rand(B, L, 96, seed=1), rand(B, N, 56, seed=2), where(B, L, 4, 5), where(B, N, 2, 6)
+    mask = rand(B, N, seed=7) < 0.8
+    y = r(x, pos, s, spos, key_mask=mask)
+    g = rand(*y.shape, seed=8)
+    got, = torch.autograd.grad(y, r.to_kv.bias, g)
+    p = {n: t.detach().double() for n, t in r.named_parameters()}
+    each = p["to_kv.bias"].expand(B, N, -1).clone().requires_grad_(True)          # a bias of each state's own
+    p["to_kv.bias"] = each
+    z = plain(r, p, x.double(), pos.double(), s.double(), spos.double(), mask)
+    d, = torch.autograd.grad(z, each, g.double())
+    half, bound = r.kv_heads * r.head_dim, 18 * R.bound_of(torch.float32)
+    want = d.sum((0, 1))
+    assert rel(got[half:], want[half:]) <= bound
+    assert (got[:half] - want[:half]).norm().item() <= bound * d[..., :half].abs().sum((0, 1)).norm().item()
