@@ -114,13 +114,6 @@ __device__ __forceinline__ void turn_runs(float (&a)[W], float (&b)[W], const fl
 }
 
 template <typename T, int W>
-__device__ __forceinline__ void load_run(const T* p, float (&f)[W]) {
-  T v[W];
-  __builtin_memcpy(v, p, sizeof(v));
-#pragma unroll
-  for (int j = 0; j < W; ++j) f[j] = (float)v[j];
-}
-template <typename T, int W>
 __device__ __forceinline__ void store_run(T* p, const float (&f)[W]) {
   T v[W];
 #pragma unroll
