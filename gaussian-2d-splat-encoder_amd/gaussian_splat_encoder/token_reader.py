@@ -77,7 +77,7 @@ class TokenReader(nn.Module):
                                              key_mask=key_mask))
 
     def new_cache(self, sequences, tokens, page=64, dtype=torch.bfloat16, device="cuda", masked=False):
-        """A cache with room for `tokens` states of each sequence, and its tables."""
+        """A cache with room for `tokens` states of each sequence, and its tables. dtype: the states' (keys and values have it)."""
         cache = PagedCache.empty(sequences * -(-tokens // page), page, self.kv_heads, self.head_dim, dtype, device, masked)
         return cache, cache.tables(sequences)
 

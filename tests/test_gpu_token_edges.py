@@ -285,3 +285,22 @@ def test_reader_gradients_of_key_and_value_biases(kind):
     want = d.sum((0, 1))
     assert rel(got[half:], want[half:]) <= bound
     assert (got[:half] - want[:half]).norm().item() <= bound * d[..., :half].abs().sum((0, 1)).norm().item()
+
+
+def test_the_documented_example_runs():
+    """The lines on tokens in the readme, with what its reader has: eight sequences of one new token in bfloat16, a frame's latents
+    as the encoder gives them (float32)."""
+    import os
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "README.md")
+    with open(at) as f:
+        blocks = [b.split("```")[0] for b in f.read().split("```python\n")[1:]]
+    code, = [b for b in blocks if "cached_attention" in b]
+    env = dict(torch=torch, q=rand(8, 1, 8, 64, dt=torch.bfloat16), k=rand(8, 1, 4, 64, dt=torch.bfloat16, seed=1),
+               v=rand(8, 1, 4, 64, dt=torch.bfloat16, seed=2), positions=rand(8, 1, 3, seed=3), p=rand(8, 1, 3, seed=3),
+               x=rand(4, 100, 256), h=rand(4, 100, 256, seed=4), g=rand(256, seed=5), w1=rand(256, seed=6), w2=rand(256, seed=7),
+               latents=rand(1, 500, 128, seed=8), splat_positions=rand(1, 500, 3, seed=9), tokens=rand(1, 5, 256, seed=10),
+               token_positions=rand(5, 3, seed=11))
+    before = env["tokens"]
+    exec(compile(code, at, "exec"), env)
+    assert torch.equal(env["o"].view(8, 4, 2, 64), env["v"][:, 0, :, None].expand(8, 4, 2, 64))    # one token: its value
+    assert env["tokens"].shape == before.shape and torch.equal(env["tokens"], before)              # a new layer's gates are closed
