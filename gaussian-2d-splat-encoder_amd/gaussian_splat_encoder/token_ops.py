@@ -168,6 +168,7 @@ class PagedCache:
         if k.requires_grad or v.requires_grad:
             raise ValueError("a cache's pages must not require a gradient")
         self.k, self.v, self.live = k, v, live
+        self._shared = any(n > 1 and st == 0 for t in (k, v, live) if t is not None for n, st in zip(t.shape, t.stride()))
         self.pages, self.page, self.heads, self.head_dim = k.shape
 
     @classmethod
@@ -227,6 +228,8 @@ def cache_append(cache, tables, lengths, k, v, counts=None, positions=None, axes
     that are False do not count (all do by default). Every tensor is on the device: a captured call follows them. For autograd
     a call is a write in place of the cache's tensors."""
     _of_cache(cache, positions, axes, k, v)
+    if cache._shared:
+        raise ValueError("a cache of expanded tensors, whose tokens share memory, is only read")
     B, T = k.shape[:2] if k.dim() == 4 else (0, 0)
     if k.dim() != 4 or k.shape != v.shape or k.shape[2:] != cache.k.shape[2:]:
         raise ValueError(f"k and v must be [B, T, {cache.heads}, {cache.head_dim}], got {list(k.shape)} and {list(v.shape)}")

@@ -100,3 +100,16 @@ def test_one_bfloat16_value_for_two_would_show(H, Hk, D, n):
     own = rel(want.to(b), want)
     assert rel(attend(q, True).to(b), want) > 1.1 * own
     assert rel(attend(q.to(b).double(), False).to(b), want) > 1.5 * own
+
+
+def test_an_append_into_expanded_pages_is_refused(no_launch):
+    """Tokens that share memory may be read, but a call would write many of them to one place."""
+    one = t(1, 8, 2, 16)
+    for c in (F.PagedCache(one.expand(4, 8, 2, 16), t(4, 8, 2, 16)), F.PagedCache(t(4, 8, 2, 16), t(4, 1, 2, 16).expand(4, 8, 2, 16)),
+              F.PagedCache(t(4, 8, 2, 16), t(4, 8, 2, 16), t(4, 1, dtype=torch.bool).expand(4, 8))):
+        append, read = calls(t(1, 1, 2), c)
+        with pytest.raises(ValueError, match="share memory"):
+            append()
+        read()
+    calls(t(1, 1, 2), F.PagedCache(one.expand(1, 8, 2, 16), one))[0]()      # one page: nothing is shared
+    assert no_launch == ["splat_cached_attention"] * 3 + ["splat_cache_append"]
