@@ -12,15 +12,17 @@
 // and sums, accumulators and partial results are 32-bit floats. Probabilities, and queries that were turned, are taken as sums
 // of two bf16 values: matrix instructions wait for memory here, and a single rounding would show next to the result's own.
 //
-// Tokens past the length or marked dead are not read and count as zeros; their places hold a neighbour's values, zeros for floats,
-// so that an infinite value that counts stays infinite (368,640 tokens of 4 heads of 64 floats, 60% live, 102 us, 100 without;
-// bf16 would still multiply it by a probability's second part, of either sign or zero, and give NaN). Tokens after a causal query
-// have probability zero; a tile whose values there are not finite is multiplied query by query with those values as zeros.
+// Tokens past the length or marked dead are not read and count as zeros; their places hold a neighbour's values, zeros for
+// floats, so that an infinite value that counts stays infinite (368,640 tokens of 4 heads of 64 floats, 60% live, 102 us, 100
+// without; bf16 would still multiply it by a probability's second part, of either sign or zero, and give NaN). Tokens after a
+// causal query have probability zero; a tile whose values there are not finite is multiplied query by query with those values
+// as zeros.
 //
-// Measured: one token in each of sixteen sequences of 0 to 32,768 tokens, 32 heads over 8 of 128 bf16 (1.06 GB) 187 us, 5.7
-// TB/s; one token over 368,640, of which 60% count, 4 heads of 64 bf16 (226 MB) 49 us, 4.6 TB/s, with a join of 190 pieces 5;
-// one over 900 tokens 7.7 us, six loads behind each other, and a join of 4. Many rows are not what this is for: 1,024 tokens of
-// 32 heads over 8,192 take 683 us (190 TFLOP/s), rows of 32 a workgroup and two products for one.
+// Measured: one token in each of sixteen sequences of 0 to 32,768 tokens, 32 heads over 8 of 128 bf16 (1.06 GB) 188 us, 5.6
+// TB/s, floats (2.1 GB) 372 with the join, 5.7; one token over 368,640, of which 60% count, 4 heads of 64 bf16 (226 MB) 48 us, 4.7
+// TB/s, with a join of 190 pieces 5, of floats, all live (755 MB), 141 with the join, 5.4 TB/s; one over 900 tokens 8.1 us, six
+// loads behind each other, and a join of 4. Many rows are not what this is for: 1,024 tokens of 32 heads over 8,192 take 626 us
+// (205 TFLOP/s), rows of 32 a workgroup and two products for one.
 #include <algorithm>
 
 #include "token_common.h"

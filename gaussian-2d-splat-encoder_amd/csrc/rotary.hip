@@ -6,7 +6,7 @@
 //
 // All of it is bound by memory. A thread has a unit of W pairs (16 bytes a run where the axes allow it) of a token, computes
 // their angles once in 64 bits and turns the unit in several heads; a token's threads lie side by side, so that a wave's loads
-// cover whole heads. Measured (a large copy moves 4.9 TB/s here): 147,456 tokens of 4 heads of 64 bf16 33.7 us each way (4.5
+// cover whole heads. Measured (a large copy moves 4.9 TB/s here): 147,456 tokens of 4 heads of 64 bf16 35 us each way (4.3
 // TB/s); 92,160 tokens of 4 heads of 64 bf16 appended 48 us (3.9 TB/s), whose writes go to a page and head of their own each.
 #include <algorithm>
 
@@ -241,9 +241,10 @@ __global__ __launch_bounds__(kThreads) void k_append(Append n, const T* __restri
 }
 
 // Threads of a token and tokens of a workgroup. A thread turns several heads by the angles it computes once, two at a time, as
-// long as `lanes` threads are left. 36,864 tokens, 8 heads of 64 floats: 2^18 29.7 us, 2^19 28.0; appending 8,192 tokens of 8
-// heads of 128: 2^18 15.0, 2^19 18.2; 92,160 of 4 heads of 64: 48.0 and 49.8. (Four heads at a time: 30.7 us for the first of
-// these; the next token's loads under way while one is turned: 31.0, as the registers cost waves.)
+// long as `lanes` threads are left. Rotations, 2^18, 2^19 and 2^20, us: 36,864 tokens of 8 heads of 64 floats 34.1, 32.5, 34.2;
+// 8,192 of 32 of 128 bf16 32.6, 29.3, 32.1; 4,096 of 16 of 64 floats 10.4, 11.1, 11.0. Appends: 8,192 of 8 of 128 bf16 15.2,
+// 18.4, 18.4; 92,160 of 4 of 64 bf16 46.1, 45.1, 45.7; 36,864 of 8 of 64 floats 64.1, 61.1, 61.8. (Four heads at a time, or the
+// next token's loads under way while one is turned, cost more waves than they gain.)
 constexpr long long kTurnLanes = 1 << 19, kAppendLanes = 1 << 18;
 template <typename N>
 int seats(N& n, const Units& u, int H, long long lanes) {

@@ -17,7 +17,7 @@
 //
 // Bound by memory: 73,728 x 256 bf16 with a gate of each image's (a large copy moves 4.9 TB/s here) forward 38 us (151 MB, 4.0
 // TB/s), backward 52 (227 MB, 4.4 TB/s), the join of 512 partial sums 5, the launch and two rounds of loads. (Stores that pass the
-// caches by take 4 us off the forward alone, and cost the product that reads its result 7.)
+// caches by take a tenth off the forward alone, and cost the product that reads its result as much again.)
 #include <algorithm>
 
 #include "feat_common.h"
@@ -108,7 +108,7 @@ using Vals = float[K][kV<T>];
 
 // A row's chunks as they lie in memory. Lanes past C load the first chunk, and where C is not whole chunks (!Whole) the lane of
 // the last ones loads the row's last 16 bytes, so that no load has a condition of its own and the next row's are under way
-// while this one is worked on (60,033 x 333 bf16 in training: 203 us with conditions, 169 without).
+// while this one is worked on (60,033 x 333 bf16 in training: 338 us with conditions, 250 without).
 template <typename T, int K>
 using Raw = Chunk<T>[K];
 
@@ -519,9 +519,11 @@ __global__ __launch_bounds__(kJoin) void k_token_norm_join(TokenNorm a, int wgs,
   }
 }
 
-// At most 8 values a lane. Rows of 65 to 128 chunks: of floats two chunks in each lane of a wave (73,728 x 300 in training 106 us,
-// one in each of two waves 118), of bf16 one in each of two waves (18,432 x 1,024 94 us, two a lane 112); 4,096 bf16 values one
-// in each of eight waves (102 us, two in each of four 117); 517 floats one in each of four waves (57 us, three a lane 65).
+// At most 8 values a lane. Training passes, us, this rule's side first. Rows of 65 to 128 chunks: of floats two chunks in each
+// lane of a wave, or one in each of two waves (36,864 rows of 400 channels 131 and 135, of 512 156 and 159); of bf16 one in each
+// of two waves, or two a lane (24,576 x 640 109 and 135, 18,432 x 1,024 97 and 119). Up to 512 chunks of bf16 one in each of
+// eight waves, or two in each of four (6,144 x 3,000 119 and 151, 4,608 x 4,096 103 and 129). Up to 192 chunks of floats one in
+// each of four waves, or three a lane (5,001 x 517 48 and 62, 16,384 x 600 106 and 113, 12,288 x 768 87 and 95).
 struct Shape {
   int tpr, k, rows;   // threads of a row; chunks of a thread; rows of a workgroup at a time
   bool whole, lean;
@@ -596,8 +598,10 @@ unsigned plan(TokenNorm& n, const Shape& s, long long target) {
 }
 
 // Workgroups aimed at: what the card holds at once, by the registers of a lane (four waves a SIMD; in the backward three or two
-// for 4 or 8 values a lane, four of 1,024 threads, whose registers spill). Backward of 73,728 x 256 bf16, with its join: 512
-// workgroups 55 us, 768 69, 1,024 60; of 5,001 x 517 floats 768 39 us, 512 45, 1,024 50.
+// for 4 or 8 values a lane, four of 1,024 threads, whose registers spill). Training passes for 2, 3 and 4 waves, us: bf16
+// 73,728 x 256 97, 110, 101 (64 to 1,024 channels the same to 3%), 4,608 x 4,096 103, 123, 114, 2,304 x 8,192 274, 226, 209;
+// floats of four values a lane 36,864 x 256 85, 82, 86, 9,216 x 1,024 87, 84, 86, 5,001 x 517 49, 47, 56; of eight 73,728 x 300
+// 204, 231, 209, 4,608 x 2,048 87, 97, 96. (More waves than fit are a second round, shorter than the first.)
 long long resident(const Shape& s, int dtype, bool back) {
   const int values = s.k * (dtype == kF32 ? 4 : 8), waves = !back || s.tpr == 1024 ? 4 : values == 4 ? 3 : 2;
   return 256LL * waves * 4 * 64 / std::max(256, s.tpr);

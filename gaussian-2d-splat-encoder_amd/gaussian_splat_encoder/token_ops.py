@@ -50,7 +50,8 @@ class RotaryAxes:
         except OverflowError:
             rates = [math.inf]
         if not all(abs(r) <= _MAX_FLOAT for r in rates):
-            raise ValueError(f"rates scale * base ** (-2 i / dims) must be finite float32, got base {self.base}, scale {self.scale}")
+            raise ValueError(f"rates scale * base ** (-2 i / dims) must be finite float32, got base {self.base}, scale "
+                             f"{self.scale}")
         self._c = SplatRotation(len(self.dims), int(self.interleaved), (ctypes.c_int * 4)(*self.dims),
                                 (ctypes.c_double * 64)(*(r * 2 / math.pi for r in rates)))
 

@@ -1,5 +1,5 @@
 """TokenReader: a layer of tokens that read states with positions (the splats of a stream of frames, a map's cells, earlier
-tokens), dense in training and over a paged cache in serving:
+tokens), dense in training and over a paged cache in serving (there also in order, which the dense attention has no mode for):
 
     a = attention(turn(q(norm(x))), turn(k(states)), v(states))     y = x + gate norm(out(a))     y + gate norm(fc2(gelu(fc1(norm(y)))))
 
@@ -77,7 +77,8 @@ class TokenReader(nn.Module):
                                              key_mask=key_mask))
 
     def new_cache(self, sequences, tokens, page=64, dtype=torch.bfloat16, device="cuda", masked=False):
-        """A cache with room for `tokens` states of each sequence, and its tables. dtype: the states' (keys and values have it)."""
+        """A cache with room for `tokens` states of each sequence, and its tables. dtype: the states', which keys and values
+        have too."""
         cache = PagedCache.empty(sequences * -(-tokens // page), page, self.kv_heads, self.head_dim, dtype, device, masked)
         return cache, cache.tables(sequences)
 

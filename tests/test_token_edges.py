@@ -87,7 +87,8 @@ def test_one_bfloat16_value_for_two_would_show(H, Hk, D, n):
     from _feature_ref import rel
     b = torch.bfloat16
     g = torch.Generator().manual_seed(1)
-    q, k, v = ((torch.randn(12, *s, D, generator=g) * f).to(b).double() for s, f in (((H,), 1.3), ((n, Hk), 1.3), ((n, Hk), 1.0)))
+    q, k, v = ((torch.randn(12, *s, D, generator=g) * f).to(b).double()
+               for s, f in (((H,), 1.3), ((n, Hk), 1.3), ((n, Hk), 1.0)))
     k, v = k.repeat_interleave(H // Hk, 2), v.repeat_interleave(H // Hk, 2)
     q = R.rotary(q[:, None], torch.full((12, 1, 1), 12345.0, dtype=torch.float64), F.RotaryAxes((D,)))[:, 0]
 
@@ -105,7 +106,8 @@ def test_one_bfloat16_value_for_two_would_show(H, Hk, D, n):
 def test_an_append_into_expanded_pages_is_refused(no_launch):
     """Tokens that share memory may be read, but a call would write many of them to one place."""
     one = t(1, 8, 2, 16)
-    for c in (F.PagedCache(one.expand(4, 8, 2, 16), t(4, 8, 2, 16)), F.PagedCache(t(4, 8, 2, 16), t(4, 1, 2, 16).expand(4, 8, 2, 16)),
+    for c in (F.PagedCache(one.expand(4, 8, 2, 16), t(4, 8, 2, 16)),
+              F.PagedCache(t(4, 8, 2, 16), t(4, 1, 2, 16).expand(4, 8, 2, 16)),
               F.PagedCache(t(4, 8, 2, 16), t(4, 8, 2, 16), t(4, 1, dtype=torch.bool).expand(4, 8))):
         append, read = calls(t(1, 1, 2), c)
         with pytest.raises(ValueError, match="share memory"):
